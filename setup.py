@@ -28,6 +28,9 @@ setup(
             sources=SOURCES,
             include_dirs=[os.path.join(HERE, CSRC)],
             extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": NVCC},
+            # the process's own C++ runtime: where a toolchain has only the static archive, a second
+            # copy of it inside the extension crashes as soon as an error message prints a number
+            extra_link_args=["-l:libstdc++.so.6"],
         )
     ],
     cmdclass={"build_ext": BuildExtension.with_options(use_ninja=True)},
