@@ -1644,6 +1644,156 @@ torch::Tensor ce_online_bwd(torch::Tensor h, torch::Tensor W, torch::Tensor labe
   return dh;
 }
 
+// ------------------------------------------------------------ serving
+// (rows, channels) of packed or per-row tokens: unit channel stride, any row stride
+void check_rows(const torch::Tensor& t, const torch::Tensor& like, int64_t rows, int64_t cols, const char* op,
+                const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == like.scalar_type() && t.dim() == 2 &&
+                  t.size(0) == rows && t.size(1) == cols && (t.stride(1) == 1 || cols == 1),
+              op, ": ", name, " must be a ", like.scalar_type(), " tensor of ", rows, " rows and ", cols,
+              " channels with unit channel stride on ", like.device(), ", got ", t.scalar_type(), " ", t.sizes());
+}
+
+void check_flat(const torch::Tensor& t, const torch::Tensor& like, at::ScalarType dt, int64_t numel, const char* op,
+                const char* name) {
+  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == dt && t.is_contiguous() && t.numel() == numel, op, ": ",
+              name, " must be a contiguous ", dt, " tensor of ", numel, " values on ", like.device(), ", got ",
+              t.scalar_type(), " ", t.sizes());
+}
+
+struct SeqArgs {
+  const int *cu, *slots;
+  int B, L;
+};
+
+// Sequences of T packed rows: from cu_seqlens, or rows of L tokens each.
+SeqArgs seq_args(const torch::Tensor& like, int64_t T, int64_t L, int64_t S, const c10::optional<torch::Tensor>& cu,
+                 const c10::optional<torch::Tensor>& slots, const char* op) {
+  SeqArgs a{nullptr, nullptr, 0, (int)L};
+  if (cu.has_value()) {
+    TORCH_CHECK(cu->numel() >= 1, op, ": cu_seqlens must hold at least one offset");
+    check_flat(*cu, like, at::kInt, cu->numel(), op, "cu_seqlens");
+    a.cu = cu->data_ptr<int>();
+    a.B = (int)cu->numel() - 1;
+  } else {
+    a.B = (int)(L > 0 ? T / L : 0);
+  }
+  if (slots.has_value()) {
+    check_flat(*slots, like, at::kInt, a.B, op, "slots");
+    a.slots = slots->data_ptr<int>();
+  } else {
+    TORCH_CHECK(a.B <= S, op, ": ", a.B, " sequences need a state slot each, the state has ", S);
+  }
+  TORCH_CHECK(a.B <= 65535, op, ": at most 65535 sequences in one call, got ", a.B);
+  return a;
+}
+
+torch::Tensor selective_scan(const torch::Tensor& x, const torch::Tensor& dt, const torch::Tensor& A,
+                             const torch::Tensor& Bm, const torch::Tensor& Cm, const torch::Tensor& conv_w,
+                             const c10::optional<torch::Tensor>& conv_b, const torch::Tensor& conv_state,
+                             const torch::Tensor& state, int64_t L, const c10::optional<torch::Tensor>& cu,
+                             const c10::optional<torch::Tensor>& slots, double dt_min, double dt_max) {
+  const char* op = "selective_scan";
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, op, ": x must be a CUDA tensor of (tokens, channels) rows");
+  TORCH_CHECK(state.dim() == 4 && state.scalar_type() == at::kFloat && state.is_contiguous() &&
+                  state.device() == x.device(),
+              op, ": state must be a contiguous fp32 (slots, heads, head dim, states) tensor on ", x.device());
+  const int64_t T = x.size(0), C = x.size(1), S = state.size(0), H = state.size(1), P = state.size(2), N = state.size(3);
+  TORCH_CHECK(H * P == C && C > 0, op, ": ", H, " heads of ", P, " channels do not make ", C);
+  TORCH_CHECK(T < (1ll << 31) && C < (1ll << 24), op, ": sizes out of range");
+  check_rows(x, x, T, C, op, "x");
+  check_rows(dt, x, T, C, op, "dt");
+  check_rows(Bm, x, T, N, op, "B");
+  check_rows(Cm, x, T, N, op, "C");
+  check_flat(A, x, at::kFloat, H, op, "A");
+  check_flat(conv_w, x, conv_w.scalar_type(), C * 4, op, "conv_w (channels, 4)");
+  if (conv_b.has_value()) check_flat(*conv_b, x, at::kFloat, C, op, "conv_b");
+  check_flat(conv_state, x, x.scalar_type(), S * 3 * C, op, "conv_state (slots, 3, channels)");
+  const SeqArgs q = seq_args(x, T, L, S, cu, slots, op);
+  const c10::cuda::CUDAGuard guard(x.device());
+  auto y = torch::empty({T, C}, x.options());
+  const int rc = ahb_selective_scan(x.data_ptr(), x.stride(0), dt.data_ptr(), dt.stride(0), A.data_ptr<float>(),
+                                    Bm.data_ptr(), Bm.stride(0), Cm.data_ptr(), Cm.stride(0), conv_w.data_ptr(),
+                                    dt_code(conv_w), opt_ptr(conv_b), conv_state.data_ptr(), state.data_ptr<float>(),
+                                    q.cu, q.slots, y.data_ptr(), q.B, q.L, (int)T, (int)C, (int)P, (int)N, (int)S,
+                                    dt_code(x), (float)dt_min, (float)dt_max, cur_stream());
+  TORCH_CHECK(rc == 0, op, ": no kernel for ", N, " states");
+  check_launch(op);
+  return y;
+}
+
+torch::Tensor gdn2_recurrent(const std::vector<torch::Tensor>& in, const std::vector<torch::Tensor>& conv_w,
+                             const std::vector<c10::optional<torch::Tensor>>& conv_b, const torch::Tensor& decay_a,
+                             const torch::Tensor& conv_state, const torch::Tensor& state, int64_t L,
+                             const c10::optional<torch::Tensor>& cu, const c10::optional<torch::Tensor>& slots) {
+  const char* op = "gdn2_recurrent";
+  static const char* names[6] = {"q", "k", "v", "b", "w", "f"};
+  TORCH_CHECK(in.size() == 6 && conv_w.size() == 3 && conv_b.size() == 3, op, ": six inputs, three convolutions");
+  const torch::Tensor& x = in[0];
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, op, ": q must be a CUDA tensor of (tokens, channels) rows");
+  TORCH_CHECK(state.dim() == 4 && state.scalar_type() == at::kFloat && state.is_contiguous() &&
+                  state.device() == x.device() && state.size(2) == state.size(3),
+              op, ": state must be a contiguous fp32 (slots, heads, D, D) tensor on ", x.device());
+  const int64_t T = x.size(0), d = x.size(1), S = state.size(0), H = state.size(1), D = state.size(2);
+  TORCH_CHECK(H * D == d && d > 0, op, ": ", H, " heads of ", D, " channels do not make ", d);
+  TORCH_CHECK(T < (1ll << 31) && H < (1ll << 16), op, ": sizes out of range");
+  const void* ip[6];
+  int64_t rs[6];
+  for (int i = 0; i < 6; ++i) {
+    check_rows(in[i], x, T, d, op, names[i]);
+    ip[i] = in[i].data_ptr();
+    rs[i] = in[i].stride(0);
+  }
+  const void* wp[3];
+  const float* bp[3];
+  for (int i = 0; i < 3; ++i) {
+    check_flat(conv_w[i], x, conv_w[0].scalar_type(), d * 4, op, "conv_w (channels, 4)");
+    if (conv_b[i].has_value()) check_flat(*conv_b[i], x, at::kFloat, d, op, "conv_b");
+    wp[i] = conv_w[i].data_ptr();
+    bp[i] = opt_ptr(conv_b[i]);
+  }
+  check_flat(decay_a, x, at::kFloat, H, op, "decay_a");
+  check_flat(conv_state, x, x.scalar_type(), S * 9 * d, op, "conv_state (slots, 3, 3, channels)");
+  const SeqArgs q = seq_args(x, T, L, S, cu, slots, op);
+  const c10::cuda::CUDAGuard guard(x.device());
+  auto y = torch::empty({T, d}, x.options());
+  const int rc = ahb_gdn_recurrent(ip, rs, wp, dt_code(conv_w[0]), bp, decay_a.data_ptr<float>(), conv_state.data_ptr(),
+                                   state.data_ptr<float>(), q.cu, q.slots, y.data_ptr(), q.B, q.L, (int)T, (int)H,
+                                   (int)D, (int)S, dt_code(x), cur_stream());
+  TORCH_CHECK(rc == 0, op, ": no kernel for head dim ", D);
+  check_launch(op);
+  return y;
+}
+
+std::vector<torch::Tensor> sample(const torch::Tensor& logits, const torch::Tensor& noise,
+                                  const torch::Tensor& temperature, const torch::Tensor& top_k,
+                                  const torch::Tensor& top_p, const torch::Tensor& min_p) {
+  const char* op = "sample";
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.size(1) > 0, op,
+              ": logits must be a CUDA tensor of (rows, vocabulary)");
+  const int64_t B = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(V < (1ll << 31) && B < (1ll << 31), op, ": sizes out of range");
+  check_rows(logits, logits, B, V, op, "logits");
+  TORCH_CHECK(noise.device() == logits.device() && noise.scalar_type() == at::kFloat && noise.dim() == 2 &&
+                  noise.size(0) == B && noise.size(1) == V && (noise.stride(1) == 1 || V == 1),
+              op, ": noise must be an fp32 tensor of the logits' shape with unit column stride, got ",
+              noise.scalar_type(), " ", noise.sizes());
+  check_flat(temperature, logits, at::kFloat, B, op, "temperature");
+  check_flat(top_k, logits, at::kInt, B, op, "top_k");
+  check_flat(top_p, logits, at::kFloat, B, op, "top_p");
+  check_flat(min_p, logits, at::kFloat, B, op, "min_p");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  auto tokens = torch::empty({B}, logits.options().dtype(at::kLong));
+  auto logprobs = torch::empty({B}, logits.options().dtype(at::kFloat));
+  const int rc = ahb_sample(logits.data_ptr(), logits.stride(0), dt_code(logits), noise.data_ptr<float>(),
+                            noise.stride(0), temperature.data_ptr<float>(), top_k.data_ptr<int>(),
+                            top_p.data_ptr<float>(), min_p.data_ptr<float>(), tokens.data_ptr<int64_t>(),
+                            logprobs.data_ptr<float>(), (int)B, (int)V, cur_stream());
+  TORCH_CHECK(rc == 0, op, ": failed with code ", rc);
+  check_launch(op);
+  return {tokens, logprobs};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1736,4 +1886,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bias_grad_acc", &bias_grad_acc);
   m.def("sum_slots", &sum_slots);
   m.def("memcpy_async", &memcpy_async);
+  m.def("selective_scan", &selective_scan);
+  m.def("gdn2_recurrent", &gdn2_recurrent);
+  m.def("sample", &sample);
 }

@@ -247,3 +247,24 @@ int ahb_ce_gemm(bool bwd, const void* h, int64_t rows, int d, const void* W, int
                 bool pair);
 void ahb_ce_combine(const void* partials, int ntiles, const int64_t* labels, int64_t T, int V, float ls, float* lse,
                     float* loss_sum, float* count, cudaStream_t st);
+
+// Serving (state carried between calls).  Sequence b is tokens cu[b] .. cu[b + 1] of the T packed rows
+// (cu null: rows b L .. b L + L) and keeps its state in slot slots[b] (null: slot b) of S; a slot outside
+// [0, S) gives zero outputs and touches no state.  Row strides (xs, ...) in elements, unit channel
+// stride.  Return 0, -1 for a size without a kernel, -2 for too many sequences.
+// selective_scan.cu: x, dt (T, C), Bm, Cm (T, N), conv_w (C, 4), conv_state (S, 3, C), state
+// (S, C / P, P, N) fp32, y (T, C); N in {32, 64, 128}.
+int ahb_selective_scan(const void* x, int64_t xs, const void* dt, int64_t dts, const float* A, const void* Bm,
+                       int64_t bs, const void* Cm, int64_t cs, const void* conv_w, int wdtype, const float* conv_b,
+                       void* conv_state, float* state, const int* cu, const int* slots, void* y, int B, int L, int T,
+                       int C, int P, int N, int S, int dtype, float dt_min, float dt_max, cudaStream_t st);
+// gdn_recurrent.cu: in = q, k, v, b, w, f (T, H D), conv_state (S, 3, 3, H D), state (S, H, D, D) fp32;
+// D in {64, 96, 128}.
+int ahb_gdn_recurrent(const void* const in[6], const int64_t rs[6], const void* const conv_w[3], int wdtype,
+                      const float* const conv_b[3], const float* decay_a, void* conv_state, float* state,
+                      const int* cu, const int* slots, void* y, int B, int L, int T, int H, int D, int S, int dtype,
+                      cudaStream_t st);
+// sample.cu: logits (B, V) of `dtype`, noise (B, V) fp32, per-row settings; tokens, logprobs (B,)
+int ahb_sample(const void* logits, int64_t ls, int dtype, const float* noise, int64_t ns, const float* temperature,
+               const int* top_k, const float* top_p, const float* min_p, int64_t* tokens, float* logprobs, int B, int V,
+               cudaStream_t st);

@@ -153,6 +153,66 @@ def grouped_ffn(x_sorted, group_sizes, w1, w2, w3, act: str, group_sizes_cpu=Non
     return R.grouped_ffn(x_sorted, sizes, w1.to(dt), w2.to(dt), None if w3 is None else w3.to(dt), act)
 
 
+# ---------------------------------------------------------------- serving (state carried between calls)
+def selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, cu_seqlens=None, slots=None,
+                   dt_min: float = 1e-2, dt_max: float = 1.0) -> torch.Tensor:
+    """Mamba2's short causal convolution and scan from and into a kept state; no gradient.
+
+    ``x`` (the scan's input before the convolution) and ``dt`` (before softplus, its bias added)
+    have ``C`` channels in ``A.numel()`` heads, ``Bm`` and ``Cm`` have ``N`` states::
+
+        xc_t = clip(silu(sum_j conv_w[:, j] x_{t-3+j} + conv_b), 1e3),  dt_t = clamp(softplus(dt_t), dt_min, dt_max)
+        S_t  = e^{max(dt_t A, -20)} S_{t-1} + dt_t xc_t B_t^T,          y_t = S_t C_t
+
+    Tokens come as ``(T, C)`` rows packed by ``cu_seqlens`` (int32, ``sequences + 1`` offsets on the
+    device; sequences of any length, also none), as ``(B, L, C)``, or as ``(B, C)`` rows of one token
+    each.  ``conv_state (S, 3, C)`` holds the last three rows of ``x`` in its dtype and ``state
+    (S, H, P, N)`` the fp32 scan state; both are updated in place.  Sequence ``i`` owns slot
+    ``slots[i]`` (int32, all different; default ``i``); one with a slot outside ``[0, S)`` is padding:
+    zeros come out and no state is touched.  Returns ``y`` shaped like ``x``."""
+    if use_cuda(x):
+        return _k().selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, cu_seqlens, slots, dt_min,
+                                   dt_max)
+    return R.selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, cu_seqlens, slots, dt_min, dt_max)
+
+
+def gdn2_recurrent(q, k, v, b, w, f, conv_w, conv_b, decay_a, conv_state, state, cu_seqlens=None,
+                   slots=None) -> torch.Tensor:
+    """GDN-2 token by token from and into a kept state (single tokens and a few at once; ``gdn2``
+    is the chunked form for long sequences); no gradient.
+
+    The six inputs are the layer's projections before convolution and gates, ``d = H D`` channels
+    each; ``conv_w`` / ``conv_b`` are the three convolutions of ``q, k, v``::
+
+        q, k, v = silu(conv(.)); v clipped to 50; q, k l2-normalised per head
+        h <- diag(exp(-e^decay_a softplus(f))) h;  n = sigmoid(w) v - (sigmoid(b) k)^T h
+        h <- h + k n^T;  o = q^T h
+
+    Tokens, ``cu_seqlens`` and ``slots`` as in ``selective_scan``; ``conv_state (S, 3, 3, d)`` holds
+    the last three rows of ``q, k, v`` (in that order) and ``state (S, H, D, D)`` the fp32 state, both
+    updated in place.  Returns ``o`` shaped like ``q``."""
+    if use_cuda(q):
+        return _k().gdn2_recurrent(q, k, v, b, w, f, conv_w, conv_b, decay_a, conv_state, state, cu_seqlens, slots)
+    return R.gdn2_recurrent(q, k, v, b, w, f, conv_w, conv_b, decay_a, conv_state, state, cu_seqlens, slots)
+
+
+def sample(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """The next token of every row of ``logits (B, V)`` from given noise; returns ``(tokens int64,
+    logprobs fp32)``.
+
+    ``noise (B, V)`` fp32 holds Exp(1) draws (``torch.empty(B, V).exponential_()``).  The settings are
+    numbers or ``(B,)`` tensors.  Tokens are ranked by (logit descending, index ascending); of the
+    row's distribution ``softmax(logits / temperature)`` those are kept whose rank is below ``top_k``
+    (0 or less: no limit), with less than ``top_p`` of the mass ranked before them (the first one
+    always), and with at least ``min_p`` times the first one's probability.  The token is the kept
+    one with the largest ``log p - log noise`` (ties: lowest index), which draws from the kept ones by
+    their probability.  ``temperature <= 0`` takes the first token and tempers by 1 for ``logprobs``,
+    the log-probability before anything is cut.  NaN and ``-inf`` logits are never drawn; a row
+    of nothing else gives token -1 and ``-inf``."""
+    if use_cuda(logits):
+        return _k().sample(logits, noise, temperature, top_k, top_p, min_p)
+    return R.sample(logits, noise, temperature, top_k, top_p, min_p)
+
 # ---------------------------------------------------------------- loss
 def cross_entropy(hidden: torch.Tensor, labels: torch.Tensor, weight: torch.Tensor,
                   label_smoothing: float, chunk: int = 2048):

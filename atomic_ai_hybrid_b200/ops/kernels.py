@@ -889,6 +889,58 @@ def newton_schulz3(g, steps: int = 3, eps: float = 1e-4):
     return out.reshape(g.shape)
 
 
+# ----------------------------------------------------------------- serving (state carried between calls)
+def _flat_rows(t):
+    """``(B, L, C)`` or ``(T, C)`` as ``(T, C)`` rows of unit channel stride (a column slice stays a view)."""
+    if t.dim() == 3:
+        t = t.reshape(-1, t.shape[2])
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, cu_seqlens, slots, dt_min, dt_max):
+    """See ``ops.selective_scan``; bf16 or fp32 tokens and 32, 64 or 128 states (others run the PyTorch form)."""
+    if state.shape[-1] not in (32, 64, 128):
+        _unsupported(f"selective_scan N={state.shape[-1]}")
+        return R.selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, cu_seqlens, slots, dt_min, dt_max)
+    if x.dim() == 2:
+        return ext().selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, 1, cu_seqlens, slots, dt_min,
+                                    dt_max)
+    R.check_no_offsets(cu_seqlens)
+    y = ext().selective_scan(_flat_rows(x), _flat_rows(dt), A, _flat_rows(Bm), _flat_rows(Cm), conv_w, conv_b,
+                             conv_state, state, x.shape[1], None, slots, dt_min, dt_max)
+    return y.view(x.shape)
+
+
+def gdn2_recurrent(q, k, v, b, w, f, conv_w, conv_b, decay_a, conv_state, state, cu_seqlens, slots):
+    """See ``ops.gdn2_recurrent``; bf16 or fp32 tokens and head dims 64, 96, 128 (others run the PyTorch form)."""
+    if state.shape[-1] not in (64, 96, 128):
+        _unsupported(f"gdn2_recurrent D={state.shape[-1]}")
+        return R.gdn2_recurrent(q, k, v, b, w, f, conv_w, conv_b, decay_a, conv_state, state, cu_seqlens, slots)
+    if q.dim() == 2:
+        return ext().gdn2_recurrent((q, k, v, b, w, f), conv_w, conv_b, decay_a, conv_state, state, 1, cu_seqlens,
+                                    slots)
+    R.check_no_offsets(cu_seqlens)
+    y = ext().gdn2_recurrent([_flat_rows(t) for t in (q, k, v, b, w, f)], conv_w, conv_b, decay_a, conv_state, state,
+                             q.shape[1], None, slots)
+    return y.view(q.shape)
+
+
+def _per_row(v, like, dtype):
+    """A setting as a ``(B,)`` tensor of ``dtype`` on the rows' device."""
+    if isinstance(v, torch.Tensor):
+        return v if v.dtype == dtype and v.device == like.device else v.to(device=like.device, dtype=dtype)
+    return torch.full((like.shape[0],), v, dtype=dtype, device=like.device)
+
+
+def sample(logits, noise, temperature, top_k, top_p, min_p):
+    """See ``ops.sample``; bf16 or fp32 logits."""
+    f32 = torch.float32
+    tokens, logprobs = ext().sample(logits, noise, _per_row(temperature, logits, f32),
+                                    _per_row(top_k, logits, torch.int32), _per_row(top_p, logits, f32),
+                                    _per_row(min_p, logits, f32))
+    return tokens, logprobs
+
+
 # ----------------------------------------------------------------- fused optimizer
 _WD = {"muon": 0.01, "lion": 0.1, "adamw_decay": 0.01, "adamw_nodecay": 0.0, "frozen": 0.0}
 _ORDER = ("muon", "lion", "adamw_decay", "adamw_nodecay", "frozen")

@@ -297,6 +297,134 @@ def grouped_ffn(x_sorted: Tensor, group_sizes, w1: Tensor, w2: Tensor, w3: Optio
     return torch.cat(outs, 0) if outs else x_sorted.new_zeros(0, w2.shape[-1])
 
 
+# --------------------------------------------------------------------------
+# Serving: state carried between calls (updated in place)
+# --------------------------------------------------------------------------
+def check_no_offsets(cu_seqlens) -> None:
+    if cu_seqlens is not None:
+        raise ValueError("cu_seqlens packs (T, channels) rows; (B, L, channels) tokens have none")
+
+
+def _sequences(x: Tensor, cu_seqlens, slots, n_slots: int):
+    """``[(slot, start, end)]`` of the sequences in the flattened rows of ``x``; slot -1 is padding."""
+    if x.dim() == 3:
+        check_no_offsets(cu_seqlens)
+        cu = [i * x.shape[1] for i in range(x.shape[0] + 1)]
+    elif cu_seqlens is not None:
+        T = x.shape[0]
+        cu = [min(max(c, 0), T) for c in cu_seqlens.tolist()]
+    else:
+        cu = list(range(x.shape[0] + 1))
+    which = list(range(len(cu) - 1)) if slots is None else slots.tolist()
+    if len(which) != len(cu) - 1:
+        raise ValueError(f"{len(cu) - 1} sequences, {len(which)} slots")
+    if slots is None and len(which) > n_slots:
+        raise ValueError(f"{len(which)} sequences need a state slot each, the state has {n_slots}")
+    return [(s if 0 <= s < n_slots else -1, a, max(a, e)) for s, a, e in zip(which, cu[:-1], cu[1:])]
+
+
+def _window_conv(x: Tensor, window: Tensor, w: Tensor, b: Optional[Tensor], acc):
+    """SiLU of the causal convolution of one sequence ``(l, C)`` after ``window (3, C)``; the new window."""
+    ext = torch.cat([window, x], 0)
+    l = x.shape[0]
+    y = sum(ext[j:j + l].to(acc) * w[:, j].to(acc) for j in range(4))
+    return F.silu(y if b is None else y + b.to(acc)), ext[l:]
+
+
+@torch.no_grad()
+def selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, cu_seqlens=None, slots=None,
+                   dt_min: float = 1e-2, dt_max: float = 1.0):
+    """Token-serial form of ``ops.selective_scan`` (the states are kept in ``state``'s dtype)."""
+    S, H, P, N = state.shape
+    C = H * P
+    acc = _acc_dtype(state)
+    flat = lambda t, n: t.reshape(-1, n)  # noqa: E731
+    xf, dtf, Bf, Cf = flat(x, C), flat(dt, C), flat(Bm, N), flat(Cm, N)
+    y = torch.zeros(xf.shape, dtype=x.dtype, device=x.device)
+    a_chan = A.to(acc).repeat_interleave(P)
+    for slot, s, e in _sequences(x, cu_seqlens, slots, S):
+        if slot < 0 or e == s:
+            continue
+        xc, window = _window_conv(xf[s:e], conv_state[slot], conv_w, conv_b, acc)
+        conv_state[slot] = window
+        step = torch.nan_to_num(F.softplus(dtf[s:e].to(acc)).clamp(dt_min, dt_max), nan=0.0)
+        a = torch.exp((step * a_chan).clamp(min=-20.0))
+        u = step * sanitize(xc, 1e3)
+        Bs, Cs = sanitize(Bf[s:e].to(acc), 1e3), sanitize(Cf[s:e].to(acc), 1e3)
+        h = state[slot].to(acc).view(C, N)
+        for t in range(e - s):
+            h = h * a[t][:, None] + u[t][:, None] * Bs[t]
+            y[s + t] = (h @ Cs[t]).to(y.dtype)
+        state[slot] = h.view(H, P, N)
+    return y.view(x.shape)
+
+
+@torch.no_grad()
+def gdn2_recurrent(q, k, v, b, w, f, conv_w, conv_b, decay_a, conv_state, state, cu_seqlens=None, slots=None):
+    """Token-serial form of ``ops.gdn2_recurrent``."""
+    S, H, D, _ = state.shape
+    d = H * D
+    acc = _acc_dtype(state)
+    rows = [t.reshape(-1, d) for t in (q, k, v, b, w, f)]
+    o = torch.zeros(rows[0].shape, dtype=q.dtype, device=q.device)
+    rate = torch.exp(decay_a.to(acc).clamp(-20.0, 20.0))[:, None]
+    for slot, s, e in _sequences(q, cu_seqlens, slots, S):
+        if slot < 0 or e == s:
+            continue
+        qkv = []
+        for m in range(3):
+            y, conv_state[slot, m] = _window_conv(rows[m][s:e], conv_state[slot, m], conv_w[m], conv_b[m], acc)
+            qkv.append(y.view(-1, H, D))
+        qs, ks = (sanitize(t * torch.rsqrt((t * t).sum(-1, keepdim=True) + 1e-12), 1e3) for t in qkv[:2])
+        vs = sanitize(qkv[2], 50.0)
+        erase, write = (sanitize(torch.sigmoid(t[s:e].to(acc)), 1.0).view(-1, H, D) for t in rows[3:5])
+        g = torch.nan_to_num(-rate * F.softplus(rows[5][s:e].to(acc)).view(-1, H, D), nan=0.0).clamp(min=-1e3)
+        h = state[slot].to(acc)
+        for t in range(e - s):
+            h = h * torch.exp(g[t])[..., None]
+            new = write[t] * vs[t] - torch.einsum("hk,hkv->hv", erase[t] * ks[t], h)
+            h = h + ks[t][..., None] * new[:, None]
+            o[s + t] = torch.einsum("hk,hkv->hv", qs[t], h).reshape(d).to(o.dtype)
+        state[slot] = h
+    return o.view(q.shape)
+
+
+@torch.no_grad()
+def sample(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """``ops.sample`` by sorting each row."""
+    B, V = logits.shape
+    acc = _acc_dtype(logits)
+
+    def setting(t, dtype):
+        t = t if isinstance(t, torch.Tensor) else torch.full((B,), t)
+        return t.to(device=logits.device, dtype=dtype)[:, None]
+
+    l = logits.to(acc)
+    l = torch.where(torch.isnan(l), -math.inf, l).clamp(max=torch.finfo(torch.float32).max)
+    T, k = setting(temperature, acc), setting(top_k, torch.long)
+    greedy = ~(T > 0)
+    k = torch.where(greedy, 1, torch.where(k <= 0, V, k))
+    T = torch.where(greedy, 1.0, T)
+    ranked, index = torch.sort(l, dim=1, descending=True, stable=True)
+    top = ranked[:, :1]
+    empty = top == -math.inf
+    nd = torch.where(empty, -math.inf, (ranked - top) / T)  # -d
+    mass = torch.exp(nd)
+    before = torch.cumsum(mass, 1) - mass
+    total = mass.sum(1, keepdim=True)
+    rank = torch.arange(V, device=l.device)[None]
+    first = rank == 0
+    kept = (rank < k) & (first | (before < setting(top_p, acc) * total)) & (first | (mass >= setting(min_p, acc)))
+    kept &= ranked > -math.inf
+    score = nd - torch.log(noise.to(acc).gather(1, index))
+    score = torch.where(kept, torch.nan_to_num(score, nan=-math.inf, posinf=math.inf, neginf=-math.inf), -math.inf)
+    best = score.max(1, keepdim=True).values
+    tokens = torch.where(kept & (score == best), index, V).min(1, keepdim=True).values
+    tokens = torch.where(empty, -1, tokens)
+    logp = (l.gather(1, tokens.clamp(min=0)) - top) / T - torch.log(total)
+    return tokens[:, 0], torch.where(empty, -math.inf, logp)[:, 0].to(torch.float64 if acc == torch.float64 else torch.float32)
+
+
 def newton_schulz3(g: Tensor, steps: int = 3, eps: float = 1e-4) -> Tensor:
     """Reference Muon orthogonalisation (reference `optimizer.py:53-77`)."""
     if g.ndim == 3:
