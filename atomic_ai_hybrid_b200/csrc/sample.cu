@@ -42,15 +42,47 @@ struct SampleArgs {
   int resident;  // the CTA's part of the row fits in shared memory
 };
 
-constexpr int kBins = 512;
+constexpr int kBins = 512, kMaxCtas = 8;
 constexpr float kBinsPerLog2 = 12.f;  // bins of 6 % in probability over the top 2^-42; finer for a flatter row
 constexpr float kSlack = 1e-5f;       // rounding of the fp32 mass sums
 
+// What the threads of a cluster bring together: the race's leader as an ordered key (score, then lowest
+// index) with its logit, a mass, an index and a count, the largest and least logit.
 struct alignas(16) Part {
-  float v;
-  int i;
-  float l, w;
+  uint32_t score, place;  // order_of(score), ~index; 0: none
+  float logit, mass;
+  int first, count;
+  float most, least;
+  AHB_DEVICE static Part none() { return {0u, 0u, 0.f, 0.f, INT_MAX, 0, -INFINITY, INFINITY}; }
+  AHB_DEVICE int index() const { return (int)~place; }
+  template <int F>
+  AHB_DEVICE void take(const Part& b);
 };
+enum { RACE = 1, MASS = 2, FIRST = 4, COUNT = 8, RANGE = 16 };
+
+template <int F>
+AHB_DEVICE void Part::take(const Part& b) {
+  if (F & RACE) {
+    const bool t = b.score > score || (b.score == score && b.place > place);
+    logit = t ? b.logit : logit;
+    score = t ? b.score : score;
+    place = t ? b.place : place;
+  }
+  if (F & MASS) mass += b.mass;
+  if (F & FIRST) first = min(first, b.first);
+  if (F & COUNT) count += b.count;
+  if (F & RANGE) {
+    most = fmaxf(most, b.most);
+    least = fminf(least, b.least);
+  }
+}
+
+// monotone maps between floats (no NaN) and unsigned / signed integers
+AHB_DEVICE uint32_t order_of(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+AHB_DEVICE float value_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 
 AHB_DEVICE float ex2(float x) {
   float y;
@@ -58,43 +90,29 @@ AHB_DEVICE float ex2(float x) {
   return y;
 }
 
-// larger value, then lower index
-AHB_DEVICE bool beats(float v, int i, const Part& b) { return v > b.v || (v == b.v && i < b.i); }
-
-AHB_DEVICE Part shfl_xor(const Part& p, int o) {
-  return {__shfl_xor_sync(0xffffffffu, p.v, o), __shfl_xor_sync(0xffffffffu, p.i, o),
-          __shfl_xor_sync(0xffffffffu, p.l, o), __shfl_xor_sync(0xffffffffu, p.w, o)};
+// The fields F over a warp; every lane gets the result (the same bits: the additions are symmetric).
+template <int F>
+AHB_DEVICE Part warp_part(Part p) {
+  constexpr uint32_t all = 0xffffffffu;
+  if (F & RACE) {
+    const uint32_t score = __reduce_max_sync(all, p.score);
+    const uint32_t place = __reduce_max_sync(all, p.score == score ? p.place : 0u);
+    const uint32_t who = __ballot_sync(all, p.score == score && p.place == place);
+    p.logit = __shfl_sync(all, p.logit, __ffs(who) - 1);
+    p.score = score;
+    p.place = place;
+  }
+  if (F & MASS) p.mass = warp_sum(p.mass);
+  if (F & FIRST) p.first = __reduce_min_sync(all, p.first);
+  if (F & COUNT) p.count = __reduce_add_sync(all, p.count);
+  if (F & RANGE) {
+    p.most = value_of(__reduce_max_sync(all, order_of(p.most)));
+    p.least = value_of(__reduce_min_sync(all, order_of(p.least)));
+  }
+  return p;
 }
-// winner of (v, i) with its l; sum of w
-struct TakeBest {
-  AHB_DEVICE static Part none() { return {-INFINITY, INT_MAX, 0.f, 0.f}; }
-  AHB_DEVICE Part operator()(Part a, const Part& b) const {
-    const float w = a.w + b.w;
-    if (beats(b.v, b.i, a)) a = b;
-    a.w = w;
-    return a;
-  }
-};
-// larger v, then lower i; smaller l
-struct TakeRange {
-  AHB_DEVICE static Part none() { return {-INFINITY, INT_MAX, INFINITY, 0.f}; }
-  AHB_DEVICE Part operator()(Part a, const Part& b) const {
-    const float l = fminf(a.l, b.l);
-    if (beats(b.v, b.i, a)) a = b;
-    a.l = l;
-    return a;
-  }
-};
-// sums of i and w
-struct TakeSum {
-  AHB_DEVICE static Part none() { return {0.f, 0, 0.f, 0.f}; }
-  AHB_DEVICE Part operator()(Part a, const Part& b) const {
-    a.i += b.i;
-    a.w += b.w;
-    return a;
-  }
-};
 
+// 16 bytes of logits
 template <typename T> struct Vec;
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
@@ -107,8 +125,15 @@ template <> struct Vec<__nv_bfloat16> {
     const uint32_t h = __float_as_uint(v) >> 16;
     w = j & 1 ? (w & 0xffffu) | (h << 16) : (w & 0xffff0000u) | h;
   }
-  // +inf counts as the largest value of the type
-  AHB_DEVICE static float most() { return __uint_as_float(0x7f7f0000u); }
+  // NaN becomes -inf, +inf the largest value of the type (max and min return the operand that is not NaN)
+  AHB_DEVICE static void clean(uint4& r) {
+    const uint32_t lo = 0xff80ff80u, hi = 0x7f7f7f7fu;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t& w = k == 0 ? r.x : k == 1 ? r.y : k == 2 ? r.z : r.w;
+      asm("max.bf16x2 %0, %0, %1;\n\tmin.bf16x2 %0, %0, %2;" : "+r"(w) : "r"(lo), "r"(hi));
+    }
+  }
 };
 template <> struct Vec<float> {
   static constexpr int N = 4;
@@ -118,42 +143,57 @@ template <> struct Vec<float> {
   AHB_DEVICE static void put(uint4& r, int j, float v) {
     (j == 0 ? r.x : j == 1 ? r.y : j == 2 ? r.z : r.w) = __float_as_uint(v);
   }
-  AHB_DEVICE static float most() { return FLT_MAX; }
+  AHB_DEVICE static void clean(uint4& r) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) put(r, j, fminf(fmaxf(get(r, j), -INFINITY), FLT_MAX));
+  }
 };
+template <typename T>
+AHB_DEVICE float largest(const uint4& r) {
+  float m = Vec<T>::get(r, 0);
+#pragma unroll
+  for (int j = 1; j < Vec<T>::N; ++j) m = fmaxf(m, Vec<T>::get(r, j));
+  return m;
+}
 
-// Combines the threads' parts, then the CTAs' in rank order; every thread gets the result.  `mine` are
-// two slots used in turn: one is rewritten only after the barrier that follows its last reading.
-template <int NT, class Op>
-AHB_DEVICE Part combine(Part p, Op op, Part* warps, Part* mine, int turn, int ctas) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) p = op(p, shfl_xor(p, o));
-  if (lane == 0) warps[threadIdx.x >> 5] = p;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    p = lane < NT / 32 ? warps[lane] : Op::none();
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) p = op(p, shfl_xor(p, o));
-    if (lane == 0) mine[turn] = p;
+// Combines the parts of all threads of the cluster; every thread gets the result.  Each warp puts its
+// part into every CTA's shared memory before the barrier, and every warp combines them all after it from
+// its own: one barrier, and no remote read waits.  `parts` are two sets of slots used in turn: one is
+// rewritten only after the barrier that follows its last reading.
+template <int F, int NT>
+AHB_DEVICE Part combine(Part p, Part (*parts)[kMaxCtas * NT / 32], int turn, int rank, int ctas) {
+  constexpr int NW = NT / 32;
+  const int lane = threadIdx.x & 31, at = rank * NW + (threadIdx.x >> 5);
+  p = warp_part<F>(p);
+  if (ctas == 1) {
+    if (lane == 0) parts[turn][at] = p;
+    __syncthreads();
+  } else {
+    if (lane < ctas) {
+      const uint32_t a = mapa_shared(&parts[turn][at], lane);
+      if (F & (RACE | MASS))
+        asm volatile("st.shared::cluster.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(p.score), "r"(p.place),
+                     "r"(__float_as_uint(p.logit)), "r"(__float_as_uint(p.mass)) : "memory");
+      if (F & (FIRST | COUNT | RANGE))
+        asm volatile("st.shared::cluster.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a + 16), "r"((uint32_t)p.first),
+                     "r"((uint32_t)p.count), "r"(__float_as_uint(p.most)), "r"(__float_as_uint(p.least)) : "memory");
+    }
+    cluster_sync();
   }
-  cluster_sync();
-  p = Op::none();
-  for (int r = 0; r < ctas; ++r) {
-    const uint32_t a = mapa_shared(&mine[turn], r);
-    uint32_t x, y, z, w;
-    asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x), "=r"(y), "=r"(z), "=r"(w) : "r"(a) : "memory");
-    p = op(p, Part{__uint_as_float(x), (int)y, __uint_as_float(z), __uint_as_float(w)});
-  }
-  return p;
+  p = Part::none();
+#pragma unroll
+  for (int u = 0; u < kMaxCtas * NW / 32; ++u)
+    if (u * 32 + lane < ctas * NW) p.take<F>(parts[turn][u * 32 + lane]);
+  return warp_part<F>(p);
 }
 
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT) sample_kernel(SampleArgs p, int ctas) {
   using X = Vec<T>;
-  constexpr int N = X::N;
+  constexpr int N = X::N, U = 16 / N;
   extern __shared__ __align__(16) uint4 keep[];
-  __shared__ Part warps[NT / 32], mine[2];
-  __shared__ int hist[kBins];
+  __shared__ Part parts[2][kMaxCtas * NT / 32];
+  __shared__ int hist[kBins + 32];   // then a place per lane for what is beyond the bins
   __shared__ int count_to[kBins];    // tokens in bins up to and with this one
   __shared__ float most_to[kBins];   // and the most mass they can stand for
   __shared__ float2 wsum[kBins / 32];
@@ -162,46 +202,39 @@ __global__ void __launch_bounds__(NT) sample_kernel(SampleArgs p, int ctas) {
   const int tid = threadIdx.x, rank = (int)cluster_ctarank();
   const int64_t row = blockIdx.x / ctas;
   const T* l = static_cast<const T*>(p.logits) + row * p.ls;
-  const float* q = p.noise + row * p.ns;
+  const float* noise = p.noise + row * p.ns;
   const float temp = p.temperature[row];
   const bool greedy = !(temp > 0.f);
   const float inv = greedy ? 1.f : fminf(fmaxf(1.f / temp, 1e-30f), 1e30f);
   const float c = inv * 1.4426950408889634f;  // logits to log2 of a probability
   const int kr = p.top_k[row], k = kr <= 0 || kr > p.V ? p.V : kr;
   const float top_p = p.top_p[row], min_p = fminf(p.min_p[row], 1.f);
-  const float most_x = min_p > 0.f ? -__log2f(min_p) : INFINITY;
   const bool by_rank = !greedy && k < p.V, by_mass = !greedy && top_p < 1.f;
   int turn = 0;
 
   // vectors [v0, v1) of the row in 16-byte lines; its first element is element `skew` of line 0
   const int skew = (int)((reinterpret_cast<uintptr_t>(l) & 15) / sizeof(T));
   const int v0 = rank * p.chunk, v1 = min(v0 + p.chunk, (skew + p.V + N - 1) / N);
+  const bool q4 = (reinterpret_cast<uintptr_t>(noise - skew) & 15) == 0;  // noise in 16-byte pieces beside it
   auto fetch = [&](int v) {
-    uint4 r = make_uint4(0, 0, 0, 0);
     const int i = v * N - skew;
     if (i >= 0 && i + N <= p.V) return __ldg(reinterpret_cast<const uint4*>(l + i));
+    uint4 r = make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int j = 0; j < N; ++j) X::put(r, j, i + j >= 0 && i + j < p.V ? to_f(l[i + j]) : -INFINITY);
     return r;
   };
-  auto clean = [&](uint4& r) {  // NaN never drawn, +inf as the largest value
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float x = X::get(r, j);
-      if (!(x < INFINITY)) X::put(r, j, x != x ? -INFINITY : X::most());
-    }
-  };
   auto line = [&](int v) {
     if (p.resident) return keep[v - v0];
     uint4 r = fetch(v);
-    clean(r);
+    X::clean(r);
     return r;
   };
 
   // pass 1: the row into shared memory, its largest and least values
   for (int b = tid; b < kBins; b += NT) hist[b] = 0;
   if (tid == 0) first_out = kBins;
-  Part range = TakeRange::none();
+  Part range = Part::none();
   for (int v = v0 + tid; v < v1; v += 4 * NT) {
     uint4 r[4];
 #pragma unroll
@@ -210,22 +243,18 @@ __global__ void __launch_bounds__(NT) sample_kernel(SampleArgs p, int ctas) {
 #pragma unroll
     for (int u = 0; u < 4; ++u)
       if (v + u * NT < v1) {
-        clean(r[u]);
+        X::clean(r[u]);
         if (p.resident) keep[v + u * NT - v0] = r[u];
+        range.most = fmaxf(range.most, largest<T>(r[u]));
 #pragma unroll
         for (int j = 0; j < N; ++j) {
           const float x = X::get(r[u], j);
-          if (x > range.v) {
-            range.v = x;
-            range.i = (v + u * NT) * N - skew + j;
-          }
-          if (x > -INFINITY) range.l = fminf(range.l, x);
+          range.least = fminf(range.least, x == -INFINITY ? INFINITY : x);
         }
       }
   }
-  range = combine<NT>(range, TakeRange(), warps, mine, turn ^= 1, ctas);
-  const float top = range.v;
-  const int top_i = range.i;
+  range = combine<RANGE, NT>(range, parts, turn ^= 1, rank, ctas);
+  const float top = range.most;
   if (top == -INFINITY) {  // nothing can be drawn
     if (rank == 0 && tid == 0) {
       p.tokens[row] = -1;
@@ -234,118 +263,208 @@ __global__ void __launch_bounds__(NT) sample_kernel(SampleArgs p, int ctas) {
     cluster_sync();  // the other CTAs may still be reading this one's part
     return;
   }
-  const float bins = fmaxf(kBinsPerLog2, (kBins - 1) / fmaxf((top - range.l) * c, 1e-20f));
+  const float bins = fmaxf(kBinsPerLog2, (kBins - 1) / fmaxf((top - range.least) * c, 1e-20f));
 
-  // the race over tokens ranked before (bound_l, bound_i), in bins before `out`
-  float out = INFINITY, bound_l = -INFINITY;
-  int bound_i = INT_MAX;
-  auto race_line = [&](const uint4& r, int i0, Part& best) {
+  // The race over line r: tokens with y = (top - x) c bins below `limit` (bins left in, min_p) and, in
+  // later rounds, ranked before (bound_l, bound_i).
+  float limit = min_p > 0.f ? -__log2f(min_p) * bins * (1.f + 1e-6f) + 1e-30f : INFINITY;
+  float bound_l = 0.f;
+  int bound_i = 0;
+  bool bounded = false;
+  float best_s, best_l;
+  int best_i;
+  auto race_lines = [&](int v) {  // lines v, v + NT, ... of this thread, their noise on the way together
+    uint4 r[U];
+    float q[U][N];
+    bool in[U];
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float x = X::get(r, j), x2 = (top - x) * c;
-      if (x2 * bins < out && x2 <= most_x && (x > bound_l || (x == bound_l && i0 + j < bound_i))) {
-        float s = -x2 - __log2f(__ldg(q + i0 + j));
-        s = s != s ? -INFINITY : s;
-        if (beats(s, i0 + j, best)) best = {s, i0 + j, x, best.w};
+    for (int u = 0; u < U; ++u) {
+      const int w = v + u * NT, i0 = w * N - skew;
+      in[u] = w < v1;
+      if (in[u]) {
+        r[u] = line(w);
+        in[u] = (top - largest<T>(r[u])) * c * bins < limit;
+      }
+      if (in[u]) {
+        if (q4 && i0 >= 0 && i0 + N <= p.V) {
+#pragma unroll
+          for (int j = 0; j < N; j += 4) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(noise + i0 + j));
+            q[u][j] = f.x;
+            q[u][j + 1] = f.y;
+            q[u][j + 2] = f.z;
+            q[u][j + 3] = f.w;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < N; ++j) q[u][j] = (unsigned)(i0 + j) < (unsigned)p.V ? __ldg(noise + i0 + j) : 1.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!in[u]) continue;
+      const int i0 = (v + u * NT) * N - skew;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float x = X::get(r[u], j), x2 = (top - x) * c, s = -x2 - __log2f(q[u][j]);
+        bool win = (x2 * bins < limit) & (s > best_s);  // a thread's indices ascend: ties stay with the lowest
+        if (bounded) win = win & ((x > bound_l) | ((x == bound_l) & (i0 + j < bound_i)));
+        best_s = win ? s : best_s;
+        best_i = win ? i0 + j : best_i;
+        best_l = win ? x : best_l;
       }
     }
   };
-  // pass 2: the mass beside the first token's, and the histogram where a rule needs one, else the race
+
+  // pass 2: the mass beside one first token's, the first token's index, and the histogram where a rule
+  // needs it, else the race itself
   const bool binned = by_rank || by_mass;
-  Part best = TakeBest::none();
+  Part best = Part::none();
+  best_s = -INFINITY;
   for (int v = v0 + tid; v < v1; v += NT) {
     const uint4 r = line(v);
     const int i0 = v * N - skew;
+    float e[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float x2 = (top - X::get(r, j)) * c, e = ex2(-x2);
-      best.w += i0 + j == top_i ? 0.f : e;
-      if (binned && x2 < INFINITY) atomicAdd(&hist[(int)fminf(x2 * bins, kBins - 1)], 1);
+    for (int j = 0; j < N; ++j) e[j] = ex2((X::get(r, j) - top) * c);
+    if (binned) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {  // floor(y) from the sum with 2^23, rounded towards zero
+        const float y = (top - X::get(r, j)) * c * bins;
+        const int at = __float_as_int(__fadd_rz(y, 8388608.f)) - 0x4b000000;
+        atomicAdd(&hist[y < (float)(kBins - 1) ? at : kBins + (tid & 31)], 1);
+      }
     }
-    if (!binned && !greedy) race_line(r, i0, best);
+    if (largest<T>(r) == top) {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (X::get(r, j) == top) {
+          e[j] = 0.f;
+          ++best.count;
+          best.first = min(best.first, i0 + j);
+        }
+    }
+#pragma unroll
+    for (int j = 1; j < N; ++j) e[0] += e[j];
+    best.mass += e[0];
   }
-  best = combine<NT>(best, TakeBest(), warps, mine, turn ^= 1, ctas);
-  const float rest = best.w, z = 1.f + rest;
+  if (!binned && !greedy)
+    for (int v = v0 + tid; v < v1; v += U * NT) race_lines(v);
+  auto leader = [&](Part& p) {
+    if (best_s > -INFINITY) {
+      p.score = order_of(best_s);
+      p.place = ~(uint32_t)best_i;
+      p.logit = best_l;
+    }
+  };
+  leader(best);
+  best = combine<RACE | MASS | FIRST | COUNT, NT>(best, parts, turn ^= 1, rank, ctas);
+  // tokens as likely as the first count 1 each; the first itself stays out so that `rest` keeps its bits
+  const int top_i = best.first;
+  const float rest = best.mass + (float)(best.count - 1), z = 1.f + rest;
 
   if (binned) {
     // counts of all CTAs, summed up to each bin; the least and the most mass they can stand for
-    int n = 0;
-    float lo = 0.f, hi = 0.f;
-    int cn = 0;
-    if (tid < kBins) {
-      for (int r = 0; r < ctas; ++r) {
-        int a;
-        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(a) : "r"(mapa_shared(&hist[tid], r)) : "memory");
-        n += a;
+    constexpr int PB = NT < kBins ? kBins / NT : 1;  // consecutive bins of a thread
+    int cn[PB], c_all = 0;
+    float lo[PB], hi[PB], lo_all = 0.f, hi_all = 0.f;
+    const int bin0 = tid * PB;
+    if (bin0 < kBins) {
+#pragma unroll
+      for (int u = 0; u < PB; ++u) {
+        int a[kMaxCtas], n = 0;
+#pragma unroll
+        for (int r = 0; r < kMaxCtas; ++r) {
+          a[r] = 0;
+          if (r < ctas) asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(a[r]) : "r"(mapa_shared(&hist[bin0 + u], r)));
+        }
+#pragma unroll
+        for (int r = 0; r < kMaxCtas; ++r) n += a[r];
+        cn[u] = c_all += n;
+        lo[u] = lo_all += n * ex2(-(bin0 + u + 1) / bins);
+        hi[u] = hi_all += n * ex2(-(bin0 + u) / bins);
       }
-      cn = n;
-      lo = tid == kBins - 1 ? 0.f : n * ex2(-(tid + 1) / bins);
-      hi = n * ex2(-tid / bins);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int a = __shfl_up_sync(0xffffffffu, cn, o);
-        const float b = __shfl_up_sync(0xffffffffu, lo, o), d = __shfl_up_sync(0xffffffffu, hi, o);
+        const int a = __shfl_up_sync(0xffffffffu, c_all, o);
+        const float b = __shfl_up_sync(0xffffffffu, lo_all, o), d = __shfl_up_sync(0xffffffffu, hi_all, o);
         if ((tid & 31) >= o) {
-          cn += a;
-          lo += b;
-          hi += d;
+          c_all += a;
+          lo_all += b;
+          hi_all += d;
         }
       }
       if ((tid & 31) == 31) {
-        wcnt[tid >> 5] = cn;
-        wsum[tid >> 5] = make_float2(lo, hi);
+        wcnt[tid >> 5] = c_all;
+        wsum[tid >> 5] = make_float2(lo_all, hi_all);
       }
+      // up to and without this thread's bins
+      c_all -= cn[PB - 1];
+      lo_all -= lo[PB - 1];
+      hi_all -= hi[PB - 1];
     }
     __syncthreads();
-    if (tid < kBins) {
+    if (bin0 < kBins) {
       for (int w = 0; w < (tid >> 5); ++w) {
-        cn += wcnt[w];
-        lo += wsum[w].x;
-        hi += wsum[w].y;
+        c_all += wcnt[w];
+        lo_all += wsum[w].x;
+        hi_all += wsum[w].y;
       }
-      count_to[tid] = cn;
-      most_to[tid] = hi;
-      // everything in the bins after this one is out if the bins up to it already fill a rule
-      if ((by_rank && cn >= k) || (by_mass && lo >= top_p * z * (1.f + kSlack))) atomicMin(&first_out, tid + 1);
+#pragma unroll
+      for (int u = 0; u < PB; ++u) {
+        count_to[bin0 + u] = c_all + cn[u];
+        most_to[bin0 + u] = hi_all + hi[u];
+        // everything in the bins after this one is out if the bins up to it already fill a rule
+        if ((by_rank && c_all + cn[u] >= k) || (by_mass && lo_all + lo[u] >= top_p * z * (1.f + kSlack)))
+          atomicMin(&first_out, bin0 + u + 1);
+      }
     }
     __syncthreads();
-    out = first_out < kBins ? (float)first_out : INFINITY;
+    if (first_out < kBins - 1) limit = fminf(limit, (float)first_out);
   }
 
   float won_l = top;
   int won_i = top_i;
   for (bool again = binned; !greedy;) {
     if (again) {
-      best = TakeBest::none();
-      for (int v = v0 + tid; v < v1; v += NT) race_line(line(v), v * N - skew, best);
-      best = combine<NT>(best, TakeBest(), warps, mine, turn ^= 1, ctas);
+      best = Part::none();
+      best_s = -INFINITY;
+      for (int v = v0 + tid; v < v1; v += U * NT) race_lines(v);
+      leader(best);
+      best = combine<RACE, NT>(best, parts, turn ^= 1, rank, ctas);
     }
-    if (best.i == INT_MAX || best.i == top_i) break;
-    won_l = best.l;
-    won_i = best.i;
-    if (!binned) break;
-    const float x2 = (top - won_l) * c;
-    const int bin = (int)fminf(x2 * bins, kBins - 1);
-    if ((!by_rank || count_to[bin] <= k) && (!by_mass || most_to[bin] * (1.f + kSlack) < top_p * z)) break;
-    Part before = TakeSum::none();
-    for (int v = v0 + tid; v < v1; v += NT) {
-      const uint4 r = line(v);
+    if (best.score == 0u || best.index() == top_i) break;
+    if (binned) {
+      // surely kept by the histogram's bounds, or ranked exactly
+      const float y = (top - best.logit) * c * bins;
+      const int bin = y < (float)(kBins - 1) ? (int)y : kBins - 1;
+      if (bin == kBins - 1 || (by_rank && count_to[bin] > k) || (by_mass && most_to[bin] * (1.f + kSlack) >= top_p * z)) {
+        Part before = Part::none();
+        for (int v = v0 + tid; v < v1; v += NT) {
+          const uint4 r = line(v);
+          if (largest<T>(r) < best.logit) continue;
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float x = X::get(r, j);
-        if (x > won_l || (x == won_l && v * N - skew + j < won_i)) {
-          before.i += 1;
-          before.w += ex2(-(top - x) * c);
+          for (int j = 0; j < N; ++j) {
+            const float x = X::get(r, j);
+            if ((x > best.logit) | ((x == best.logit) & (v * N - skew + j < best.index()))) {
+              before.count += 1;
+              before.mass += ex2(-(top - x) * c);
+            }
+          }
+        }
+        before = combine<MASS | COUNT, NT>(before, parts, turn ^= 1, rank, ctas);
+        if ((by_rank && before.count >= k) || (by_mass && !(before.mass < top_p * z))) {
+          bound_l = best.logit;
+          bound_i = best.index();
+          bounded = again = true;
+          continue;
         }
       }
     }
-    before = combine<NT>(before, TakeSum(), warps, mine, turn ^= 1, ctas);
-    if ((!by_rank || before.i < k) && (!by_mass || before.w < top_p * z)) break;
-    bound_l = won_l;
-    bound_i = won_i;
-    won_l = top;
-    won_i = top_i;
-    again = true;
+    won_l = best.logit;
+    won_i = best.index();
+    break;
   }
   if (rank == 0 && tid == 0) {
     p.tokens[row] = won_i;
@@ -397,6 +516,9 @@ int ahb_sample(const void* logits, int64_t ls, int dtype, const float* noise, in
   size_t smem = (size_t)p.chunk * 16;
   p.resident = smem <= (size_t)kMaxSlice;
   if (!p.resident) smem = 0;
-  if (dtype == AHB_BF16) return launch<__nv_bfloat16, 512>(p, B, ctas, smem, st);
-  return launch<float, 512>(p, B, ctas, smem, st);
+  // Few CTAs: more warps to hide each other's latency.  Many: the longer part per warp pays for the
+  // meetings of the cluster (256 x 128256 fp32: 127 us against 220 us).
+  if (B * ctas <= 2 * 148)
+    return dtype == AHB_BF16 ? launch<__nv_bfloat16, 512>(p, B, ctas, smem, st) : launch<float, 512>(p, B, ctas, smem, st);
+  return dtype == AHB_BF16 ? launch<__nv_bfloat16, 256>(p, B, ctas, smem, st) : launch<float, 256>(p, B, ctas, smem, st);
 }

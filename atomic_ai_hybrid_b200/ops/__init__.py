@@ -206,7 +206,7 @@ def sample(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     (0 or less: no limit), with less than ``top_p`` of the mass ranked before them (the first one
     always), and with at least ``min_p`` times the first one's probability.  The token is the kept
     one with the largest ``log p - log noise`` (ties: lowest index), which draws from the kept ones by
-    their probability.  ``temperature <= 0`` takes the first token and tempers by 1 for ``logprobs``,
+    their probability (a row without any such score gives the first).  ``temperature <= 0`` takes the first token and tempers by 1 for ``logprobs``,
     the log-probability before anything is cut.  NaN and ``-inf`` logits are never drawn; a row
     of nothing else gives token -1 and ``-inf``."""
     if use_cuda(logits):

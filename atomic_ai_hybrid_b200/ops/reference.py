@@ -420,7 +420,7 @@ def sample(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     score = torch.where(kept, torch.nan_to_num(score, nan=-math.inf, posinf=math.inf, neginf=-math.inf), -math.inf)
     best = score.max(1, keepdim=True).values
     tokens = torch.where(kept & (score == best), index, V).min(1, keepdim=True).values
-    tokens = torch.where(empty, -1, tokens)
+    tokens = torch.where(empty, -1, torch.where(best > -math.inf, tokens, index[:, :1]))
     logp = (l.gather(1, tokens.clamp(min=0)) - top) / T - torch.log(total)
     return tokens[:, 0], torch.where(empty, -math.inf, logp)[:, 0].to(torch.float64 if acc == torch.float64 else torch.float32)
 
