@@ -1700,7 +1700,7 @@ torch::Tensor selective_scan(const torch::Tensor& x, const torch::Tensor& dt, co
               op, ": state must be a contiguous fp32 (slots, heads, head dim, states) tensor on ", x.device());
   const int64_t T = x.size(0), C = x.size(1), S = state.size(0), H = state.size(1), P = state.size(2), N = state.size(3);
   TORCH_CHECK(H * P == C && C > 0, op, ": ", H, " heads of ", P, " channels do not make ", C);
-  TORCH_CHECK(T < (1ll << 31) && C < (1ll << 24), op, ": sizes out of range");
+  TORCH_CHECK(T < (1ll << 30) && C < (1ll << 22), op, ": sizes out of range");
   check_rows(x, x, T, C, op, "x");
   check_rows(dt, x, T, C, op, "dt");
   check_rows(Bm, x, T, N, op, "B");
@@ -1712,12 +1712,17 @@ torch::Tensor selective_scan(const torch::Tensor& x, const torch::Tensor& dt, co
   const SeqArgs q = seq_args(x, T, L, S, cu, slots, op);
   const c10::cuda::CUDAGuard guard(x.device());
   auto y = torch::empty({T, C}, x.options());
+  int64_t floats = 0;
+  const int seg = ahb_selective_scan_plan(q.B, q.L, (int)T, (int)C, (int)N, q.cu != nullptr, dt_code(x), &floats);
+  torch::Tensor work;
+  if (floats > 0) work = torch::empty({floats}, state.options());
   const int rc = ahb_selective_scan(x.data_ptr(), x.stride(0), dt.data_ptr(), dt.stride(0), A.data_ptr<float>(),
                                     Bm.data_ptr(), Bm.stride(0), Cm.data_ptr(), Cm.stride(0), conv_w.data_ptr(),
                                     dt_code(conv_w), opt_ptr(conv_b), conv_state.data_ptr(), state.data_ptr<float>(),
                                     q.cu, q.slots, y.data_ptr(), q.B, q.L, (int)T, (int)C, (int)P, (int)N, (int)S,
-                                    dt_code(x), (float)dt_min, (float)dt_max, cur_stream());
-  TORCH_CHECK(rc == 0, op, ": no kernel for ", N, " states");
+                                    dt_code(x), (float)dt_min, (float)dt_max, seg,
+                                    floats > 0 ? work.data_ptr<float>() : nullptr, cur_stream());
+  TORCH_CHECK(rc == 0, op, ": failed with code ", rc, " for ", N, " states");
   check_launch(op);
   return y;
 }

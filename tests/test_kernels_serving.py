@@ -71,7 +71,7 @@ def test_scan_tokens(C, P, N, dtype):
 
 
 @pytest.mark.parametrize("lens", [[1], [2], [3], [15], [16], [17], [33], [0, 5, 0, 1, 70], [129, 64, 1, 255], [300], [1100, 3, 513]])
-@pytest.mark.parametrize("C,P,N,dtype", [(256, 64, 128, BF), (192, 192, 64, BF), (72, 8, 32, BF), (64, 64, 128, F32)])
+@pytest.mark.parametrize("C,P,N,dtype", [(256, 64, 128, BF), (192, 192, 64, BF), (72, 8, 32, BF), (21, 7, 128, BF), (64, 64, 128, F32)])
 def test_scan_prompts(lens, C, P, N, dtype):
     a = _scan_inputs(lens, C, P, N, dtype, seed=sum(lens) + C)
     _check_scan(a, _cu(lens))
@@ -81,6 +81,24 @@ def test_scan_long_prompt():
     """Many segments: the state is handed from one to the next."""
     lens = [5000, 1, 2500]
     _check_scan(_scan_inputs(lens, 512, 64, 128, BF, seed=3), _cu(lens))
+
+
+@pytest.mark.parametrize("N", [32, 64, 128])
+def test_scan_strong_decays(N):
+    """Steps and rates from no decay to the -20 clamp at every token, side by side."""
+    lens = [45, 700, 64]
+    a = _scan_inputs(lens, 256, 8, N, BF, seed=12)
+    a["A"] = -torch.logspace(-3, 2, 32, device=dev)[torch.randperm(32, generator=_gen(1), device=dev)].contiguous()
+    a["dt"] = (torch.randn(sum(lens), 256, generator=_gen(2), device=dev) * 4).to(BF)
+    # A = -1e-3 forgets with 1 - e^{-1e-5}: no room for REL there, but 700 tokens take 700 * 6 * 2^-24 at most
+    ref = {k: _d(v) for k, v in a.items()}
+    ref["conv_state"], ref["state"] = ref["conv_state"].clone(), ref["state"].clone()
+    y64 = R.selective_scan(**ref, cu_seqlens=_cu(lens))
+    y = ops.selective_scan(**a, cu_seqlens=_cu(lens))
+    top = ref["state"].abs().max()
+    rel = 700 * 6 * 2.0 ** -24
+    assert ((a["state"].double() - ref["state"]).abs() <= rel * top).all()
+    assert ((y.double() - y64).abs() <= 2.0 ** -8 * y64.abs() + rel * top * ref["Cm"].abs().sum(-1, keepdim=True)).all()
 
 
 def test_scan_padded_and_strided_inputs():
