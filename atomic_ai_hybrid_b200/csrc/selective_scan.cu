@@ -147,7 +147,6 @@ struct PromptArgs {
   float* decays;  // (segments, C): log2 of a segment's decay
 };
 
-constexpr int kBlock = 32, kWarps = 4, kChan = 16 * kWarps;
 constexpr float kSpan = 86.f, kLog2e = 1.4426950408889634f;
 
 struct Segment { int b, first, count, index; SeqRange seq; };  // sequence, its first segment's number, its segments, which one
@@ -201,17 +200,46 @@ AHB_DEVICE float ex2(float x) {
   return y;
 }
 
+AHB_DEVICE float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two floats in one instruction (the two channels of a lane, or two columns of an accumulator row)
+AHB_DEVICE float2 both(float x) { return make_float2(x, x); }
+AHB_DEVICE float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+AHB_DEVICE float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+AHB_DEVICE float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+AHB_DEVICE float2 max2(float2 a, float b) { return make_float2(fmaxf(a.x, b), fmaxf(a.y, b)); }
+
 // log(1 + e^x) to about 2^-22: max(x, 0) + log1p(z) with z = e^{-|x|}, log1p(z) = 2 atanh(z / (2 + z)) as
-// its power series (the argument is at most 1/3; the first term left out is below 5e-9 of the sum)
-AHB_DEVICE float softplus_series(float x) {
-  const float z = ex2(-fabsf(x) * kLog2e), s = __fdividef(z, 2.f + z), w = s * s;
-  float p = fmaf(w, 2.f / 13.f, 2.f / 11.f);
-  p = fmaf(w, p, 2.f / 9.f);
-  p = fmaf(w, p, 2.f / 7.f);
-  p = fmaf(w, p, 2.f / 5.f);
-  p = fmaf(w, p, 2.f / 3.f);
-  p = fmaf(w, p, 2.f);
-  return fmaf(s, p, fmaxf(x, 0.f));
+// its power series (the argument is at most 1/3; the first term left out is below 2e-7 of the sum)
+AHB_DEVICE float2 softplus2(float2 x) {
+  const float2 z = make_float2(ex2(-fabsf(x.x) * kLog2e), ex2(-fabsf(x.y) * kLog2e)), d = add2(z, both(2.f));
+  const float2 s = mul2(z, make_float2(rcp(d.x), rcp(d.y))), w = mul2(s, s);
+  float2 p = fma2(w, both(2.f / 11.f), both(2.f / 9.f));
+  p = fma2(w, p, both(2.f / 7.f));
+  p = fma2(w, p, both(2.f / 5.f));
+  p = fma2(w, p, both(2.f / 3.f));
+  p = fma2(w, p, both(2.f));
+  return fma2(s, p, max2(x, 0.f));
 }
 
 AHB_DEVICE void ldsm4(uint32_t r[4], const void* p) {
@@ -231,11 +259,12 @@ AHB_DEVICE uint32_t clip2(uint32_t x) {
 AHB_DEVICE float lo16(uint32_t x) { return __uint_as_float(x << 16); }
 AHB_DEVICE float hi16(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
+AHB_DEVICE float2 both16(uint32_t x) { return make_float2(lo16(x), hi16(x)); }
+
 // the next bf16 term of two floats, which keep what it leaves
-AHB_DEVICE uint32_t term2(float& x, float& y) {
-  const uint32_t h = pack2(x, y);
-  x -= lo16(h);
-  y -= hi16(h);
+AHB_DEVICE uint32_t term2(float2& v) {
+  const uint32_t h = pack2(v.x, v.y);
+  v = add2(v, make_float2(-lo16(h), -hi16(h)));
   return h;
 }
 
@@ -259,44 +288,52 @@ AHB_DEVICE void store_pair(bf16* row, int c, int C, bool pairs, uint32_t v) {
   }
 }
 
+// Two warps share 16 channels: each makes V for its 16 of the block's 32 tokens and keeps half of the
+// states (32 accumulator registers a thread at N = 128, so that 16 warps fit an SM and hide each other's
+// latencies: 12 warps with whole states were issuing 42 % of the time).
+constexpr int kBlock = 32, kGroups = 4, kWarps = 2 * kGroups, kChan = 16 * kGroups;
+
 template <int N>
 struct BlockSmem {
   static constexpr int LD = N + 8;    // row strides that spread ldmatrix rows over the banks
-  static constexpr int LT = kBlock + 4;
+  static constexpr int LT = kBlock + 4, LV = kBlock + 8;
   bf16 b[2][kBlock][LD];
   bf16 c[2][kBlock][LD];
-  bf16 cb[2][kBlock][kBlock + 8];     // C B^T below the diagonal: high and low terms
-  float v[kWarps][16][LT];            // a warp's V (or u) per channel and token, then its outputs
-  float d[kWarps][16][LT];            // decays for a warp that goes token by token
+  bf16 cb[2][kBlock][LV];             // C B^T below the diagonal: high and low terms
+  bf16 v[kGroups][3][16][LV];         // the terms of V per channel and token
+  float y[kGroups][2][16][LT];        // both warps' parts of the outputs
+  float u[kGroups][16][LT];           // a group's inputs and decays where it goes token by token
+  float d[kGroups][16][LT];
+  float span[kGroups][2][16];         // log2 decay of each half block
 };
 
-// Multiplies the accumulator rows (channels) by factors that lane l holds for channels 2 (l % 8) + {0, 1}.
+// Multiplies the accumulator rows (channels) by factors that lane l holds for channel l % 16.
 template <int NT>
-AHB_DEVICE void scale_rows(float (*S)[4], float f0, float f1) {
+AHB_DEVICE void scale_rows(float (*S)[4], float f) {
   const int g = (threadIdx.x & 31) >> 2;
-  const float a0 = __shfl_sync(0xffffffffu, f0, g >> 1), a1 = __shfl_sync(0xffffffffu, f1, g >> 1);
-  const float b0 = __shfl_sync(0xffffffffu, f0, 4 + (g >> 1)), b1 = __shfl_sync(0xffffffffu, f1, 4 + (g >> 1));
-  const float r0 = g & 1 ? a1 : a0, r1 = g & 1 ? b1 : b0;
+  const float2 r0 = both(__shfl_sync(0xffffffffu, f, g)), r1 = both(__shfl_sync(0xffffffffu, f, g + 8));
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
-    S[j][0] *= r0;
-    S[j][1] *= r0;
-    S[j][2] *= r1;
-    S[j][3] *= r1;
+    const float2 u = mul2(make_float2(S[j][0], S[j][1]), r0), v = mul2(make_float2(S[j][2], S[j][3]), r1);
+    S[j][0] = u.x;
+    S[j][1] = u.y;
+    S[j][2] = v.x;
+    S[j][3] = v.y;
   }
 }
 
 template <typename W, int N, bool STATE>
-__global__ void __launch_bounds__(kWarps * 32, 3) scan_block_kernel(PromptArgs pa) {
-  constexpr int NT = N / 8;
+__global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs pa) {
+  constexpr int M = N / 2, NT = M / 8;      // this warp's states, their accumulator tiles
   using Smem = BlockSmem<N>;
   extern __shared__ __align__(16) unsigned char raw[];
   Smem& sm = *reinterpret_cast<Smem*>(raw);
   const ScanArgs& p = pa.a;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = warp >> 1, half = warp & 1;
   const int g = lane >> 2, q = lane & 3;    // accumulator rows g, g + 8; columns 2 q, 2 q + 1
-  const int i = lane & 7, tg = lane >> 3;   // channels 2 i, 2 i + 1 of tokens [8 tg, 8 tg + 8)
-  const int c0 = blockIdx.y * kChan + warp * 16, ca = c0 + 2 * i;
+  const int i = lane & 7, tg = lane >> 3;   // channels 2 i, 2 i + 1 of tokens tk .. tk + 3
+  const int tk = half * 16 + tg * 4;
+  const int c0 = blockIdx.y * kChan + grp * 16, ca = c0 + 2 * i;
   const Segment sg = find_segment(p, pa.seg, blockIdx.x);
   if (sg.b < 0) return;
   if (STATE && sg.index == sg.count - 1) return;  // its end state comes with its outputs
@@ -310,33 +347,28 @@ __global__ void __launch_bounds__(kWarps * 32, 3) scan_block_kernel(PromptArgs p
                      ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(dt) | reinterpret_cast<uintptr_t>(p.conv_state)) & 3) == 0;
   if (slot < 0) {
     if (!STATE)
-      for (int t = start + tg; t < end; t += 4) store_pair(y + (int64_t)t * p.C, ca, p.C, ypairs, 0u);
+      for (int t = start + half * 4 + tg; t < end; t += 8) store_pair(y + (int64_t)t * p.C, ca, p.C, ypairs, 0u);
     return;
   }
 
-  float w[2][4], bias[2], A2[2];
+  float2 w[4], bias, A2;
+  {
+    const bool h0 = ca < p.C, h1 = ca + 1 < p.C;
+    const W* taps = static_cast<const W*>(p.conv_w) + (int64_t)ca * 4;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const bool has = ca + e < p.C;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) w[e][j] = has ? to_f(static_cast<const W*>(p.conv_w)[(int64_t)(ca + e) * 4 + j]) : 0.f;
-    bias[e] = has && p.conv_b ? p.conv_b[ca + e] : 0.f;
-    A2[e] = has ? p.A[(ca + e) / p.P] * kLog2e : 0.f;
+    for (int j = 0; j < 4; ++j) w[j] = make_float2(h0 ? to_f(taps[j]) : 0.f, h1 ? to_f(taps[4 + j]) : 0.f);
+    bias = make_float2(h0 && p.conv_b ? p.conv_b[ca] : 0.f, h1 && p.conv_b ? p.conv_b[ca + 1] : 0.f);
+    A2 = make_float2(h0 ? p.A[ca / p.P] * kLog2e : 0.f, h1 ? p.A[(ca + 1) / p.P] * kLog2e : 0.f);
   }
-  // the three rows of x before the segment
   bf16* const win = static_cast<bf16*>(p.conv_state) + (int64_t)slot * 3 * p.C;
-  uint32_t before[3], carry[3];
-#pragma unroll
-  for (int j = 0; j < 3; ++j)
-    before[j] = carry[j] = sg.index == 0 ? load_pair(win + j * p.C, ca, p.C, pairs)
-                                         : load_pair(x + (int64_t)(start - 3 + j) * p.xs, ca, p.C, pairs);
 
   float S[NT][4];
   float* const slot_state = p.state + (int64_t)slot * p.C * N;
   float* const seg_state = pa.states + (int64_t)(sg.first + sg.index) * p.C * N;
   const bool has0 = c0 + g < p.C, has1 = c0 + g + 8 < p.C;
+  const int64_t at_state = (int64_t)(c0 + g) * N + half * M + 2 * q;
   {
-    const float* src = (sg.count == 1 ? slot_state : seg_state) + (int64_t)(c0 + g) * N + 2 * q;
+    const float* src = (sg.count == 1 ? slot_state : seg_state) + at_state;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       float2 u = make_float2(0.f, 0.f), v = u;
@@ -350,12 +382,13 @@ __global__ void __launch_bounds__(kWarps * 32, 3) scan_block_kernel(PromptArgs p
   }
 
   // block rows of B and C: every thread copies, and later clips, the same 16-byte pieces
-  constexpr int PIECES = kBlock * N / 8 / (kWarps * 32);
+  constexpr int ALL = kBlock * N / 8, PIECES = (ALL + kWarps * 32 - 1) / (kWarps * 32);
   const bool wide = (((p.bs | p.cs) & 7) == 0) && ((reinterpret_cast<uintptr_t>(p.Bm) | reinterpret_cast<uintptr_t>(p.Cm)) & 15) == 0;
   auto copy_rows = [&](const void* from, int64_t stride, bf16 (*to)[Smem::LD], int t0) {
 #pragma unroll
     for (int m = 0; m < PIECES; ++m) {
       const int piece = tid + m * kWarps * 32, row = piece / (N / 8), col = piece % (N / 8) * 8;
+      if (ALL % (kWarps * 32) != 0 && piece >= ALL) break;
       const bf16* src = static_cast<const bf16*>(from) + (int64_t)(t0 + row) * stride + col;
       if (t0 + row >= end) {
         *reinterpret_cast<uint4*>(&to[row][col]) = make_uint4(0, 0, 0, 0);
@@ -371,6 +404,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) scan_block_kernel(PromptArgs p
 #pragma unroll
     for (int m = 0; m < PIECES; ++m) {
       const int piece = tid + m * kWarps * 32;
+      if (ALL % (kWarps * 32) != 0 && piece >= ALL) break;
       uint4* at = reinterpret_cast<uint4*>(&rows[piece / (N / 8)][piece % (N / 8) * 8]);
       const uint4 r = *at;
       *at = make_uint4(clip2(r.x), clip2(r.y), clip2(r.z), clip2(r.w));
@@ -381,217 +415,228 @@ __global__ void __launch_bounds__(kWarps * 32, 3) scan_block_kernel(PromptArgs p
     if (!STATE) copy_rows(p.Cm, p.cs, sm.c[buf], t0);
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  uint32_t xr[8], dr[8];
+  // this lane's tokens; lanes of the warp's first tokens also hold the three rows before them
+  uint32_t xr[4], dr[4], hr[3];
   auto load_tokens = [&](int t0) {
+    const bf16* xp = x + (int64_t)(t0 + tk) * p.xs;
+    const bf16* dp = dt + (int64_t)(t0 + tk) * p.dts;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int t = t0 + tg * 8 + k;
-      xr[k] = t < end ? load_pair(x + (int64_t)t * p.xs, ca, p.C, pairs) : 0u;
-      dr[k] = t < end ? load_pair(dt + (int64_t)t * p.dts, ca, p.C, pairs) : 0u;
+    for (int k = 0; k < 4; ++k) {
+      const bool in = t0 + tk + k < end;
+      xr[k] = in ? load_pair(xp + k * p.xs, ca, p.C, pairs) : 0u;
+      dr[k] = in ? load_pair(dp + k * p.dts, ca, p.C, pairs) : 0u;
+    }
+    if (tg == 0) {
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        const int t = t0 + tk + j - 3, back = t - sg.seq.start;
+        hr[j] = back < 0 ? load_pair(win + (back + 3) * p.C, ca, p.C, pairs)
+                         : t < end ? load_pair(x + (int64_t)t * p.xs, ca, p.C, pairs) : 0u;
+      }
     }
   };
 
   copy_block(start, 0);
   load_tokens(start);
-  float pend[2] = {0.f, 0.f}, total[2] = {0.f, 0.f};  // log2 of the scale S still lacks, of the segment's decay
-  float (*const vt)[Smem::LT] = sm.v[warp];
-  float (*const dl)[Smem::LT] = sm.d[warp];
+  float pend = 0.f, total = 0.f;  // of channel lane % 16: log2 of the scale S still lacks, of the segment's decay
   int buf = 0;
   for (int t0 = start; t0 < end; t0 += kBlock, buf ^= 1) {
     const int n = min(kBlock, end - t0);
     // convolution, step and input of this lane's channels and tokens
-    float E[8][2], u[8][2];
+    float2 E[4], u[4];
     {
-      uint32_t xs[11];
+      uint32_t xs[7];
 #pragma unroll
       for (int j = 0; j < 3; ++j) {
-        const uint32_t last = __shfl_sync(0xffffffffu, xr[5 + j], (lane + 24) & 31);
-        xs[j] = tg == 0 ? carry[j] : last;
-        carry[j] = last;
+        const uint32_t last = __shfl_up_sync(0xffffffffu, xr[1 + j], 8);
+        xs[j] = tg == 0 ? hr[j] : last;
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) xs[3 + k] = xr[k];
+      for (int k = 0; k < 4; ++k) xs[3 + k] = xr[k];
+      float2 odd = both(0.f);  // NaN as soon as an input is not finite
+      float most = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const bool in = tg * 8 + k < n;
+      for (int k = 0; k < 4; ++k) {
+        float2 a = bias;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float a = bias[e];
+        for (int j = 0; j < 4; ++j) a = fma2(w[j], both16(xs[k + j]), a);
+        const float2 t = mul2(a, both(-kLog2e)), d = add2(make_float2(ex2(t.x), ex2(t.y)), both(1.f));
+        u[k] = mul2(a, make_float2(rcp(d.x), rcp(d.y)));
+        most = fmaxf(most, fmaxf(fabsf(u[k].x), fabsf(u[k].y)));
+        const float2 r = both16(dr[k]), sp = softplus2(r);
+        E[k] = make_float2(fminf(fmaxf(sp.x, p.dt_min), p.dt_max), fminf(fmaxf(sp.y, p.dt_min), p.dt_max));
+        odd = fma2(add2(a, r), both(0.f), odd);
+      }
+      if (__any_sync(0xffffffffu, (odd.x != odd.x) | (odd.y != odd.y) | (most > kClip))) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) a = fmaf(w[e][j], e ? hi16(xs[k + j]) : lo16(xs[k + j]), a);
-          const float xc = sanitize(__fdividef(a, 1.f + ex2(-a * kLog2e)), kClip);
-          const float r = e ? hi16(dr[k]) : lo16(dr[k]);
-          float step = fminf(fmaxf(softplus_series(r), p.dt_min), p.dt_max);
-          step = in && r == r ? step : 0.f;
-          E[k][e] = fmaxf(step * A2[e], kMinDA * kLog2e);
-          u[k][e] = step * xc;
+        for (int k = 0; k < 4; ++k) {
+          const float2 r = both16(dr[k]);
+          u[k] = make_float2(sanitize(u[k].x, kClip), sanitize(u[k].y, kClip));
+          E[k] = make_float2(r.x != r.x ? 0.f : E[k].x, r.y != r.y ? 0.f : E[k].y);
         }
+      }
+      if (n < kBlock) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (tk + k >= n) E[k] = both(0.f);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        u[k] = mul2(u[k], E[k]);
+        E[k] = max2(mul2(E[k], A2), kMinDA * kLog2e);
       }
     }
     if (t0 + kBlock < end) load_tokens(t0 + kBlock);
-    // decays summed along the tokens, over the four lanes of a channel
-    float mid[2], last[2], off[2];
+    // decays summed along the warp's half block, over the four lanes of a channel
+    const float2 sum = add2(add2(E[0], E[1]), add2(E[2], E[3]));
+    float2 incl = sum, v = make_float2(__shfl_up_sync(0xffffffffu, sum.x, 8), __shfl_up_sync(0xffffffffu, sum.y, 8));
+    if (tg >= 1) incl = add2(incl, v);
+    v = make_float2(__shfl_up_sync(0xffffffffu, incl.x, 16), __shfl_up_sync(0xffffffffu, incl.y, 16));
+    if (tg >= 2) incl = add2(incl, v);
+    const float2 whole = make_float2(__shfl_sync(0xffffffffu, incl.x, 24 + i), __shfl_sync(0xffffffffu, incl.y, 24 + i));
+    if (tg == 0) *reinterpret_cast<float2*>(&sm.span[grp][half][2 * i]) = whole;
+    // E: the first half ends at the reference, the second starts from it
+    float2 run = add2(incl, make_float2(-sum.x, -sum.y));
+    if (half == 0) run = add2(run, make_float2(-whole.x, -whole.y));
+    // for a group that has to go token by token: its inputs and decays as they are
+    *reinterpret_cast<float4*>(&sm.u[grp][2 * i][tk]) = make_float4(u[0].x, u[1].x, u[2].x, u[3].x);
+    *reinterpret_cast<float4*>(&sm.u[grp][2 * i + 1][tk]) = make_float4(u[0].y, u[1].y, u[2].y, u[3].y);
+    *reinterpret_cast<float4*>(&sm.d[grp][2 * i][tk]) = make_float4(E[0].x, E[1].x, E[2].x, E[3].x);
+    *reinterpret_cast<float4*>(&sm.d[grp][2 * i + 1][tk]) = make_float4(E[0].y, E[1].y, E[2].y, E[3].y);
+    float2 V[4];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float sum = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) sum += E[k][e];
-      float incl = sum, v = __shfl_up_sync(0xffffffffu, incl, 8);
-      if (tg >= 1) incl += v;
-      v = __shfl_up_sync(0xffffffffu, incl, 16);
-      if (tg >= 2) incl += v;
-      mid[e] = __shfl_sync(0xffffffffu, incl, 8 + i);
-      last[e] = __shfl_sync(0xffffffffu, incl, 24 + i);
-      off[e] = incl - sum - mid[e];
-      total[e] += last[e];
+    for (int k = 0; k < 4; ++k) {
+      run = add2(run, E[k]);
+      V[k] = mul2(u[k], make_float2(ex2(-run.x), ex2(-run.y)));
+      E[k] = run;
     }
-    const bool heavy = __any_sync(0xffffffffu, (mid[0] < -kSpan) | (mid[1] < -kSpan) | (last[0] - mid[0] < -kSpan) | (last[1] - mid[1] < -kSpan));
-    __syncwarp();  // the previous block's outputs have left vt
+    float2 V0[2] = {{V[0].x, V[1].x}, {V[2].x, V[3].x}}, V1[2] = {{V[0].y, V[1].y}, {V[2].y, V[3].y}};
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float v[8];
-      if (heavy) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = E[k][e];
-        *reinterpret_cast<float4*>(&dl[2 * i + e][8 * tg]) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>(&dl[2 * i + e][8 * tg + 4]) = make_float4(v[4], v[5], v[6], v[7]);
-      }
-      float run = off[e];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        run += E[k][e];
-        E[k][e] = run;
-        v[k] = heavy ? u[k][e] : u[k][e] * ex2(-run);
-      }
-      *reinterpret_cast<float4*>(&vt[2 * i + e][8 * tg]) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4*>(&vt[2 * i + e][8 * tg + 4]) = make_float4(v[4], v[5], v[6], v[7]);
+    for (int m = 0; m < 3; ++m) {
+      *reinterpret_cast<uint2*>(&sm.v[grp][m][2 * i][tk]) = make_uint2(term2(V0[0]), term2(V0[1]));
+      *reinterpret_cast<uint2*>(&sm.v[grp][m][2 * i + 1][tk]) = make_uint2(term2(V1[0]), term2(V1[1]));
     }
-    // S takes the scale it lacks and goes to the block's reference.  S itself may stand at 2^kSpan, so the two
-    // scales go in one after the other where their product would leave the floats' range.
-    if (__any_sync(0xffffffffu, (pend[0] + mid[0] < -120.f) | (pend[1] + mid[1] < -120.f))) {
-      scale_rows<NT>(S, ex2(pend[0]), ex2(pend[1]));
-      pend[0] = pend[1] = 0.f;
-    }
-    scale_rows<NT>(S, ex2(pend[0] + (heavy ? 0.f : mid[0])), ex2(pend[1] + (heavy ? 0.f : mid[1])));
-#pragma unroll
-    for (int e = 0; e < 2; ++e) pend[e] = heavy ? 0.f : last[e] - mid[e];
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     clip_rows(sm.b[buf]);
     if (!STATE) clip_rows(sm.c[buf]);
-    __syncthreads();  // the block's rows are there; every warp is done with the other buffer and with cb
+    __syncthreads();  // the block's rows, V and spans are there; every warp is done with the other buffer and with cb
     if (t0 + kBlock < end) copy_block(t0 + kBlock, buf ^ 1);
+    const float mid = sm.span[grp][0][lane & 15], tail = sm.span[grp][1][lane & 15];
+    total += mid + tail;
+    const bool heavy = __any_sync(0xffffffffu, fminf(mid, tail) < -kSpan);
+    // S takes the scale it lacks and goes to the block's reference.  S itself may stand at 2^kSpan, so the two
+    // scales go in one after the other where their product would leave the floats' range.
+    if (__any_sync(0xffffffffu, pend + mid < -120.f)) {
+      scale_rows<NT>(S, ex2(pend));
+      pend = 0.f;
+    }
+    scale_rows<NT>(S, ex2(heavy ? pend : pend + mid));
+    pend = heavy ? 0.f : tail;
 
     const int mrow = lane & 15, mcol = (lane >> 4) * 8;  // ldmatrix: rows of a 16 x 16 piece, its column half
     const int xrow = (lane & 7) + (lane >> 4) * 8, xcol = ((lane >> 3) & 1) * 8;  // two 8-row halves, each with both column halves
     if (!STATE) {
-      // C B^T, 16 x 16 pieces (0,0), (16,0), (16,16) by warps 0 to 2
-      if (warp < 3) {
-        const int tb = warp == 0 ? 0 : 16, sb = warp == 2 ? 16 : 0;
-        float acc[2][4];
+      // C B^T in 16 x 8 pieces of (0,0), (16,0), (16,16) by warps 0 to 5
+      if (warp < 6) {
+        const int tb = warp < 2 ? 0 : 16, sb = (warp < 4 ? 0 : 16) + (warp & 1) * 8;
+        float acc[2][4];  // even and odd k apart: half the chain of dependent products
         zero_acc<2>(acc);
 #pragma unroll
-        for (int k = 0; k < N; k += 16) {
+        for (int k = 0; k < N; k += 32) {
           uint32_t a[4], b[4];
+          ldsm4(b, &sm.b[buf][sb + (lane & 7)][k + (lane >> 3) * 8]);
           ldsm4(a, &sm.c[buf][tb + mrow][k + mcol]);
-          ldsm4(b, &sm.b[buf][sb + xrow][k + xcol]);
           mma16816(acc[0], a, b);
+          ldsm4(a, &sm.c[buf][tb + mrow][k + 16 + mcol]);
           mma16816(acc[1], a, b + 2);
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int t = tb + g + 8 * h, s = sb + 8 * j + 2 * q;
-            float v0 = s <= t ? acc[j][2 * h] : 0.f, v1 = s + 1 <= t ? acc[j][2 * h + 1] : 0.f;
-            *reinterpret_cast<uint32_t*>(&sm.cb[0][t][s]) = term2(v0, v1);
-            *reinterpret_cast<uint32_t*>(&sm.cb[1][t][s]) = pack2(v0, v1);
-          }
+        for (int h = 0; h < 2; ++h) {
+          const int t = tb + g + 8 * h, s = sb + 2 * q;
+          float2 v = make_float2(s <= t ? acc[0][2 * h] + acc[1][2 * h] : 0.f, s + 1 <= t ? acc[0][2 * h + 1] + acc[1][2 * h + 1] : 0.f);
+          *reinterpret_cast<uint32_t*>(&sm.cb[0][t][s]) = term2(v);
+          *reinterpret_cast<uint32_t*>(&sm.cb[1][t][s]) = pack2(v.x, v.y);
+        }
       }
       __syncthreads();
-    } else {
-      __syncwarp();
     }
 
+    // A product waits for the one before it on the same accumulators, so consecutive ones go to different ones.
+    float Y[4][4];
+    if (!STATE) zero_acc<4>(Y);
     if (!heavy) {
-      // V as left operands: rows are channels, columns tokens
-      uint32_t vf[2][3][4];
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float2 v = *reinterpret_cast<const float2*>(&vt[g + (r & 1) * 8][ks * 16 + (r >> 1) * 8 + 2 * q]);
-          vf[ks][0][r] = term2(v.x, v.y);
-          vf[ks][1][r] = term2(v.x, v.y);
-          vf[ks][2][r] = pack2(v.x, v.y);
-        }
       if (!STATE) {
-        float Y[4][4];
-        zero_acc<4>(Y);
 #pragma unroll
-        for (int k = 0; k < N / 16; ++k) {  // S C^T
-          uint32_t sh[4], sl[4], b[4];
-          float s8[8] = {S[2 * k][0], S[2 * k][1], S[2 * k][2], S[2 * k][3], S[2 * k + 1][0], S[2 * k + 1][1], S[2 * k + 1][2], S[2 * k + 1][3]};
+        for (int k = 0; k < M / 16; ++k) {  // Y += S C^T over this warp's states
+          uint32_t sh[4], sl[4], cf[2][4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            sh[r] = term2(s8[2 * r], s8[2 * r + 1]);
-            sl[r] = pack2(s8[2 * r], s8[2 * r + 1]);
+            float2 v = make_float2(S[2 * k + (r >> 1)][(r & 1) * 2], S[2 * k + (r >> 1)][(r & 1) * 2 + 1]);
+            sh[r] = term2(v);
+            sl[r] = pack2(v.x, v.y);
           }
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            ldsm4(b, &sm.c[buf][16 * h + xrow][16 * k + xcol]);
-            mma16816(Y[2 * h], sh, b);
-            mma16816(Y[2 * h + 1], sh, b + 2);
-            mma16816(Y[2 * h], sl, b);
-            mma16816(Y[2 * h + 1], sl, b + 2);
-          }
-        }
+          for (int h = 0; h < 2; ++h) ldsm4(cf[h], &sm.c[buf][16 * h + xrow][half * M + 16 * k + xcol]);
 #pragma unroll
-        for (int pc = 0; pc < 3; ++pc) {  // V (C B^T)^T, the same three pieces
-          const int h = pc == 0 ? 0 : 1, ks = pc == 2 ? 1 : 0;
-          uint32_t bh[4], bl[4];
-          ldsm4(bh, &sm.cb[0][16 * h + xrow][16 * ks + xcol]);
-          ldsm4(bl, &sm.cb[1][16 * h + xrow][16 * ks + xcol]);
+          for (int j = 0; j < 4; ++j) mma16816(Y[j], sh, cf[j >> 1] + 2 * (j & 1));
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            mma16816(Y[2 * h + j], vf[ks][0], bh + 2 * j);
-            mma16816(Y[2 * h + j], vf[ks][0], bl + 2 * j);
-            mma16816(Y[2 * h + j], vf[ks][1], bh + 2 * j);
-          }
-        }
-        __syncwarp();  // V has been read by every lane
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          *reinterpret_cast<float2*>(&vt[g][8 * j + 2 * q]) = make_float2(Y[j][0], Y[j][1]);
-          *reinterpret_cast<float2*>(&vt[g + 8][8 * j + 2 * q]) = make_float2(Y[j][2], Y[j][3]);
+          for (int j = 0; j < 4; ++j) mma16816(Y[j], sl, cf[j >> 1] + 2 * (j & 1));
         }
       }
 #pragma unroll
-      for (int j = 0; j < N / 16; ++j)  // S += V^T B
+      for (int ks = 0; ks < 2; ++ks) {
+        uint32_t vf[3][4];
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          uint32_t b[4];
-          ldsm4_t(b, &sm.b[buf][16 * ks + mrow][16 * j + mcol]);
+        for (int m = 0; m < 3; ++m) ldsm4(vf[m], &sm.v[grp][m][mrow][16 * ks + mcol]);
+        if (!STATE) {  // Y += V (C B^T)^T: the pieces (0,0) and (16,16) by one warp, (16,0) by the other
+          if (half == 0 || ks == 0) {
+            const int tb = half == 0 ? 16 * ks : 16;
+            uint32_t bh[4], bl[4];
+            ldsm4(bh, &sm.cb[0][tb + xrow][16 * ks + xcol]);
+            ldsm4(bl, &sm.cb[1][tb + xrow][16 * ks + xcol]);
+            if (tb == 0) {
 #pragma unroll
-          for (int m = 0; m < 3; ++m) {
-            mma16816(S[2 * j], vf[ks][m], b);
-            mma16816(S[2 * j + 1], vf[ks][m], b + 2);
+              for (int m = 0; m < 3; ++m)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) mma16816(Y[j], vf[m == 2], (m == 1 ? bl : bh) + 2 * j);
+            } else {
+#pragma unroll
+              for (int m = 0; m < 3; ++m)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) mma16816(Y[2 + j], vf[m == 2], (m == 1 ? bl : bh) + 2 * j);
+            }
           }
         }
+        uint32_t bf[M / 16][4];  // S += V^T B
+#pragma unroll
+        for (int j = 0; j < M / 16; ++j) ldsm4_t(bf[j], &sm.b[buf][16 * ks + mrow][half * M + 16 * j + mcol]);
+#pragma unroll
+        for (int m = 0; m < 3; ++m)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) mma16816(S[j], vf[m], bf[j >> 1] + 2 * (j & 1));
+      }
+      if (!STATE) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          *reinterpret_cast<float2*>(&sm.y[grp][half][g][8 * j + 2 * q]) = make_float2(Y[j][0], Y[j][1]);
+          *reinterpret_cast<float2*>(&sm.y[grp][half][g + 8][8 * j + 2 * q]) = make_float2(Y[j][2], Y[j][3]);
+        }
+      }
     } else {
       for (int t = 0; t < n; ++t) {
-        const float a0 = ex2(dl[g][t]), a1 = ex2(dl[g + 8][t]), u0 = vt[g][t], u1 = vt[g + 8][t];
+        const float a0 = ex2(sm.d[grp][g][t]), a1 = ex2(sm.d[grp][g + 8][t]), u0 = sm.u[grp][g][t], u1 = sm.u[grp][g + 8][t];
         float y0 = 0.f, y1 = 0.f;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const uint32_t bb = *reinterpret_cast<const uint32_t*>(&sm.b[buf][t][8 * j + 2 * q]);
-          S[j][0] = fmaf(a0, S[j][0], u0 * lo16(bb));
-          S[j][1] = fmaf(a0, S[j][1], u0 * hi16(bb));
-          S[j][2] = fmaf(a1, S[j][2], u1 * lo16(bb));
-          S[j][3] = fmaf(a1, S[j][3], u1 * hi16(bb));
+          const float2 bb = both16(*reinterpret_cast<const uint32_t*>(&sm.b[buf][t][half * M + 8 * j + 2 * q]));
+          S[j][0] = fmaf(a0, S[j][0], u0 * bb.x);
+          S[j][1] = fmaf(a0, S[j][1], u0 * bb.y);
+          S[j][2] = fmaf(a1, S[j][2], u1 * bb.x);
+          S[j][3] = fmaf(a1, S[j][3], u1 * bb.y);
           if (!STATE) {
-            const uint32_t cc = *reinterpret_cast<const uint32_t*>(&sm.c[buf][t][8 * j + 2 * q]);
-            y0 = fmaf(lo16(cc), S[j][0], fmaf(hi16(cc), S[j][1], y0));
-            y1 = fmaf(lo16(cc), S[j][2], fmaf(hi16(cc), S[j][3], y1));
+            const float2 cc = both16(*reinterpret_cast<const uint32_t*>(&sm.c[buf][t][half * M + 8 * j + 2 * q]));
+            y0 = fmaf(cc.x, S[j][0], fmaf(cc.y, S[j][1], y0));
+            y1 = fmaf(cc.x, S[j][2], fmaf(cc.y, S[j][3], y1));
           }
         }
         if (!STATE) {
@@ -599,48 +644,47 @@ __global__ void __launch_bounds__(kWarps * 32, 3) scan_block_kernel(PromptArgs p
           y1 += __shfl_xor_sync(0xffffffffu, y1, 1);
           y0 += __shfl_xor_sync(0xffffffffu, y0, 2);
           y1 += __shfl_xor_sync(0xffffffffu, y1, 2);
-          if (q == 0) {  // the four lanes have read u there
-            vt[g][t] = y0;
-            vt[g + 8][t] = y1;
+          if (q == 0) {
+            sm.y[grp][half][g][t] = y0;
+            sm.y[grp][half][g + 8][t] = y1;
           }
         }
       }
     }
+    // the pair's outputs are there, and it is done with V, u and d
+    asm volatile("bar.sync %0, 64;" ::"r"(grp + 1) : "memory");
     if (!STATE) {
-      __syncwarp();
+      const float4 a0 = *reinterpret_cast<const float4*>(&sm.y[grp][0][2 * i][tk]), b0 = *reinterpret_cast<const float4*>(&sm.y[grp][1][2 * i][tk]);
+      const float4 a1 = *reinterpret_cast<const float4*>(&sm.y[grp][0][2 * i + 1][tk]), b1 = *reinterpret_cast<const float4*>(&sm.y[grp][1][2 * i + 1][tk]);
+      const float2 o[4] = {{a0.x + b0.x, a1.x + b1.x}, {a0.y + b0.y, a1.y + b1.y}, {a0.z + b0.z, a1.z + b1.z}, {a0.w + b0.w, a1.w + b1.w}};
+      bf16* row = y + (int64_t)(t0 + tk) * p.C;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int t = 8 * tg + k;
-        const float y0 = vt[2 * i][t], y1 = vt[2 * i + 1][t];
-        if (t < n)
-          store_pair(y + (int64_t)(t0 + t) * p.C, ca, p.C, ypairs, heavy ? pack2(y0, y1) : pack2(y0 * ex2(E[k][0]), y1 * ex2(E[k][1])));
+      for (int k = 0; k < 4; ++k, row += p.C) {
+        const float2 r = heavy ? o[k] : mul2(o[k], make_float2(ex2(E[k].x), ex2(E[k].y)));
+        if (tk + k < n) store_pair(row, ca, p.C, ypairs, pack2(r.x, r.y));
       }
     }
   }
 
   // the end state, with the scale it lacks
   if (STATE || sg.index == sg.count - 1) {
-    scale_rows<NT>(S, ex2(pend[0]), ex2(pend[1]));
-    float* dst = (STATE ? seg_state : slot_state) + (int64_t)(c0 + g) * N + 2 * q;
+    scale_rows<NT>(S, ex2(pend));
+    float* dst = (STATE ? seg_state : slot_state) + at_state;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       if (has0) *reinterpret_cast<float2*>(dst + 8 * j) = make_float2(S[j][0], S[j][1]);
       if (has1) *reinterpret_cast<float2*>(dst + 8 * N + 8 * j) = make_float2(S[j][2], S[j][3]);
     }
-    if (STATE && tg == 0) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (ca + e < p.C) pa.decays[(int64_t)(sg.first + sg.index) * p.C + ca + e] = total[e];
-    }
+    if (STATE && half == 0 && lane < 16 && c0 + lane < p.C) pa.decays[(int64_t)(sg.first + sg.index) * p.C + c0 + lane] = total;
   }
   // the first segment's block alone reads the window, so it may write it
-  if (!STATE && sg.index == 0 && tg == 0) {
+  if (!STATE && sg.index == 0 && half == 0 && tg == 0) {
     const int len = sg.seq.end - sg.seq.start;
     uint32_t nw[3];
 #pragma unroll
     for (int j = 0; j < 3; ++j) {
       const int at = len + j - 3;
-      nw[j] = at >= 0 ? load_pair(x + (int64_t)(sg.seq.start + at) * p.xs, ca, p.C, pairs) : at == -2 ? before[1] : before[2];
+      nw[j] = at >= 0 ? load_pair(x + (int64_t)(sg.seq.start + at) * p.xs, ca, p.C, pairs) : load_pair(win + (3 + at) * p.C, ca, p.C, pairs);
     }
 #pragma unroll
     for (int j = 0; j < 3; ++j) store_pair(win + j * p.C, ca, p.C, pairs, nw[j]);
