@@ -256,6 +256,15 @@ AHB_DEVICE uint32_t clip2(uint32_t x) {
   return __heq2_mask(v, v) & *reinterpret_cast<const uint32_t*>(&c);
 }
 
+// whether eight bf16 are all within +-1000 (false for NaN)
+AHB_DEVICE bool within(const uint4& r) {
+  const uint32_t a[4] = {r.x & 0x7fff7fffu, r.y & 0x7fff7fffu, r.z & 0x7fff7fffu, r.w & 0x7fff7fffu};
+  __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162*>(&a[0]);
+#pragma unroll
+  for (int j = 1; j < 4; ++j) m = __hmax2_nan(m, *reinterpret_cast<const __nv_bfloat162*>(&a[j]));
+  return __hble2(m, __floats2bfloat162_rn(kClip, kClip));
+}
+
 AHB_DEVICE float lo16(uint32_t x) { return __uint_as_float(x << 16); }
 AHB_DEVICE float hi16(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
@@ -270,18 +279,17 @@ AHB_DEVICE uint32_t term2(float2& v) {
 
 using bf16 = __nv_bfloat16;
 
-// Channels c, c + 1 of a row as two bf16; `pairs`: both in one 4-byte access
+// Channels c, c + 1 of a row as two bf16 (0 past the last); `pairs`: both exist, in one 4-byte access
 AHB_DEVICE uint32_t load_pair(const bf16* row, int c, int C, bool pairs) {
-  if (c >= C) return 0u;
   if (pairs) return __ldg(reinterpret_cast<const unsigned int*>(row + c));
+  if (c >= C) return 0u;
   const uint16_t* r = reinterpret_cast<const uint16_t*>(row) + c;
   return __ldg(r) | (c + 1 < C ? (uint32_t)__ldg(r + 1) << 16 : 0u);
 }
 AHB_DEVICE void store_pair(bf16* row, int c, int C, bool pairs, uint32_t v) {
-  if (c >= C) return;
-  if (pairs) {
+  if (pairs && c < C) {
     *reinterpret_cast<uint32_t*>(row + c) = v;
-  } else {
+  } else if (c < C) {
     uint16_t* r = reinterpret_cast<uint16_t*>(row) + c;
     r[0] = (uint16_t)v;
     if (c + 1 < C) r[1] = (uint16_t)(v >> 16);
@@ -322,7 +330,9 @@ AHB_DEVICE void scale_rows(float (*S)[4], float f) {
   }
 }
 
-template <typename W, int N, bool STATE>
+// FAST: 4-byte access to channel pairs, 16-byte access to rows of B and C, whole groups of 16 channels
+// (the other form takes any alignment, stride and number of channels).
+template <typename W, int N, bool STATE, bool FAST>
 __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs pa) {
   constexpr int M = N / 2, NT = M / 8;      // this warp's states, their accumulator tiles
   using Smem = BlockSmem<N>;
@@ -333,7 +343,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs p
   const int g = lane >> 2, q = lane & 3;    // accumulator rows g, g + 8; columns 2 q, 2 q + 1
   const int i = lane & 7, tg = lane >> 3;   // channels 2 i, 2 i + 1 of tokens tk .. tk + 3
   const int tk = half * 16 + tg * 4;
-  const int c0 = blockIdx.y * kChan + grp * 16, ca = c0 + 2 * i;
+  // with whole groups, those past the last channel repeat its group and store nothing
+  const int c1 = blockIdx.y * kChan + grp * 16, c0 = FAST ? min(c1, p.C - 16) : c1, ca = c0 + 2 * i;
+  const bool mine = !FAST || c1 < p.C;
   const Segment sg = find_segment(p, pa.seg, blockIdx.x);
   if (sg.b < 0) return;
   if (STATE && sg.index == sg.count - 1) return;  // its end state comes with its outputs
@@ -342,11 +354,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs p
   bf16* const y = static_cast<bf16*>(p.y);
   const bf16* const x = static_cast<const bf16*>(p.x);
   const bf16* const dt = static_cast<const bf16*>(p.dt);
-  const bool ypairs = (p.C & 1) == 0;
-  const bool pairs = ypairs && ((p.xs | p.dts) & 1) == 0 &&
-                     ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(dt) | reinterpret_cast<uintptr_t>(p.conv_state)) & 3) == 0;
+  const bool ypairs = FAST || (p.C & 1) == 0;
+  const bool pairs = FAST;
   if (slot < 0) {
-    if (!STATE)
+    if (!STATE && mine)
       for (int t = start + half * 4 + tg; t < end; t += 8) store_pair(y + (int64_t)t * p.C, ca, p.C, ypairs, 0u);
     return;
   }
@@ -365,7 +376,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs p
   float S[NT][4];
   float* const slot_state = p.state + (int64_t)slot * p.C * N;
   float* const seg_state = pa.states + (int64_t)(sg.first + sg.index) * p.C * N;
-  const bool has0 = c0 + g < p.C, has1 = c0 + g + 8 < p.C;
+  const bool has0 = FAST || c0 + g < p.C, has1 = FAST || c0 + g + 8 < p.C;
   const int64_t at_state = (int64_t)(c0 + g) * N + half * M + 2 * q;
   {
     const float* src = (sg.count == 1 ? slot_state : seg_state) + at_state;
@@ -382,32 +393,32 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs p
   }
 
   // block rows of B and C: every thread copies, and later clips, the same 16-byte pieces
-  constexpr int ALL = kBlock * N / 8, PIECES = (ALL + kWarps * 32 - 1) / (kWarps * 32);
-  const bool wide = (((p.bs | p.cs) & 7) == 0) && ((reinterpret_cast<uintptr_t>(p.Bm) | reinterpret_cast<uintptr_t>(p.Cm)) & 15) == 0;
+  constexpr int ALL = kBlock * N / 8, PIECES = (ALL + kWarps * 32 - 1) / (kWarps * 32), STEP = kWarps * 32 / (N / 8);
+  const int prow = tid / (N / 8), pcol = tid % (N / 8) * 8;  // piece m: row prow + m STEP
   auto copy_rows = [&](const void* from, int64_t stride, bf16 (*to)[Smem::LD], int t0) {
+    const bf16* src = static_cast<const bf16*>(from) + (int64_t)(t0 + prow) * stride + pcol;
 #pragma unroll
-    for (int m = 0; m < PIECES; ++m) {
-      const int piece = tid + m * kWarps * 32, row = piece / (N / 8), col = piece % (N / 8) * 8;
-      if (ALL % (kWarps * 32) != 0 && piece >= ALL) break;
-      const bf16* src = static_cast<const bf16*>(from) + (int64_t)(t0 + row) * stride + col;
+    for (int m = 0; m < PIECES; ++m, src += STEP * stride) {
+      const int row = prow + m * STEP;
+      if (ALL % (kWarps * 32) != 0 && row >= kBlock) break;
       if (t0 + row >= end) {
-        *reinterpret_cast<uint4*>(&to[row][col]) = make_uint4(0, 0, 0, 0);
-      } else if (wide) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(&to[row][col])), "l"(src) : "memory");
+        *reinterpret_cast<uint4*>(&to[row][pcol]) = make_uint4(0, 0, 0, 0);
+      } else if (FAST) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(&to[row][pcol])), "l"(src) : "memory");
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) to[row][col + k] = src[k];
+        for (int k = 0; k < 8; ++k) to[row][pcol + k] = src[k];
       }
     }
   };
   auto clip_rows = [&](bf16 (*rows)[Smem::LD]) {
 #pragma unroll
     for (int m = 0; m < PIECES; ++m) {
-      const int piece = tid + m * kWarps * 32;
-      if (ALL % (kWarps * 32) != 0 && piece >= ALL) break;
-      uint4* at = reinterpret_cast<uint4*>(&rows[piece / (N / 8)][piece % (N / 8) * 8]);
+      const int row = prow + m * STEP;
+      if (ALL % (kWarps * 32) != 0 && row >= kBlock) break;
+      uint4* at = reinterpret_cast<uint4*>(&rows[row][pcol]);
       const uint4 r = *at;
-      *at = make_uint4(clip2(r.x), clip2(r.y), clip2(r.z), clip2(r.w));
+      if (!within(r)) *at = make_uint4(clip2(r.x), clip2(r.y), clip2(r.z), clip2(r.w));
     }
   };
   auto copy_block = [&](int t0, int buf) {
@@ -418,13 +429,25 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs p
   // this lane's tokens; lanes of the warp's first tokens also hold the three rows before them
   uint32_t xr[4], dr[4], hr[3];
   auto load_tokens = [&](int t0) {
-    const bf16* xp = x + (int64_t)(t0 + tk) * p.xs;
-    const bf16* dp = dt + (int64_t)(t0 + tk) * p.dts;
+    const bf16* xp = x + (int64_t)(t0 + tk) * p.xs + ca;
+    const bf16* dp = dt + (int64_t)(t0 + tk) * p.dts + ca;
+    if (FAST && t0 + kBlock <= end && (half == 1 || t0 > sg.seq.start)) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        xr[k] = __ldg(reinterpret_cast<const unsigned int*>(xp + k * p.xs));
+        dr[k] = __ldg(reinterpret_cast<const unsigned int*>(dp + k * p.dts));
+      }
+      if (tg == 0) {
+#pragma unroll
+        for (int j = 0; j < 3; ++j) hr[j] = __ldg(reinterpret_cast<const unsigned int*>(xp + (j - 3) * p.xs));
+      }
+      return;
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const bool in = t0 + tk + k < end;
-      xr[k] = in ? load_pair(xp + k * p.xs, ca, p.C, pairs) : 0u;
-      dr[k] = in ? load_pair(dp + k * p.dts, ca, p.C, pairs) : 0u;
+      xr[k] = in ? load_pair(xp - ca + k * p.xs, ca, p.C, pairs) : 0u;
+      dr[k] = in ? load_pair(dp - ca + k * p.dts, ca, p.C, pairs) : 0u;
     }
     if (tg == 0) {
 #pragma unroll
@@ -495,35 +518,37 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs p
     if (tg >= 2) incl = add2(incl, v);
     const float2 whole = make_float2(__shfl_sync(0xffffffffu, incl.x, 24 + i), __shfl_sync(0xffffffffu, incl.y, 24 + i));
     if (tg == 0) *reinterpret_cast<float2*>(&sm.span[grp][half][2 * i]) = whole;
-    // E: the first half ends at the reference, the second starts from it
-    float2 run = add2(incl, make_float2(-sum.x, -sum.y));
-    if (half == 0) run = add2(run, make_float2(-whole.x, -whole.y));
-    // for a group that has to go token by token: its inputs and decays as they are
-    *reinterpret_cast<float4*>(&sm.u[grp][2 * i][tk]) = make_float4(u[0].x, u[1].x, u[2].x, u[3].x);
-    *reinterpret_cast<float4*>(&sm.u[grp][2 * i + 1][tk]) = make_float4(u[0].y, u[1].y, u[2].y, u[3].y);
-    *reinterpret_cast<float4*>(&sm.d[grp][2 * i][tk]) = make_float4(E[0].x, E[1].x, E[2].x, E[3].x);
-    *reinterpret_cast<float4*>(&sm.d[grp][2 * i + 1][tk]) = make_float4(E[0].y, E[1].y, E[2].y, E[3].y);
-    float2 V[4];
+    asm volatile("bar.sync %0, 64;" ::"r"(grp + 1) : "memory");  // the pair's spans are there
+    const float mid = sm.span[grp][0][lane & 15], tail = sm.span[grp][1][lane & 15];
+    const bool heavy = __any_sync(0xffffffffu, fminf(mid, tail) < -kSpan);
+    if (heavy) {  // V would leave the floats' range: the group goes token by token, on these
+      *reinterpret_cast<float4*>(&sm.u[grp][2 * i][tk]) = make_float4(u[0].x, u[1].x, u[2].x, u[3].x);
+      *reinterpret_cast<float4*>(&sm.u[grp][2 * i + 1][tk]) = make_float4(u[0].y, u[1].y, u[2].y, u[3].y);
+      *reinterpret_cast<float4*>(&sm.d[grp][2 * i][tk]) = make_float4(E[0].x, E[1].x, E[2].x, E[3].x);
+      *reinterpret_cast<float4*>(&sm.d[grp][2 * i + 1][tk]) = make_float4(E[0].y, E[1].y, E[2].y, E[3].y);
+    } else {
+      // E: the first half ends at the reference, the second starts from it
+      float2 run = add2(incl, make_float2(-sum.x, -sum.y));
+      if (half == 0) run = add2(run, make_float2(-whole.x, -whole.y));
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      run = add2(run, E[k]);
-      V[k] = mul2(u[k], make_float2(ex2(-run.x), ex2(-run.y)));
-      E[k] = run;
-    }
-    float2 V0[2] = {{V[0].x, V[1].x}, {V[2].x, V[3].x}}, V1[2] = {{V[0].y, V[1].y}, {V[2].y, V[3].y}};
+      for (int k = 0; k < 4; ++k) {
+        run = add2(run, E[k]);
+        u[k] = mul2(u[k], make_float2(ex2(-run.x), ex2(-run.y)));
+        E[k] = run;
+      }
+      float2 V0[2] = {{u[0].x, u[1].x}, {u[2].x, u[3].x}}, V1[2] = {{u[0].y, u[1].y}, {u[2].y, u[3].y}};
 #pragma unroll
-    for (int m = 0; m < 3; ++m) {
-      *reinterpret_cast<uint2*>(&sm.v[grp][m][2 * i][tk]) = make_uint2(term2(V0[0]), term2(V0[1]));
-      *reinterpret_cast<uint2*>(&sm.v[grp][m][2 * i + 1][tk]) = make_uint2(term2(V1[0]), term2(V1[1]));
+      for (int m = 0; m < 3; ++m) {
+        *reinterpret_cast<uint2*>(&sm.v[grp][m][2 * i][tk]) = make_uint2(term2(V0[0]), term2(V0[1]));
+        *reinterpret_cast<uint2*>(&sm.v[grp][m][2 * i + 1][tk]) = make_uint2(term2(V1[0]), term2(V1[1]));
+      }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     clip_rows(sm.b[buf]);
     if (!STATE) clip_rows(sm.c[buf]);
     __syncthreads();  // the block's rows, V and spans are there; every warp is done with the other buffer and with cb
     if (t0 + kBlock < end) copy_block(t0 + kBlock, buf ^ 1);
-    const float mid = sm.span[grp][0][lane & 15], tail = sm.span[grp][1][lane & 15];
     total += mid + tail;
-    const bool heavy = __any_sync(0xffffffffu, fminf(mid, tail) < -kSpan);
     // S takes the scale it lacks and goes to the block's reference.  S itself may stand at 2^kSpan, so the two
     // scales go in one after the other where their product would leave the floats' range.
     if (__any_sync(0xffffffffu, pend + mid < -120.f)) {
@@ -661,13 +686,13 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs p
 #pragma unroll
       for (int k = 0; k < 4; ++k, row += p.C) {
         const float2 r = heavy ? o[k] : mul2(o[k], make_float2(ex2(E[k].x), ex2(E[k].y)));
-        if (tk + k < n) store_pair(row, ca, p.C, ypairs, pack2(r.x, r.y));
+        if (mine && tk + k < n) store_pair(row, ca, p.C, ypairs, pack2(r.x, r.y));
       }
     }
   }
 
   // the end state, with the scale it lacks
-  if (STATE || sg.index == sg.count - 1) {
+  if (mine && (STATE || sg.index == sg.count - 1)) {
     scale_rows<NT>(S, ex2(pend));
     float* dst = (STATE ? seg_state : slot_state) + at_state;
 #pragma unroll
@@ -678,7 +703,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs p
     if (STATE && half == 0 && lane < 16 && c0 + lane < p.C) pa.decays[(int64_t)(sg.first + sg.index) * p.C + c0 + lane] = total;
   }
   // the first segment's block alone reads the window, so it may write it
-  if (!STATE && sg.index == 0 && half == 0 && tg == 0) {
+  if (!STATE && mine && sg.index == 0 && half == 0 && tg == 0) {
     const int len = sg.seq.end - sg.seq.start;
     uint32_t nw[3];
 #pragma unroll
@@ -735,15 +760,15 @@ int64_t max_segments(int B, int L, int T, bool packed, int seg) {
   return packed ? (int64_t)T / seg + B : (int64_t)B * ((L + seg - 1) / seg);
 }
 
-template <typename W, int N>
+template <typename W, int N, bool FAST>
 int launch_prompt(const ScanArgs& a, int seg, float* work, cudaStream_t st) {
   static bool ready[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -3;
   const int bytes = (int)sizeof(BlockSmem<N>);
   if (!ready[dev]) {
-    if (cudaFuncSetAttribute(scan_block_kernel<W, N, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
-        cudaFuncSetAttribute(scan_block_kernel<W, N, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    if (cudaFuncSetAttribute(scan_block_kernel<W, N, true, FAST>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
+        cudaFuncSetAttribute(scan_block_kernel<W, N, false, FAST>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
       return -3;
     ready[dev] = true;
   }
@@ -751,11 +776,19 @@ int launch_prompt(const ScanArgs& a, int seg, float* work, cudaStream_t st) {
   const PromptArgs p{a, seg, (int)segs, work, work + segs * a.C * N};
   const dim3 grid((unsigned)segs, (unsigned)((a.C + kChan - 1) / kChan));
   if (segs > a.B) {
-    scan_block_kernel<W, N, true><<<grid, kWarps * 32, bytes, st>>>(p);
+    scan_block_kernel<W, N, true, FAST><<<grid, kWarps * 32, bytes, st>>>(p);
     scan_join_kernel<N><<<dim3((unsigned)(((int64_t)a.C * (N / 4) + 255) / 256), (unsigned)a.B), 256, 0, st>>>(p);
   }
-  scan_block_kernel<W, N, false><<<grid, kWarps * 32, bytes, st>>>(p);
+  scan_block_kernel<W, N, false, FAST><<<grid, kWarps * 32, bytes, st>>>(p);
   return 0;
+}
+
+template <typename W, int N>
+int launch_prompt(const ScanArgs& a, int seg, float* work, cudaStream_t st) {
+  const auto low = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+  const bool fast = a.C % 16 == 0 && ((a.xs | a.dts) & 1) == 0 && ((a.bs | a.cs) & 7) == 0 &&
+                    ((low(a.x) | low(a.dt) | low(a.conv_state)) & 3) == 0 && ((low(a.Bm) | low(a.Cm)) & 15) == 0;
+  return fast ? launch_prompt<W, N, true>(a, seg, work, st) : launch_prompt<W, N, false>(a, seg, work, st);
 }
 
 template <typename T, typename W>
@@ -780,9 +813,11 @@ int by_state(const ScanArgs& p, int N, int seg, float* work, cudaStream_t st) {
 int ahb_selective_scan_plan(int B, int L, int T, int C, int N, int packed, int dtype, int64_t* floats) {
   *floats = 0;
   if (dtype != AHB_BF16 || B == 0 || T < 4 * (int64_t)B) return 0;
-  const int64_t groups = (C + kChan - 1) / kChan;
-  int64_t seg = T * groups / (2 * 3 * 148);
-  seg = std::min<int64_t>(1 << 30, std::max<int64_t>(256, (seg + kBlock - 1) / kBlock * kBlock));
+  // Two blocks of 64 channels run on an SM.  Sequences that fill them stay whole (a segment more costs
+  // another state pass over it); others are cut so that one wave of blocks holds all segments.
+  const int64_t groups = (C + kChan - 1) / kChan, wave = 2 * 148;
+  int64_t seg = packed ? T * groups / wave : (L + std::max<int64_t>(1, wave / (B * groups)) - 1) / std::max<int64_t>(1, wave / (B * groups));
+  seg = std::min<int64_t>(1 << 30, std::max<int64_t>(128, (seg + kBlock - 1) / kBlock * kBlock));
   const int64_t segs = max_segments(B, L, T, packed != 0, (int)seg);
   if (segs > B) *floats = segs * C * (N + 1);
   return (int)seg;
