@@ -273,7 +273,8 @@ AHB_DEVICE float2 both16(uint32_t x) { return make_float2(lo16(x), hi16(x)); }
 // the next bf16 term of two floats, which keep what it leaves
 AHB_DEVICE uint32_t term2(float2& v) {
   const uint32_t h = pack2(v.x, v.y);
-  v = add2(v, make_float2(-lo16(h), -hi16(h)));
+  v.x -= lo16(h);
+  v.y -= hi16(h);
   return h;
 }
 
