@@ -743,16 +743,23 @@ __global__ void __launch_bounds__(256) scan_join_kernel(PromptArgs pa) {
   if (at >= (int64_t)p.C * (N / 4)) return;
   const int c = (int)(at / (N / 4));
   float4 run = reinterpret_cast<const float4*>(p.state + (int64_t)slot * p.C * N)[at];
-  for (int s = first; s < first + count; ++s) {
-    float4* seg = reinterpret_cast<float4*>(pa.states + (int64_t)s * p.C * N) + at;
-    if (s == first + count - 1) {
-      *seg = run;
-      break;
-    }
-    const float4 own = *seg;
-    const float f = ex2(pa.decays[(int64_t)s * p.C + c]);
-    *seg = run;
-    run = make_float4(fmaf(f, run.x, own.x), fmaf(f, run.y, own.y), fmaf(f, run.z, own.z), fmaf(f, run.w, own.w));
+  constexpr int AHEAD = 8;  // segments whose end states are on the way together
+  for (int s0 = 0; s0 < count; s0 += AHEAD) {
+    float4 own[AHEAD];
+    float f[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (s0 + k < count - 1) {
+        own[k] = *(reinterpret_cast<const float4*>(pa.states + (int64_t)(first + s0 + k) * p.C * N) + at);
+        f[k] = ex2(pa.decays[(int64_t)(first + s0 + k) * p.C + c]);
+      }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (s0 + k < count) {
+        *(reinterpret_cast<float4*>(pa.states + (int64_t)(first + s0 + k) * p.C * N) + at) = run;
+        if (s0 + k < count - 1)
+          run = make_float4(fmaf(f[k], run.x, own[k].x), fmaf(f[k], run.y, own[k].y), fmaf(f[k], run.z, own[k].z), fmaf(f[k], run.w, own[k].w));
+      }
   }
 }
 
