@@ -1701,6 +1701,7 @@ torch::Tensor selective_scan(const torch::Tensor& x, const torch::Tensor& dt, co
   const int64_t T = x.size(0), C = x.size(1), S = state.size(0), H = state.size(1), P = state.size(2), N = state.size(3);
   TORCH_CHECK(H * P == C && C > 0, op, ": ", H, " heads of ", P, " channels do not make ", C);
   TORCH_CHECK(T < (1ll << 30) && C < (1ll << 22), op, ": sizes out of range");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(state.data_ptr()) % 16 == 0, op, ": state must start at a 16-byte boundary");
   check_rows(x, x, T, C, op, "x");
   check_rows(dt, x, T, C, op, "dt");
   check_rows(Bm, x, T, N, op, "B");
@@ -1741,7 +1742,8 @@ torch::Tensor gdn2_recurrent(const std::vector<torch::Tensor>& in, const std::ve
               op, ": state must be a contiguous fp32 (slots, heads, D, D) tensor on ", x.device());
   const int64_t T = x.size(0), d = x.size(1), S = state.size(0), H = state.size(1), D = state.size(2);
   TORCH_CHECK(H * D == d && d > 0, op, ": ", H, " heads of ", D, " channels do not make ", d);
-  TORCH_CHECK(T < (1ll << 31) && H < (1ll << 16), op, ": sizes out of range");
+  TORCH_CHECK(T < (1ll << 30) && H < (1ll << 16), op, ": sizes out of range");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(state.data_ptr()) % 16 == 0, op, ": state must start at a 16-byte boundary");
   const void* ip[6];
   int64_t rs[6];
   for (int i = 0; i < 6; ++i) {
@@ -1765,7 +1767,7 @@ torch::Tensor gdn2_recurrent(const std::vector<torch::Tensor>& in, const std::ve
   const int rc = ahb_gdn_recurrent(ip, rs, wp, dt_code(conv_w[0]), bp, decay_a.data_ptr<float>(), conv_state.data_ptr(),
                                    state.data_ptr<float>(), q.cu, q.slots, y.data_ptr(), q.B, q.L, (int)T, (int)H,
                                    (int)D, (int)S, dt_code(x), cur_stream());
-  TORCH_CHECK(rc == 0, op, ": no kernel for head dim ", D);
+  TORCH_CHECK(rc == 0, op, ": failed with code ", rc, " for head dim ", D);
   check_launch(op);
   return y;
 }
