@@ -1772,7 +1772,7 @@ torch::Tensor gdn2_recurrent(const std::vector<torch::Tensor>& in, const std::ve
   return y;
 }
 
-std::vector<torch::Tensor> sample(const torch::Tensor& logits, const torch::Tensor& noise,
+std::tuple<torch::Tensor, torch::Tensor> sample(const torch::Tensor& logits, const torch::Tensor& noise,
                                   const torch::Tensor& temperature, const torch::Tensor& top_k,
                                   const torch::Tensor& top_p, const torch::Tensor& min_p) {
   const char* op = "sample";

@@ -246,11 +246,8 @@ __global__ void __launch_bounds__(NT) sample_kernel(SampleArgs p, int ctas) {
         X::clean(r[u]);
         if (p.resident) keep[v + u * NT - v0] = r[u];
         range.most = fmaxf(range.most, largest<T>(r[u]));
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const float x = X::get(r[u], j);
-          range.least = fminf(range.least, x == -INFINITY ? INFINITY : x);
-        }
+        const float x = X::get(r[u], 0);  // one value a line is enough to size the bins
+        range.least = fminf(range.least, x == -INFINITY ? INFINITY : x);
       }
   }
   range = combine<RANGE, NT>(range, parts, turn ^= 1, rank, ctas);
@@ -263,7 +260,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(SampleArgs p, int ctas) {
     cluster_sync();  // the other CTAs may still be reading this one's part
     return;
   }
-  const float bins = fmaxf(kBinsPerLog2, (kBins - 1) / fmaxf((top - range.least) * c, 1e-20f));
+  const float bins = range.least < INFINITY ? fminf(fmaxf(kBinsPerLog2, (kBins - 1) / fmaxf((top - range.least) * c, 1e-20f)), 1e6f) : kBinsPerLog2;
 
   // The race over line r: tokens with y = (top - x) c bins below `limit` (bins left in, min_p) and, in
   // later rounds, ranked before (bound_l, bound_i).

@@ -170,7 +170,7 @@ def selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, cu_seqle
     (S, H, P, N)`` the fp32 scan state; both are updated in place.  Sequence ``i`` owns slot
     ``slots[i]`` (int32, all different; default ``i``); one with a slot outside ``[0, S)`` is padding:
     zeros come out and no state is touched.  Returns ``y`` shaped like ``x``."""
-    if use_cuda(x):
+    if x.is_cuda and _IMPL == "cuda":
         return _k().selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, cu_seqlens, slots, dt_min,
                                    dt_max)
     return R.selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, cu_seqlens, slots, dt_min, dt_max)
@@ -191,7 +191,7 @@ def gdn2_recurrent(q, k, v, b, w, f, conv_w, conv_b, decay_a, conv_state, state,
     Tokens, ``cu_seqlens`` and ``slots`` as in ``selective_scan``; ``conv_state (S, 3, 3, d)`` holds
     the last three rows of ``q, k, v`` (in that order) and ``state (S, H, D, D)`` the fp32 state, both
     updated in place.  Returns ``o`` shaped like ``q``."""
-    if use_cuda(q):
+    if q.is_cuda and _IMPL == "cuda":
         return _k().gdn2_recurrent(q, k, v, b, w, f, conv_w, conv_b, decay_a, conv_state, state, cu_seqlens, slots)
     return R.gdn2_recurrent(q, k, v, b, w, f, conv_w, conv_b, decay_a, conv_state, state, cu_seqlens, slots)
 
@@ -209,7 +209,7 @@ def sample(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     their probability (a row without any such score gives the first).  ``temperature <= 0`` takes the first token and tempers by 1 for ``logprobs``,
     the log-probability before anything is cut.  NaN and ``-inf`` logits are never drawn; a row
     of nothing else gives token -1 and ``-inf``."""
-    if use_cuda(logits):
+    if logits.is_cuda and _IMPL == "cuda":
         return _k().sample(logits, noise, temperature, top_k, top_p, min_p)
     return R.sample(logits, noise, temperature, top_k, top_p, min_p)
 

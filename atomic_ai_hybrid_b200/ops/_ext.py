@@ -23,8 +23,10 @@ class _Counted:
             return fn
 
         def call(*a, **k):
-            launch_counter.add(name, a, k)
+            if launch_counter.on:
+                launch_counter.add(name, a, k)
             return fn(*a, **k)
+        setattr(self, name, call)  # found without __getattr__ from now on
         return call
 
 

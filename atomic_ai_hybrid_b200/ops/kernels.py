@@ -928,17 +928,15 @@ def gdn2_recurrent(q, k, v, b, w, f, conv_w, conv_b, decay_a, conv_state, state,
 def _per_row(v, like, dtype):
     """A setting as a ``(B,)`` tensor of ``dtype`` on the rows' device."""
     if isinstance(v, torch.Tensor):
-        return v if v.dtype == dtype and v.device == like.device else v.to(device=like.device, dtype=dtype)
+        return v if v.dtype is dtype and v.is_cuda else v.to(device=like.device, dtype=dtype)
     return torch.full((like.shape[0],), v, dtype=dtype, device=like.device)
 
 
 def sample(logits, noise, temperature, top_k, top_p, min_p):
     """See ``ops.sample``; bf16 or fp32 logits."""
     f32 = torch.float32
-    tokens, logprobs = ext().sample(logits, noise, _per_row(temperature, logits, f32),
-                                    _per_row(top_k, logits, torch.int32), _per_row(top_p, logits, f32),
-                                    _per_row(min_p, logits, f32))
-    return tokens, logprobs
+    return ext().sample(logits, noise, _per_row(temperature, logits, f32), _per_row(top_k, logits, torch.int32),
+                        _per_row(top_p, logits, f32), _per_row(min_p, logits, f32))
 
 
 # ----------------------------------------------------------------- fused optimizer
