@@ -22,6 +22,12 @@ from ..utils.diag import DIAG
 from .layers import Dense, RMSNorm, lecun_normal_, tp_world_rank
 
 
+def _serving():
+    """The running ``serving(...)`` call (tokens on kept state), or None."""
+    from ..serving.state import get_serving
+    return get_serving()
+
+
 def _shard_vec(full: torch.Tensor) -> nn.Parameter:
     """A per-channel / per-head parameter from its full-size initial value: under tensor
     parallelism this rank's piece of it (every rank draws the full value)."""
@@ -90,6 +96,9 @@ class GatedDeltaNet2(nn.Module):
         return self.out_proj(o)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        sv = _serving()
+        if sv is not None:
+            return sv.gdn2(self, x)
         cp = get_cp()
         if ops.use_cuda(x) and cp is None:
             return self._forward_fused(x)
@@ -189,6 +198,9 @@ class Mamba2(nn.Module):
         return self.out_proj(out)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        sv = _serving()
+        if sv is not None:
+            return sv.mamba2(self, x)
         cp = get_cp()
         if ops.use_cuda(x) and cp is None:
             from ..ops import kernels as K
@@ -250,6 +262,9 @@ class MLA(nn.Module):
         self.W_o = Dense(d, d, tp="row")
 
     def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+        sv = _serving()
+        if sv is not None:
+            return sv.mla(self, x)
         H = self.n_heads
         dh = self.cfg.d_model // self.cfg.n_heads
         tp = get_tp()

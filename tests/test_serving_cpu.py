@@ -1,0 +1,180 @@
+"""Serving on the CPU: the operators' PyTorch forms against direct formulas, a model on kept state against
+its forward over whole sequences, generation, refusals."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from atomic_ai_hybrid_b200 import get_preset, ops
+from atomic_ai_hybrid_b200.models import HybridMoEModel
+from atomic_ai_hybrid_b200.ops import reference as R
+from atomic_ai_hybrid_b200.serving import DecodeState, Generator, load_weights, serving
+
+
+def test_selective_scan_is_conv_and_token_serial_scan():
+    """From zero state it is the layer's convolution, step and scan (64 bits: differences are rounding)."""
+    g = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)  # noqa: E731
+    B, L, H, P, N = 2, 23, 3, 8, 32
+    C = H * P
+    x, dt, Bm, Cm, w, b, A = r(B, L, C), r(B, L, C), r(B, L, N), r(B, L, N), r(C, 4), r(C), -r(H).exp()
+    conv, state = torch.zeros(B, 3, C, dtype=torch.float64), torch.zeros(B, H, P, N, dtype=torch.float64)
+    y = ops.selective_scan(x, dt, A, Bm, Cm, w, b, conv, state)
+    xc = R.causal_conv1d(x, w, b, True).view(B, L, H, P)
+    step = F.softplus(dt).clamp(1e-2, 1.0).view(B, L, H, P)
+    want, s = R.ssd_token_serial(step, A, Bm, Cm, xc)
+    torch.testing.assert_close(y.view(want.shape), want, rtol=1e-10, atol=1e-10)
+    torch.testing.assert_close(state, s, rtol=1e-10, atol=1e-10)
+    assert torch.equal(conv, x[:, -3:])
+
+
+def test_gdn2_recurrent_is_conv_norm_gates_and_delta_rule():
+    g = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)  # noqa: E731
+    B, L, H, D = 2, 9, 2, 16
+    d = H * D
+    q, k, v, b, w, f = (r(B, L, d) for _ in range(6))
+    cw, cb, a = [r(d, 4) for _ in range(3)], [r(d) for _ in range(3)], r(H)
+    conv, state = torch.zeros(B, 3, 3, d, dtype=torch.float64), torch.zeros(B, H, D, D, dtype=torch.float64)
+    o = ops.gdn2_recurrent(q, k, v, b, w, f, cw, cb, a, conv, state)
+    shp = (B, L, H, D)
+    qc, kc, vc = (R.causal_conv1d(t, cw[i], cb[i], True).view(shp) for i, t in enumerate((q, k, v)))
+    norm = lambda t: t * torch.rsqrt(t.square().sum(-1, keepdim=True) + 1e-12)  # noqa: E731
+    gl = -a.exp()[:, None] * F.softplus(f.view(shp))
+    want, h = R.gdn2_token_serial(norm(qc), norm(kc), vc.clamp(-50, 50), gl, torch.sigmoid(b).view(shp), torch.sigmoid(w).view(shp))
+    torch.testing.assert_close(o.view(shp), want, rtol=1e-10, atol=1e-10)
+    torch.testing.assert_close(state, h, rtol=1e-10, atol=1e-10)
+    assert torch.equal(conv, torch.stack([q, k, v], 1)[:, :, -3:])
+
+
+def test_sequences_in_parts_and_padding_slots():
+    g = torch.Generator().manual_seed(2)
+    r = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)  # noqa: E731
+    T, H, P, N = 12, 2, 4, 32
+    C = H * P
+    x, dt, Bm, Cm, w, A = r(T, C), r(T, C), r(T, N), r(T, N), r(C, 4), -r(H).exp()
+    one = [torch.zeros(4, 3, C, dtype=torch.float64), torch.zeros(4, H, P, N, dtype=torch.float64)]
+    two = [t.clone() for t in one]
+    cu = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    y = ops.selective_scan(x, dt, A, Bm, Cm, w, None, *one, cu_seqlens=cu(0, 7, 7, 12), slots=cu(2, 0, 1))
+    parts = [ops.selective_scan(x[a:e], dt[a:e], A, Bm[a:e], Cm[a:e], w, None, *two, cu_seqlens=cu(0, e - a), slots=cu(s))
+             for a, e, s in ((0, 3, 2), (3, 7, 2), (7, 8, 1), (8, 12, 1))]
+    torch.testing.assert_close(torch.cat(parts), y)
+    for p, q in zip(one, two):
+        torch.testing.assert_close(p, q)
+    assert (one[1][[0, 3]] == 0).all()
+    before = [t.clone() for t in one]
+    y = ops.selective_scan(x[:1], dt[:1], A, Bm[:1], Cm[:1], w, None, *one, slots=cu(-1))
+    assert (y == 0).all() and all(torch.equal(p, q) for p, q in zip(one, before))
+    with pytest.raises(ValueError, match="slot each"):
+        ops.selective_scan(x, dt, A, Bm, Cm, w, None, *one)
+    with pytest.raises(ValueError, match="cu_seqlens packs"):
+        ops.selective_scan(x[None], dt[None], A, Bm[None], Cm[None], w, None, *one, cu_seqlens=cu(0, 12))
+
+
+def test_sample_rules_and_frequencies():
+    logits = torch.tensor([[2.0, 1.0, 2.0, -1.0, float("-inf"), float("nan")]])
+    ones = torch.ones(1, 6)
+    assert ops.sample(logits, ones, temperature=0.0)[0].item() == 0
+    pull = torch.tensor([[9.0, 1.0, 3.0, 1e-6, 1e-9, 1e-9]])
+    assert ops.sample(logits, pull)[0].item() == 3
+    assert ops.sample(logits, pull, top_k=3)[0].item() == 1
+    assert ops.sample(logits, pull, top_k=2)[0].item() == 2
+    # masses 1, 1, 0.368, 0.050 of 2.418 by rank: 0.414 are ranked before the second, 0.827 before the third
+    assert ops.sample(logits, pull, top_p=0.5)[0].item() == 2
+    assert ops.sample(logits, pull, top_p=0.4)[0].item() == 0
+    assert ops.sample(logits, pull, top_p=0.3)[0].item() == 0
+    assert ops.sample(logits, pull, min_p=0.9)[0].item() == 2
+    none = torch.full((1, 3), float("-inf"))
+    tok, lp = ops.sample(none, torch.ones(1, 3))
+    assert tok.item() == -1 and lp.item() == -math.inf
+    p = torch.softmax(torch.tensor([0.3, -0.2, 1.0, 0.0]), 0)
+    n = 4000
+    noise = torch.empty(n, 4).exponential_(generator=torch.Generator().manual_seed(3))
+    count = torch.bincount(ops.sample(p.log()[None].repeat(n, 1), noise)[0], minlength=4).float()
+    assert ((count - n * p).abs() <= 5 * (n * p * (1 - p)).sqrt()).all()
+
+
+def _model(preset, **kw):
+    torch.manual_seed(0)
+    cfg = get_preset(preset, **kw)
+    return HybridMoEModel(cfg, compute_dtype=torch.float32).eval(), cfg
+
+
+@pytest.mark.parametrize("preset,kw", [("tiny", dict(num_layers=2, layer_types=("mamba2", "gdn2"))), ("reference_tiny", {})])
+def test_kept_state_equals_whole_sequences(preset, kw):
+    """Prompts of uneven lengths, then tokens, give the hidden rows of a forward over the whole sequences.  The two
+    run different (fp32) orders of the same sums through a few layers of norms: 1e-3 of the rows' size."""
+    model, cfg = _model(preset, **kw)
+    L = 64
+    ids = torch.randint(0, cfg.vocab_size, (2, L), generator=torch.Generator().manual_seed(1))
+    with torch.no_grad():
+        whole, _ = model(ids)
+    gen = Generator(model, 4, max_len=L)
+    slots, lens = [3, 1], [17, 40]
+    logits = gen.prefill([ids[0, :17].tolist(), ids[1, :40].tolist()], slots)
+    rows = torch.stack([whole[0, 16], whole[1, 39]])
+    want = rows @ model.lm_weight().t()
+    assert (logits - want).norm() <= 1e-3 * want.norm()
+    for _ in range(20):
+        logits = gen.step(torch.stack([ids[i, n] for i, n in enumerate(lens)]), slots)
+        want = torch.stack([whole[i, n] for i, n in enumerate(lens)]) @ model.lm_weight().t()
+        assert (logits - want).norm() <= 1e-3 * want.norm()
+        lens = [n + 1 for n in lens]
+    assert gen.state.lengths == [0, 60, 0, 37]
+
+
+def test_generate_stops_and_repeats():
+    model, cfg = _model("tiny", num_layers=2, layer_types=("mamba2", "gdn2"))
+    gen = Generator(model, 3)
+    prompts = [[1, 2, 3], [7], [5, 6]]
+    run = lambda **kw: gen.generate(prompts, 12, top_k=20, generator=torch.Generator().manual_seed(4), **kw)  # noqa: E731
+    a, la = run()
+    assert [len(t) for t in a] == [12, 12, 12] and all(len(x) == len(y) for x, y in zip(a, la))
+    assert run()[0] == a
+    greedy = gen.generate(prompts, 6, temperature=0.0)[0]
+    assert greedy == gen.generate(prompts, 6, temperature=[0.0, 0.0, 0.0])[0]
+    stop = a[1][4]
+    b, _ = run(stop_token=stop)
+    assert b[1] == a[1][:a[1].index(stop) + 1]
+    assert gen.generate(prompts, 0) == ([[], [], []], [[], [], []])
+
+
+def test_serving_refusals(tmp_path):
+    model, cfg = _model("reference_tiny")
+    with pytest.raises(ValueError, match="max_len"):
+        DecodeState(model, 2)
+    gen = Generator(model, 2, max_len=8)
+    with pytest.raises(ValueError, match="room for 2"):
+        gen.generate([[1]] * 3, 1)
+    with pytest.raises(ValueError, match="at least one token"):
+        gen.generate([[]], 1)
+    with pytest.raises(ValueError, match="max_len=8"):
+        gen.prefill([list(range(9))], [0])
+    with pytest.raises(ValueError, match="different"):
+        gen.prefill([[1], [2]], [0, 0])
+    with serving(gen.state, [0], [1]):
+        with pytest.raises(RuntimeError, match="not nested"):
+            with serving(gen.state, [1], [1]):
+                pass
+    with pytest.raises(FileNotFoundError):
+        load_weights(model, str(tmp_path))
+
+
+def test_load_weights_from_a_training_checkpoint(tmp_path):
+    from atomic_ai_hybrid_b200.ckpt import CheckpointManager
+    from atomic_ai_hybrid_b200.training.trainer import Trainer
+
+    model, cfg = _model("tiny", num_layers=2, layer_types=("mamba2", "gdn2"))
+    tr = Trainer(model, total_steps=4, compute_dtype=torch.float32, device=torch.device("cpu"))
+    mgr = CheckpointManager(str(tmp_path), "latest")
+    mgr.save(3, tr, {}, asynchronous=False)
+    mgr.finalize()
+    torch.manual_seed(9)
+    other = HybridMoEModel(cfg, compute_dtype=torch.float32)
+    assert load_weights(other, str(tmp_path)) == []
+    ids = torch.randint(0, cfg.vocab_size, (1, 64))
+    with torch.no_grad():  # the routed experts are stored in bf16
+        a, b = model.eval()(ids)[0], other.eval()(ids)[0]
+    assert (a - b).norm() <= 2e-2 * a.norm()
