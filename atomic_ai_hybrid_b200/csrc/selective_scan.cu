@@ -30,7 +30,7 @@ AHB_DEVICE float dt_of(float raw, float lo, float hi) {
   return raw != raw ? 0.f : fminf(fmaxf(softplusf_(raw), lo), hi);
 }
 
-// ---------------------------------------------------------------- token form
+// ---------------------------------------------------------------- a few tokens per sequence, or fp32
 // One warp carries CH channels of one sequence through its tokens: lane l holds states
 // [l V, l V + V) of each channel in registers (N = 32 V), lanes 0..CH-1 also hold the convolution
 // window of one channel and turn its row into (decay, dt xc).
@@ -116,8 +116,137 @@ __global__ void __launch_bounds__(WARPS * 32) scan_token_kernel(ScanArgs p) {
   }
 }
 
+// ---------------------------------------------------------------- one token per sequence
+// Bound by the state's bytes, read once and written once.  A warp takes G groups of R channels of one
+// sequence; the next group's rows are on their way while one is worked on.  Lane c of the first R G turns
+// channel c's row into (decay, dt xc).
+
+// Sums v[0..R) over the warp; lane l gets the sum number `sum_index<R>(l)`: every step adds half of the values'
+// halves across lanes, so R sums take R - 1 + 5 - log2 R shuffles.
+template <int R>
+AHB_DEVICE float warp_sums(float (&v)[R]) {
+  const int lane = threadIdx.x & 31;
+  int w = 16;
+#pragma unroll
+  for (int r = R / 2; r >= 1; r /= 2, w /= 2) {
+    const bool hi = lane & w;
+#pragma unroll
+    for (int i = 0; i < r; ++i) {
+      const float give = hi ? v[i] : v[i + r], keep = hi ? v[i + r] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, w);
+    }
+  }
+#pragma unroll
+  for (; w >= 1; w /= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], w);
+  return v[0];
+}
+template <int R>
+AHB_DEVICE int sum_index(int lane) {
+  int at = 0, w = 16;
+#pragma unroll
+  for (int r = R / 2; r >= 1; r /= 2, w /= 2) at += lane & w ? r : 0;
+  return at;
+}
+
+template <int V> struct Floats;
+template <> struct Floats<4> { using type = float4; };
+template <> struct Floats<2> { using type = float2; };
+template <> struct Floats<1> { using type = float; };
+
+template <int V>
+AHB_DEVICE void load_states(float (&h)[V], const float* p) {
+  const auto r = __ldcs(reinterpret_cast<const typename Floats<V>::type*>(p));
+#pragma unroll
+  for (int i = 0; i < V; ++i) h[i] = reinterpret_cast<const float*>(&r)[i];
+}
+template <int V>
+AHB_DEVICE void store_states(float* p, const float (&h)[V]) {
+  typename Floats<V>::type r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) reinterpret_cast<float*>(&r)[i] = h[i];
+  __stcs(reinterpret_cast<typename Floats<V>::type*>(p), r);
+}
+
+template <typename T, typename W, int N, int R, int G>
+__global__ void __launch_bounds__(128) scan_step_kernel(ScanArgs p) {
+  constexpr int V = N / 32;
+  const int lane = threadIdx.x & 31, b = blockIdx.y;
+  const int c0 = (blockIdx.x * 4 + (threadIdx.x >> 5)) * R * G;
+  if (c0 >= p.C) return;
+  const int slot = seq_slot(p.slots, b, p.S), c = c0 + lane;
+  const bool mine = lane < R * G && c < p.C;
+  T* y = static_cast<T*>(p.y) + (int64_t)b * p.C;
+  if (slot < 0) {
+    if (mine) y[c] = from_f<T>(0.f);
+    return;
+  }
+  float* S0 = p.state + ((int64_t)slot * p.C + c0) * N + lane * V;
+  float h[2][R][V];
+  auto fetch = [&](int k) {
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+      if (c0 + k * R + j < p.C) load_states<V>(h[k & 1][j], S0 + (k * R + j) * N);
+  };
+  fetch(0);
+  float a = 0.f, u = 0.f;
+  if (mine) {
+    T* win = static_cast<T*>(p.conv_state) + (int64_t)slot * 3 * p.C + c;
+    float w[4];
+    load_taps(w, static_cast<const W*>(p.conv_w) + (int64_t)c * 4);
+    const float bias = p.conv_b ? p.conv_b[c] : 0.f, A = p.A[c / p.P];
+    const float x0 = to_f(win[0]), x1 = to_f(win[p.C]), x2 = to_f(win[2 * p.C]);
+    const T x = static_cast<const T*>(p.x)[(int64_t)b * p.xs + c];
+    const float dt = dt_of(to_f(static_cast<const T*>(p.dt)[(int64_t)b * p.dts + c]), p.dt_min, p.dt_max);
+    a = exp_decay(fmaxf(dt * A, kMinDA));
+    u = dt * sanitize(conv_silu(w, bias, x0, x1, x2, to_f(x)), kClip);
+    win[0] = from_f<T>(x1);
+    win[p.C] = from_f<T>(x2);
+    win[2 * p.C] = x;
+  }
+  float Bv[V], Cv[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    Bv[i] = sanitize(to_f(static_cast<const T*>(p.Bm)[(int64_t)b * p.bs + lane * V + i]), kClip);
+    Cv[i] = sanitize(to_f(static_cast<const T*>(p.Cm)[(int64_t)b * p.cs + lane * V + i]), kClip);
+  }
+#pragma unroll
+  for (int k = 0; k < G; ++k) {
+    if (k + 1 < G) fetch(k + 1);
+    float sum[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const float aj = __shfl_sync(0xffffffffu, a, k * R + j), uj = __shfl_sync(0xffffffffu, u, k * R + j);
+      sum[j] = 0.f;
+      if (c0 + k * R + j < p.C) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          h[k & 1][j][i] = fmaf(aj, h[k & 1][j][i], uj * Bv[i]);
+          sum[j] = fmaf(Cv[i], h[k & 1][j][i], sum[j]);
+        }
+        store_states<V>(S0 + (k * R + j) * N, h[k & 1][j]);
+      }
+    }
+    const float out = warp_sums<R>(sum);
+    const int at = c0 + k * R + sum_index<R>(lane);
+    if (lane % (32 / R) == 0 && at < p.C) y[at] = from_f<T>(out);
+  }
+}
+
+template <typename T, typename W, int N, int R, int G>
+void launch_step(const ScanArgs& p, cudaStream_t st) {
+  const dim3 grid((p.C + 4 * R * G - 1) / (4 * R * G), p.B);
+  scan_step_kernel<T, W, N, R, G><<<grid, 128, 0, st>>>(p);
+}
+
 template <typename T, typename W, int N>
 void launch_token(const ScanArgs& p, cudaStream_t st) {
+  if (p.cu == nullptr && p.L == 1) {
+    // 32 channels a warp use every lane and keep two groups of rows on their way; where that leaves an SM
+    // fewer than 8 warps, 8 channels a warp spread the loads
+    if ((int64_t)p.B * p.C < 32 * 8 * 148) launch_step<T, W, N, 8, 1>(p, st);
+    else launch_step<T, W, N, 1024 / N, N / 32>(p, st);
+    return;
+  }
   constexpr int CH = 8, WARPS = 4;
   const dim3 grid((p.C + CH * WARPS - 1) / (CH * WARPS), p.B);
   scan_token_kernel<T, W, N, CH, WARPS><<<grid, WARPS * 32, 0, st>>>(p);
