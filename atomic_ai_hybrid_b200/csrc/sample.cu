@@ -235,20 +235,28 @@ __global__ void __launch_bounds__(NT) sample_kernel(SampleArgs p, int ctas) {
   for (int b = tid; b < kBins; b += NT) hist[b] = 0;
   if (tid == 0) first_out = kBins;
   Part range = Part::none();
-  for (int v = v0 + tid; v < v1; v += 4 * NT) {
-    uint4 r[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (v + u * NT < v1) r[u] = fetch(v + u * NT);
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (v + u * NT < v1) {
-        X::clean(r[u]);
-        if (p.resident) keep[v + u * NT - v0] = r[u];
-        range.most = fmaxf(range.most, largest<T>(r[u]));
-        const float x = X::get(r[u], 0);  // one value a line is enough to size the bins
-        range.least = fminf(range.least, x == -INFINITY ? INFINITY : x);
-      }
+  auto take = [&](uint4 r) {
+    range.most = fmaxf(range.most, largest<T>(r));
+    const float x = X::get(r, 0);  // one value a line is enough to size the bins
+    range.least = fminf(range.least, x == -INFINITY ? INFINITY : x);
+  };
+  if (p.resident) {  // all on their way at once; a thread reads only the lines it copied
+    for (int v = v0 + tid; v < v1; v += NT) {
+      const int i = v * N - skew;
+      if (i >= 0 && i + N <= p.V)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&keep[v - v0])), "l"(l + i) : "memory");
+      else
+        keep[v - v0] = fetch(v);
+    }
+    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+    for (int v = v0 + tid; v < v1; v += NT) {
+      uint4 r = keep[v - v0];
+      X::clean(r);
+      keep[v - v0] = r;
+      take(r);
+    }
+  } else {
+    for (int v = v0 + tid; v < v1; v += NT) take(line(v));
   }
   range = combine<RANGE, NT>(range, parts, turn ^= 1, rank, ctas);
   const float top = range.most;
