@@ -327,9 +327,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(SampleArgs p, int ctas) {
   const bool binned = by_rank || by_mass;
   Part best = Part::none();
   best_s = -INFINITY;
-  for (int v = v0 + tid; v < v1; v += NT) {
-    const uint4 r = line(v);
-    const int i0 = v * N - skew;
+  auto weigh = [&](const uint4& r, int i0) {
     float e[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) e[j] = ex2((X::get(r, j) - top) * c);
@@ -353,7 +351,16 @@ __global__ void __launch_bounds__(NT) sample_kernel(SampleArgs p, int ctas) {
 #pragma unroll
     for (int j = 1; j < N; ++j) e[0] += e[j];
     best.mass += e[0];
+  };
+  int v = v0 + tid;
+  for (; v + (U - 1) * NT < v1; v += U * NT) {  // several lines' arithmetic side by side
+    uint4 r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) r[u] = line(v + u * NT);
+#pragma unroll
+    for (int u = 0; u < U; ++u) weigh(r[u], (v + u * NT) * N - skew);
   }
+  for (; v < v1; v += NT) weigh(line(v), v * N - skew);
   if (!binned && !greedy)
     for (int v = v0 + tid; v < v1; v += U * NT) race_lines(v);
   auto leader = [&](Part& p) {
