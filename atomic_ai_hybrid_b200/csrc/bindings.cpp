@@ -4,6 +4,7 @@
 // without the framework.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include "launchers.h"
@@ -1645,6 +1646,12 @@ torch::Tensor ce_online_bwd(torch::Tensor h, torch::Tensor W, torch::Tensor labe
 }
 
 // ------------------------------------------------------------ serving
+// An output of a call that the host's own time bounds: straight from the caching allocator, without the
+// dispatcher (0.7 us less than torch::empty).
+torch::Tensor new_output(at::IntArrayRef size, at::ScalarType dt, const torch::Tensor& like) {
+  return at::detail::empty_cuda(size, dt, like.device(), c10::nullopt);
+}
+
 // (rows, channels) of packed or per-row tokens: unit channel stride, any row stride
 void check_rows(const torch::Tensor& t, const torch::Tensor& like, int64_t rows, int64_t cols, const char* op,
                 const char* name) {
@@ -1712,11 +1719,11 @@ torch::Tensor selective_scan(const torch::Tensor& x, const torch::Tensor& dt, co
   check_flat(conv_state, x, x.scalar_type(), S * 3 * C, op, "conv_state (slots, 3, channels)");
   const SeqArgs q = seq_args(x, T, L, S, cu, slots, op);
   const c10::cuda::CUDAGuard guard(x.device());
-  auto y = torch::empty({T, C}, x.options());
+  auto y = new_output({T, C}, x.scalar_type(), x);
   int64_t floats = 0;
   const int seg = ahb_selective_scan_plan(q.B, q.L, (int)T, (int)C, (int)N, q.cu != nullptr, dt_code(x), &floats);
   torch::Tensor work;
-  if (floats > 0) work = torch::empty({floats}, state.options());
+  if (floats > 0) work = new_output({floats}, at::kFloat, x);
   const int rc = ahb_selective_scan(x.data_ptr(), x.stride(0), dt.data_ptr(), dt.stride(0), A.data_ptr<float>(),
                                     Bm.data_ptr(), Bm.stride(0), Cm.data_ptr(), Cm.stride(0), conv_w.data_ptr(),
                                     dt_code(conv_w), opt_ptr(conv_b), conv_state.data_ptr(), state.data_ptr<float>(),
@@ -1763,7 +1770,7 @@ torch::Tensor gdn2_recurrent(const std::vector<torch::Tensor>& in, const std::ve
   check_flat(conv_state, x, x.scalar_type(), S * 9 * d, op, "conv_state (slots, 3, 3, channels)");
   const SeqArgs q = seq_args(x, T, L, S, cu, slots, op);
   const c10::cuda::CUDAGuard guard(x.device());
-  auto y = torch::empty({T, d}, x.options());
+  auto y = new_output({T, d}, x.scalar_type(), x);
   const int rc = ahb_gdn_recurrent(ip, rs, wp, dt_code(conv_w[0]), bp, decay_a.data_ptr<float>(), conv_state.data_ptr(),
                                    state.data_ptr<float>(), q.cu, q.slots, y.data_ptr(), q.B, q.L, (int)T, (int)H,
                                    (int)D, (int)S, dt_code(x), cur_stream());
@@ -1790,8 +1797,8 @@ std::tuple<torch::Tensor, torch::Tensor> sample(const torch::Tensor& logits, con
   check_flat(top_p, logits, at::kFloat, B, op, "top_p");
   check_flat(min_p, logits, at::kFloat, B, op, "min_p");
   const c10::cuda::CUDAGuard guard(logits.device());
-  auto tokens = torch::empty({B}, logits.options().dtype(at::kLong));
-  auto logprobs = torch::empty({B}, logits.options().dtype(at::kFloat));
+  auto tokens = new_output({B}, at::kLong, logits);
+  auto logprobs = new_output({B}, at::kFloat, logits);
   const int rc = ahb_sample(logits.data_ptr(), logits.stride(0), dt_code(logits), noise.data_ptr<float>(),
                             noise.stride(0), temperature.data_ptr<float>(), top_k.data_ptr<int>(),
                             top_p.data_ptr<float>(), min_p.data_ptr<float>(), tokens.data_ptr<int64_t>(),
