@@ -43,7 +43,7 @@ struct SampleArgs {
 };
 
 constexpr int kBins = 512, kMaxCtas = 8;
-constexpr float kBinsPerLog2 = 12.f;  // bins of 6 % in probability over the top 2^-42; finer for a flatter row
+constexpr float kBinsPerLog2 = 24.f;  // bins of 6 % in probability over the top 2^-42; finer for a flatter row
 constexpr float kSlack = 1e-5f;       // rounding of the fp32 mass sums
 
 // What the threads of a cluster bring together: the race's leader as an ordered key (score, then lowest
