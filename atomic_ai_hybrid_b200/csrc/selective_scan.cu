@@ -273,8 +273,10 @@ struct PromptArgs {
   ScanArgs a;
   int seg;        // tokens per segment, a multiple of 32
   int segments;   // that `states` and `decays` have room for
+  int blocks;     // that `rows` has room for
   float* states;  // (segments, C, N): the segments' own end states, then their start states
   float* decays;  // (segments, C): log2 of a segment's decay
+  __nv_bfloat16* rows;  // (blocks, BlockRows<N>): what all channels share of a block
 };
 
 constexpr float kSpan = 86.f, kLog2e = 1.4426950408889634f;
@@ -324,6 +326,17 @@ AHB_DEVICE Segment find_segment(const ScanArgs& p, int seg, int id) {
   return r;
 }
 
+// Blocks of 32 tokens in the sequences before b.  Every warp counts by itself.
+AHB_DEVICE int blocks_before(const ScanArgs& p, int b) {
+  if (p.cu == nullptr) return b * ((p.L + 31) / 32);
+  int n = 0;
+  for (int o = threadIdx.x & 31; o < b; o += 32) {
+    const SeqRange q = seq_range(p.cu, o, p.L, p.T);
+    n += (q.end - q.start + 31) / 32;
+  }
+  return __reduce_add_sync(0xffffffffu, n);
+}
+
 // log(1 + e^x) to about 2^-22: max(x, 0) + log1p(z) with z = e^{-|x|}, log1p(z) = 2 atanh(z / (2 + z)) as
 // its power series (the argument is at most 1/3; the first term left out is below 2e-7 of the sum)
 AHB_DEVICE float2 softplus2(float2 x) {
@@ -349,15 +362,6 @@ AHB_DEVICE uint32_t clip2(uint32_t x) {
   const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&x);
   const __nv_bfloat162 c = __hmin2(__hmax2(v, __floats2bfloat162_rn(-kClip, -kClip)), __floats2bfloat162_rn(kClip, kClip));
   return __heq2_mask(v, v) & *reinterpret_cast<const uint32_t*>(&c);
-}
-
-// whether eight bf16 are all within +-1000 (false for NaN)
-AHB_DEVICE bool within(const uint4& r) {
-  const uint32_t a[4] = {r.x & 0x7fff7fffu, r.y & 0x7fff7fffu, r.z & 0x7fff7fffu, r.w & 0x7fff7fffu};
-  __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162*>(&a[0]);
-#pragma unroll
-  for (int j = 1; j < 4; ++j) m = __hmax2_nan(m, *reinterpret_cast<const __nv_bfloat162*>(&a[j]));
-  return __hble2(m, __floats2bfloat162_rn(kClip, kClip));
 }
 
 AHB_DEVICE float lo16(uint32_t x) { return __uint_as_float(x << 16); }
@@ -397,13 +401,74 @@ AHB_DEVICE void store_pair(bf16* row, int c, int C, bool pairs, uint32_t v) {
 // latencies: 12 warps with whole states were issuing 42 % of the time).
 constexpr int kBlock = 32, kGroups = 4, kWarps = 2 * kGroups, kChan = 16 * kGroups;
 
+// A block's rows of B and C, clipped, zeros past the sequence's end, and C B^T up to the diagonal in two bf16
+// terms: made once (scan_rows_kernel), read by every group of channels.
+template <int N>
+struct BlockRows {
+  bf16 b[kBlock][N], c[kBlock][N], cb[2][kBlock][kBlock];
+};
+
+template <int N>
+__global__ void __launch_bounds__(192) scan_rows_kernel(PromptArgs pa) {
+  constexpr int LD = N + 8;
+  __shared__ bf16 sb[kBlock][LD], sc[kBlock][LD];
+  const ScanArgs& p = pa.a;
+  const Segment sg = find_segment(p, kBlock, blockIdx.x);
+  if (sg.b < 0) return;
+  BlockRows<N>& out = reinterpret_cast<BlockRows<N>*>(pa.rows)[blockIdx.x];
+  const int tid = threadIdx.x, t0 = sg.seq.start + sg.index * kBlock;
+  const bool wide = ((p.bs | p.cs) & 7) == 0 && ((reinterpret_cast<uintptr_t>(p.Bm) | reinterpret_cast<uintptr_t>(p.Cm)) & 15) == 0;
+  for (int piece = tid; piece < kBlock * N / 8; piece += 192) {
+    const int row = piece / (N / 8), col = piece % (N / 8) * 8;
+    uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if (t0 + row < sg.seq.end) {
+      const bf16* from[2] = {static_cast<const bf16*>(p.Bm) + (int64_t)(t0 + row) * p.bs + col,
+                             static_cast<const bf16*>(p.Cm) + (int64_t)(t0 + row) * p.cs + col};
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        if (wide) {
+          v[m] = __ldg(reinterpret_cast<const uint4*>(from[m]));
+        } else {
+          const uint16_t* f = reinterpret_cast<const uint16_t*>(from[m]);
+          v[m] = make_uint4(f[0] | (uint32_t)f[1] << 16, f[2] | (uint32_t)f[3] << 16, f[4] | (uint32_t)f[5] << 16, f[6] | (uint32_t)f[7] << 16);
+        }
+        v[m] = make_uint4(clip2(v[m].x), clip2(v[m].y), clip2(v[m].z), clip2(v[m].w));
+      }
+    }
+    *reinterpret_cast<uint4*>(&sb[row][col]) = *reinterpret_cast<uint4*>(&out.b[row][col]) = v[0];
+    *reinterpret_cast<uint4*>(&sc[row][col]) = *reinterpret_cast<uint4*>(&out.c[row][col]) = v[1];
+  }
+  __syncthreads();
+  // one warp each: 16 x 8 pieces of (0,0), (16,0), (16,16); nothing reads the fourth quarter
+  const int lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+  const int tb = warp < 2 ? 0 : 16, cb = (warp < 4 ? 0 : 16) + (warp & 1) * 8;
+  float acc[2][4];
+  zero_acc<2>(acc);
+#pragma unroll
+  for (int k = 0; k < N; k += 32) {
+    uint32_t a[4], b[4];
+    ldsm4(b, &sb[cb + (lane & 7)][k + (lane >> 3) * 8]);
+    ldsm4(a, &sc[tb + (lane & 15)][k + (lane >> 4) * 8]);
+    mma16816(acc[0], a, b);
+    ldsm4(a, &sc[tb + (lane & 15)][k + 16 + (lane >> 4) * 8]);
+    mma16816(acc[1], a, b + 2);
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int t = tb + g + 8 * h, c = cb + 2 * q;
+    float2 v = make_float2(c <= t ? acc[0][2 * h] + acc[1][2 * h] : 0.f, c + 1 <= t ? acc[0][2 * h + 1] + acc[1][2 * h + 1] : 0.f);
+    *reinterpret_cast<uint32_t*>(&out.cb[0][t][c]) = term2(v);
+    *reinterpret_cast<uint32_t*>(&out.cb[1][t][c]) = pack2(v.x, v.y);
+  }
+}
+
 template <int N>
 struct BlockSmem {
   static constexpr int LD = N + 8;    // row strides that spread ldmatrix rows over the banks
   static constexpr int LT = kBlock + 4, LV = kBlock + 8;
   bf16 b[2][kBlock][LD];
   bf16 c[2][kBlock][LD];
-  bf16 cb[2][kBlock][LV];             // C B^T below the diagonal: high and low terms
+  bf16 cb[2][2][kBlock][LV];          // C B^T up to the diagonal: high and low terms
   bf16 v[kGroups][3][16][LV];         // the terms of V per channel and token
   float y[kGroups][2][16][LT];        // both warps' parts of the outputs
   float u[kGroups][16][LT];           // a group's inputs and decays where it goes token by token
@@ -426,8 +491,8 @@ AHB_DEVICE void scale_rows(float (*S)[4], float f) {
   }
 }
 
-// FAST: 4-byte access to channel pairs, 16-byte access to rows of B and C, whole groups of 16 channels
-// (the other form takes any alignment, stride and number of channels).
+// FAST: 4-byte access to channel pairs, whole groups of 16 channels (the other form takes any alignment,
+// stride and number of channels).
 template <typename W, int N, bool STATE, bool FAST>
 __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs pa) {
   constexpr int M = N / 2, NT = M / 8;      // this warp's states, their accumulator tiles
@@ -488,38 +553,23 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs p
     }
   }
 
-  // block rows of B and C: every thread copies, and later clips, the same 16-byte pieces
-  constexpr int ALL = kBlock * N / 8, PIECES = (ALL + kWarps * 32 - 1) / (kWarps * 32), STEP = kWarps * 32 / (N / 8);
-  const int prow = tid / (N / 8), pcol = tid % (N / 8) * 8;  // piece m: row prow + m STEP
-  auto copy_rows = [&](const void* from, int64_t stride, bf16 (*to)[Smem::LD], int t0) {
-    const bf16* src = static_cast<const bf16*>(from) + (int64_t)(t0 + prow) * stride + pcol;
+  const int block0 = blocks_before(p, sg.b) + sg.index * (pa.seg / kBlock);
+  if (block0 + (end - start + kBlock - 1) / kBlock > pa.blocks) return;  // offsets that overlap
+  auto copy_block = [&](int block, int buf) {
+    const BlockRows<N>& from = reinterpret_cast<const BlockRows<N>*>(pa.rows)[block];
+    auto copy = [&](bf16* to, const bf16* f) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(f) : "memory");
+    };
 #pragma unroll
-    for (int m = 0; m < PIECES; ++m, src += STEP * stride) {
-      const int row = prow + m * STEP;
-      if (ALL % (kWarps * 32) != 0 && row >= kBlock) break;
-      if (t0 + row >= end) {
-        *reinterpret_cast<uint4*>(&to[row][pcol]) = make_uint4(0, 0, 0, 0);
-      } else if (FAST) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(&to[row][pcol])), "l"(src) : "memory");
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) to[row][pcol + k] = src[k];
-      }
+    for (int piece = tid; piece < kBlock * N / 8; piece += kWarps * 32) {
+      const int row = piece / (N / 8), col = piece % (N / 8) * 8;
+      copy(&sm.b[buf][row][col], &from.b[row][col]);
+      if (!STATE) copy(&sm.c[buf][row][col], &from.c[row][col]);
     }
-  };
-  auto clip_rows = [&](bf16 (*rows)[Smem::LD]) {
-#pragma unroll
-    for (int m = 0; m < PIECES; ++m) {
-      const int row = prow + m * STEP;
-      if (ALL % (kWarps * 32) != 0 && row >= kBlock) break;
-      uint4* at = reinterpret_cast<uint4*>(&rows[row][pcol]);
-      const uint4 r = *at;
-      if (!within(r)) *at = make_uint4(clip2(r.x), clip2(r.y), clip2(r.z), clip2(r.w));
+    if (!STATE) {
+      const int m = tid >> 7, row = (tid >> 2) & 31, col = (tid & 3) * 8;  // 2 x 32 x 4 pieces, one a thread
+      copy(&sm.cb[buf][m][row][col], &from.cb[m][row][col]);
     }
-  };
-  auto copy_block = [&](int t0, int buf) {
-    copy_rows(p.Bm, p.bs, sm.b[buf], t0);
-    if (!STATE) copy_rows(p.Cm, p.cs, sm.c[buf], t0);
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   // this lane's tokens; lanes of the warp's first tokens also hold the three rows before them
@@ -555,7 +605,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs p
     }
   };
 
-  copy_block(start, 0);
+  copy_block(block0, 0);
   load_tokens(start);
   float pend = 0.f, total = 0.f;  // of channel lane % 16: log2 of the scale S still lacks, of the segment's decay
   int buf = 0;
@@ -640,10 +690,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs p
       }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    clip_rows(sm.b[buf]);
-    if (!STATE) clip_rows(sm.c[buf]);
-    __syncthreads();  // the block's rows, V and spans are there; every warp is done with the other buffer and with cb
-    if (t0 + kBlock < end) copy_block(t0 + kBlock, buf ^ 1);
+    __syncthreads();  // the block's rows are there, and V; every warp is done with the other buffer
+    if (t0 + kBlock < end) copy_block(block0 + (t0 - start) / kBlock + 1, buf ^ 1);
     total += mid + tail;
     // S takes the scale it lacks and goes to the block's reference.  S itself may stand at 2^kSpan, so the two
     // scales go in one after the other where their product would leave the floats' range.
@@ -656,31 +704,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs p
 
     const int mrow = lane & 15, mcol = (lane >> 4) * 8;  // ldmatrix: rows of a 16 x 16 piece, its column half
     const int xrow = (lane & 7) + (lane >> 4) * 8, xcol = ((lane >> 3) & 1) * 8;  // two 8-row halves, each with both column halves
-    if (!STATE) {
-      // C B^T in 16 x 8 pieces of (0,0), (16,0), (16,16) by warps 0 to 5
-      if (warp < 6) {
-        const int tb = warp < 2 ? 0 : 16, sb = (warp < 4 ? 0 : 16) + (warp & 1) * 8;
-        float acc[2][4];  // even and odd k apart: half the chain of dependent products
-        zero_acc<2>(acc);
-#pragma unroll
-        for (int k = 0; k < N; k += 32) {
-          uint32_t a[4], b[4];
-          ldsm4(b, &sm.b[buf][sb + (lane & 7)][k + (lane >> 3) * 8]);
-          ldsm4(a, &sm.c[buf][tb + mrow][k + mcol]);
-          mma16816(acc[0], a, b);
-          ldsm4(a, &sm.c[buf][tb + mrow][k + 16 + mcol]);
-          mma16816(acc[1], a, b + 2);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int t = tb + g + 8 * h, s = sb + 2 * q;
-          float2 v = make_float2(s <= t ? acc[0][2 * h] + acc[1][2 * h] : 0.f, s + 1 <= t ? acc[0][2 * h + 1] + acc[1][2 * h + 1] : 0.f);
-          *reinterpret_cast<uint32_t*>(&sm.cb[0][t][s]) = term2(v);
-          *reinterpret_cast<uint32_t*>(&sm.cb[1][t][s]) = pack2(v.x, v.y);
-        }
-      }
-      __syncthreads();
-    }
 
     // A product waits for the one before it on the same accumulators, so consecutive ones go to different ones.
     float Y[4][4];
@@ -713,8 +736,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs p
           if (half == 0 || ks == 0) {
             const int tb = half == 0 ? 16 * ks : 16;
             uint32_t bh[4], bl[4];
-            ldsm4(bh, &sm.cb[0][tb + xrow][16 * ks + xcol]);
-            ldsm4(bl, &sm.cb[1][tb + xrow][16 * ks + xcol]);
+            ldsm4(bh, &sm.cb[buf][0][tb + xrow][16 * ks + xcol]);
+            ldsm4(bl, &sm.cb[buf][1][tb + xrow][16 * ks + xcol]);
             if (tb == 0) {
 #pragma unroll
               for (int m = 0; m < 3; ++m)
@@ -875,9 +898,12 @@ int launch_prompt(const ScanArgs& a, int seg, float* work, cudaStream_t st) {
       return -3;
     ready[dev] = true;
   }
-  const int64_t segs = max_segments(a.B, a.L, a.T, a.cu != nullptr, seg);
-  const PromptArgs p{a, seg, (int)segs, work, work + segs * a.C * N};
+  const bool packed = a.cu != nullptr;
+  const int64_t segs = max_segments(a.B, a.L, a.T, packed, seg), blocks = max_segments(a.B, a.L, a.T, packed, kBlock);
+  float* const states = work + blocks * (int64_t)(sizeof(BlockRows<N>) / 4);
+  const PromptArgs p{a, seg, (int)segs, (int)blocks, states, states + segs * a.C * N, reinterpret_cast<bf16*>(work)};
   const dim3 grid((unsigned)segs, (unsigned)((a.C + kChan - 1) / kChan));
+  scan_rows_kernel<N><<<(unsigned)blocks, 192, 0, st>>>(p);
   if (segs > a.B) {
     scan_block_kernel<W, N, true, FAST><<<grid, kWarps * 32, bytes, st>>>(p);
     scan_join_kernel<N><<<dim3((unsigned)(((int64_t)a.C * (N / 4) + 255) / 256), (unsigned)a.B), 256, 0, st>>>(p);
@@ -889,8 +915,7 @@ int launch_prompt(const ScanArgs& a, int seg, float* work, cudaStream_t st) {
 template <typename W, int N>
 int launch_prompt(const ScanArgs& a, int seg, float* work, cudaStream_t st) {
   const auto low = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
-  const bool fast = a.C % 16 == 0 && ((a.xs | a.dts) & 1) == 0 && ((a.bs | a.cs) & 7) == 0 &&
-                    ((low(a.x) | low(a.dt) | low(a.conv_state)) & 3) == 0 && ((low(a.Bm) | low(a.Cm)) & 15) == 0;
+  const bool fast = a.C % 16 == 0 && ((a.xs | a.dts) & 1) == 0 && ((low(a.x) | low(a.dt) | low(a.conv_state)) & 3) == 0;
   return fast ? launch_prompt<W, N, true>(a, seg, work, st) : launch_prompt<W, N, false>(a, seg, work, st);
 }
 
@@ -922,7 +947,8 @@ int ahb_selective_scan_plan(int B, int L, int T, int C, int N, int packed, int d
   int64_t seg = packed ? T * groups / wave : (L + std::max<int64_t>(1, wave / (B * groups)) - 1) / std::max<int64_t>(1, wave / (B * groups));
   seg = std::min<int64_t>(1 << 30, std::max<int64_t>(128, (seg + kBlock - 1) / kBlock * kBlock));
   const int64_t segs = max_segments(B, L, T, packed != 0, (int)seg);
-  if (segs > B) *floats = segs * C * (N + 1);
+  const int64_t rows = (int64_t)(2 * kBlock * N + 2 * kBlock * kBlock) / 2;  // of a block, in floats
+  *floats = max_segments(B, L, T, packed != 0, kBlock) * rows + (segs > B ? segs * C * (N + 1) : 0);
   return (int)seg;
 }
 
