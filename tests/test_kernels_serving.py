@@ -70,7 +70,7 @@ def test_scan_tokens(C, P, N, dtype):
     _check_scan(a, None)
 
 
-@pytest.mark.parametrize("lens", [[1], [2], [3], [15], [16], [17], [33], [0, 5, 0, 1, 70], [129, 64, 1, 255], [300], [1100, 3, 513]])
+@pytest.mark.parametrize("lens", [[1], [2], [3], [15], [16], [17], [33], [0, 5, 0, 1, 70], [129, 64, 1, 255], [300], [1100, 3, 513], [1, 2, 3, 0, 15, 16, 17, 31, 32, 33, 200]])
 @pytest.mark.parametrize("C,P,N,dtype", [(256, 64, 128, BF), (192, 192, 64, BF), (72, 8, 32, BF), (21, 7, 128, BF), (64, 64, 128, F32)])
 def test_scan_prompts(lens, C, P, N, dtype):
     a = _scan_inputs(lens, C, P, N, dtype, seed=sum(lens) + C)
