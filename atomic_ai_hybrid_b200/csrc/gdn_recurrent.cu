@@ -5,6 +5,7 @@
 //   beta = sigmoid(b), omega = sigmoid(w),  alpha = exp(max(-e^a softplus(f), -1e3))     per channel
 //   h <- diag(alpha) h;  n = omega v - (beta k)^T h;  h <- h + k n^T;  o = q^T h         h (D, D) per head
 #include "launchers.h"
+#include "packed.cuh"
 #include "recurrent.cuh"
 
 namespace {
@@ -51,11 +52,14 @@ struct Channel {
   }
 };
 
-AHB_DEVICE float4 operator*(const float4& a, float b) { return make_float4(a.x * b, a.y * b, a.z * b, a.w * b); }
+AHB_DEVICE float2 lo2(const float4& v) { return make_float2(v.x, v.y); }
+AHB_DEVICE float2 hi2(const float4& v) { return make_float2(v.z, v.w); }
+AHB_DEVICE float4 join(float2 a, float2 b) { return make_float4(a.x, a.y, b.x, b.y); }
+AHB_DEVICE float4 operator*(const float4& a, float b) { return join(mul2(lo2(a), both(b)), mul2(hi2(a), both(b))); }
 AHB_DEVICE float4 fma4(float a, const float4& b, const float4& c) {
-  return make_float4(fmaf(a, b.x, c.x), fmaf(a, b.y, c.y), fmaf(a, b.z, c.z), fmaf(a, b.w, c.w));
+  return join(fma2(both(a), lo2(b), lo2(c)), fma2(both(a), hi2(b), hi2(c)));
 }
-AHB_DEVICE float4 operator+(const float4& a, const float4& b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
+AHB_DEVICE float4 operator+(const float4& a, const float4& b) { return join(add2(lo2(a), lo2(b)), add2(hi2(a), hi2(b))); }
 
 template <typename T>
 AHB_DEVICE void store4(T* p, const float4& v) {
@@ -206,15 +210,25 @@ __global__ void __launch_bounds__(2 * D, 2) gdn_tokens_kernel(GdnArgs p) {
   // threads below D: q, v and the write gate of channel c; the others: k, the erase gate and the decay
   const int half = tid / D, c = tid - half * D, ch = h * D + c, len = r.end - r.start;
   T* cs = static_cast<T*>(p.conv_state) + (int64_t)slot * 9 * d + ch;
-  Channel a, v;
-  a.template load<T, W>(p, half, ch, d, cs);
-  if (half == 0) v.template load<T, W>(p, 2, ch, d, cs);
-  const float rate = rate_of(p.decay_a[h]);
   auto in = [&](int e, int t) { return to_f(static_cast<const T*>(p.in[e])[(int64_t)(r.start + t) * p.rs[e] + ch]); };
+  // row t of convolution e, the window's for t < 0
+  auto seen = [&](int e, int t) { return t >= 0 ? in(e, t) : to_f(cs[(e * 3 + 3 + t) * d]); };
 
   float4 s[R], n = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int t0 = 0; t0 < len; t0 += TB) {
     const int cnt = min(TB, len - t0);
+    // the channel's parameters are read again every TB tokens rather than held beside the state
+    Channel a, v;
+    a.template load<T, W>(p, half, ch, d, cs);
+    if (half == 0) v.template load<T, W>(p, 2, ch, d, cs);
+    if (t0) {
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        a.win[j] = in(half, t0 - 3 + j);
+        if (half == 0) v.win[j] = in(2, t0 - 3 + j);
+      }
+    }
+    const float rate = rate_of(p.decay_a[h]);
     float qk[TB], gate[TB], other[TB];  // all on their way together; past the last token its values again
 #pragma unroll
     for (int t = 0; t < TB; ++t) {
@@ -307,10 +321,16 @@ __global__ void __launch_bounds__(2 * D, 2) gdn_tokens_kernel(GdnArgs p) {
   }
 #pragma unroll
   for (int i = 0; i < R; ++i) st[i * Q] = s[i];
+  float wa[3], wv3[3];
 #pragma unroll
   for (int j = 0; j < 3; ++j) {
-    cs[(half * 3 + j) * d] = from_f<T>(a.win[j]);
-    if (half == 0) cs[(6 + j) * d] = from_f<T>(v.win[j]);
+    wa[j] = seen(half, len - 3 + j);
+    wv3[j] = half == 0 ? seen(2, len - 3 + j) : 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < 3; ++j) {
+    cs[(half * 3 + j) * d] = from_f<T>(wa[j]);
+    if (half == 0) cs[(6 + j) * d] = from_f<T>(wv3[j]);
   }
 }
 
