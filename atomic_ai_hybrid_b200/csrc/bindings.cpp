@@ -1786,7 +1786,7 @@ std::tuple<torch::Tensor, torch::Tensor> sample(const torch::Tensor& logits, con
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.size(1) > 0, op,
               ": logits must be a CUDA tensor of (rows, vocabulary)");
   const int64_t B = logits.size(0), V = logits.size(1);
-  TORCH_CHECK(V < (1ll << 31) && B < (1ll << 31), op, ": sizes out of range");
+  TORCH_CHECK(V < (1ll << 30) && B < (1ll << 27), op, ": sizes out of range");
   check_rows(logits, logits, B, V, op, "logits");
   TORCH_CHECK(noise.device() == logits.device() && noise.scalar_type() == at::kFloat && noise.dim() == 2 &&
                   noise.size(0) == B && noise.size(1) == V && (noise.stride(1) == 1 || V == 1),

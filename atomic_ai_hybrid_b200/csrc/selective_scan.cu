@@ -270,13 +270,17 @@ void launch_token(const ScanArgs& p, cudaStream_t st) {
 // from the block's start, m = c after 16 tokens and E_t = c_t - m per channel p,
 //   Y[t,p]  = 2^{E_t} ( C_t . (2^m S) + sum_{s <= t} (C_t . B_s) V_s )       V_s = 2^{-E_s} u_s
 //   S'      = 2^{E_end} ( 2^m S + sum_s V_s B_s )
-// so one factor V serves the output and the state, and C B^T is shared by all channels.  The exponents
-// stay below 2^kSpan as long as neither half block decays by more; a warp whose channels do
-// takes its block token by token instead.  Both sums run on m16n8k16 bf16 products with fp32 accumulators:
+// so one factor V serves the output and the state, and C B^T is shared by all channels.  The factors
+// stay below 2^kSpan as long as neither half block decays by more: 2^76 times the largest u (2^10), C . B
+// (2^27) and 32 terms is far from the floats' end.  Channels that decay faster (over 3.3 nats a token on
+// average; none of 2.1 M channel-blocks at dt around 0.06 and A up to -16) take their block token by
+// token.  Both sums run on m16n8k16 bf16 products with fp32 accumulators:
 // a warp keeps the fp32 state of 16 channels as accumulators (channels are rows), which the next
 // block's C S product takes back as its left operand without leaving the registers.  B and C are bf16
 // already; the fp32 factors go in as bf16 terms: V in three (24 bits, the state loses nothing), S and
-// C B^T in two (2^-17, for outputs rounded to bf16).  tcgen05 would have the state in TMEM, where
+// C B^T in two (2^-17, for outputs rounded to bf16).  Sums of exponents up to
+// kSpan carry 2^-18 each: the state of a channel that loses 4 powers of two a token is good to about 3e-6, that of
+// the usual ones (under 0.5) to 3e-7.  tcgen05 would have the state in TMEM, where
 // rescaling it per channel and block costs a round trip through the registers it is spared here.
 //
 // Long sequences are cut into segments of `seg` tokens.  A first launch finds every segment's state from
@@ -292,7 +296,7 @@ struct PromptArgs {
   __nv_bfloat16* rows;  // (blocks, BlockRows<N>): what all channels share of a block
 };
 
-constexpr float kSpan = 86.f, kLog2e = 1.4426950408889634f;
+constexpr float kSpan = 76.f, kLog2e = 1.4426950408889634f;
 
 struct Segment { int b, first, count, index; SeqRange seq; };  // sequence, its first segment's number, its segments, which one
 
@@ -679,7 +683,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs p
     if (tg == 0) *reinterpret_cast<float2*>(&sm.span[grp][half][2 * i]) = whole;
     asm volatile("bar.sync %0, 64;" ::"r"(grp + 1) : "memory");  // the pair's spans are there
     const float mid = sm.span[grp][0][lane & 15], tail = sm.span[grp][1][lane & 15];
-    const bool heavy = __any_sync(0xffffffffu, fminf(mid, tail) < -kSpan);
+    const bool heavy = __any_sync(0xffffffffu, fmaxf(fabsf(mid), fabsf(tail)) > kSpan);
     if (heavy) {  // V would leave the floats' range: the group goes token by token, on these
       *reinterpret_cast<float4*>(&sm.u[grp][2 * i][tk]) = make_float4(u[0].x, u[1].x, u[2].x, u[3].x);
       *reinterpret_cast<float4*>(&sm.u[grp][2 * i + 1][tk]) = make_float4(u[0].y, u[1].y, u[2].y, u[3].y);
@@ -708,7 +712,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs p
     total += mid + tail;
     // S takes the scale it lacks and goes to the block's reference.  S itself may stand at 2^kSpan, so the two
     // scales go in one after the other where their product would leave the floats' range.
-    if (__any_sync(0xffffffffu, pend + mid < -120.f)) {
+    if (__any_sync(0xffffffffu, fabsf(pend + mid) > 120.f)) {
       scale_rows<NT>(S, ex2(pend));
       pend = 0.f;
     }

@@ -159,7 +159,7 @@ def selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, cu_seqle
     """Mamba2's short causal convolution and scan from and into a kept state; no gradient.
 
     ``x`` (the scan's input before the convolution) and ``dt`` (before softplus, its bias added)
-    have ``C`` channels in ``A.numel()`` heads, ``Bm`` and ``Cm`` have ``N`` states::
+    have ``C`` channels in ``A.numel()`` heads (``A`` negative), ``Bm`` and ``Cm`` have ``N`` states::
 
         xc_t = clip(silu(sum_j conv_w[:, j] x_{t-3+j} + conv_b), 1e3),  dt_t = clamp(softplus(dt_t), dt_min, dt_max)
         S_t  = e^{max(dt_t A, -20)} S_{t-1} + dt_t xc_t B_t^T,          y_t = S_t C_t

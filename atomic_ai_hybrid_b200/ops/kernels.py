@@ -906,6 +906,8 @@ def selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, cu_seqle
         return ext().selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, 1, cu_seqlens, slots, dt_min,
                                     dt_max)
     R.check_no_offsets(cu_seqlens)
+    if x.shape[1] == 0:
+        return torch.empty_like(x)
     y = ext().selective_scan(_flat_rows(x), _flat_rows(dt), A, _flat_rows(Bm), _flat_rows(Cm), conv_w, conv_b,
                              conv_state, state, x.shape[1], None, slots, dt_min, dt_max)
     return y.view(x.shape)
@@ -920,6 +922,8 @@ def gdn2_recurrent(q, k, v, b, w, f, conv_w, conv_b, decay_a, conv_state, state,
         return ext().gdn2_recurrent((q, k, v, b, w, f), conv_w, conv_b, decay_a, conv_state, state, 1, cu_seqlens,
                                     slots)
     R.check_no_offsets(cu_seqlens)
+    if q.shape[1] == 0:
+        return torch.empty_like(q)
     y = ext().gdn2_recurrent([_flat_rows(t) for t in (q, k, v, b, w, f)], conv_w, conv_b, decay_a, conv_state, state,
                              q.shape[1], None, slots)
     return y.view(q.shape)

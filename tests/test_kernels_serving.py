@@ -168,6 +168,25 @@ def test_scan_extreme_values(L):
     assert ((a["state"].double() - ref["state"]).abs()[a["slots"].long()][0, 0, small] <= REL * 1e4).all()
 
 
+@pytest.mark.parametrize("A", [-0.05, -3.0, -5.0])
+def test_scan_largest_values(A):
+    """Every input at its clip, decays on both sides of the change from blocks to single tokens (A dt = 3.3 a token):
+    nothing overflows, and errors stay in proportion to the sums of absolute values."""
+    L = 90
+    a = _scan_inputs([L], 64, 64, 128, BF, seed=6)
+    sign = lambda t, s: torch.where(torch.rand(t.shape, generator=_gen(s), device=dev) < 0.5, -1.0, 1.0).to(BF)  # noqa: E731
+    a["x"], a["dt"] = sign(a["x"], 1) * 1e30, torch.full_like(a["dt"], 60.0)
+    a["Bm"], a["Cm"], a["A"][:] = sign(a["Bm"], 2) * 1e4, sign(a["Cm"], 3) * 1e4, A
+    ref = {k: _d(v) for k, v in a.items()}
+    ref["conv_state"], ref["state"] = ref["conv_state"].clone(), ref["state"].clone()
+    y64 = R.selective_scan(**ref, cu_seqlens=_cu([L]))
+    y = ops.selective_scan(**a, cu_seqlens=_cu([L]))
+    most = 1e6 / -math.expm1(A)  # of a state
+    assert torch.isfinite(y).all()
+    assert ((a["state"].double() - ref["state"]).abs() <= REL * most).all()
+    assert ((y.double() - y64).abs() <= 2.0 ** -8 * y64.abs() + REL * most * 128e3).all()
+
+
 def test_scan_bad_offsets_stay_in_bounds():
     """Offsets outside the rows or in the wrong order never reach outside the buffers."""
     lens = [20, 30]
@@ -190,6 +209,8 @@ def test_scan_on_another_stream_and_empty():
     torch.cuda.current_stream().wait_stream(s)
     e = _scan_inputs([0], 128, 64, 64, BF)
     assert ops.selective_scan(**e, cu_seqlens=_cu([0])).shape == (0, 128)
+    rows = {k: v.unflatten(0, (2, 0)) if k in ("x", "dt", "Bm", "Cm") else v for k, v in _scan_inputs([0, 0], 128, 64, 64, BF).items()}
+    assert ops.selective_scan(**rows).shape == (2, 0, 128)
 
 
 def test_scan_refusals():
