@@ -22,10 +22,13 @@ from ..parallel.tp import get_tp
 
 _SERVING = None
 
-# GDN-2 prompts from this length run on the chunked scan (one launch per 64 tokens and head is in flight at
-# once); shorter ones cost less token by token: 8 tokens take 14 us there, the chunked path's
-# padding, convolutions and two scan launches over 100 us.
-GDN_CHUNKED_FROM = 64
+# GDN-2 prompts of at least this many tokens, in at most this many (sequence, head) pairs, run on the chunked
+# training scan.  It runs a head's chunks side by side, but each call pays 0.9 ms of separate launches for padding,
+# convolutions and gates; token by token a head takes 1.3 us a token on an SM of its own.  Whole mixer of
+# 16 heads of 128, chunked against token by token: 1 sequence of 512 tokens 1.20 and 0.94 ms, 768 1.21 and 1.27,
+# 4096 1.8 and 5.7; 4 sequences of 768 1.50 and 1.40, 1024 1.65 and 1.75, 4096 4.4 and 6.3; 6 of 1024 2.06 and 1.84,
+# 4096 6.4 and 6.8; 32 of 1024 8.3 and 5.5.
+GDN_CHUNKED_FROM, GDN_CHUNKED_HEADS = 768, 64
 
 
 def get_serving():
@@ -121,7 +124,8 @@ class _Call:
     def gdn2(self, mod: GatedDeltaNet2, x: torch.Tensor) -> torch.Tensor:
         c = self.state.layers[mod]
         *ins, og = mod.projections(x)
-        if self.lens is not None and max(self.lens) >= GDN_CHUNKED_FROM and mod.d_head == 128 and ops.use_cuda(x):
+        if (self.lens is not None and max(self.lens) >= GDN_CHUNKED_FROM and len(self.lens) * mod.n_heads <= GDN_CHUNKED_HEADS
+                and mod.d_head == 128 and ops.use_cuda(x)):
             o = self._gdn2_chunked(mod, c, ins)
         else:
             convs = [mod.q_conv_w, mod.k_conv_w, mod.v_conv_w], [mod.q_conv_b, mod.k_conv_b, mod.v_conv_b]
@@ -145,7 +149,7 @@ class _Call:
         return self._pad
 
     def _gdn2_chunked(self, mod, c, ins):
-        """Long prompts: the training kernels' convolution and chunked scan on padded rows, from and into the state."""
+        """Long prompts of few heads: the training kernels' convolution and chunked scan on padded rows, from and into the state."""
         row, has, n = self._padded()
         H, D = mod.n_heads, mod.d_head
         B, L = row.shape

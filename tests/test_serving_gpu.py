@@ -5,7 +5,7 @@ import torch
 
 from atomic_ai_hybrid_b200 import get_preset, ops
 from atomic_ai_hybrid_b200.models import HybridMoEModel
-from atomic_ai_hybrid_b200.serving import Generator
+from atomic_ai_hybrid_b200.serving import Generator, state
 
 pytestmark = pytest.mark.gpu
 dev = "cuda"
@@ -25,10 +25,12 @@ def _close(a, b, tol):
         ((a.float() - b.float()).norm() / b.float().norm()).item()
 
 
-def test_kept_state_equals_whole_sequences():
+@pytest.mark.parametrize("chunked_from", [64, 768])
+def test_kept_state_equals_whole_sequences(chunked_from, monkeypatch):
     """Against the training forward, whose scans multiply bf16 operands (2^-9 each, several in a row: up to 2e-2 a layer)
     where these keep fp32: 5e-2 of the logits' size over two layers.  Every expert is chosen for every token: a
     top-k choice that flips on a near tie is another output altogether."""
+    monkeypatch.setattr(state, "GDN_CHUNKED_FROM", chunked_from)
     model, cfg = _model(num_layers=2, n_routed_experts=2, num_experts=3)
     L = 192
     ids = torch.randint(0, cfg.vocab_size, (3, L), generator=torch.Generator().manual_seed(1)).to(dev)
@@ -42,7 +44,7 @@ def test_kept_state_equals_whole_sequences():
     for k in range(2):
         logits = gen.step(torch.stack([ids[i, n + k] for i, n in enumerate(lens)]), slots)
         _close(logits, torch.stack([want[i, n + k] for i, n in enumerate(lens)]), 5e-2)
-    # a conversation continued by a second prompt through the chunked scan
+    # a conversation continued by a second prompt (from 64 tokens on: through the chunked scan)
     logits = gen.prefill([ids[0, 102:180].tolist()], [4], fresh=False)
     _close(logits, want[0, 179:180], 5e-2)
 
