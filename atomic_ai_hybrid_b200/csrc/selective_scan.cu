@@ -282,15 +282,18 @@ void launch_token(const ScanArgs& p, cudaStream_t st) {
 // already; the fp32 factors go in as bf16 terms: V in three (24 bits, the state loses nothing), S and
 // C B^T in two (2^-17, for outputs rounded to bf16).  Sums of exponents up to
 // kSpan carry 2^-18 each: the state of a channel that loses 4 powers of two a token is good to about 3e-6, that of
-// the usual ones (under 0.5) to 3e-7.  tcgen05 would have the state in TMEM, where
-// rescaling it per channel and block costs a round trip through the registers it is spared here.
+// the usual ones (under 0.5) to 3e-7.  A form on tcgen05 with the state in TMEM as accumulator and as tf32 operand
+// was built and measured: its 22 products of 128 x 32 a block take about 60 cycles each, four times their
+// arithmetic (the left operand's read), and 128 channels a group meet the token-by-token case more
+// often: 416 us in place of 559 for 8 prompts of 2048 x 4096 channels, but 200 for 215, 104 for 98 on
+// ragged ones, and 32 for 12 on 16 tokens that decay fast; its outputs carry 2^-11 where these carry 2^-17.
 //
 // What all channels share, the clipped rows of B and C and C B^T, is made first (scan_rows_kernel; made by every
 // block of channels instead it costs 10 %).  Long sequences are cut into segments of `seg` tokens: a launch
 // finds every segment's state from zero and its decay, the next one hands the states on from segment to
 // segment (scan_join_kernel), and the last one runs the segments from their true states with outputs.
 //
-// One prompt of 8192 tokens, 2048 channels, 128 states: 220 us (17 ms token by token), 8 of 2048 tokens with
+// One prompt of 8192 tokens, 2048 channels, 128 states: 215 us (17 ms token by token), 8 of 2048 tokens with
 // 4096 channels: 559 us.  Neither HBM (8 %) nor the tensor pipe (38 %) is the end of it: 1.9 thousand
 // instructions for 16 channels of a block issue 47 % of the time at the 16 warps that 128 registers leave.
 struct PromptArgs {
@@ -969,9 +972,19 @@ int ahb_selective_scan_plan(int B, int L, int T, int C, int N, int packed, int d
   // 128 sequences: 123 and 190, 212 and 194, 395 and 203 us.
   if (dtype != AHB_BF16 || B == 0 || T < 16 * (int64_t)B) return 0;
   // Two blocks of 64 channels run on an SM.  Sequences that fill them stay whole (a segment more costs
-  // another state pass over it); others are cut so that one wave of blocks holds all segments.
+  // another state pass over it); others are cut so that one wave of blocks holds all segments.  Of several packed
+  // sequences the host knows the mean length: they are cut by their tokens' share of a wave, and at the mean
+  // where that is not much longer (4 of 512 tokens, 4096 channels: 84 us whole, 136 us cut at their share of 448).
   const int64_t groups = (C + kChan - 1) / kChan, wave = 2 * 148;
-  int64_t seg = packed ? T * groups / wave : (L + std::max<int64_t>(1, wave / (B * groups)) - 1) / std::max<int64_t>(1, wave / (B * groups));
+  int64_t seg;
+  if (packed && B > 1) {
+    const int64_t mean = (T + B - 1) / B;
+    seg = T * groups / wave;
+    if (4 * seg > 3 * mean) seg = std::max(seg, mean);
+  } else {
+    const int64_t n = packed ? T : L, cuts = std::max<int64_t>(1, wave / (B * groups));
+    seg = (n + cuts - 1) / cuts;
+  }
   seg = std::min<int64_t>(1 << 30, std::max<int64_t>(128, (seg + kBlock - 1) / kBlock * kBlock));
   const int64_t segs = max_segments(B, L, T, packed != 0, (int)seg);
   const int64_t rows = (int64_t)(2 * kBlock * N + 2 * kBlock * kBlock) / 2;  // of a block, in floats
