@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(SampleArgs p, int ctas) {
   __shared__ int wcnt[kBins / 32];
   __shared__ int first_out;
   const int tid = threadIdx.x, rank = (int)cluster_ctarank();
+  if (ctas > 1) cluster_arrive();  // this CTA has started: the others may write into its shared memory
   const int64_t row = blockIdx.x / ctas;
   const T* l = static_cast<const T*>(p.logits) + row * p.ls;
   const float* noise = p.noise + row * p.ns;
@@ -256,6 +257,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(SampleArgs p, int ctas) {
   } else {
     for (int v = v0 + tid; v < v1; v += NT) take(line(v));
   }
+  if (ctas > 1) cluster_wait();  // for the others' start, which the copy of the row has covered
   range = combine<RANGE, NT>(range, parts, turn ^= 1, rank, ctas);
   const float top = range.most;
   if (top == -INFINITY) {  // nothing can be drawn

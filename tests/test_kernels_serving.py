@@ -464,6 +464,16 @@ def test_sample_frequencies():
     assert ((count - n * q).abs() <= 5 * (n * q * (1 - q)).sqrt() + 1e-6).all()
 
 
+@pytest.mark.parametrize("B,V,dtype", [(1, 65537, BF), (5, 40001, F32), (37, 131073, BF), (40, 100003, F32), (150, 128257, BF)])
+def test_sample_clusters_start_together(B, V, dtype):
+    """Rows split over clusters of 2 to 8 CTAs whose parts differ in length, and calls one after another that leave no
+    SM idle between them: a CTA is written to by its cluster only once it runs, so every call gives the same."""
+    logits, noise = _logits(B, V, dtype, seed=V)
+    tokens = _check_sample(logits, noise, temperature=0.8, top_k=50, top_p=0.9)
+    again = [ops.sample(logits, noise, temperature=0.8, top_k=50, top_p=0.9) for _ in range(40)]
+    assert all(torch.equal(t, tokens) and torch.equal(lp, again[0][1]) for t, lp in again)
+
+
 def test_sample_refusals():
     logits, noise = _logits(3, 100, BF, seed=1)
 
