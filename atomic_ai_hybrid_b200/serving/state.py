@@ -16,6 +16,7 @@ import torch.nn.functional as F
 
 from .. import ops
 from ..models.mixers import MLA, GatedDeltaNet2, Mamba2
+from ..models.moe import MoE
 from ..ops import reference as R
 from ..parallel.cp import get_cp
 from ..parallel.tp import get_tp
@@ -44,6 +45,9 @@ class DecodeState:
     def __init__(self, model, slots: int, max_len: int = 0):
         if get_tp() is not None or get_cp() is not None:
             raise ValueError("serving runs on one rank's whole model: tensor and context parallelism are for training")
+        if any(isinstance(m, MoE) and m.ep_world > 1 for m in model.modules()):
+            raise ValueError("serving runs on one rank's whole model: this rank holds a part of the experts only, and every "
+                             "layer would wait for the other ranks")
         p = next(model.parameters())
         self.device, self.dtype, self.slots, self.max_len = p.device, model.compute_dtype, slots, max_len
         self.lengths = [0] * slots

@@ -178,3 +178,17 @@ def test_load_weights_from_a_training_checkpoint(tmp_path):
     with torch.no_grad():  # the routed experts are stored in bf16
         a, b = model.eval()(ids)[0], other.eval()(ids)[0]
     assert (a - b).norm() <= 2e-2 * a.norm()
+
+
+def test_expert_parallel_models_are_refused():
+    """A rank that holds some of the experts would wait for the others in every layer."""
+    from atomic_ai_hybrid_b200.parallel.context import ParallelContext, get_parallel_context, set_parallel_context
+
+    before = get_parallel_context()
+    set_parallel_context(ParallelContext(ep_world=2))
+    try:
+        model, _ = _model("tiny", num_layers=2, layer_types=("mamba2", "gdn2"))
+    finally:
+        set_parallel_context(before)
+    with pytest.raises(ValueError, match="experts"):
+        Generator(model, 1)
