@@ -28,7 +28,7 @@ from .. import ops
 from ..config import ModelConfig
 from ..ops import reference as R
 from ..parallel.context import dp_mean, get_parallel_context
-from .layers import Dense, lecun_normal_
+from .layers import Dense, lecun_normal_, serving_call
 
 ROUTER_LOGIT_CLIP = 8.0
 ROUTER_TEMP_INIT = 10.0
@@ -78,6 +78,11 @@ class MoE(nn.Module):
                     w._ahb_ep_local = True
 
     # ------------------------------------------------------------------ router
+    @staticmethod
+    def _over_ranks(t: torch.Tensor) -> torch.Tensor:
+        """A statistic's mean over the data-parallel ranks; its own in a serving call, which one rank makes alone."""
+        return dp_mean(t) if serving_call() is None else t
+
     def route(self, flat_x: torch.Tensor, stats: Dict[str, torch.Tensor]):
         E, k = self.E, self.k
         if ops.use_cuda(flat_x) and flat_x.dtype == torch.bfloat16:
@@ -110,7 +115,7 @@ class MoE(nn.Module):
             0, top_idx.reshape(-1), torch.ones(top_idx.numel(), device=flat_x.device, dtype=torch.float32))
         stats["assignment_frac"] = (counts / (flat_x.shape[0] * k)).detach()
         probs = torch.nan_to_num(torch.softmax(logits, -1), nan=0.0, posinf=0.0, neginf=0.0)
-        mean_probs = dp_mean(probs.mean(0))  # batch-global, as the reference's GSPMD mean
+        mean_probs = self._over_ranks(probs.mean(0))  # batch-global, as the reference's GSPMD mean
         stats["aux_loss"] = E * (mean_probs * mean_probs).sum()
         stats["z_loss"] = torch.logsumexp(logits, -1).square().mean()
         stats["expert_utilization"] = mean_probs.detach()
@@ -143,7 +148,7 @@ class MoE(nn.Module):
         stats["max_abs_logit_preclip"] = scal[1].detach()
         stats["min_col_norm"] = kern.square().sum(0).sqrt().min().detach()
         stats["assignment_frac"] = (counts / (T * k)).detach()
-        mean_probs = dp_mean(psum / T)  # batch-global, as the reference's GSPMD mean
+        mean_probs = self._over_ranks(psum / T)  # batch-global, as the reference's GSPMD mean
         stats["aux_loss"] = E * (mean_probs * mean_probs).sum()
         stats["z_loss"] = lse_sq.reshape(()) / T
         stats["expert_utilization"] = mean_probs.detach()

@@ -192,3 +192,21 @@ def test_expert_parallel_models_are_refused():
         set_parallel_context(before)
     with pytest.raises(ValueError, match="experts"):
         Generator(model, 1)
+
+
+def test_answering_takes_no_part_in_collectives(monkeypatch):
+    """One data-parallel rank may answer while the others do not: nothing of its forward is reduced over them."""
+    from atomic_ai_hybrid_b200.models import moe
+
+    model, cfg = _model("tiny", num_layers=2, layer_types=("mamba2", "gdn2"))
+    gen = Generator(model, 1)
+    want = gen.prefill([[1, 2, 3]], [0])
+
+    def reduced(t):
+        raise AssertionError("a collective in a serving call")
+
+    monkeypatch.setattr(moe, "dp_mean", reduced)
+    assert torch.equal(gen.prefill([[1, 2, 3]], [0]), want)
+    gen.step(torch.tensor([4]), [0])
+    with pytest.raises(AssertionError, match="a collective"):
+        model(torch.ones(1, 64, dtype=torch.long))
