@@ -1720,6 +1720,7 @@ torch::Tensor selective_scan(const torch::Tensor& x, const torch::Tensor& dt, co
   const SeqArgs q = seq_args(x, T, L, S, cu, slots, op);
   const c10::cuda::CUDAGuard guard(x.device());
   auto y = new_output({T, C}, x.scalar_type(), x);
+  if (q.B == 0) y.zero_();  // no sequence, and no kernel
   int64_t floats = 0;
   const int seg = ahb_selective_scan_plan(q.B, q.L, (int)T, (int)C, (int)N, q.cu != nullptr, dt_code(x), &floats);
   torch::Tensor work;
@@ -1771,6 +1772,7 @@ torch::Tensor gdn2_recurrent(const std::vector<torch::Tensor>& in, const std::ve
   const SeqArgs q = seq_args(x, T, L, S, cu, slots, op);
   const c10::cuda::CUDAGuard guard(x.device());
   auto y = new_output({T, d}, x.scalar_type(), x);
+  if (q.B == 0) y.zero_();  // no sequence, and no kernel
   const int rc = ahb_gdn_recurrent(ip, rs, wp, dt_code(conv_w[0]), bp, decay_a.data_ptr<float>(), conv_state.data_ptr(),
                                    state.data_ptr<float>(), q.cu, q.slots, y.data_ptr(), q.B, q.L, (int)T, (int)H,
                                    (int)D, (int)S, dt_code(x), cur_stream());

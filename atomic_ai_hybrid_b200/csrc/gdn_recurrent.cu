@@ -197,12 +197,17 @@ __global__ void __launch_bounds__(2 * D, 2) gdn_tokens_kernel(GdnArgs p) {
   const SeqRange r = seq_range(p.cu, b, p.L, p.T);
   const int slot = seq_slot(p.slots, b, p.S);
   T* y = static_cast<T*>(p.y) + h * D;
-  if (slot < 0) {
+  auto clear_open = [&] {  // last, when nothing of the recurrence is held: 0.4 us of 15 (0.5 to 2 us at other places)
+    if (p.cu == nullptr || tid >= D) return;
+    const OpenRows open(p.cu, p.B, p.T);
+    for (int i = b; i < open.count; i += p.B) y[(int64_t)open.row(i) * d + tid] = from_f<T>(0.f);
+  };
+  if (slot < 0 || r.start == r.end) {
     for (int t = r.start; t < r.end; ++t)
       if (tid < D) y[(int64_t)t * d + tid] = from_f<T>(0.f);
+    clear_open();
     return;
   }
-  if (r.start == r.end) return;
   const int g = tid / Q, m = tid % Q;
   float4* st = reinterpret_cast<float4*>(p.state + ((int64_t)slot * p.H + h) * D * D) + g * R * Q + m;
 #pragma unroll
@@ -335,6 +340,7 @@ __global__ void __launch_bounds__(2 * D, 2) gdn_tokens_kernel(GdnArgs p) {
     cs[(half * 3 + j) * d] = from_f<T>(wa[j]);
     if (half == 0) cs[(6 + j) * d] = from_f<T>(wv3[j]);
   }
+  clear_open();
 }
 
 template <typename T, typename W, int D>
@@ -349,11 +355,10 @@ int launch(const GdnArgs& p, cudaStream_t st) {
       return -3;
     ready[dev] = true;
   }
-  const dim3 grid(p.H, p.B);
   if (p.cu == nullptr && p.L == 1)
-    gdn_token_kernel<T, W, D><<<grid, 2 * D, bytes, st>>>(p);
+    gdn_token_kernel<T, W, D><<<dim3(p.H, p.B), 2 * D, bytes, st>>>(p);
   else
-    gdn_tokens_kernel<T, W, D><<<grid, 2 * D, bytes, st>>>(p);
+    gdn_tokens_kernel<T, W, D><<<dim3(p.H, p.B), 2 * D, bytes, st>>>(p);
   return 0;
 }
 

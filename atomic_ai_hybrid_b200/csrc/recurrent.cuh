@@ -14,6 +14,18 @@ AHB_DEVICE SeqRange seq_range(const int* cu, int b, int L, int T) {
   return {s, min(max(__ldg(cu + b + 1), s), T)};
 }
 
+// Rows that no sequence covers, [0, cu[0]) and [cu[B], T).  Every block of a call with offsets clears some of them, so
+// that no row of the output keeps what its memory held before.
+struct OpenRows {
+  int head, tail, count;
+  AHB_DEVICE OpenRows(const int* cu, int B, int T) {
+    head = min(max(__ldg(cu), 0), T);
+    tail = min(max(__ldg(cu + B), head), T);
+    count = head + T - tail;
+  }
+  AHB_DEVICE int row(int i) const { return i < head ? i : tail + i - head; }
+};
+
 // State slot of sequence b, -1 if it has none (a padding row): such rows give zeros, touch no state.
 AHB_DEVICE int seq_slot(const int* slots, int b, int S) {
   const int s = slots ? __ldg(slots + b) : b;

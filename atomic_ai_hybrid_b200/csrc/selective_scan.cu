@@ -66,6 +66,12 @@ template <typename T, typename W, int N, int CH, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32) scan_token_kernel(ScanArgs p) {
   constexpr int V = N / 32;
   const int lane = threadIdx.x & 31, b = blockIdx.y;
+  if (blockIdx.x * WARPS * CH >= p.C) {  // beside the channels, in calls with offsets
+    const OpenRows open(p.cu, p.B, p.T);
+    for (int i = b; i < open.count; i += p.B)
+      for (int c = threadIdx.x; c < p.C; c += WARPS * 32) static_cast<T*>(p.y)[(int64_t)open.row(i) * p.C + c] = from_f<T>(0.f);
+    return;
+  }
   const int c0 = (blockIdx.x * WARPS + (threadIdx.x >> 5)) * CH;
   if (c0 >= p.C) return;
   const SeqRange r = seq_range(p.cu, b, p.L, p.T);
@@ -263,7 +269,7 @@ void launch_token(const ScanArgs& p, cudaStream_t st) {
     return;
   }
   constexpr int CH = 8, WARPS = 4;
-  const dim3 grid((p.C + CH * WARPS - 1) / (CH * WARPS), p.B);
+  const dim3 grid((p.C + CH * WARPS - 1) / (CH * WARPS) + (p.cu != nullptr), p.B);
   scan_token_kernel<T, W, N, CH, WARPS><<<grid, WARPS * 32, 0, st>>>(p);
 }
 
@@ -299,8 +305,6 @@ void launch_token(const ScanArgs& p, cudaStream_t st) {
 struct PromptArgs {
   ScanArgs a;
   int seg;        // tokens per segment, a multiple of 32
-  int segments;   // that `states` and `decays` have room for
-  int blocks;     // that `rows` has room for
   float* states;  // (segments, C, N): the segments' own end states, then their start states
   float* decays;  // (segments, C): log2 of a segment's decay
   __nv_bfloat16* rows;  // (blocks, BlockRows<N>): what all channels share of a block
@@ -308,11 +312,36 @@ struct PromptArgs {
 
 constexpr float kSpan = 76.f, kLog2e = 1.4426950408889634f;
 
-struct Segment { int b, first, count, index; SeqRange seq; };  // sequence, its first segment's number, its segments, which one
+struct Segment {  // sequence, its first segment's number, its segments, which one, the blocks of 32 tokens before it
+  int b, first, count, index, blocks;
+  SeqRange seq;
+};
+
+AHB_DEVICE int offset_of(const ScanArgs& p, int b) { return min(max(__ldg(p.cu + b), 0), p.T); }
+
+// Sequences b0 + lane of packed rows.  A sequence starts at the largest offset up to its own (`reach`: up to b0, then
+// up to b0 + 32): where offsets fall it is empty, so all sequences together never have more than T tokens and their
+// segments and blocks fit their places.
+AHB_DEVICE SeqRange rising_ranges(const ScanArgs& p, int b0, int& reach) {
+  const int lane = threadIdx.x & 31;
+  int end = max(reach, b0 + lane < p.B ? offset_of(p, b0 + lane + 1) : 0);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, end, o);
+    if (lane >= o) end = max(end, v);
+  }
+  const int before = __shfl_up_sync(0xffffffffu, end, 1);
+  const SeqRange r{lane == 0 ? reach : before, end};
+  reach = __shfl_sync(0xffffffffu, end, 31);
+  return r;
+}
+AHB_DEVICE SeqRange range_of_lane(SeqRange q, int lane) {
+  return {__shfl_sync(0xffffffffu, q.start, lane), __shfl_sync(0xffffffffu, q.end, lane)};
+}
 
 // Segment number `id` over all sequences in order; b = -1 past the last.  Every warp looks by itself.
 AHB_DEVICE Segment find_segment(const ScanArgs& p, int seg, int id) {
-  Segment r{-1, 0, 0, 0, {0, 0}};
+  Segment r{-1, 0, 0, 0, 0, {0, 0}};
   if (p.cu == nullptr) {
     const int n = (p.L + seg - 1) / seg;
     if (n > 0 && id < n * p.B) {
@@ -320,18 +349,16 @@ AHB_DEVICE Segment find_segment(const ScanArgs& p, int seg, int id) {
       r.first = r.b * n;
       r.count = n;
       r.index = id - r.first;
+      r.blocks = r.b * ((p.L + 31) / 32);
       r.seq = seq_range(p.cu, r.b, p.L, p.T);
     }
     return r;
   }
   const int lane = threadIdx.x & 31;
-  int base = 0;
+  int base = 0, reach = offset_of(p, 0);
   for (int b0 = 0; b0 < p.B; b0 += 32) {
-    int n = 0;
-    if (b0 + lane < p.B) {
-      const SeqRange q = seq_range(p.cu, b0 + lane, p.L, p.T);
-      n = (q.end - q.start + seg - 1) / seg;
-    }
+    const SeqRange q = rising_ranges(p, b0, reach);
+    const int n = (q.end - q.start + seg - 1) / seg, blocks = (q.end - q.start + 31) / 32;
     int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -345,23 +372,14 @@ AHB_DEVICE Segment find_segment(const ScanArgs& p, int seg, int id) {
       r.count = __shfl_sync(0xffffffffu, n, src);
       r.first = base + __shfl_sync(0xffffffffu, incl, src) - r.count;
       r.index = id - r.first;
-      r.seq = seq_range(p.cu, r.b, p.L, p.T);
+      r.blocks += __reduce_add_sync(0xffffffffu, lane < src ? blocks : 0);
+      r.seq = range_of_lane(q, src);
       return r;
     }
     base += __shfl_sync(0xffffffffu, incl, 31);
+    r.blocks += __reduce_add_sync(0xffffffffu, blocks);
   }
   return r;
-}
-
-// Blocks of 32 tokens in the sequences before b.  Every warp counts by itself.
-AHB_DEVICE int blocks_before(const ScanArgs& p, int b) {
-  if (p.cu == nullptr) return b * ((p.L + 31) / 32);
-  int n = 0;
-  for (int o = threadIdx.x & 31; o < b; o += 32) {
-    const SeqRange q = seq_range(p.cu, o, p.L, p.T);
-    n += (q.end - q.start + 31) / 32;
-  }
-  return __reduce_add_sync(0xffffffffu, n);
 }
 
 // log(1 + e^x) to about 2^-22: max(x, 0) + log1p(z) with z = e^{-|x|}, log1p(z) = 2 atanh(z / (2 + z)) as
@@ -535,6 +553,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs p
   const int c1 = blockIdx.y * kChan + grp * 16, c0 = FAST ? min(c1, p.C - 16) : c1, ca = c0 + 2 * i;
   const bool mine = !FAST || c1 < p.C;
   const Segment sg = find_segment(p, pa.seg, blockIdx.x);
+  if (!STATE && p.cu != nullptr) {  // every block clears some of the rows without a sequence
+    const OpenRows open(p.cu, p.B, p.T);
+    const int c = blockIdx.y * kChan + 2 * lane;
+    for (int i = blockIdx.x * kWarps + warp; i < open.count; i += gridDim.x * kWarps)
+      store_pair(static_cast<bf16*>(p.y) + (int64_t)open.row(i) * p.C, c, p.C, FAST || (p.C & 1) == 0, 0u);
+  }
   if (sg.b < 0) return;
   if (STATE && sg.index == sg.count - 1) return;  // its end state comes with its outputs
   const int slot = seq_slot(p.slots, sg.b, p.S);
@@ -580,8 +604,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_block_kernel(PromptArgs p
     }
   }
 
-  const int block0 = blocks_before(p, sg.b) + sg.index * (pa.seg / kBlock);
-  if (block0 + (end - start + kBlock - 1) / kBlock > pa.blocks) return;  // offsets that overlap
+  const int block0 = sg.blocks + sg.index * (pa.seg / kBlock);
   auto copy_block = [&](int block, int buf) {
     const BlockRows<N>& from = reinterpret_cast<const BlockRows<N>*>(pa.rows)[block];
     auto copy = [&](bf16* to, const bf16* f) {
@@ -870,20 +893,20 @@ __global__ void __launch_bounds__(256) scan_join_kernel(PromptArgs pa) {
   const int b = blockIdx.y;
   const int slot = seq_slot(p.slots, b, p.S);
   if (slot < 0) return;
-  const SeqRange r = seq_range(p.cu, b, p.L, p.T);
-  const int count = (r.end - r.start + pa.seg - 1) / pa.seg;
-  if (count < 2) return;
-  int first = b * count;
+  SeqRange r = seq_range(nullptr, b, p.L, p.T);
+  int first = 0;
   if (p.cu != nullptr) {
     const int lane = threadIdx.x & 31;
-    first = 0;
-    for (int o = lane; o < b; o += 32) {
-      const SeqRange q = seq_range(p.cu, o, p.L, p.T);
-      first += (q.end - q.start + pa.seg - 1) / pa.seg;
+    int reach = offset_of(p, 0);
+    for (int b0 = 0; b0 <= b; b0 += 32) {
+      const SeqRange q = rising_ranges(p, b0, reach);
+      first += __reduce_add_sync(0xffffffffu, b0 + lane < b ? (q.end - q.start + pa.seg - 1) / pa.seg : 0);
+      r = range_of_lane(q, b & 31);
     }
-    first = __reduce_add_sync(0xffffffffu, first);
   }
-  if (first + count > pa.segments) return;  // offsets that overlap
+  const int count = (r.end - r.start + pa.seg - 1) / pa.seg;
+  if (p.cu == nullptr) first = b * count;
+  if (count < 2) return;
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= (int64_t)p.C * (N / 4)) return;
   const int c = (int)(at / (N / 4));
@@ -908,7 +931,8 @@ __global__ void __launch_bounds__(256) scan_join_kernel(PromptArgs pa) {
   }
 }
 
-// Segments of T tokens in B sequences: as many as any packing of them can have
+// Segments of T tokens in B sequences: as many as any packing of them can have (a sequence of l tokens has fewer than
+// l / seg + 1)
 int64_t max_segments(int B, int L, int T, bool packed, int seg) {
   return packed ? (int64_t)T / seg + B : (int64_t)B * ((L + seg - 1) / seg);
 }
@@ -928,7 +952,7 @@ int launch_prompt(const ScanArgs& a, int seg, float* work, cudaStream_t st) {
   const bool packed = a.cu != nullptr;
   const int64_t segs = max_segments(a.B, a.L, a.T, packed, seg), blocks = max_segments(a.B, a.L, a.T, packed, kBlock);
   float* const states = work + blocks * (int64_t)(sizeof(BlockRows<N>) / 4);
-  const PromptArgs p{a, seg, (int)segs, (int)blocks, states, states + segs * a.C * N, reinterpret_cast<bf16*>(work)};
+  const PromptArgs p{a, seg, states, states + segs * a.C * N, reinterpret_cast<bf16*>(work)};
   const dim3 grid((unsigned)segs, (unsigned)((a.C + kChan - 1) / kChan));
   scan_rows_kernel<N><<<(unsigned)blocks, 192, 0, st>>>(p);
   if (segs > a.B) {

@@ -165,7 +165,8 @@ def selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, cu_seqle
         S_t  = e^{max(dt_t A, -20)} S_{t-1} + dt_t xc_t B_t^T,          y_t = S_t C_t
 
     Tokens come as ``(T, C)`` rows packed by ``cu_seqlens`` (int32, ``sequences + 1`` offsets on the
-    device; sequences of any length, also none), as ``(B, L, C)``, or as ``(B, C)`` rows of one token
+    device, none below the one before; sequences of any length, also none; rows that none covers come out
+    as zeros), as ``(B, L, C)``, or as ``(B, C)`` rows of one token
     each.  ``conv_state (S, 3, C)`` holds the last three rows of ``x`` in its dtype and ``state
     (S, H, P, N)`` the fp32 scan state; both are updated in place.  Sequence ``i`` owns slot
     ``slots[i]`` (int32, all different; default ``i``); one with a slot outside ``[0, S)`` is padding:

@@ -200,6 +200,52 @@ def test_scan_bad_offsets_stay_in_bounds():
     assert torch.equal(a["state"][other], canary[other])
 
 
+def _poisoned(shape, dtype):
+    """Leaves NaN in the memory that the next output of this shape takes; returns its address."""
+    t = torch.full(shape, math.nan, device=dev, dtype=dtype)
+    return t.data_ptr()
+
+
+# offsets of 60 rows that leave rows uncovered at either end, in falling order, out of range, or have no sequence
+OPEN = [[0, 20, 50], [7, 20, 60], [3, 3, 40], [60, 60, 60], [0, 0, 0], [9], [40, 10, 50], [0, 50, 20], [50, 30, 10], [-5, 20, 9000]]
+
+
+@pytest.mark.parametrize("cu", OPEN)
+@pytest.mark.parametrize("form", ["blocks", "blocks of any width", "tokens"])
+def test_scan_rows_of_no_sequence_are_zero(cu, form):
+    T, C = 60, 21 if form == "blocks of any width" else 80
+    a = _scan_inputs([T // 2] * 2, C, C, 64, F32 if form == "tokens" else BF, seed=4)
+    a["slots"] = a["slots"][:len(cu) - 1].contiguous()
+    cu_dev = torch.tensor(cu, dtype=torch.int32, device=dev)
+    ref = {k: _d(v) for k, v in a.items()}
+    ref["conv_state"], ref["state"] = ref["conv_state"].clone(), ref["state"].clone()
+    want = R.selective_scan(**ref, cu_seqlens=cu_dev)
+    at = _poisoned(a["x"].shape, a["x"].dtype)
+    y = ops.selective_scan(**a, cu_seqlens=cu_dev)
+    assert y.data_ptr() == at and torch.isfinite(y).all()
+    if all(s <= e for s, e in zip(cu, cu[1:])):  # falling offsets promise finite values only
+        assert (y[(want == 0).all(1)] == 0).all()
+        assert (y.double() - want).abs().max() <= 2.0 ** -7 * want.abs().max()
+
+
+def test_scan_open_rows_beside_many_sequences():
+    """More rows than blocks that clear them, more sequences than a warp looks at together, cut and whole."""
+    for lens, T in (([1] * 70, 900), ([40, 0, 3] * 25, 9000), ([3000, 500], 12000)):
+        a = _scan_inputs([T], 64, 64, 32, BF, seed=5, pool=len(lens) + 2)
+        a["slots"] = torch.randperm(len(lens) + 2, generator=_gen(1), device=dev)[:len(lens)].to(torch.int32)
+        head = 33
+        cu = (_cu(lens) + head).contiguous()
+        used = {k: v[head:head + sum(lens)] if k in ("x", "dt", "Bm", "Cm") else v.clone() if "state" in k else v
+                for k, v in a.items()}
+        want = ops.selective_scan(**used, cu_seqlens=_cu(lens))
+        at = _poisoned(a["x"].shape, BF)
+        y = ops.selective_scan(**a, cu_seqlens=cu)
+        assert y.data_ptr() == at
+        assert (y[:head] == 0).all() and (y[head + sum(lens):] == 0).all()
+        # cut elsewhere, the same sums in another order
+        assert (y[head:head + sum(lens)].float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
+
+
 def test_scan_on_another_stream_and_empty():
     a = _scan_inputs([64, 2], 256, 64, 128, BF, seed=8)
     s = torch.cuda.Stream()
@@ -295,6 +341,22 @@ def test_gdn_padding_slots_and_streams():
     idle = torch.ones(before[0].shape[0], dtype=torch.bool, device=dev)
     idle[a["slots"][[0, 2]].long()] = False
     assert torch.equal(a["state"][idle], before[0][idle]) and torch.equal(a["conv_state"][idle], before[1][idle])
+
+
+@pytest.mark.parametrize("cu", OPEN)
+def test_gdn_rows_of_no_sequence_are_zero(cu):
+    a = _gdn_inputs([30, 30], 2, 64, BF, seed=4)
+    a["slots"] = a["slots"][:len(cu) - 1].contiguous()
+    cu_dev = torch.tensor(cu, dtype=torch.int32, device=dev)
+    ref = {k: _d(v) for k, v in a.items()}
+    ref["conv_state"], ref["state"] = ref["conv_state"].clone(), ref["state"].clone()
+    want = R.gdn2_recurrent(**ref, cu_seqlens=cu_dev)
+    at = _poisoned(a["q"].shape, BF)
+    o = ops.gdn2_recurrent(**a, cu_seqlens=cu_dev)
+    assert o.data_ptr() == at and torch.isfinite(o).all()
+    if all(s <= e for s, e in zip(cu, cu[1:])):
+        assert (o[(want == 0).all(1)] == 0).all()
+        assert (o.double() - want).abs().max() <= 2.0 ** -7 * want.abs().max()
 
 
 def test_gdn_matches_chunked_scan():
