@@ -83,6 +83,10 @@ class MoE(nn.Module):
         """A statistic's mean over the data-parallel ranks; its own in a serving call, which one rank makes alone."""
         return dp_mean(t) if serving_call() is None else t
 
+    def _noisy(self) -> bool:
+        """Router noise and dropout are for training forwards; a serving call has none, whatever the mode."""
+        return self.training and serving_call() is None
+
     def route(self, flat_x: torch.Tensor, stats: Dict[str, torch.Tensor]):
         E, k = self.E, self.k
         if ops.use_cuda(flat_x) and flat_x.dtype == torch.bfloat16:
@@ -106,7 +110,7 @@ class MoE(nn.Module):
         stats["max_abs_logit_preclip"] = logits.abs().max().detach()
         stats["min_col_norm"] = kern.square().sum(0).sqrt().min().detach()
         logits = R.sanitize(logits.clamp(-ROUTER_LOGIT_CLIP, ROUTER_LOGIT_CLIP), 1e3)
-        if self.training and self.cfg.router_noise_std > 0:
+        if self._noisy() and self.cfg.router_noise_std > 0:
             logits = logits + self.cfg.router_noise_std * torch.randn_like(logits)
         biased = logits + self.expert_bias.detach().float()[None, :]
         top_idx = torch.topk(biased, k, dim=-1).indices
@@ -138,7 +142,7 @@ class MoE(nn.Module):
         stats["router_max_cos"] = (gram - eye).abs().max().detach()
         temp = self.router_temp.float().clamp(1.0, 15.0).reshape(1)
         noise = None
-        if self.training and self.cfg.router_noise_std > 0:
+        if self._noisy() and self.cfg.router_noise_std > 0:
             noise = self.cfg.router_noise_std * torch.randn(T, E, device=flat_x.device)
         gate, psum, lse_sq, top_idx, counts, scal = K.router(flat_x, kn, temp, self.expert_bias.detach().float(),
                                                              noise, k)
@@ -170,7 +174,7 @@ class MoE(nn.Module):
                 h = F.silu(h1) * h3
         else:
             h = R.gelu_tanh(self.shared_w1(flat))
-        if self.training and self.cfg.dropout_rate > 0:
+        if self._noisy() and self.cfg.dropout_rate > 0:
             h = F.dropout(h, self.cfg.dropout_rate)
         return self.shared_w2(h)
 

@@ -7,6 +7,7 @@ import torch
 
 from .. import ops
 from ..models.hybrid import flax_path
+from ..optim.store import default_keep_fp32
 from .state import DecodeState, serving
 
 
@@ -33,21 +34,27 @@ def load_weights(model, root: str, slot: str = "latest", step: Optional[int] = N
     return fresh
 
 
+def compute_weights(model):
+    """Keeps ``model``'s matrices in its compute dtype from here on, those that training computes with in fp32 (router,
+    norms, biases) apart: half the memory, and no rounding at every token.  Parameters that a trainer's store holds
+    already are its views, and stay.  Returns ``model``."""
+    for n, p in model.named_parameters():
+        if not default_keep_fp32(n, p) and not hasattr(p, "_ahb_grad_acc"):
+            p.data = p.data.to(model.compute_dtype)
+    return model
+
+
 class Generator:
     """Answers up to ``max_sequences`` prompts at a time.
 
-    ``model`` is put into evaluation mode; on a GPU its matrices are kept in the compute dtype from
-    here on (the training stores' own compute copy is already).  ``max_len`` bounds prompt plus answer
-    for models with MLA layers.  On a GPU, models without MLA replay the token step from one CUDA
-    graph per batch size."""
+    ``model`` stays as it is, in training mode or not and owned by a trainer or not: its weights are read where they
+    are at every token, matrices of another dtype than the compute dtype are rounded on the way (``compute_weights``
+    keeps them rounded).  ``max_len`` bounds prompt plus answer for models with MLA layers.  On a GPU, models without
+    MLA replay the token step from one CUDA graph per batch size."""
 
     def __init__(self, model, max_sequences: int, max_len: int = 0, cuda_graph: bool = True):
-        self.model = model.eval()
+        self.model = model
         p = next(model.parameters())
-        if p.is_cuda:
-            for q in model.parameters():
-                if q.ndim >= 2 and q.dtype != model.compute_dtype:
-                    q.data = q.data.to(model.compute_dtype)
         self.device = p.device
         self.state = DecodeState(model, max_sequences, max_len)
         self.cuda_graph = cuda_graph and p.is_cuda and not self.state.has_mla

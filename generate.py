@@ -17,7 +17,7 @@ import torch  # noqa: E402
 
 from atomic_ai_hybrid_b200.config import get_preset, load_yaml_config  # noqa: E402
 from atomic_ai_hybrid_b200.models import HybridMoEModel  # noqa: E402
-from atomic_ai_hybrid_b200.serving import Generator, load_weights  # noqa: E402
+from atomic_ai_hybrid_b200.serving import Generator, compute_weights, load_weights  # noqa: E402
 
 
 def parse(argv=None):
@@ -63,7 +63,7 @@ def main(argv=None) -> None:
         fresh = load_weights(model, a.ckpt_root, a.ckpt_slot, a.ckpt_step)
         if fresh:
             print(f"[generate] not in the checkpoint, left as initialised: {', '.join(fresh[:8])}", file=sys.stderr)
-    gen = Generator(model, len(prompts), max_len=max(map(len, prompts)) + a.max_new_tokens, cuda_graph=not a.no_graph)
+    gen = Generator(compute_weights(model), len(prompts), max_len=max(map(len, prompts)) + a.max_new_tokens, cuda_graph=not a.no_graph)
     began = time.perf_counter()
     tokens, logprobs = gen.generate(prompts, a.max_new_tokens, a.temperature, a.top_k, a.top_p, a.min_p, a.stop_token,
                                     torch.Generator(device=device).manual_seed(a.seed))

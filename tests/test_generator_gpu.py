@@ -1,0 +1,88 @@
+"""What a Generator leaves of the model that it is given, and what it sees of that model's changes, on the GPU."""
+import pytest
+import torch
+
+from atomic_ai_hybrid_b200 import get_preset
+from atomic_ai_hybrid_b200.models import HybridMoEModel
+from atomic_ai_hybrid_b200.serving import DecodeState, Generator, compute_weights, serving
+
+pytestmark = pytest.mark.gpu
+dev = "cuda"
+
+
+def _model(**kw):
+    torch.manual_seed(0)
+    cfg = get_preset("hybrid_1b", **{**dict(d_model=256, n_heads=2, n_heads_ssm=4, num_layers=4, d_ff=256, n_routed_experts=8,
+                                            top_k=2, vocab_size=1024, d_state=128), **kw})
+    with torch.device(dev):
+        return HybridMoEModel(cfg, compute_dtype=torch.bfloat16), cfg
+
+
+def _weights(model):
+    return {n: (p.data_ptr(), p.dtype, p.detach().clone()) for n, p in model.named_parameters()}
+
+
+def _unchanged(model, before):
+    for n, p in model.named_parameters():
+        ptr, dtype, value = before[n]
+        assert p.data_ptr() == ptr and p.dtype is dtype and torch.equal(p, value), n
+
+
+def _direct(model, ids):
+    """Logits after ``ids`` on a state of their own, without a Generator."""
+    with torch.no_grad(), serving(DecodeState(model, 1), [0], [len(ids)]):
+        h, _ = model(torch.tensor([ids], device=dev))
+    return h[0, -1:] @ model.lm_weight().to(h.dtype).t()
+
+
+@pytest.mark.parametrize("training", [True, False])
+def test_generator_leaves_the_model_alone(training):
+    """Weights, their dtypes (the router's fp32 among them) and the mode; its logits are those of the model as it was
+    before, from the same kernels on the same weights: equal up to the order of sums that atomics may take."""
+    model, cfg = _model()
+    model.train(training)
+    before = _weights(model)
+    ids = torch.randint(0, cfg.vocab_size, (40,), generator=torch.Generator().manual_seed(1)).tolist()
+    want = _direct(model, ids)
+    gen = Generator(model, 2)
+    got = gen.prefill([ids], [1])
+    assert (got - want).float().norm() <= 1e-3 * want.float().norm()
+    gen.generate([ids, [3]], 6)
+    _unchanged(model, before)
+    assert all(m.training == training for m in model.modules())
+
+
+def test_generating_between_training_steps():
+    """A trainer's model answers and goes on training: its parameters stay the store's views."""
+    from atomic_ai_hybrid_b200.training.trainer import Trainer
+
+    model, cfg = _model(num_layers=2)
+    tr = Trainer(model, total_steps=8, optimizer="adamw", device=torch.device(dev))
+    g = torch.Generator().manual_seed(2)
+    first = _weights(model)
+    for _ in range(3):
+        ids = torch.randint(0, 16, (2, 65), generator=g).to(dev)
+        loss = tr.train_step([{"input_ids": ids[:, :-1], "labels": ids[:, 1:]}])["loss"]
+        assert torch.isfinite(loss)
+        before = _weights(model)
+        compute_weights(model)
+        tokens, _ = Generator(model, 2).generate([[1, 2, 3], [4]], 5, top_k=8)
+        assert [len(t) for t in tokens] == [5, 5]
+        _unchanged(model, before)
+        for s in tr.store.segs:
+            assert s.param.data_ptr() == tr.store.compute_view(s).data_ptr(), s.name
+    assert not torch.equal(model.layer_0.moe.router, first["layer_0.moe.router"][2])  # the steps reached the model
+    tr.close()
+
+
+def test_compute_weights_keeps_what_training_keeps():
+    """Matrices in bf16, the router and the vectors in fp32; the logits are the same, as every product rounds its
+    matrix to bf16 either way."""
+    model, cfg = _model(num_layers=2)
+    want = _direct(model, [5, 6, 7])
+    assert compute_weights(model) is model
+    for n, p in model.named_parameters():
+        assert p.dtype is (torch.float32 if p.ndim < 2 or n.endswith("router") else torch.bfloat16), n
+    got = _direct(model, [5, 6, 7])
+    # the convolutions' taps (2^-9 of their values) are the one difference, seen through two layers
+    assert (got - want).float().norm() <= 2e-2 * want.float().norm()

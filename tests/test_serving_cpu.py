@@ -210,3 +210,16 @@ def test_answering_takes_no_part_in_collectives(monkeypatch):
     gen.step(torch.tensor([4]), [0])
     with pytest.raises(AssertionError, match="a collective"):
         model(torch.ones(1, 64, dtype=torch.long))
+
+
+def test_generator_leaves_mode_and_weights_alone():
+    """A model in training mode answers without router noise and dropout, and stays in training mode."""
+    model, cfg = _model("reference_tiny", dropout_rate=0.5, router_noise_std=1.0)
+    want = Generator(model, 1, max_len=16).prefill([[1, 2, 3]], [0])
+    model.train()
+    before = {n: (p.data_ptr(), p.dtype) for n, p in model.named_parameters()}
+    gen = Generator(model, 1, max_len=16)
+    assert all(m.training for m in model.modules())
+    assert torch.equal(gen.prefill([[1, 2, 3]], [0]), want)
+    gen.generate([[1, 2, 3]], 4)
+    assert {n: (p.data_ptr(), p.dtype) for n, p in model.named_parameters()} == before
