@@ -58,8 +58,7 @@ class DecodeState:
             if isinstance(m, Mamba2):
                 H, C = m.n_heads, m.cfg.d_inner
                 self.layers[m] = dict(conv=torch.zeros(slots, 3, C, **kw),
-                                      state=torch.zeros(slots, H, C // H, m.cfg.d_state, **f32),
-                                      A=-torch.exp(m.A_log.detach().float().clamp(-20.0, 20.0)))
+                                      state=torch.zeros(slots, H, C // H, m.cfg.d_state, **f32))
             elif isinstance(m, GatedDeltaNet2):
                 H, D = m.n_heads, m.d_head
                 self.layers[m] = dict(conv=torch.zeros(slots, 3, 3, H * D, **kw), state=torch.zeros(slots, H, D, D, **f32))
@@ -103,9 +102,17 @@ class _Call:
                 ends.append(ends[-1] + n)
             self.starts = ends
             self.cu = torch.tensor(ends, dtype=torch.int32, device=dev)
-        self._pad = None
+        self._pad = self._rates = None
 
     # ------------------------------------------------------------ Mamba2
+    def _decay_rates(self):
+        """``A = -exp(A_log)`` of every Mamba2 layer, from the weights as they are now: four launches a call for all."""
+        if self._rates is None:
+            mods = [m for m in self.state.layers if isinstance(m, Mamba2)]
+            logs = torch._foreach_clamp_min([m.A_log.detach().float() for m in mods], -20.0)
+            self._rates = dict(zip(mods, torch._foreach_neg(torch._foreach_exp(torch._foreach_clamp_max(logs, 20.0)))))
+        return self._rates
+
     def mamba2(self, mod: Mamba2, x: torch.Tensor) -> torch.Tensor:
         c = self.state.layers[mod]
         xz = mod.in_projection(x)
@@ -116,7 +123,7 @@ class _Call:
             Bm, Cm, dt = K.linear_multi(x_bc, [(m.kernel, m.bias) for m in (mod.B_proj, mod.C_proj, mod.dt_proj)])
         else:
             Bm, Cm, dt = mod.B_proj(x_bc), mod.C_proj(x_bc), mod.dt_proj(x_bc)
-        y = ops.selective_scan(x_bc[0], dt[0], c["A"], Bm[0], Cm[0], mod.conv_w.detach(), mod.conv_b.detach(), c["conv"],
+        y = ops.selective_scan(x_bc[0], dt[0], self._decay_rates()[mod], Bm[0], Cm[0], mod.conv_w.detach(), mod.conv_b.detach(), c["conv"],
                                c["state"], cu_seqlens=self.cu, slots=self.slots_dev)[None]
         if ops.use_cuda(x) and x.dtype == torch.bfloat16:
             from ..ops import kernels as K

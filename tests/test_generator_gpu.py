@@ -86,3 +86,17 @@ def test_compute_weights_keeps_what_training_keeps():
     got = _direct(model, [5, 6, 7])
     # the convolutions' taps (2^-9 of their values) are the one difference, seen through two layers
     assert (got - want).float().norm() <= 2e-2 * want.float().norm()
+
+
+def test_captured_steps_follow_the_weights():
+    """Weights changed in place after a graph was captured, Mamba2's decay rates among them, are those it runs on."""
+    model, cfg = _model(num_layers=2)
+    gen = Generator(model, 2)
+    run = lambda g: g.generate([[1, 2, 3], [9]], 24, top_k=50, generator=torch.Generator(device=dev).manual_seed(4))  # noqa: E731
+    old = run(gen)
+    with torch.no_grad():
+        for n, p in model.named_parameters():
+            if n.endswith("A_log") or n.endswith("final_norm.scale"):
+                p += 0.5
+    new = run(gen)
+    assert new[0] == run(Generator(model, 2))[0] and new[1] != old[1]

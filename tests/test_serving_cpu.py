@@ -223,3 +223,23 @@ def test_generator_leaves_mode_and_weights_alone():
     assert torch.equal(gen.prefill([[1, 2, 3]], [0]), want)
     gen.generate([[1, 2, 3]], 4)
     assert {n: (p.data_ptr(), p.dtype) for n, p in model.named_parameters()} == before
+
+
+@pytest.mark.parametrize("change", ["load", "step"])
+def test_answers_follow_the_weights(change, tmp_path):
+    """New weights in the model, Mamba2's decay rates among them, are what the next call of an older Generator runs on."""
+    model, cfg = _model("tiny", num_layers=2, layer_types=("mamba2", "gdn2"))
+    gen = Generator(model, 1)
+    gen.generate([[1, 2, 3]], 3)
+    torch.manual_seed(5)
+    other = HybridMoEModel(cfg, compute_dtype=torch.float32)
+    with torch.no_grad():
+        if change == "load":
+            model.load_state_dict(other.state_dict())
+        else:
+            for n, p in model.named_parameters():
+                if n.endswith("A_log"):
+                    p += 1.0
+            other.load_state_dict(model.state_dict())
+    ids = [5, 6, 7, 8, 9]
+    assert torch.equal(gen.prefill([ids], [0]), Generator(other, 1).prefill([ids], [0]))
