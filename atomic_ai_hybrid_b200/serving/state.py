@@ -8,6 +8,7 @@ conversations and its mixers run on this state; everything else in the model is 
 from __future__ import annotations
 
 import contextlib
+import contextvars
 import math
 from typing import Dict, List, Optional
 
@@ -21,7 +22,8 @@ from ..ops import reference as R
 from ..parallel.cp import get_cp
 from ..parallel.tp import get_tp
 
-_SERVING = None
+# the running call of this thread (of this context): forwards elsewhere are ordinary ones meanwhile
+_SERVING: contextvars.ContextVar[Optional["_Call"]] = contextvars.ContextVar("serving", default=None)
 
 # GDN-2 prompts of at least this many tokens, in at most this many (sequence, head) pairs, run on the chunked
 # training scan.  It runs a head's chunks side by side, but each call pays 0.9 ms of separate launches for padding,
@@ -33,8 +35,8 @@ GDN_CHUNKED_FROM, GDN_CHUNKED_HEADS = 768, 64
 
 
 def get_serving():
-    """The running call's ``_Call``, or None outside ``serving(...)``."""
-    return _SERVING
+    """The ``_Call`` that this thread is in, or None outside ``serving(...)``."""
+    return _SERVING.get()
 
 
 class DecodeState:
@@ -216,9 +218,9 @@ class _Call:
 def serving(state: DecodeState, slots: List[int], lens: Optional[List[int]] = None, slots_dev=None):
     """Runs a model's forwards on ``state``: ``(1, T)`` tokens of ``len(slots)`` conversations packed one
     after another, ``lens[i]`` of them each (None: one each).  ``slots_dev`` is ``slots`` as an int32 tensor
-    on the device, where the caller has it."""
-    global _SERVING
-    if _SERVING is not None:
+    on the device, where the caller has it.  It holds for the thread that enters it; a state serves one call at a
+    time."""
+    if _SERVING.get() is not None:
         raise RuntimeError("serving(...) is not nested")
     if len(set(slots)) != len(slots) or any(not 0 <= s < state.slots for s in slots):
         raise ValueError(f"slots must be different and below {state.slots}: {slots}")
@@ -226,10 +228,11 @@ def serving(state: DecodeState, slots: List[int], lens: Optional[List[int]] = No
         raise ValueError("every sequence of a call adds at least one token")
     if state.has_mla and any(state.lengths[s] + n > state.max_len for s, n in zip(slots, lens or [1] * len(slots))):
         raise ValueError(f"a conversation would grow past max_len={state.max_len}")
-    _SERVING = _Call(state, slots, lens, slots_dev)
+    call = _Call(state, slots, lens, slots_dev)
+    token = _SERVING.set(call)
     try:
-        yield _SERVING
+        yield call
         for s, n in zip(slots, lens or [1] * len(slots)):
             state.lengths[s] += n
     finally:
-        _SERVING = None
+        _SERVING.reset(token)

@@ -243,3 +243,34 @@ def test_answers_follow_the_weights(change, tmp_path):
             other.load_state_dict(model.state_dict())
     ids = [5, 6, 7, 8, 9]
     assert torch.equal(gen.prefill([ids], [0]), Generator(other, 1).prefill([ids], [0]))
+
+
+def test_other_threads_are_not_serving():
+    """While one thread answers, another thread's forward of the same or of another model is an ordinary one, and
+    another Generator can answer there."""
+    import threading
+
+    model, cfg = _model("tiny", num_layers=2, layer_types=("mamba2", "gdn2"))
+    ids = torch.randint(0, cfg.vocab_size, (1, 64), generator=torch.Generator().manual_seed(3))
+    with torch.no_grad():
+        want = model(ids)[0]
+    gen, second = Generator(model, 2), Generator(model, 1)
+    answer = second.prefill([[1, 2]], [0])
+    got = {}
+
+    def work():
+        try:
+            with torch.no_grad():
+                got["forward"] = model(ids)[0]
+                got["other"] = HybridMoEModel(cfg, compute_dtype=torch.float32)(ids)[0]
+            got["answer"] = second.prefill([[1, 2]], [0])
+        except Exception as e:  # noqa: BLE001
+            got["error"] = e
+
+    with serving(gen.state, [0], [64]):
+        t = threading.Thread(target=work)
+        t.start()
+        t.join()
+    assert "error" not in got, got["error"]
+    assert torch.equal(got["forward"], want) and torch.equal(got["answer"], answer)
+    assert all((c[n] == 0).all() for c in gen.state.layers.values() for n in ("conv", "state"))
