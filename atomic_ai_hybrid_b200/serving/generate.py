@@ -68,11 +68,9 @@ class Generator:
     def prefill(self, prompts: Sequence[Sequence[int]], slots: List[int], fresh: bool = True) -> torch.Tensor:
         """Reads ``prompts`` into ``slots`` (``fresh``: as new conversations) and returns the logits
         ``(prompts, vocabulary)`` after their last tokens."""
-        if fresh:
-            self.state.reset(slots)
         lens = [len(p) for p in prompts]
         ids = torch.cat([torch.as_tensor(p, dtype=torch.long) for p in prompts]).to(self.device)
-        with serving(self.state, slots, lens) as call:
+        with serving(self.state, slots, lens, fresh=fresh) as call:
             h, _ = self.model(ids[None])
             last = call.cu[1:].long() - 1
         return self._logits(h[0, last])

@@ -79,8 +79,13 @@ class DecodeState:
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for c in self.layers.values() for t in c.values())
 
+    def check_slots(self, slots: List[int]) -> None:
+        if len(set(slots)) != len(slots) or any(not 0 <= s < self.slots for s in slots):
+            raise ValueError(f"slots must be different and below {self.slots}: {slots}")
+
     def reset(self, slots: List[int]) -> None:
         """Makes the conversations in ``slots`` new ones."""
+        self.check_slots(slots)
         idx = torch.tensor(slots, device=self.device)
         for cache in self.layers.values():
             for name in ("conv", "state"):
@@ -215,19 +220,21 @@ class _Call:
 
 
 @contextlib.contextmanager
-def serving(state: DecodeState, slots: List[int], lens: Optional[List[int]] = None, slots_dev=None):
+def serving(state: DecodeState, slots: List[int], lens: Optional[List[int]] = None, slots_dev=None, fresh: bool = False):
     """Runs a model's forwards on ``state``: ``(1, T)`` tokens of ``len(slots)`` conversations packed one
-    after another, ``lens[i]`` of them each (None: one each).  ``slots_dev`` is ``slots`` as an int32 tensor
-    on the device, where the caller has it.  It holds for the thread that enters it; a state serves one call at a
-    time."""
+    after another, ``lens[i]`` of them each (None: one each; ``fresh``: as new conversations).  ``slots_dev`` is
+    ``slots`` as an int32 tensor on the device, where the caller has it.  It holds for the thread that enters it; a
+    state serves one call at a time."""
     if _SERVING.get() is not None:
         raise RuntimeError("serving(...) is not nested")
-    if len(set(slots)) != len(slots) or any(not 0 <= s < state.slots for s in slots):
-        raise ValueError(f"slots must be different and below {state.slots}: {slots}")
+    state.check_slots(slots)
     if lens is not None and (len(lens) != len(slots) or min(lens, default=1) < 1):
         raise ValueError("every sequence of a call adds at least one token")
-    if state.has_mla and any(state.lengths[s] + n > state.max_len for s, n in zip(slots, lens or [1] * len(slots))):
+    if state.has_mla and any((0 if fresh else state.lengths[s]) + n > state.max_len
+                             for s, n in zip(slots, lens or [1] * len(slots))):
         raise ValueError(f"a conversation would grow past max_len={state.max_len}")
+    if fresh:
+        state.reset(slots)
     call = _Call(state, slots, lens, slots_dev)
     token = _SERVING.set(call)
     try:

@@ -274,3 +274,23 @@ def test_other_threads_are_not_serving():
     assert "error" not in got, got["error"]
     assert torch.equal(got["forward"], want) and torch.equal(got["answer"], answer)
     assert all((c[n] == 0).all() for c in gen.state.layers.values() for n in ("conv", "state"))
+
+
+@pytest.mark.parametrize("prompts,slots,match", [([[1]], [3], "below 3"), ([[1]], [-1], "below 3"), ([[1], [2]], [1, 1], "different"),
+                                                 ([[1], []], [0, 1], "at least one"), ([[1]], [0, 1], "at least one"),
+                                                 ([[1] * 17], [0], "max_len=16")])
+def test_refused_prompts_leave_the_conversations(prompts, slots, match):
+    """Slots are checked on the host before anything is reset or indexed (out of range on a GPU they would end the
+    process), and a refused call changes nothing."""
+    model, cfg = _model("reference_tiny")
+    gen = Generator(model, 3, max_len=16)
+    gen.prefill([[1, 2, 3], [4, 5]], [0, 1])
+    kept = [{n: t.clone() for n, t in c.items()} for c in gen.state.layers.values()]
+    with pytest.raises(ValueError, match=match):
+        gen.prefill(prompts, slots)
+    assert gen.state.lengths == [3, 2, 0]
+    assert all(torch.equal(c[n], k[n]) for c, k in zip(gen.state.layers.values(), kept) for n in k)
+    if match == "below 3":
+        with pytest.raises(ValueError, match=match):
+            gen.state.reset(slots)
+    assert gen.prefill([[1] * 14], [0], fresh=True).shape == (1, cfg.vocab_size)
