@@ -111,6 +111,11 @@ class _Call:
             self.cu = torch.tensor(ends, dtype=torch.int32, device=dev)
         self._pad = self._rates = None
 
+    def _check_rows(self, x: torch.Tensor) -> None:
+        want = len(self.slots) if self.lens is None else sum(self.lens)
+        if x.shape[0] != 1 or x.shape[1] != want:
+            raise ValueError(f"this call has {want} tokens packed in one row, the forward {x.shape[1]} in {x.shape[0]}")
+
     # ------------------------------------------------------------ Mamba2
     def _decay_rates(self):
         """``A = -exp(A_log)`` of every Mamba2 layer, from the weights as they are now: four launches a call for all."""
@@ -121,6 +126,7 @@ class _Call:
         return self._rates
 
     def mamba2(self, mod: Mamba2, x: torch.Tensor) -> torch.Tensor:
+        self._check_rows(x)
         c = self.state.layers[mod]
         xz = mod.in_projection(x)
         di = xz.shape[-1] // 2
@@ -140,6 +146,7 @@ class _Call:
 
     # ------------------------------------------------------------ GDN-2
     def gdn2(self, mod: GatedDeltaNet2, x: torch.Tensor) -> torch.Tensor:
+        self._check_rows(x)
         c = self.state.layers[mod]
         *ins, og = mod.projections(x)
         if (self.lens is not None and max(self.lens) >= GDN_CHUNKED_FROM and len(self.lens) * mod.n_heads <= GDN_CHUNKED_HEADS
@@ -195,6 +202,7 @@ class _Call:
     def mla(self, mod: MLA, x: torch.Tensor) -> torch.Tensor:
         """Keys and values kept rotated per slot; the products are PyTorch's attention, as under
         context parallelism."""
+        self._check_rows(x)
         st, c = self.state, self.state.layers[mod]
         H, D = mod.n_heads, mod.cfg.d_model // mod.cfg.n_heads
         lens = self.lens or [1] * len(self.slots)

@@ -294,3 +294,19 @@ def test_refused_prompts_leave_the_conversations(prompts, slots, match):
         with pytest.raises(ValueError, match=match):
             gen.state.reset(slots)
     assert gen.prefill([[1] * 14], [0], fresh=True).shape == (1, cfg.vocab_size)
+
+
+def test_forwards_of_other_shapes_are_refused():
+    """Inside a call the model takes (1, tokens of the call): other counts would index past the rows, a second batch row
+    would be dropped."""
+    model, cfg = _model("tiny", num_layers=2, layer_types=("gdn2", "mamba2"))
+    state = DecodeState(model, 3)
+    for lens, shape in (([5], (1, 4)), ([5], (1, 6)), ([5, 2], (2, 5)), (None, (1, 3)), ([3, 3], (2, 6))):
+        with torch.no_grad(), serving(state, list(range(len(lens or [1]))), lens):
+            with pytest.raises(ValueError, match="packed"):
+                model(torch.ones(shape, dtype=torch.long))
+    assert all((c[n] == 0).all() for c in state.layers.values() for n in ("conv", "state"))
+    blockdar, _ = _model("reference_tiny", num_layers=3, layer_types=("mla",) * 3)
+    with torch.no_grad(), serving(DecodeState(blockdar, 1, 8), [0], [4]):
+        with pytest.raises(ValueError, match="packed"):
+            blockdar(torch.ones((1, 3), dtype=torch.long))
