@@ -69,7 +69,10 @@ class Generator:
         """Reads ``prompts`` into ``slots`` (``fresh``: as new conversations) and returns the logits
         ``(prompts, vocabulary)`` after their last tokens."""
         lens = [len(p) for p in prompts]
-        ids = torch.cat([torch.as_tensor(p, dtype=torch.long) for p in prompts]).to(self.device)
+        ids = torch.cat([torch.as_tensor(p, dtype=torch.long) for p in prompts])
+        if ids.numel() and not 0 <= int(ids.min()) <= int(ids.max()) < self.model.cfg.vocab_size:
+            raise ValueError(f"prompts need token ids of the vocabulary, [0, {self.model.cfg.vocab_size})")
+        ids = ids.to(self.device)
         with serving(self.state, slots, lens, fresh=fresh) as call:
             h, _ = self.model(ids[None])
             last = call.cu[1:].long() - 1

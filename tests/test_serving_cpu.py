@@ -310,3 +310,14 @@ def test_forwards_of_other_shapes_are_refused():
     with torch.no_grad(), serving(DecodeState(blockdar, 1, 8), [0], [4]):
         with pytest.raises(ValueError, match="packed"):
             blockdar(torch.ones((1, 3), dtype=torch.long))
+
+
+def test_prompts_outside_the_vocabulary_are_refused():
+    """The embedding kernel would take the nearest row for such an id."""
+    model, cfg = _model("tiny", num_layers=2, layer_types=("mamba2", "gdn2"))
+    gen = Generator(model, 2)
+    gen.prefill([[1, 2]], [0])
+    for bad in (-1, cfg.vocab_size):
+        with pytest.raises(ValueError, match="vocabulary"):
+            gen.prefill([[1], [3, bad]], [0, 1])
+    assert gen.state.lengths == [2, 0]
