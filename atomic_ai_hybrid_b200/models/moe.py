@@ -162,6 +162,11 @@ class MoE(nn.Module):
         return top_idx, gate
 
     # ------------------------------------------------------------------ forward
+    def has_kernels(self, dtype: torch.dtype) -> bool:
+        """The grouped GEMM tiles need bf16, d_model and d_ff in multiples of 256; other sizes read the experts' counts
+        on the host."""
+        return dtype == torch.bfloat16 and self.cfg.d_model % 256 == 0 and self.cfg.d_ff % 256 == 0
+
     def _shared(self, flat: torch.Tensor) -> torch.Tensor:
         if self.swiglu:
             if ops.use_cuda(flat) and flat.dtype == torch.bfloat16:
@@ -198,8 +203,7 @@ class MoE(nn.Module):
             if shared is not None:
                 out = out + shared.float()
             return R.sanitize(out, 1e3).view(Bsz, L, d).to(x.dtype)
-        # the grouped GEMM tiles need d_model and d_ff in multiples of 256
-        if ops.use_cuda(flat) and x.dtype == torch.bfloat16 and d % 256 == 0 and self.cfg.d_ff % 256 == 0:
+        if ops.use_cuda(flat) and self.has_kernels(x.dtype):
             from ..ops import kernels as K
             out = K.moe_forward(flat, top_idx, gate, self.routed_w1, self.routed_w2, self.routed_w3, shared,
                                 "swiglu" if self.swiglu else "gelu")

@@ -890,6 +890,9 @@ def newton_schulz3(g, steps: int = 3, eps: float = 1e-4):
 
 
 # ----------------------------------------------------------------- serving (state carried between calls)
+SCAN_STATES, RECURRENT_HEADS = (32, 64, 128), (64, 96, 128)  # sizes with kernels
+
+
 def _flat_rows(t):
     """``(B, L, C)`` or ``(T, C)`` as ``(T, C)`` rows of unit channel stride (a column slice stays a view)."""
     if t.dim() == 3:
@@ -899,7 +902,7 @@ def _flat_rows(t):
 
 def selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, cu_seqlens, slots, dt_min, dt_max):
     """See ``ops.selective_scan``; bf16 or fp32 tokens and 32, 64 or 128 states (others run the PyTorch form)."""
-    if state.shape[-1] not in (32, 64, 128):
+    if state.shape[-1] not in SCAN_STATES:
         _unsupported(f"selective_scan N={state.shape[-1]}")
         return R.selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, cu_seqlens, slots, dt_min, dt_max)
     if x.dim() == 2:
@@ -915,7 +918,7 @@ def selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, cu_seqle
 
 def gdn2_recurrent(q, k, v, b, w, f, conv_w, conv_b, decay_a, conv_state, state, cu_seqlens, slots):
     """See ``ops.gdn2_recurrent``; bf16 or fp32 tokens and head dims 64, 96, 128 (others run the PyTorch form)."""
-    if state.shape[-1] not in (64, 96, 128):
+    if state.shape[-1] not in RECURRENT_HEADS:
         _unsupported(f"gdn2_recurrent D={state.shape[-1]}")
         return R.gdn2_recurrent(q, k, v, b, w, f, conv_w, conv_b, decay_a, conv_state, state, cu_seqlens, slots)
     if q.dim() == 2:

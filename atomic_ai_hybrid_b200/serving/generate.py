@@ -50,14 +50,14 @@ class Generator:
     ``model`` stays as it is, in training mode or not and owned by a trainer or not: its weights are read where they
     are at every token, matrices of another dtype than the compute dtype are rounded on the way (``compute_weights``
     keeps them rounded).  ``max_len`` bounds prompt plus answer for models with MLA layers.  On a GPU, models without
-    MLA replay the token step from one CUDA graph per batch size."""
+    MLA whose sizes all have kernels replay the token step from one CUDA graph per batch size; others launch it."""
 
     def __init__(self, model, max_sequences: int, max_len: int = 0, cuda_graph: bool = True):
         self.model = model
         p = next(model.parameters())
         self.device = p.device
         self.state = DecodeState(model, max_sequences, max_len)
-        self.cuda_graph = cuda_graph and p.is_cuda and not self.state.has_mla
+        self.cuda_graph = cuda_graph
         self._graphs = {}
 
     # ------------------------------------------------------------ forwards
@@ -144,7 +144,8 @@ class Generator:
         t, lp = ops.sample(self.prefill(prompts, slots), noise(torch.empty(B, V, device=dev)), *rules)
         steps = [(t, lp)]
         done = (t < 0) | (t == stop_token) if stop_token is not None else t < 0
-        if self.cuda_graph and max_new_tokens > 1:
+        replay = self.cuda_graph and max_new_tokens > 1 and self.state.on_device()
+        if replay:
             graph, buf = self._graph_step(slots)
             for name, v in zip(("temperature", "top_k", "top_p", "min_p"), rules):
                 buf[name].copy_(v)
@@ -152,7 +153,7 @@ class Generator:
         for i in range(1, max_new_tokens):
             if i % 16 == 0 and bool(done.all()):  # the host waits for the device every 16 tokens only
                 break
-            if self.cuda_graph:
+            if replay:
                 noise(buf["noise"])
                 graph.replay()
                 t, lp = (o.clone() for o in buf["out"])

@@ -50,6 +50,7 @@ class DecodeState:
         if any(isinstance(m, MoE) and m.ep_world > 1 for m in model.modules()):
             raise ValueError("serving runs on one rank's whole model: this rank holds a part of the experts only, and every "
                              "layer would wait for the other ranks")
+        self.model = model
         p = next(model.parameters())
         self.device, self.dtype, self.slots, self.max_len = p.device, model.compute_dtype, slots, max_len
         self.lengths = [0] * slots
@@ -75,6 +76,15 @@ class DecodeState:
     @property
     def has_mla(self) -> bool:
         return any("k" in c for c in self.layers.values())
+
+    def on_device(self) -> bool:
+        """Whether a token step runs without a host read, as a CUDA graph needs it: every layer's sizes have kernels."""
+        from ..ops import kernels as K
+        if self.device.type != "cuda" or ops.get_impl() != "cuda" or self.has_mla:
+            return False
+        return all((not isinstance(m, Mamba2) or m.cfg.d_state in K.SCAN_STATES)
+                   and (not isinstance(m, GatedDeltaNet2) or m.d_head in K.RECURRENT_HEADS)
+                   and (not isinstance(m, MoE) or m.has_kernels(self.dtype)) for m in self.model.modules())
 
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for c in self.layers.values() for t in c.values())

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from atomic_ai_hybrid_b200 import get_preset
+from atomic_ai_hybrid_b200 import get_preset, ops
 from atomic_ai_hybrid_b200.models import HybridMoEModel
 from atomic_ai_hybrid_b200.serving import DecodeState, Generator, compute_weights, serving
 
@@ -100,3 +100,19 @@ def test_captured_steps_follow_the_weights():
                 p += 0.5
     new = run(gen)
     assert new[0] == run(Generator(model, 2))[0] and new[1] != old[1]
+
+
+@pytest.mark.parametrize("kw", [dict(d_model=128, d_ff=128), dict(d_state=16), dict(n_heads=8), dict(compute_dtype=torch.float32), dict()])
+@pytest.mark.parametrize("impl", ["cuda", "eager"])
+def test_sizes_without_kernels_are_launched(kw, impl):
+    """A layer that reads on the host cannot be captured: the token step is launched, with the same answer as ever."""
+    kw = dict(kw)
+    dtype = kw.pop("compute_dtype", torch.bfloat16)
+    model, cfg = _model(num_layers=2, **kw)
+    model.compute_dtype = dtype
+    run = lambda graph: Generator(model, 2, cuda_graph=graph).generate(  # noqa: E731
+        [[1, 2, 3], [9]], 6, top_k=50, generator=torch.Generator(device=dev).manual_seed(4))
+    with ops.impl(impl):
+        gen = Generator(model, 2)
+        assert gen.state.on_device() == (not kw and dtype is torch.bfloat16 and impl == "cuda")
+        assert run(True)[0] == run(False)[0]
