@@ -58,7 +58,7 @@ class Generator:
         self.device = p.device
         self.state = DecodeState(model, max_sequences, max_len)
         self.cuda_graph = cuda_graph
-        self._graphs = {}
+        self._graphs, self._captured = {}, None
 
     # ------------------------------------------------------------ forwards
     def _logits(self, h: torch.Tensor) -> torch.Tensor:
@@ -87,6 +87,10 @@ class Generator:
 
     def _graph_step(self, slots: List[int]):
         """The token step over ``slots`` and its sampling as one graph; returns it with its buffers."""
+        where = [(p.data_ptr(), p.dtype) for p in self.model.parameters()]
+        if where != self._captured:  # a graph reads the weights by address: they have moved since
+            self._graphs.clear()
+            self._captured = where
         key = tuple(slots)
         if key not in self._graphs:
             B, V = len(slots), self.model.cfg.vocab_size

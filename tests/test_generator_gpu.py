@@ -116,3 +116,27 @@ def test_sizes_without_kernels_are_launched(kw, impl):
         gen = Generator(model, 2)
         assert gen.state.on_device() == (not kw and dtype is torch.bfloat16 and impl == "cuda")
         assert run(True)[0] == run(False)[0]
+
+
+@pytest.mark.parametrize("move", ["compute_weights", "trainer"])
+def test_captured_steps_find_moved_weights(move):
+    """Parameters that moved to other memory after a capture (into a trainer's store, to another dtype) and changed
+    there: the graph is captured again."""
+    from atomic_ai_hybrid_b200.training.trainer import Trainer
+
+    model, cfg = _model(num_layers=2)
+    gen = Generator(model, 2)
+    run = lambda g: g.generate([[1, 2, 3], [9]], 24, top_k=50, generator=torch.Generator(device=dev).manual_seed(4))  # noqa: E731
+    old = run(gen)
+    if move == "compute_weights":
+        compute_weights(model)
+    else:
+        tr = Trainer(model, total_steps=4, optimizer="adamw", device=torch.device(dev))
+    with torch.no_grad():
+        for n, p in model.named_parameters():
+            if p.ndim == 2 and not n.startswith("embed"):
+                p *= 0.5
+    new = run(gen)
+    assert new[0] == run(Generator(model, 2))[0] and new[1] != old[1]
+    if move == "trainer":
+        tr.close()
