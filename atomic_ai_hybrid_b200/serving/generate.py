@@ -112,16 +112,19 @@ class Generator:
             lengths = list(self.state.lengths)
             side = torch.cuda.Stream(device=dev)
             side.wait_stream(torch.cuda.current_stream(dev))
-            with torch.cuda.stream(side):
-                run()
-            torch.cuda.current_stream(dev).wait_stream(side)
             graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph):
-                buf["out"] = run()
-            for c, k in zip(self.state.layers.values(), kept):
-                for n, t in k.items():
-                    c[n].copy_(t)
-            self.state.lengths = lengths
+            try:
+                with torch.cuda.stream(side):
+                    run()
+                torch.cuda.current_stream(dev).wait_stream(side)
+                with torch.cuda.graph(graph):
+                    buf["out"] = run()
+            finally:
+                torch.cuda.current_stream(dev).wait_stream(side)
+                for c, k in zip(self.state.layers.values(), kept):
+                    for n, t in k.items():
+                        c[n].copy_(t)
+                self.state.lengths = lengths
             self._graphs[key] = graph, buf
         return self._graphs[key]
 

@@ -140,3 +140,22 @@ def test_captured_steps_find_moved_weights(move):
     assert new[0] == run(Generator(model, 2))[0] and new[1] != old[1]
     if move == "trainer":
         tr.close()
+
+
+def test_a_failed_capture_leaves_the_conversations(monkeypatch):
+    """States and lengths after a step that cannot be captured are those before it."""
+    model, cfg = _model(num_layers=2)
+    gen = Generator(model, 2)
+    gen.prefill([[1, 2, 3], [4]], [0, 1])
+    kept = [{n: t.clone() for n, t in c.items()} for c in gen.state.layers.values()]
+
+    def broken(*a):
+        raise RuntimeError("no sampling today")
+
+    with monkeypatch.context() as m:
+        m.setattr(ops, "sample", broken)
+        with pytest.raises(RuntimeError, match="no sampling"):
+            gen._graph_step([0, 1])
+    assert gen.state.lengths == [3, 1] and not gen._graphs
+    assert all(torch.equal(c[n], k[n]) for c, k in zip(gen.state.layers.values(), kept) for n in k)
+    assert [len(t) for t in gen.generate([[1, 2, 3], [4]], 4)[0]] == [4, 4]
