@@ -44,6 +44,9 @@ def compute_weights(model):
     return model
 
 
+MAX_GRAPHS = 8  # captured token steps that a Generator keeps, one per batch size; a capture launches the step twice
+
+
 class Generator:
     """Answers up to ``max_sequences`` prompts at a time.
 
@@ -58,7 +61,7 @@ class Generator:
         self.device = p.device
         self.state = DecodeState(model, max_sequences, max_len)
         self.cuda_graph = cuda_graph
-        self._graphs, self._captured = {}, None
+        self._graphs, self._captured, self._rows = {}, None, None
 
     # ------------------------------------------------------------ forwards
     def _logits(self, h: torch.Tensor) -> torch.Tensor:
@@ -93,12 +96,17 @@ class Generator:
             self._captured = where
         key = tuple(slots)
         if key not in self._graphs:
-            B, V = len(slots), self.model.cfg.vocab_size
-            dev = self.device
-            buf = dict(tokens=torch.zeros(B, dtype=torch.long, device=dev), noise=torch.ones(B, V, device=dev),
-                       temperature=torch.ones(B, device=dev), top_k=torch.zeros(B, dtype=torch.int32, device=dev),
-                       top_p=torch.ones(B, device=dev), min_p=torch.zeros(B, device=dev),
-                       slots=torch.tensor(slots, dtype=torch.int32, device=dev))  # all that the graph reads by address
+            while len(self._graphs) >= MAX_GRAPHS:  # the one that was used least recently
+                self._graphs.pop(next(iter(self._graphs)))
+            B, V, dev = len(slots), self.model.cfg.vocab_size, self.device
+            if self._rows is None:  # what the graphs read by address: rows of the same buffers, as they run one at a time
+                n = self.state.slots
+                self._rows = dict(tokens=torch.zeros(n, dtype=torch.long, device=dev), noise=torch.ones(n, V, device=dev),
+                                  temperature=torch.ones(n, device=dev), top_k=torch.zeros(n, dtype=torch.int32, device=dev),
+                                  top_p=torch.ones(n, device=dev), min_p=torch.zeros(n, device=dev))
+                self._pool = torch.cuda.graph_pool_handle()
+            buf = {name: t[:B] for name, t in self._rows.items()}
+            buf["slots"] = torch.tensor(slots, dtype=torch.int32, device=dev)
 
             def run():
                 with serving(self.state, slots, slots_dev=buf["slots"]):
@@ -117,7 +125,7 @@ class Generator:
                 with torch.cuda.stream(side):
                     run()
                 torch.cuda.current_stream(dev).wait_stream(side)
-                with torch.cuda.graph(graph):
+                with torch.cuda.graph(graph, pool=self._pool):
                     buf["out"] = run()
             finally:
                 torch.cuda.current_stream(dev).wait_stream(side)
@@ -125,8 +133,10 @@ class Generator:
                     for n, t in k.items():
                         c[n].copy_(t)
                 self.state.lengths = lengths
-            self._graphs[key] = graph, buf
-        return self._graphs[key]
+        else:
+            graph, buf = self._graphs.pop(key)
+        self._graphs[key] = graph, buf
+        return graph, buf
 
     # ------------------------------------------------------------ generation
     @torch.no_grad()

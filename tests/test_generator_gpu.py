@@ -159,3 +159,23 @@ def test_a_failed_capture_leaves_the_conversations(monkeypatch):
     assert gen.state.lengths == [3, 1] and not gen._graphs
     assert all(torch.equal(c[n], k[n]) for c, k in zip(gen.state.layers.values(), kept) for n in k)
     assert [len(t) for t in gen.generate([[1, 2, 3], [4]], 4)[0]] == [4, 4]
+
+
+def test_graphs_of_many_batch_sizes_are_bounded():
+    """Answers to every batch size, twice around: a bounded number of graphs is kept, their buffers are shared, and
+    memory does not grow."""
+    from atomic_ai_hybrid_b200.serving import generate
+
+    model, cfg = _model(num_layers=2, vocab_size=50304)
+    gen, plain = Generator(model, 12), Generator(model, 12, cuda_graph=False)
+    held = []
+    for turn in range(3):
+        for B in range(1, 13):
+            run = lambda g: g.generate([[i + 1, 7] for i in range(B)], 4, top_k=50,  # noqa: E731
+                                       generator=torch.Generator(device=dev).manual_seed(B))
+            got = run(gen)
+            assert len(gen._graphs) <= generate.MAX_GRAPHS
+            assert turn or got[0] == run(plain)[0]
+        torch.cuda.synchronize()
+        held.append(torch.cuda.memory_reserved())
+    assert held[2] <= held[1]
