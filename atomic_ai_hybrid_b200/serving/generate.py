@@ -104,7 +104,8 @@ class Generator:
                 self._rows = dict(tokens=torch.zeros(n, dtype=torch.long, device=dev), noise=torch.ones(n, V, device=dev),
                                   temperature=torch.ones(n, device=dev), top_k=torch.zeros(n, dtype=torch.int32, device=dev),
                                   top_p=torch.ones(n, device=dev), min_p=torch.zeros(n, device=dev))
-                self._pool = torch.cuda.graph_pool_handle()
+                # one stream, of the model's device, for every capture: the allocator keeps a stream's memory for it
+                self._pool, self._side = torch.cuda.graph_pool_handle(), torch.cuda.Stream(device=dev)
             buf = {name: t[:B] for name, t in self._rows.items()}
             buf["slots"] = torch.tensor(slots, dtype=torch.int32, device=dev)
 
@@ -118,14 +119,14 @@ class Generator:
             # warm up and capture on a copy of what the step changes
             kept = [{n: c[n].clone() for n in ("conv", "state")} for c in self.state.layers.values()]
             lengths = list(self.state.lengths)
-            side = torch.cuda.Stream(device=dev)
+            side = self._side
             side.wait_stream(torch.cuda.current_stream(dev))
             graph = torch.cuda.CUDAGraph()
             try:
                 with torch.cuda.stream(side):
                     run()
                 torch.cuda.current_stream(dev).wait_stream(side)
-                with torch.cuda.graph(graph, pool=self._pool):
+                with torch.cuda.graph(graph, pool=self._pool, stream=side):
                     buf["out"] = run()
             finally:
                 torch.cuda.current_stream(dev).wait_stream(side)

@@ -179,3 +179,23 @@ def test_graphs_of_many_batch_sizes_are_bounded():
         torch.cuda.synchronize()
         held.append(torch.cuda.memory_reserved())
     assert held[2] <= held[1]
+
+
+def test_captures_on_the_models_device(monkeypatch):
+    """The capture runs on a stream of the model's device, whichever device is the current one (without a stream
+    PyTorch takes one of the device that was current at the process's first capture: kernels elsewhere are not
+    captured)."""
+    streams, graph = [], torch.cuda.graph
+
+    def capture(*a, **kw):
+        streams.append(kw.get("stream"))
+        return graph(*a, **kw)
+
+    monkeypatch.setattr(torch.cuda, "graph", capture)
+    home = torch.device(dev, torch.cuda.device_count() - 1)
+    model, cfg = _model(num_layers=2)
+    gen = Generator(model.to(home), 2)
+    with torch.cuda.device(0):
+        tokens = gen.generate([[1, 2, 3], [9]], 6, temperature=0.0)[0]
+    assert len(streams) == 1 and streams[0].device == home
+    assert tokens == Generator(model, 2, cuda_graph=False).generate([[1, 2, 3], [9]], 6, temperature=0.0)[0]
