@@ -13,7 +13,8 @@ from .state import DecodeState, serving
 
 def load_weights(model, root: str, slot: str = "latest", step: Optional[int] = None) -> List[str]:
     """Fills ``model`` from a training checkpoint (any parallel layout's files; the parameters keep their
-    dtypes); returns the names that the checkpoint does not hold."""
+    dtypes); returns the names that the checkpoint does not hold.  One that holds a tensor of another shape is of
+    another model: that is an error, and nothing is loaded."""
     from ..ckpt.manager import CheckpointManager, _assemble_tp, _lookup
 
     mgr = CheckpointManager(root, slot)
@@ -21,17 +22,23 @@ def load_weights(model, root: str, slot: str = "latest", step: Optional[int] = N
     if step is None:
         raise FileNotFoundError(f"no checkpoint in {root}/{slot}")
     params, _, _ = mgr.load_tensors(step)
-    fresh = []
+    found, absent, other = [], [], []
+    for n, p in model.named_parameters():
+        t = _lookup(params, flax_path(n), None)
+        if t is None:
+            t = _assemble_tp(params, flax_path(n))
+        if t is None:
+            absent.append(n)
+        elif tuple(t.shape) != tuple(p.shape):
+            other.append(f"{n} {tuple(t.shape)} for {tuple(p.shape)}")
+        else:
+            found.append((p, t))
+    if other:
+        raise ValueError(f"the checkpoint in {root}/{slot} has {len(other)} parameters of another shape: {', '.join(other[:8])}")
     with torch.no_grad():
-        for n, p in model.named_parameters():
-            t = _lookup(params, flax_path(n), None)
-            if t is None:
-                t = _assemble_tp(params, flax_path(n))
-            if t is None or tuple(t.shape) != tuple(p.shape):
-                fresh.append(n)
-            else:
-                p.copy_(t)
-    return fresh
+        for p, t in found:
+            p.copy_(t)
+    return absent
 
 
 def compute_weights(model):

@@ -60,9 +60,9 @@ def main(argv=None) -> None:
     with torch.device(device):
         model = HybridMoEModel(cfg, compute_dtype=torch.bfloat16 if device.type == "cuda" else torch.float32)
     if a.ckpt_root:
-        fresh = load_weights(model, a.ckpt_root, a.ckpt_slot, a.ckpt_step)
-        if fresh:
-            print(f"[generate] not in the checkpoint, left as initialised: {', '.join(fresh[:8])}", file=sys.stderr)
+        absent = load_weights(model, a.ckpt_root, a.ckpt_slot, a.ckpt_step)
+        if absent:
+            raise SystemExit(f"the checkpoint is of another model, without {', '.join(absent[:8])}")
     gen = Generator(compute_weights(model), len(prompts), max_len=max(map(len, prompts)) + a.max_new_tokens, cuda_graph=not a.no_graph)
     began = time.perf_counter()
     tokens, logprobs = gen.generate(prompts, a.max_new_tokens, a.temperature, a.top_k, a.top_p, a.min_p, a.stop_token,

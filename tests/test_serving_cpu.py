@@ -321,3 +321,43 @@ def test_prompts_outside_the_vocabulary_are_refused():
         with pytest.raises(ValueError, match="vocabulary"):
             gen.prefill([[1], [3, bad]], [0, 1])
     assert gen.state.lengths == [2, 0]
+
+
+def _saved(tmp_path, **kw):
+    from atomic_ai_hybrid_b200.ckpt import CheckpointManager
+    from atomic_ai_hybrid_b200.training.trainer import Trainer
+
+    model, cfg = _model("tiny", num_layers=2, **kw)
+    mgr = CheckpointManager(str(tmp_path), "latest")
+    mgr.save(3, Trainer(model, total_steps=4, compute_dtype=torch.float32, device=torch.device("cpu")), {}, asynchronous=False)
+    mgr.finalize()
+
+
+def test_weights_of_another_shape_are_refused(tmp_path):
+    """A checkpoint of another model is an error that changes nothing; names that it lacks are returned."""
+    _saved(tmp_path, d_ff=256)
+    other, cfg = _model("tiny", num_layers=2, d_ff=128)
+    before = {n: p.detach().clone() for n, p in other.named_parameters()}
+    with pytest.raises(ValueError, match="another shape.*routed_w1"):
+        load_weights(other, str(tmp_path))
+    assert all(torch.equal(p, before[n]) for n, p in other.named_parameters())
+    deeper, _ = _model("tiny", num_layers=3, d_ff=256)
+    absent = load_weights(deeper, str(tmp_path))
+    assert absent and all(n.startswith("layer_2.") for n in absent)
+
+
+def test_generate_does_not_answer_with_fresh_weights(tmp_path, capsys):
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "generate.py")
+    spec = importlib.util.spec_from_file_location("generate_command", path)
+    command = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(command)
+    _saved(tmp_path)
+    args = ["--preset", "tiny", "--ckpt-root", str(tmp_path), "--prompt", "1,2,3", "--max-new-tokens", "2"]
+    command.main(args + ["--layers", "2"])
+    assert '"tokens"' in capsys.readouterr().out
+    with pytest.raises(SystemExit, match="layer_2"):
+        command.main(args + ["--layers", "3"])
+    assert capsys.readouterr().out == ""
