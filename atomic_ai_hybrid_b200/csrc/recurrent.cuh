@@ -33,11 +33,12 @@ AHB_DEVICE int seq_slot(const int* slots, int b, int S) {
 }
 
 // e^x for x <= 0 to about one unit in the last place: x = n ln 2 + r with ln 2 in two parts (Cody and
-// Waite, 355/512 and the rest), Taylor in r to r^7 (|r| <= 0.347, remainder below 6e-9).  A decay multiplies the state once per token, so the 2^-22
-// error of the hardware's ex2 would add up over a state's memory.
+// Waite, 355/512 and the rest), Taylor in r to r^7 (|r| <= 0.347, remainder below 6e-9).  A decay multiplies the state
+// once per token, so the 2^-22 error of the hardware's ex2 would add up over a state's memory.  Growth is right too:
+// n ends at 127, the largest exponent, and r takes the rest up to infinity (2e-6 off at e^88.7, the floats' end).
 AHB_DEVICE float exp_decay(float x) {
   x = fmaxf(x, -87.f);
-  const float n = rintf(x * 1.4426950408889634f);
+  const float n = fminf(rintf(x * 1.4426950408889634f), 127.f);
   float r = fmaf(n, -355.f / 512.f, x);
   r = fmaf(n, 2.1219444005469e-4f, r);
   float p = fmaf(r, 1.f / 5040.f, 1.f / 720.f);

@@ -187,6 +187,33 @@ def test_scan_largest_values(A):
     assert ((y.double() - y64).abs() <= 2.0 ** -8 * y64.abs() + REL * most * 128e3).all()
 
 
+@pytest.mark.parametrize("N", [32, 64, 128])
+@pytest.mark.parametrize("form,dtype", [("one each", BF), ("one each", F32), ("offsets", BF), ("offsets", F32), ("block", BF)])
+def test_scan_growth(N, form, dtype):
+    """Rates above zero grow the state up to infinity, in every form alike (the layer's are below zero)."""
+    rates = torch.tensor([1.0, 20.0, 60.0, 87.9, 88.3, 88.6, 95.0, 300.0], device=dev)
+    a = _scan_inputs([1] * 3, 64, 8, N, dtype, seed=8)
+    a["A"], a["dt"] = rates, torch.full_like(a["dt"], 60.0)  # a step of 1
+    cu = None if form == "one each" else _cu([1] * 3)
+    if form == "block":  # each token first of 16 whose steps are the smallest, 1e-9 of its growth
+        lead = {n: a[n][:, None].repeat(1, 16, 1).flatten(0, 1) for n in ("x", "dt", "Bm", "Cm")}
+        lead["dt"].unflatten(0, (3, 16))[:, 1:] = -100.0
+        a.update(lead)
+        cu = _cu([16] * 3)
+    lo = dict(dt_min=1e-9) if form == "block" else {}
+    ref = {k: _d(v) for k, v in a.items()}
+    ref["conv_state"], ref["state"] = ref["conv_state"].clone(), ref["state"].clone()
+    R.selective_scan(**ref, cu_seqlens=cu, **lo)
+    ops.selective_scan(**a, cu_seqlens=cu, **lo)
+    # the last two factors are beyond the floats' end themselves, whatever they multiply
+    want, got = ref["state"].float(), a["state"]
+    mine = a["slots"].long()
+    want[mine, 6:] = want[mine, 6:].sign() * math.inf
+    assert torch.equal(torch.isinf(got), torch.isinf(want)) and torch.equal(got.sign(), want.sign())
+    finite = torch.isfinite(want)
+    assert ((got - want).abs()[finite] <= REL * want.abs()[finite].clamp(min=10.0)).all()
+
+
 def test_scan_bad_offsets_stay_in_bounds():
     """Offsets outside the rows or in the wrong order never reach outside the buffers."""
     lens = [20, 30]
