@@ -207,7 +207,8 @@ __global__ void __launch_bounds__(NT) sample_kernel(SampleArgs p, int ctas) {
   const float inv = greedy ? 1.f : fminf(fmaxf(1.f / temp, 1e-30f), 1e30f);
   const float c = inv * 1.4426950408889634f;  // logits to log2 of a probability
   const int kr = p.top_k[row], k = kr <= 0 || kr > p.V ? p.V : kr;
-  const float top_p = p.top_p[row], min_p = fminf(p.min_p[row], 1.f);
+  const float top_p = p.top_p[row], min_p = p.min_p[row];
+  const bool only_first = !(top_p > 0.f) || !(min_p <= 1.f);  // nothing else passes such a rule, NaN among them
   const bool by_rank = !greedy && k < p.V, by_mass = !greedy && top_p < 1.f;
   int turn = 0;
 
@@ -272,7 +273,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(SampleArgs p, int ctas) {
 
   // The race over line r: tokens with y = (top - x) c bins below `limit` (bins left in, min_p) and, in
   // later rounds, ranked before (bound_l, bound_i).
-  float limit = min_p > 0.f ? -__log2f(min_p) * bins * (1.f + 1e-6f) + 1e-30f : INFINITY;
+  float limit = only_first ? -1.f : min_p > 0.f ? -__log2f(min_p) * bins * (1.f + 1e-6f) + 1e-30f : INFINITY;
   float bound_l = 0.f;
   int bound_i = 0;
   bool bounded = false;

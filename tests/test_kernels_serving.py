@@ -493,6 +493,21 @@ def test_sample_ties():
     assert (ops.sample(logits, noise)[0] == 20).all()
 
 
+@pytest.mark.parametrize("kw", [dict(min_p=1.5), dict(min_p=math.nan), dict(top_p=0.0), dict(top_p=-1.0), dict(top_p=math.nan),
+                                dict(top_p=math.nan, top_k=5), dict(min_p=2.0, top_p=0.5, top_k=7)])
+@pytest.mark.parametrize("B,V", [(3, 3000), (1, 70000)])
+def test_sample_rules_that_only_the_first_passes(kw, B, V):
+    """Settings that no mass can meet keep the first token alone, not those as likely as it, and not all."""
+    logits = torch.zeros(B, V, device=dev)
+    logits[:, 7:40] = 3.0
+    noise = torch.ones(B, V, device=dev)
+    noise[:, 20] = 1e-9  # as likely as the first, and the winner of any race
+    tokens, logprobs = ops.sample(logits, noise, temperature=0.9, **kw)
+    want, wantp = R.sample(logits, noise, temperature=0.9, **kw)
+    assert (tokens == 7).all() and torch.equal(tokens, want)
+    assert ((logprobs - wantp).abs() <= 1e-5 * (1 + wantp.abs())).all()
+
+
 def test_sample_masked_rows():
     low = torch.finfo(BF).min
     B, V = 7, 2000
