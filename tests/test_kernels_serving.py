@@ -286,6 +286,18 @@ def test_scan_on_another_stream_and_empty():
     assert ops.selective_scan(**rows).shape == (2, 0, 128)
 
 
+def test_calls_repeat_themselves():
+    """The same call on the same states gives the same bits, cut into segments or not."""
+    for lens in ([1] * 5, [3, 9, 1], [700, 17, 1, 333], [4000]):
+        first = None
+        for _ in range(3):
+            a, b = _scan_inputs(lens, 256, 64, 128, BF, seed=2), _gdn_inputs([min(l, 40) for l in lens], 2, 128, BF, seed=2)
+            now = (ops.selective_scan(**a, cu_seqlens=_cu(lens)), a["state"], a["conv_state"],
+                   ops.gdn2_recurrent(**b, cu_seqlens=_cu([min(l, 40) for l in lens])), b["state"], b["conv_state"])
+            first = first or now
+            assert all(torch.equal(s, t) for s, t in zip(first, now))
+
+
 def test_scan_refusals():
     a = _scan_inputs([4], 128, 64, 64, BF)
     cu = _cu([4])
@@ -399,6 +411,62 @@ def test_gdn_matches_chunked_scan():
     serial, h64 = R.gdn2_token_serial(q, k, v, gl, torch.sigmoid(b), torch.sigmoid(w))
     # the chunked kernel's operands are bf16 (2^-9 each); the token form starts from its state
     assert (hf - h64).norm() <= 2e-2 * h64.norm()
+
+
+@pytest.mark.parametrize("lens", [[800], [70, 769, 1]])
+def test_gdn_prompt_forms_hand_over(lens):
+    """The two forms that a prompt can take in serving, the chunked scan of training and the token form, from the same
+    projections and state; then single tokens on the state of either.  Against 64 bits: the token form keeps its own
+    bound.  The chunked kernel multiplies bf16 operands (2^-9 each, a few in a row: 2e-2 of the state, as above); with
+    unit keys and gates below 1 no later token makes an error of the state larger."""
+    from atomic_ai_hybrid_b200 import get_preset
+    from atomic_ai_hybrid_b200.models.mixers import GatedDeltaNet2
+    from atomic_ai_hybrid_b200.serving.state import DecodeState, serving
+
+    torch.manual_seed(0)
+    cfg = get_preset("hybrid_1b", d_model=256, n_heads=2)
+    with torch.device(dev):
+        mod = GatedDeltaNet2(cfg)
+        mod.compute_dtype = BF
+    B, d, T, after = len(lens), 256, sum(lens), 6
+    g = _gen(3)
+    rows = [torch.randn(1, T + after * B, d, generator=g, device=dev).to(BF) for _ in range(6)]
+    start = torch.randn(B, 3, 3, d, generator=g, device=dev).to(BF), torch.randn(B, 2, 128, 128, generator=g, device=dev) * 0.1
+    par = dict(conv_w=[getattr(mod, f"{n}_conv_w").detach() for n in "qkv"],
+               conv_b=[getattr(mod, f"{n}_conv_b").detach() for n in "qkv"], decay_a=mod.decay_a.detach())
+    prompt, cu = [t[:, :T] for t in rows], _cu(lens)
+    c64 = dict(conv=start[0].double(), state=start[1].double())
+    o64 = R.gdn2_recurrent(*(t[0].double() for t in prompt), **_d(par), conv_state=c64["conv"], state=c64["state"], cu_seqlens=cu)
+
+    def states(form):
+        st = DecodeState(mod, B)
+        c = st.layers[mod]
+        c["conv"].copy_(start[0])
+        c["state"].copy_(start[1])
+        if form == "chunked":
+            with torch.no_grad(), serving(st, list(range(B)), lens) as call:
+                return c, call._gdn2_chunked(mod, c, prompt)
+        return c, ops.gdn2_recurrent(*(t[0] for t in prompt), **par, conv_state=c["conv"], state=c["state"], cu_seqlens=cu)
+
+    size = c64["state"].norm()
+    for form, tol in (("tokens", REL), ("chunked", 2e-2)):
+        c, o = states(form)
+        s64 = {n: t.clone() for n, t in c64.items()}
+        own = dict(conv=c["conv"].double(), state=c["state"].double())
+        assert torch.equal(own["conv"], s64["conv"])
+        print(f"[gdn prompt] {lens} {form}: state {(own['state'] - s64['state']).norm() / size:.1e}, outputs {(o - o64).norm() / o64.norm():.1e}")
+        assert (own["state"] - s64["state"]).norm() <= tol * size
+        assert (o - o64).norm() <= (tol + 2.0 ** -8) * o64.norm()
+        for k in range(after):
+            now = [t[0, T + k * B:T + (k + 1) * B] for t in rows]
+            y = ops.gdn2_recurrent(*now, **par, conv_state=c["conv"], state=c["state"])
+            truth = R.gdn2_recurrent(*_d(now), **_d(par), conv_state=s64["conv"], state=s64["state"])
+            cont = R.gdn2_recurrent(*_d(now), **_d(par), conv_state=own["conv"], state=own["state"])
+            assert ((y - cont).abs() <= 2.0 ** -8 * cont.abs() + REL * math.sqrt(128)).all()
+            assert (y - truth).norm() <= 2.0 ** -8 * truth.norm() + tol * size
+        assert torch.equal(c["conv"].double(), s64["conv"])
+        assert ((c["state"] - own["state"]).abs() <= REL * own["state"].abs().max().clamp(min=1.0)).all()
+        assert (c["state"] - s64["state"]).norm() <= tol * size
 
 
 def test_gdn_refusals():
@@ -576,6 +644,22 @@ def test_sample_clusters_start_together(B, V, dtype):
     tokens = _check_sample(logits, noise, temperature=0.8, top_k=50, top_p=0.9)
     again = [ops.sample(logits, noise, temperature=0.8, top_k=50, top_p=0.9) for _ in range(40)]
     assert all(torch.equal(t, tokens) and torch.equal(lp, again[0][1]) for t, lp in again)
+
+
+@pytest.mark.parametrize("V,dtype", [(409592, F32), (409605, F32), (819184, BF), (819211, BF)])
+def test_sample_rows_past_shared_memory(V, dtype):
+    """Eight CTAs keep 200 KB of a row each; a longer one (the second of each pair) is read again in every pass."""
+    logits, noise = _logits(2, V + 3, dtype, seed=V)
+    for at in (0, 3):  # a row that starts on a 16-byte line and one that does not
+        l, q = logits[:, at:at + V], noise[:, at:at + V]
+        for kw in (dict(), dict(temperature=0.0), dict(temperature=0.7, top_k=40), dict(top_p=0.8, temperature=2.0),
+                   dict(min_p=0.1), dict(temperature=1.3, top_k=1000, top_p=0.95, min_p=0.001)):
+            _check_sample(l, q, **kw)
+    logits[0, V // 2:] = -math.inf
+    logits[1] = -math.inf
+    logits[1, V - 2] = 3.0
+    _check_sample(logits, noise, top_p=0.9)
+    assert ops.sample(logits, noise)[0][1] == V - 2
 
 
 def test_sample_refusals():
