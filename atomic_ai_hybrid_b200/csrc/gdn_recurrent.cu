@@ -73,7 +73,7 @@ AHB_DEVICE void store4(T* p, const float4& v) {
 // Bound by the state's bytes.  The state waits in shared memory (asynchronous copies, 64 KB at D = 128), not
 // in registers, so that three blocks share an SM and one's arithmetic hides behind the others' copies: 128
 // sequences of 16 heads take 55 us, 0.78 of the copy rate (72 us from registers with two blocks an SM).  One
-// sequence: 5.2 us, its 16 blocks' chain of loads, sums and stores.
+// sequence: 5.5 us, its 16 blocks' chain of loads, sums and stores.
 template <typename T, typename W, int D>
 __global__ void __launch_bounds__(2 * D, 3) gdn_token_kernel(GdnArgs p) {
   constexpr int Q = D / 4, R = D / 8, NW = D / 32;
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(2 * D, 3) gdn_token_kernel(GdnArgs p) {
 // The state stays in registers from token to token.  The tokens' convolutions, norms and gates depend on
 // no state and are made for up to TB tokens at once while the state is on its way; then each token costs one
 // sweep (the last token's update, this one's decay and both sums) and one barrier.  16 sequences of 1 to 8 tokens,
-// 6 heads: 13.9 us, the dependent sweeps (1.1 us each) of 96 blocks.
+// 6 heads: 14.2 us, the dependent sweeps (1.1 us each) of 96 blocks.
 constexpr int TB = 8;
 
 template <typename T, typename W, int D>

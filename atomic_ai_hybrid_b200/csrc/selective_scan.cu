@@ -58,7 +58,8 @@ AHB_DEVICE int sum_index(int lane) {
 }
 
 // ---------------------------------------------------------------- a few tokens per sequence, or fp32
-// Bound by the chain from token to token: 0.45 us each (2048 channels), the state read and written once a call.
+// Bound by the chain from token to token: 0.5 us each (2048 channels, 64 tokens in bf16 or 1024 in fp32; 0.7 us in 8192,
+// whose rows come from HBM), the state read and written once a call.
 // One warp carries CH channels of one sequence through its tokens: lane l holds states
 // [l V, l V + V) of each channel in registers (N = 32 V), lanes 0..CH-1 also hold the convolution
 // window of one channel and turn its row into (decay, dt xc).
@@ -299,7 +300,7 @@ void launch_token(const ScanArgs& p, cudaStream_t st) {
 // finds every segment's state from zero and its decay, the next one hands the states on from segment to
 // segment (scan_join_kernel), and the last one runs the segments from their true states with outputs.
 //
-// One prompt of 8192 tokens, 2048 channels, 128 states: 215 us (17 ms token by token), 8 of 2048 tokens with
+// One prompt of 8192 tokens, 2048 channels, 128 states: 215 us (5.9 ms token by token, in fp32), 8 of 2048 tokens with
 // 4096 channels: 559 us.  Neither HBM (8 %) nor the tensor pipe (38 %) is the end of it: 1.9 thousand
 // instructions for 16 channels of a block issue 47 % of the time at the 16 warps that 128 registers leave.
 struct PromptArgs {
@@ -991,7 +992,8 @@ int by_state(const ScanArgs& p, int N, int seg, float* work, cudaStream_t st) {
 
 int ahb_selective_scan_plan(int B, int L, int T, int C, int N, int packed, int dtype, int64_t* floats) {
   *floats = 0;
-  // Blocks from 16 tokens a sequence on average (the host knows no more of packed ones).  One sequence of 2048
+  // Blocks from 16 tokens a sequence on average (the host knows no more of packed ones, so a prompt among many single
+  // tokens goes token by token: 512 tokens beside 64 of them 286 us, alone 59).  One sequence of 2048
   // channels: 8 tokens 7.3 us token by token and 10.4 us in blocks, 16 tokens 11.2 and 10.4, 32 tokens 19 and 11;
   // 128 sequences: 123 and 190, 212 and 194, 395 and 203 us.
   if (dtype != AHB_BF16 || B == 0 || T < 16 * (int64_t)B) return 0;

@@ -170,7 +170,8 @@ def selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, cu_seqle
     each.  ``conv_state (S, 3, C)`` holds the last three rows of ``x`` in its dtype and ``state
     (S, H, P, N)`` the fp32 scan state; both are updated in place.  Sequence ``i`` owns slot
     ``slots[i]`` (int32, all different; default ``i``); one with a slot outside ``[0, S)`` is padding:
-    zeros come out and no state is touched.  Returns ``y`` shaped like ``x``."""
+    zeros come out and no state is touched.  The state moves past every token given: to go back, as after drafted
+    tokens that were not accepted, copy the slots before.  Returns ``y`` shaped like ``x``."""
     if x.is_cuda and _IMPL == "cuda":
         return _k().selective_scan(x, dt, A, Bm, Cm, conv_w, conv_b, conv_state, state, cu_seqlens, slots, dt_min,
                                    dt_max)
@@ -205,10 +206,13 @@ def sample(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     numbers or ``(B,)`` tensors.  Tokens are ranked by (logit descending, index ascending); of the
     row's distribution ``softmax(logits / temperature)`` those are kept whose rank is below ``top_k``
     (0 or less: no limit), with less than ``top_p`` of the mass ranked before them (the first one
-    always), and with at least ``min_p`` times the first one's probability.  The token is the kept
+    always), and with at least ``min_p`` times the first one's probability.  Each rule looks at the whole tempered row:
+    ``top_p`` counts the mass of tokens that ``top_k`` cuts too, where samplers that renormalise after ``top_k`` keep
+    fewer tokens for the same settings.  A rule that no mass can meet (``top_p <= 0``, ``min_p > 1``, NaN) keeps the
+    first token alone.  The token is the kept
     one with the largest ``log p - log noise`` (ties: lowest index), which draws from the kept ones by
-    their probability (a row without any such score gives the first).  ``temperature <= 0`` takes the first token and tempers by 1 for ``logprobs``,
-    the log-probability before anything is cut.  NaN and ``-inf`` logits are never drawn; a row
+    their probability (a row without any such score gives the first).  ``temperature <= 0`` takes the first token and
+    tempers by 1 for ``logprobs``, the log-probability before anything is cut.  NaN and ``-inf`` logits are never drawn; a row
     of nothing else gives token -1 and ``-inf``."""
     if logits.is_cuda and _IMPL == "cuda":
         return _k().sample(logits, noise, temperature, top_k, top_p, min_p)

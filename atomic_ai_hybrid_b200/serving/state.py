@@ -31,6 +31,9 @@ _SERVING: contextvars.ContextVar[Optional["_Call"]] = contextvars.ContextVar("se
 # 16 heads of 128, chunked against token by token: 1 sequence of 512 tokens 1.20 and 0.94 ms, 768 1.21 and 1.27,
 # 4096 1.8 and 5.7; 4 sequences of 768 1.50 and 1.40, 1024 1.65 and 1.75, 4096 4.4 and 6.3; 6 of 1024 2.06 and 1.84,
 # 4096 6.4 and 6.8; 32 of 1024 8.3 and 5.5.
+# The chunked scan multiplies bf16 operands, as in the training forward that the weights come from: its state after 800
+# tokens is 4e-3 off the 64-bit one, token by token (fp32 throughout) 1e-7.  So which form a prompt took, by its length
+# and by how many others came with it, shows in its answer's last digits; the later tokens add nothing to it.
 GDN_CHUNKED_FROM, GDN_CHUNKED_HEADS = 768, 64
 
 
