@@ -19,8 +19,8 @@
 // infinities replaced), so the logits leave HBM once; partial results meet through distributed shared
 // memory and every CTA combines them in the same order.
 //
-// 1 x 151936 with every rule 10.3 us, 64 x 50304 16 us: three passes over shared memory and four meetings of the
-// cluster, one after another.  256 x 128256 fp32 120 us (greedy 57 us): 56 instructions a value; the noise of
+// 1 x 151936 with every rule 10.1 us, 64 x 50304 16 us: three passes over shared memory and four meetings of the
+// cluster, one after another.  256 x 128256 fp32 119 us (greedy 57 us): 56 instructions a value; the noise of
 // tokens that are cut is not read, 200 MB move in place of 263.
 #include "launchers.h"
 #include "packed.cuh"
@@ -522,16 +522,16 @@ int ahb_sample(const void* logits, int64_t ls, int dtype, const float* noise, in
   const int N = dtype == AHB_BF16 ? 8 : 4;
   const int lines = (V + N - 1) / N + 1;  // one more where a row starts inside a line
   // Split a row while its part would keep a second CTA off the SM (over 96 KB), or while the rows alone do
-  // not fill the SMs and a part still has four lines for every thread.  1 x 151936 bf16: 8 CTAs 10.3 us, 4 12.9,
-  // 2 18.3; 64 x 50304: 4 CTAs 16 us, 2 17.2, 8 17.8.  256 x 128256 fp32 (501 KB a row): 8 CTAs 120 us, 4 148, 2 218.
+  // not fill the SMs and a part still has four lines for every thread.  1 x 151936 bf16: 8 CTAs 10.1 us, 4 12.9,
+  // 2 18.3; 64 x 50304: 4 CTAs 16 us, 2 17.2, 8 17.8.  256 x 128256 fp32 (501 KB a row): 8 CTAs 119 us, 4 148, 2 218.
   int ctas = 1;
   while (ctas < 8 && ((lines / ctas) * 16 > 96 * 1024 || (B * ctas < 148 && lines / ctas >= 2048))) ctas *= 2;
   p.chunk = (lines + ctas - 1) / ctas;
   size_t smem = (size_t)p.chunk * 16;
   p.resident = smem <= (size_t)kMaxSlice;
   if (!p.resident) smem = 0;
-  // 512 threads while all CTAs are on the SMs at once: more warps to hide each other's latency (1 x 151936: 10.3 us,
-  // 256 threads 10.9).  Beyond that 256, so that more clusters overlap (256 x 128256 fp32: 120 us, 512 threads 223).
+  // 512 threads while all CTAs are on the SMs at once: more warps to hide each other's latency (1 x 151936: 10.1 us,
+  // 256 threads 10.9).  Beyond that 256, so that more clusters overlap (256 x 128256 fp32: 119 us, 512 threads 223).
   if (B * ctas <= 2 * 148)
     return dtype == AHB_BF16 ? launch<__nv_bfloat16, 512>(p, B, ctas, smem, st) : launch<float, 512>(p, B, ctas, smem, st);
   return dtype == AHB_BF16 ? launch<__nv_bfloat16, 256>(p, B, ctas, smem, st) : launch<float, 256>(p, B, ctas, smem, st);
