@@ -23,12 +23,6 @@ def lecun_normal_(t: torch.Tensor, fan_in: int) -> torch.Tensor:
         return nn.init.trunc_normal_(t, 0.0, std, -2 * std, 2 * std)
 
 
-def serving_call():
-    """The running ``serving(...)`` call (tokens on kept state), or None."""
-    from ..serving.state import get_serving
-    return get_serving()
-
-
 def tp_world_rank():
     """(world, rank) of the tensor-parallel group the model is built for."""
     from ..parallel.context import get_parallel_context

@@ -19,7 +19,8 @@ from ..ops import reference as R
 from ..parallel.cp import get_cp
 from ..parallel.tp import get_tp, mark_shard, shard_tensor, tp_rmsnorm
 from ..utils.diag import DIAG
-from .layers import Dense, RMSNorm, lecun_normal_, serving_call, tp_world_rank
+from ..utils.serving_call import get_serving
+from .layers import Dense, RMSNorm, lecun_normal_, tp_world_rank
 
 
 def _shard_vec(full: torch.Tensor) -> nn.Parameter:
@@ -90,7 +91,7 @@ class GatedDeltaNet2(nn.Module):
         return self.out_proj(o)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        sv = serving_call()
+        sv = get_serving()
         if sv is not None:
             return sv.gdn2(self, x)
         cp = get_cp()
@@ -192,7 +193,7 @@ class Mamba2(nn.Module):
         return self.out_proj(out)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        sv = serving_call()
+        sv = get_serving()
         if sv is not None:
             return sv.mamba2(self, x)
         cp = get_cp()
@@ -256,7 +257,7 @@ class MLA(nn.Module):
         self.W_o = Dense(d, d, tp="row")
 
     def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
-        sv = serving_call()
+        sv = get_serving()
         if sv is not None:
             return sv.mla(self, x)
         H = self.n_heads

@@ -28,7 +28,8 @@ from .. import ops
 from ..config import ModelConfig
 from ..ops import reference as R
 from ..parallel.context import dp_mean, get_parallel_context
-from .layers import Dense, lecun_normal_, serving_call
+from ..utils.serving_call import get_serving
+from .layers import Dense, lecun_normal_
 
 ROUTER_LOGIT_CLIP = 8.0
 ROUTER_TEMP_INIT = 10.0
@@ -81,11 +82,11 @@ class MoE(nn.Module):
     @staticmethod
     def _over_ranks(t: torch.Tensor) -> torch.Tensor:
         """A statistic's mean over the data-parallel ranks; its own in a serving call, which one rank makes alone."""
-        return dp_mean(t) if serving_call() is None else t
+        return dp_mean(t) if get_serving() is None else t
 
     def _noisy(self) -> bool:
         """Router noise and dropout are for training forwards; a serving call has none, whatever the mode."""
-        return self.training and serving_call() is None
+        return self.training and get_serving() is None
 
     def route(self, flat_x: torch.Tensor, stats: Dict[str, torch.Tensor]):
         E, k = self.E, self.k

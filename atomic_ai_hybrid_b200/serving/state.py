@@ -8,7 +8,6 @@ conversations and its mixers run on this state; everything else in the model is 
 from __future__ import annotations
 
 import contextlib
-import contextvars
 import math
 from typing import Dict, List, Optional
 
@@ -21,9 +20,8 @@ from ..models.moe import MoE
 from ..ops import reference as R
 from ..parallel.cp import get_cp
 from ..parallel.tp import get_tp
-
-# the running call of this thread (of this context): forwards elsewhere are ordinary ones meanwhile
-_SERVING: contextvars.ContextVar[Optional["_Call"]] = contextvars.ContextVar("serving", default=None)
+from ..utils import serving_call
+from ..utils.serving_call import get_serving
 
 # GDN-2 prompts of at least this many tokens, in at most this many (sequence, head) pairs, run on the chunked
 # training scan.  It runs a head's chunks side by side, but each call pays 0.9 ms of separate launches for padding,
@@ -35,11 +33,6 @@ _SERVING: contextvars.ContextVar[Optional["_Call"]] = contextvars.ContextVar("se
 # tokens is 4e-3 off the 64-bit one, token by token (fp32 throughout) 1e-7.  So which form a prompt took, by its length
 # and by how many others came with it, shows in its answer's last digits; the later tokens add nothing to it.
 GDN_CHUNKED_FROM, GDN_CHUNKED_HEADS = 768, 64
-
-
-def get_serving():
-    """The ``_Call`` that this thread is in, or None outside ``serving(...)``."""
-    return _SERVING.get()
 
 
 class DecodeState:
@@ -246,7 +239,7 @@ def serving(state: DecodeState, slots: List[int], lens: Optional[List[int]] = No
     after another, ``lens[i]`` of them each (None: one each; ``fresh``: as new conversations).  ``slots_dev`` is
     ``slots`` as an int32 tensor on the device, where the caller has it.  It holds for the thread that enters it; a
     state serves one call at a time."""
-    if _SERVING.get() is not None:
+    if get_serving() is not None:
         raise RuntimeError("serving(...) is not nested")
     state.check_slots(slots)
     if lens is not None and (len(lens) != len(slots) or min(lens, default=1) < 1):
@@ -257,10 +250,10 @@ def serving(state: DecodeState, slots: List[int], lens: Optional[List[int]] = No
     if fresh:
         state.reset(slots)
     call = _Call(state, slots, lens, slots_dev)
-    token = _SERVING.set(call)
+    token = serving_call.enter(call)
     try:
         yield call
         for s, n in zip(slots, lens or [1] * len(slots)):
             state.lengths[s] += n
     finally:
-        _SERVING.reset(token)
+        serving_call.leave(token)

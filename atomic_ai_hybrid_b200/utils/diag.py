@@ -25,6 +25,8 @@ from typing import Dict, List, Optional, Tuple
 
 import torch
 
+from .serving_call import get_serving
+
 STAGES = os.environ.get("GDN2_FWD_DIAG", "0") == "1"
 ALWAYS = os.environ.get("AHB_STEP_DIAG", "1") == "1"
 _CAP = 4096
@@ -41,6 +43,8 @@ class Diagnostics:
 
     # ------------------------------------------------------------ recording
     def _slot(self, kind: str, tag: str, device) -> Optional[int]:
+        if get_serving() is not None:
+            return None  # an answer's forward is no part of a training step
         key = (kind, tag)
         i = self.slots.get(key)
         if i is not None:
@@ -75,12 +79,12 @@ class Diagnostics:
 
     def nonfinite(self, tag: str, t: torch.Tensor) -> None:
         """``[FWD-DIAG]``: set when ``t`` has a NaN or an infinity."""
-        if ALWAYS:
+        if ALWAYS and get_serving() is None:
             self._put("nonfinite", tag, (~torch.isfinite(t.detach())).any())
 
     def maxabs(self, tag: str, t: torch.Tensor) -> None:
         """Largest finite magnitude of ``t`` (``[RESID-DIAG]`` above 1e3)."""
-        if ALWAYS:
+        if ALWAYS and get_serving() is None:
             self._put("maxabs", tag, torch.nan_to_num(t.detach().float(), nan=0.0, posinf=0.0, neginf=0.0)
                       .abs().amax())
 

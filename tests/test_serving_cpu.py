@@ -361,3 +361,22 @@ def test_generate_does_not_answer_with_fresh_weights(tmp_path, capsys):
     with pytest.raises(SystemExit, match="layer_2"):
         command.main(args + ["--layers", "3"])
     assert capsys.readouterr().out == ""
+
+
+def test_answers_leave_the_training_diagnostics():
+    """What an answer meets is not reported as the training step's, and its forwards take no diagnostic buffer (a
+    captured token step would keep that buffer's address)."""
+    from atomic_ai_hybrid_b200.utils.diag import DIAG
+
+    for preset, kw in (("tiny", dict(num_layers=2, layer_types=("mamba2", "gdn2"))), ("reference_tiny", {})):
+        DIAG.__init__()
+        model, cfg = _model(preset, **kw)
+        with torch.no_grad():
+            for n, p in model.named_parameters():
+                if n.endswith("out_proj.kernel"):
+                    p[0, 0] = math.nan
+        Generator(model, 1, max_len=8).prefill([[1, 2, 3]], [0])
+        assert DIAG.buf is None and DIAG.order == []
+        with torch.no_grad():
+            model(torch.ones(1, 64, dtype=torch.long))
+        assert DIAG.order  # an ordinary forward does
