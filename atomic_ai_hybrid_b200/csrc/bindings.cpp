@@ -1722,7 +1722,8 @@ torch::Tensor selective_scan(const torch::Tensor& x, const torch::Tensor& dt, co
   auto y = new_output({T, C}, x.scalar_type(), x);
   if (q.B == 0) y.zero_();  // no sequence, and no kernel
   int64_t floats = 0;
-  const int seg = ahb_selective_scan_plan(q.B, q.L, (int)T, (int)C, (int)N, q.cu != nullptr, dt_code(x), &floats);
+  int kernels = 0;
+  const int seg = ahb_selective_scan_plan(q.B, q.L, (int)T, (int)C, (int)N, q.cu != nullptr, dt_code(x), &floats, &kernels);
   torch::Tensor work;
   if (floats > 0) work = new_output({floats}, at::kFloat, x);
   const int rc = ahb_selective_scan(x.data_ptr(), x.stride(0), dt.data_ptr(), dt.stride(0), A.data_ptr<float>(),
@@ -1734,6 +1735,16 @@ torch::Tensor selective_scan(const torch::Tensor& x, const torch::Tensor& dt, co
   TORCH_CHECK(rc == 0, op, ": failed with code ", rc, " for ", N, " states");
   check_launch(op);
   return y;
+}
+
+// The kernels that selective_scan launches for these arguments
+int64_t selective_scan_kernels(const torch::Tensor& x, const torch::Tensor& state, int64_t L,
+                               const c10::optional<torch::Tensor>& cu) {
+  const int64_t T = x.size(0), B = cu.has_value() ? cu->numel() - 1 : (L > 0 ? T / L : 0);
+  int64_t floats = 0;
+  int kernels = 0;
+  ahb_selective_scan_plan((int)B, (int)L, (int)T, (int)x.size(1), (int)state.size(3), cu.has_value(), dt_code(x), &floats, &kernels);
+  return kernels;
 }
 
 torch::Tensor gdn2_recurrent(const std::vector<torch::Tensor>& in, const std::vector<torch::Tensor>& conv_w,
@@ -1903,6 +1914,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sum_slots", &sum_slots);
   m.def("memcpy_async", &memcpy_async);
   m.def("selective_scan", &selective_scan);
+  m.def("selective_scan_kernels", &selective_scan_kernels);
   m.def("gdn2_recurrent", &gdn2_recurrent);
   m.def("sample", &sample);
 }

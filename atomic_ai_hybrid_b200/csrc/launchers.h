@@ -254,8 +254,8 @@ void ahb_ce_combine(const void* partials, int ntiles, const int64_t* labels, int
 // stride.  Return 0, -1 for a size without a kernel, -2 for too many sequences.
 // selective_scan.cu: x, dt (T, C), Bm, Cm (T, N), conv_w (C, 4), conv_state (S, 3, C), state
 // (S, C / P, P, N) fp32, y (T, C); N in {32, 64, 128}.  ahb_selective_scan_plan: the tokens per segment of
-// the prompt form (0: the token form) and the fp32 values of workspace it needs.
-int ahb_selective_scan_plan(int B, int L, int T, int C, int N, int packed, int dtype, int64_t* floats);
+// the prompt form (0: the token form), the fp32 values of workspace it needs and the kernels that the call launches.
+int ahb_selective_scan_plan(int B, int L, int T, int C, int N, int packed, int dtype, int64_t* floats, int* kernels);
 int ahb_selective_scan(const void* x, int64_t xs, const void* dt, int64_t dts, const float* A, const void* Bm,
                        int64_t bs, const void* Cm, int64_t cs, const void* conv_w, int wdtype, const float* conv_b,
                        void* conv_state, float* state, const int* cu, const int* slots, void* y, int B, int L, int T,

@@ -990,8 +990,9 @@ int by_state(const ScanArgs& p, int N, int seg, float* work, cudaStream_t st) {
 
 }  // namespace
 
-int ahb_selective_scan_plan(int B, int L, int T, int C, int N, int packed, int dtype, int64_t* floats) {
+int ahb_selective_scan_plan(int B, int L, int T, int C, int N, int packed, int dtype, int64_t* floats, int* kernels) {
   *floats = 0;
+  *kernels = T == 0 || B == 0 ? 0 : 1;
   // Blocks from 16 tokens a sequence on average (the host knows no more of packed ones, so a prompt among many single
   // tokens goes token by token: 512 tokens beside 64 of them 286 us, alone 59).  One sequence of 2048
   // channels: 8 tokens 7.3 us token by token and 10.4 us in blocks, 16 tokens 11.2 and 10.4, 32 tokens 19 and 11;
@@ -1013,6 +1014,7 @@ int ahb_selective_scan_plan(int B, int L, int T, int C, int N, int packed, int d
   }
   seg = std::min<int64_t>(1 << 30, std::max<int64_t>(128, (seg + kBlock - 1) / kBlock * kBlock));
   const int64_t segs = max_segments(B, L, T, packed != 0, (int)seg);
+  *kernels = segs > B ? 4 : 2;
   const int64_t rows = (int64_t)(2 * kBlock * N + 2 * kBlock * kBlock) / 2;  // of a block, in floats
   *floats = max_segments(B, L, T, packed != 0, kBlock) * rows + (segs > B ? segs * C * (N + 1) : 0);
   return (int)seg;

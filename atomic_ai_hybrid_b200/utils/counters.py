@@ -5,10 +5,16 @@ the call's arguments)."""
 from __future__ import annotations
 
 
+def _scan_kernels(a, k):
+    from ..ops._ext import ext
+    # selective_scan(x, dt, A, B, C, conv_w, conv_b, conv_state, state, tokens a row, cu_seqlens, ...)
+    return ext()._mod.selective_scan_kernels(a[0], a[8], a[9], a[10])
+
+
 class LaunchCounter:
     MULTI = {"gdn_fwd": 2, "gdn_fwd_train": 2, "gdn_bwd": 4, "gdn_bwd_saved": 2, "ssd_fwd": 2, "ssd_fwd_train": 2,
              "ssd_bwd": 4, "moe_fwd": 7, "moe_bwd": 8, "ce_online_fwd": 2, "add_rmsnorm_bwd": 2,
-             "norm_gate_bwd": 2,
+             "norm_gate_bwd": 2, "selective_scan": _scan_kernels,
              # three GEMMs per row chunk: ce_online_bwd(h, W, labels, lse, ls, g, dW_acc, chunk_rows)
              "ce_online_bwd": lambda a, k: 3 * -(-a[0].shape[0] // a[7])}
 

@@ -298,6 +298,31 @@ def test_calls_repeat_themselves():
             assert all(torch.equal(s, t) for s, t in zip(first, now))
 
 
+@pytest.mark.parametrize("lens,dtype,kernels", [([1] * 3, BF, 1), ([5, 3], BF, 1), ([40, 40], BF, 2), ([3000], BF, 4), ([64], F32, 1)])
+def test_scan_launches_are_counted(lens, dtype, kernels):
+    """The launch counter's figure is the number of kernels in the call's CUDA graph."""
+    from cuda.bindings import runtime
+    from atomic_ai_hybrid_b200.utils.counters import launch_counter
+
+    a, cu = _scan_inputs(lens, 256, 64, 128, dtype, seed=1), _cu(lens)
+    ops.selective_scan(**a, cu_seqlens=cu)
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    before, was = launch_counter.count, launch_counter.on
+    launch_counter.enable()
+    with torch.cuda.graph(graph):
+        ops.selective_scan(**a, cu_seqlens=cu)
+    counted = launch_counter.count - before
+    if not was:
+        launch_counter.disable()
+    launch_counter.count = before
+    handle = graph.raw_cuda_graph()
+    _, _, n = runtime.cudaGraphGetNodes(handle)
+    _, nodes, _ = runtime.cudaGraphGetNodes(handle, n)
+    kinds = [runtime.cudaGraphNodeGetType(node)[1] for node in nodes]
+    assert kinds.count(runtime.cudaGraphNodeType.cudaGraphNodeTypeKernel) == kernels
+    assert counted == kernels
+
+
 def test_scan_refusals():
     a = _scan_inputs([4], 128, 64, 64, BF)
     cu = _cu([4])
