@@ -153,7 +153,9 @@ class Generator:
         """Answers to ``prompts`` (lists of token ids, at most ``max_sequences`` non-empty ones): returns
         ``(tokens, logprobs)``, one list per prompt, each at most ``max_new_tokens`` long and ending with
         ``stop_token`` where it was drawn.  The settings are numbers or one value per prompt;
-        ``generator`` (on the model's device) makes the noise."""
+        ``generator`` (on the model's device) makes the noise.  The prompts are new conversations in slots 0 to
+        ``len(prompts) - 1``, which later hold every token that was run, those after a stop among them: conversations of
+        ``prefill`` and ``step`` belong in other slots or another ``Generator``."""
         B = len(prompts)
         if not 1 <= B <= self.state.slots:
             raise ValueError(f"{B} prompts, room for {self.state.slots}")
