@@ -7,7 +7,9 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
+#include "cached_attention.h"
 #include "launchers.h"
+#include <cmath>
 #include <cstdlib>
 #include <map>
 #include <mutex>
@@ -1821,6 +1823,178 @@ std::tuple<torch::Tensor, torch::Tensor> sample(const torch::Tensor& logits, con
   return {tokens, logprobs};
 }
 
+// cache rows and what is kept of them
+void check_cache(const torch::Tensor& k, const torch::Tensor& v, const char* op) {
+  TORCH_CHECK(k.is_cuda() && k.dim() == 4 && k.is_contiguous() && v.sizes() == k.sizes() && v.is_contiguous() &&
+                  v.device() == k.device() && v.scalar_type() == k.scalar_type(),
+              op, ": k_cache and v_cache must be contiguous (slots, key heads, rows, head dim) CUDA tensors of one type");
+  TORCH_CHECK(k.data_ptr() != v.data_ptr() || k.numel() == 0, op, ": k_cache and v_cache must be different tensors");
+  TORCH_CHECK(k.size(1) > 0 && k.size(2) > 0 && k.size(3) > 0 && k.size(0) < (1ll << 30) && k.size(1) < (1ll << 15) &&
+                  k.size(2) < (1ll << 30) && k.size(3) < (1ll << 16),
+              op, ": cache sizes out of range, got ", k.sizes());
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(k.data_ptr()) | reinterpret_cast<uintptr_t>(v.data_ptr())) % 16 == 0, op,
+              ": the caches must start at 16-byte boundaries");
+}
+
+torch::Tensor cached_attention(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                               const torch::Tensor& k_cache, const torch::Tensor& v_cache, const torch::Tensor& lengths,
+                               const c10::optional<torch::Tensor>& cos, const c10::optional<torch::Tensor>& sin, int64_t L,
+                               const c10::optional<torch::Tensor>& cu, const c10::optional<torch::Tensor>& slots,
+                               const c10::optional<torch::Tensor>& prefix, const c10::optional<torch::Tensor>& seen,
+                               const c10::optional<torch::Tensor>& mass, const c10::optional<torch::Tensor>& held,
+                               double scale) {
+  const char* op = "cached_attention";
+  TORCH_CHECK(q.is_cuda() && q.dim() == 2, op, ": q must be a CUDA tensor of (tokens, channels) rows");
+  check_cache(k_cache, v_cache, op);
+  TORCH_CHECK(k_cache.device() == q.device() && k_cache.scalar_type() == at::kBFloat16 && q.scalar_type() == at::kBFloat16, op,
+              ": q and the caches must be bf16 tensors on one device, got ", q.scalar_type(), " on ", q.device(), " and ",
+              k_cache.scalar_type(), " on ", k_cache.device());
+  const int64_t T = q.size(0), S = k_cache.size(0), Hk = k_cache.size(1), M = k_cache.size(2), D = k_cache.size(3);
+  TORCH_CHECK(q.size(1) > 0 && q.size(1) % (Hk * D) == 0, op, ": ", q.size(1), " channels of q do not make heads of ", D,
+              " channels shared evenly by ", Hk, " key heads");
+  const int64_t H = q.size(1) / D;
+  TORCH_CHECK(T < (1ll << 30) && H < (1ll << 15) && T * H < (1ll << 31), op, ": sizes out of range");
+  TORCH_CHECK(std::isfinite(scale), op, ": sm_scale must be finite, got ", scale);
+  check_rows(q, q, T, H * D, op, "q");
+  check_rows(k, q, T, Hk * D, op, "k");
+  check_rows(v, q, T, Hk * D, op, "v");
+  check_flat(lengths, q, at::kInt, S, op, "lengths");
+  TORCH_CHECK(cos.has_value() == sin.has_value(), op, ": cos and sin come together");
+  TORCH_CHECK(mass.has_value() == held.has_value(), op, ": mass and held come together");
+  ahb::cattn::Args a{};
+  a.table = -1;
+  if (cos.has_value()) {
+    TORCH_CHECK(cos->dim() == 2 && cos->size(1) == D && cos->size(0) < (1ll << 31), op, ": cos must have a row of ", D,
+                " values for each position, got ", cos->sizes());
+    check_flat(*cos, q, at::kFloat, cos->numel(), op, "cos");
+    check_flat(*sin, q, at::kFloat, cos->numel(), op, "sin");
+    a.cos = cos->data_ptr<float>();
+    a.sin = sin->data_ptr<float>();
+    a.table = (int)cos->size(0);
+  }
+  if (mass.has_value()) {
+    check_flat(*mass, q, at::kFloat, S * Hk * M, op, "mass (slots, key heads, rows)");
+    check_flat(*held, q, at::kInt, S * Hk * M, op, "held (slots, key heads, rows)");
+    a.mass = mass->data_ptr<float>();
+    a.held = held->data_ptr<int>();
+  }
+  const SeqArgs s = seq_args(q, T, L, S, cu, slots, op);
+  if (prefix.has_value()) {
+    check_flat(*prefix, q, at::kInt, s.B, op, "prefix");
+    a.prefix = prefix->data_ptr<int>();
+  }
+  if (seen.has_value()) {
+    check_flat(*seen, q, at::kInt, S, op, "seen");
+    a.seen = seen->data_ptr<int>();
+  }
+  const c10::cuda::CUDAGuard guard(q.device());
+  auto o = new_output({T, H * D}, q.scalar_type(), q);
+  if (T == 0) return o;
+  if (s.B == 0) return o.zero_();  // no sequence, and no kernel
+  a.q = (const ahb::cattn::bf16*)q.data_ptr();
+  a.k = (const ahb::cattn::bf16*)k.data_ptr();
+  a.v = (const ahb::cattn::bf16*)v.data_ptr();
+  a.qs = q.stride(0);
+  a.ks = k.stride(0);
+  a.vs = v.stride(0);
+  a.kc = (ahb::cattn::bf16*)k_cache.data_ptr();
+  a.vc = (ahb::cattn::bf16*)v_cache.data_ptr();
+  a.lengths = lengths.data_ptr<int>();
+  a.cu = s.cu;
+  a.slots = s.slots;
+  a.B = s.B;
+  a.L = s.L;
+  a.T = (int)T;
+  a.S = (int)S;
+  a.M = (int)M;
+  a.H = (int)H;
+  a.Hk = (int)Hk;
+  a.D = (int)D;
+  a.scale2 = (float)(scale * 1.4426950408889634);
+  a.o = (ahb::cattn::bf16*)o.data_ptr();
+  auto work = new_output({ahb_cached_attention_bytes(a)}, at::kByte, q);
+  const int rc = ahb_cached_attention(a, work.data_ptr(), cur_stream());
+  TORCH_CHECK(rc == 0, op, ": failed with code ", rc, " for head dim ", D);
+  check_launch(op);
+  return o;
+}
+
+void cache_evict(const torch::Tensor& k_cache, const torch::Tensor& v_cache, const torch::Tensor& mass,
+                 const torch::Tensor& held, const torch::Tensor& lengths, const torch::Tensor& seen, int64_t keep,
+                 int64_t recent, const c10::optional<torch::Tensor>& slots) {
+  const char* op = "cache_evict";
+  check_cache(k_cache, v_cache, op);
+  const int64_t S = k_cache.size(0), Hk = k_cache.size(1), M = k_cache.size(2);
+  const int64_t row_bytes = k_cache.size(3) * k_cache.element_size();
+  TORCH_CHECK(row_bytes % 16 == 0, op, ": rows must be a multiple of 16 bytes, got ", row_bytes);
+  TORCH_CHECK(keep >= 1 && recent >= 0 && recent <= keep, op, ": keep must be at least 1 and recent between 0 and keep");
+  check_flat(mass, k_cache, at::kFloat, S * Hk * M, op, "mass (slots, key heads, rows)");
+  check_flat(held, k_cache, at::kInt, S * Hk * M, op, "held (slots, key heads, rows)");
+  check_flat(lengths, k_cache, at::kInt, S, op, "lengths");
+  check_flat(seen, k_cache, at::kInt, S, op, "seen");
+  int64_t n = S;
+  if (slots.has_value()) {
+    n = slots->numel();
+    check_flat(*slots, k_cache, at::kInt, n, op, "slots");
+  }
+  TORCH_CHECK(n <= 65535, op, ": at most 65535 slots in one call, got ", n);
+  if (keep >= M || n == 0) return;  // nothing holds more
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  auto work = new_output({ahb_cache_evict_bytes((int)n, (int)Hk, (int)M, (int)keep)}, at::kByte, k_cache);
+  const int rc = ahb_cache_evict(k_cache.data_ptr(), v_cache.data_ptr(), mass.data_ptr<float>(), held.data_ptr<int>(),
+                                 lengths.data_ptr<int>(), seen.data_ptr<int>(),
+                                 slots.has_value() ? slots->data_ptr<int>() : nullptr, (int)n, (int)S, (int)Hk, (int)M,
+                                 (int)row_bytes, (int)keep, (int)recent, work.data_ptr(), cur_stream());
+  TORCH_CHECK(rc == 0, op, ": failed with code ", rc);
+  check_launch(op);
+}
+
+void check_logits(const torch::Tensor& logits, const torch::Tensor& tokens, const char* op) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.size(1) > 0, op,
+              ": logits must be a CUDA tensor of (rows, vocabulary)");
+  TORCH_CHECK(logits.size(1) < (1ll << 30) && logits.size(0) < (1ll << 31), op, ": sizes out of range");
+  check_rows(logits, logits, logits.size(0), logits.size(1), op, "logits");
+  check_flat(tokens, logits, at::kLong, logits.size(0), op, "tokens");
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> token_logprobs_fwd(
+    const torch::Tensor& logits, const torch::Tensor& tokens, int64_t top, double temperature) {
+  const char* op = "token_logprobs";
+  check_logits(logits, tokens, op);
+  const int64_t R = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(top >= 0 && top <= 64 && top <= V, op, ": top must lie between 0 and 64 and the vocabulary, got ", top);
+  TORCH_CHECK(temperature > 0 && (float)temperature > 0.f && std::isfinite(1.f / (float)temperature) && std::isfinite((float)temperature),
+              op, ": temperature must be positive, with a finite reciprocal, got ", temperature);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  auto lp = new_output({R}, at::kFloat, logits), entropy = new_output({R}, at::kFloat, logits);
+  auto stats = new_output({R, 4}, at::kFloat, logits);
+  auto top_tok = new_output({R, top}, at::kLong, logits), top_lp = new_output({R, top}, at::kFloat, logits);
+  ahb_token_logprobs_fwd(logits.data_ptr(), logits.stride(0), dt_code(logits), tokens.data_ptr<int64_t>(), R, (int)V,
+                         (int)top, (float)temperature, lp.data_ptr<float>(), entropy.data_ptr<float>(), stats.data_ptr(),
+                         top > 0 ? top_tok.data_ptr<int64_t>() : nullptr, top > 0 ? top_lp.data_ptr<float>() : nullptr,
+                         cur_stream());
+  check_launch(op);
+  return {lp, entropy, stats, top_tok, top_lp};
+}
+
+torch::Tensor token_logprobs_bwd(const torch::Tensor& logits, const torch::Tensor& tokens, const torch::Tensor& stats,
+                                 const torch::Tensor& g, const torch::Tensor& ge, double temperature) {
+  const char* op = "token_logprobs";
+  check_logits(logits, tokens, op);
+  const int64_t R = logits.size(0), V = logits.size(1);
+  check_flat(stats, logits, at::kFloat, R * 4, op, "stats");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const auto gc = g.to(at::kFloat).contiguous(), gec = ge.to(at::kFloat).contiguous();
+  check_flat(gc, logits, at::kFloat, R, op, "the gradient of logprobs");
+  check_flat(gec, logits, at::kFloat, R, op, "the gradient of entropy");
+  auto dx = new_output({R, V}, logits.scalar_type(), logits);
+  ahb_token_logprobs_bwd(logits.data_ptr(), logits.stride(0), dt_code(logits), tokens.data_ptr<int64_t>(), stats.data_ptr(),
+                         gc.data_ptr<float>(), gec.data_ptr<float>(), R, (int)V, (float)temperature, dx.data_ptr(),
+                         cur_stream());
+  check_launch(op);
+  return dx;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1917,4 +2091,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("selective_scan_kernels", &selective_scan_kernels);
   m.def("gdn2_recurrent", &gdn2_recurrent);
   m.def("sample", &sample);
+  m.def("cached_attention", &cached_attention);
+  m.def("cache_evict", &cache_evict);
+  m.def("token_logprobs_fwd", &token_logprobs_fwd);
+  m.def("token_logprobs_bwd", &token_logprobs_bwd);
 }

@@ -271,3 +271,20 @@ int ahb_gdn_recurrent(const void* const in[6], const int64_t rs[6], const void* 
 int ahb_sample(const void* logits, int64_t ls, int dtype, const float* noise, int64_t ns, const float* temperature,
                const int* top_k, const float* top_p, const float* min_p, int64_t* tokens, float* logprobs, int B, int V,
                cudaStream_t st);
+// cached_attention.cu: see cached_attention.h; workspace bytes of a call, and the call (0, or -1 for a head dim without kernel)
+namespace ahb { namespace cattn { struct Args; } }
+int64_t ahb_cached_attention_bytes(const ahb::cattn::Args& a);
+int ahb_cached_attention(const ahb::cattn::Args& a, void* work, cudaStream_t st);
+// cache_evict.cu: k, v caches of (S, Hk, M) rows of row_bytes (a multiple of 16), mass and held (S, Hk, M); n_slots slots
+// (null: 0 .. n_slots - 1).  Workspace bytes of a call, and the call (0, or -1 where the device refuses the shared memory).
+int64_t ahb_cache_evict_bytes(int n_slots, int Hk, int M, int keep);
+int ahb_cache_evict(void* kc, void* vc, float* mass, int* held, const int* lengths, const int* seen, const int* slots,
+                    int n_slots, int S, int Hk, int M, int row_bytes, int keep, int recent, void* work, cudaStream_t st);
+// token_logprobs.cu: logits (R, V) of `dtype` with row stride ls; stats (R, 4) carries a row's maximum, log2 of its sum
+// and entropy to the backward; top_tok, top_lp (R, top), top <= 64; dx (R, V) contiguous
+void ahb_token_logprobs_fwd(const void* logits, int64_t ls, int dtype, const int64_t* tokens, int64_t R, int V, int top,
+                            float temperature, float* lp, float* entropy, void* stats, int64_t* top_tok, float* top_lp,
+                            cudaStream_t st);
+void ahb_token_logprobs_bwd(const void* logits, int64_t ls, int dtype, const int64_t* tokens, const void* stats,
+                            const float* g, const float* ge, int64_t R, int V, float temperature, void* dx,
+                            cudaStream_t st);

@@ -218,6 +218,82 @@ def sample(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         return _k().sample(logits, noise, temperature, top_k, top_p, min_p)
     return R.sample(logits, noise, temperature, top_k, top_p, min_p)
 
+
+def cached_attention(q, k, v, k_cache, v_cache, lengths, cos=None, sin=None, cu_seqlens=None, slots=None, prefix=None,
+                     seen=None, mass=None, held=None, sm_scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of new tokens over a kept cache, into which their keys and values go first; no gradient.
+
+    ``q`` has ``H D`` channels, ``k`` and ``v`` have ``Hk D`` (query head ``h`` reads key head ``h // (H // Hk)``),
+    before rotation; tokens, ``cu_seqlens`` and ``slots`` as in ``selective_scan``.  ``k_cache`` and ``v_cache``
+    ``(S, Hk, M, D)`` hold ``lengths[s]`` rows (int32) of slot ``s``.  Sequence ``i`` in slot ``s``::
+
+        q, k = rotated by the table rows cos, sin [seen[s] + t]  (fp32, one row a position, halves repeated)
+        q, k, v clipped to 1e3;  row lengths[s] + t of the cache <- k_t, v_t, rounded to its type
+        o_t = sum_j p_tj v_j,  p_t = softmax_j(sm_scale q_t k_j)  over the prefix's rows and own rows j <= lengths[s] + t
+
+    Without tables nothing is rotated; ``sm_scale`` is ``1 / sqrt(D)`` by default.  ``prefix`` (int32, one a sequence): the
+    slot whose rows the sequence sees before its own, any value outside ``[0, S)`` for none; neighbours in the batch
+    with the same one read its rows once for all.  ``seen`` (int32, one a slot) is the position of a slot's next token,
+    by default its rows and its prefix's.  ``mass`` (fp32) and ``held`` (int32), both ``(S, Hk, M)`` or neither: new
+    rows start with mass 0 and hold their position, then every own row's mass grows by the ``p_tj`` that it got from the call's
+    tokens and query heads (a prefix's rows gather none).
+
+    ``lengths`` and ``seen`` stay as they are, for the next layer's call: the caller moves them past the tokens.  The
+    cache is read below ``lengths`` only: what lies behind may be anything.  A
+    sequence whose slot is outside ``[0, S)``, whose rows would not fit into ``M`` or whose positions have no table row is
+    padding: zeros come out and nothing is written.  Returns ``o`` shaped like ``q``."""
+    if q.is_cuda and _IMPL == "cuda":
+        return _k().cached_attention(q, k, v, k_cache, v_cache, lengths, cos, sin, cu_seqlens, slots, prefix, seen, mass,
+                                     held, sm_scale)
+    return R.cached_attention(q, k, v, k_cache, v_cache, lengths, cos, sin, cu_seqlens, slots, prefix, seen, mass, held,
+                              sm_scale)
+
+
+def cache_evict(k_cache, v_cache, mass, held, lengths, seen, keep: int, recent: int = 0, slots=None) -> None:
+    """Thins the cache of ``cached_attention`` out to ``keep`` rows per key head, in place; no gradient.
+
+    Of the ``lengths[s]`` rows of every slot ``s`` in ``slots`` (int32, all different; default all) those are kept whose
+    position ``held`` is at least ``seen[s] - recent`` (``recent <= keep``: the newest ones) and then those with the largest
+    ``mass``, up to ``keep`` in all (ties: the lower row; NaN and ``-inf`` last).  Kept rows below ``keep`` stay where they are; the
+    others fill the rows below ``keep`` that were given up, in the order of both, with their mass and position.  What
+    lies behind is left as it was.  Slots outside ``[0, S)`` and those that hold ``keep`` rows or fewer stay as they are.
+
+    Every head keeps rows of its own.  ``lengths`` stays as it is, for the next layer's call: the caller sets it to at most ``keep``."""
+    if not 0 <= recent <= keep or keep < 1:
+        raise ValueError(f"cache_evict: keep must be at least 1 and recent between 0 and keep, got keep={keep}, recent={recent}")
+    if k_cache.is_cuda and _IMPL == "cuda":
+        return _k().cache_evict(k_cache, v_cache, mass, held, lengths, seen, keep, recent, slots)
+    return R.cache_evict(k_cache, v_cache, mass, held, lengths, seen, keep, recent, slots)
+
+
+MAX_ALTERNATIVES = 64
+
+
+def token_logprobs(logits, tokens, top: int = 0, temperature: float = 1.0):
+    """Log-probabilities of given tokens under ``p = softmax(logits / temperature)``: ``logits (R, V)``, ``tokens (R,)``
+    int64; returns ``(logprobs, entropy)``, fp32 ``(R,)`` each::
+
+        logprobs = log p[token],  entropy = -sum_v p_v log p_v
+        d logits_v = (g_logprobs ([v == token] - p_v) - g_entropy p_v (log p_v + entropy)) / temperature
+
+    with ``top`` (at most 64 and ``V``) also ``(top_tokens int64, top_logprobs fp32)``, both ``(R, top)``: the likeliest
+    ones (ties: lowest index), which carry no gradient.  A token outside ``[0, V)`` (-100, say) has log-probability 0 and no
+    gradient.  NaN and ``-inf`` logits have no probability, +inf counts as the largest finite number; a row of nothing else
+    gives ``-inf``, entropy 0, alternatives -1 and no gradient, and so do alternatives without probability.
+
+    To capture the backward pass into a CUDA graph, let go of earlier graphs of the same leaf first: PyTorch hands a leaf's
+    gradient over on the stream of its oldest living graph, and a capture that meets another stream there fails."""
+    if logits.dim() != 2 or tokens.shape != logits.shape[:1] or tokens.dtype != torch.int64:
+        raise ValueError(f"token_logprobs: one int64 token for each row of logits (R, V), got {tokens.dtype} {tuple(tokens.shape)} "
+                         f"for {tuple(logits.shape)}")
+    if not 0 <= top <= min(MAX_ALTERNATIVES, logits.shape[1]):
+        raise ValueError(f"token_logprobs: top must lie between 0 and {min(MAX_ALTERNATIVES, logits.shape[1])}, got {top}")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"token_logprobs: temperature must be positive and finite, got {temperature}")
+    if logits.is_cuda and _IMPL == "cuda":
+        return _k().token_logprobs(logits, tokens, top, temperature)
+    return R.token_logprobs(logits, tokens, top, temperature)
+
 # ---------------------------------------------------------------- loss
 def cross_entropy(hidden: torch.Tensor, labels: torch.Tensor, weight: torch.Tensor,
                   label_smoothing: float, chunk: int = 2048):

@@ -946,6 +946,61 @@ def sample(logits, noise, temperature, top_k, top_p, min_p):
                         _per_row(top_p, logits, f32), _per_row(min_p, logits, f32))
 
 
+ATTENTION_HEADS = (64, 96, 128)
+
+
+def cached_attention(q, k, v, k_cache, v_cache, lengths, cos, sin, cu_seqlens, slots, prefix, seen, mass, held, sm_scale):
+    """See ``ops.cached_attention``; bf16 and head dims 64, 96, 128 (others run the PyTorch form)."""
+    D = k_cache.shape[-1]
+    if D not in ATTENTION_HEADS or k_cache.dtype != torch.bfloat16:
+        _unsupported(f"cached_attention D={D} dtype={k_cache.dtype}")
+        return R.cached_attention(q, k, v, k_cache, v_cache, lengths, cos, sin, cu_seqlens, slots, prefix, seen, mass, held,
+                                  sm_scale)
+    scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    if q.dim() == 2:
+        return ext().cached_attention(q, k, v, k_cache, v_cache, lengths, cos, sin, 1, cu_seqlens, slots, prefix, seen,
+                                      mass, held, scale)
+    R.check_no_offsets(cu_seqlens)
+    if q.shape[1] == 0:
+        return torch.empty_like(q)
+    y = ext().cached_attention(_flat_rows(q), _flat_rows(k), _flat_rows(v), k_cache, v_cache, lengths, cos, sin,
+                               q.shape[1], None, slots, prefix, seen, mass, held, scale)
+    return y.view(q.shape)
+
+
+def cache_evict(k_cache, v_cache, mass, held, lengths, seen, keep, recent, slots):
+    """See ``ops.cache_evict``; rows of a multiple of 16 bytes, any type (others run the PyTorch form)."""
+    if k_cache.shape[-1] * k_cache.element_size() % 16:
+        _unsupported(f"cache_evict D={k_cache.shape[-1]} dtype={k_cache.dtype}")
+        return R.cache_evict(k_cache, v_cache, mass, held, lengths, seen, keep, recent, slots)
+    ext().cache_evict(k_cache, v_cache, mass, held, lengths, seen, keep, recent, slots)
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top, temperature):
+        lp, entropy, stats, index, best = ext().token_logprobs_fwd(logits, tokens, top, temperature)
+        ctx.save_for_backward(logits, tokens, stats)
+        ctx.temperature = temperature
+        ctx.mark_non_differentiable(index, best)
+        return lp, entropy, index, best
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, ge, _index, _best):
+        logits, tokens, stats = ctx.saved_tensors
+        return ext().token_logprobs_bwd(logits, tokens, stats, g, ge, ctx.temperature), None, None, None
+
+
+def token_logprobs(logits, tokens, top, temperature):
+    """See ``ops.token_logprobs``; bf16 or fp32 logits."""
+    if torch.is_grad_enabled() and logits.requires_grad:
+        lp, entropy, index, best = _TokenLogprobs.apply(logits, tokens, top, temperature)
+    else:
+        lp, entropy, _, index, best = ext().token_logprobs_fwd(logits, tokens, top, temperature)
+    return (lp, entropy, index, best) if top else (lp, entropy)
+
+
 # ----------------------------------------------------------------- fused optimizer
 _WD = {"muon": 0.01, "lion": 0.1, "adamw_decay": 0.01, "adamw_nodecay": 0.0, "frozen": 0.0}
 _ORDER = ("muon", "lion", "adamw_decay", "adamw_nodecay", "frozen")

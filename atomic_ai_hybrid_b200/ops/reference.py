@@ -425,6 +425,126 @@ def sample(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     return tokens[:, 0], torch.where(empty, -math.inf, logp)[:, 0].to(torch.float64 if acc == torch.float64 else torch.float32)
 
 
+@torch.no_grad()
+def cached_attention(q, k, v, k_cache, v_cache, lengths, cos=None, sin=None, cu_seqlens=None, slots=None, prefix=None,
+                     seen=None, mass=None, held=None, sm_scale=None):
+    """``ops.cached_attention`` sequence by sequence (float64 caches compute in float64, others in fp32)."""
+    S, Hk, M, D = k_cache.shape
+    acc = _acc_dtype(k_cache)
+    qf, kf, vf = q.reshape(-1, q.shape[-1] // D, D), k.reshape(-1, Hk, D), v.reshape(-1, Hk, D)
+    H = qf.shape[1]
+    if H % Hk:
+        raise ValueError(f"{H} query heads do not share {Hk} key heads evenly")
+    G, scale = H // Hk, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    o = torch.zeros(qf.shape, dtype=q.dtype, device=q.device)
+    rows = lengths.tolist()
+    at = None if seen is None else seen.tolist()
+    shared = None if prefix is None else prefix.tolist()
+    for i, (slot, s, e) in enumerate(_sequences(q, cu_seqlens, slots, S)):
+        n = e - s
+        if slot < 0 or n == 0 or not 0 <= rows[slot] <= M - n:
+            continue
+        pre = -1 if shared is None else shared[i]
+        if not (0 <= pre < S and 0 < rows[pre] <= M):
+            pre = -1
+        first, have = rows[slot], rows[slot] + n
+        pos = at[slot] if at is not None else first + (rows[pre] if pre >= 0 else 0)
+        if pos < 0 or (cos is not None and pos > cos.shape[0] - n):
+            continue
+        turn = (lambda t: t) if cos is None else (  # noqa: E731
+            lambda t: apply_rope(t, cos[pos:pos + n, None].to(acc), sin[pos:pos + n, None].to(acc)))
+        qs = sanitize(turn(qf[s:e].to(acc)), 1e3)
+        k_cache[slot, :, first:have] = sanitize(turn(kf[s:e].to(acc)), 1e3).to(k_cache.dtype).transpose(0, 1)
+        v_cache[slot, :, first:have] = sanitize(vf[s:e].to(acc), 1e3).to(v_cache.dtype).transpose(0, 1)
+        keys, values = k_cache[slot, :, :have], v_cache[slot, :, :have]
+        if pre >= 0:
+            keys = torch.cat([k_cache[pre, :, :rows[pre]], keys], 1)
+            values = torch.cat([v_cache[pre, :, :rows[pre]], values], 1)
+        w = torch.einsum("tkgd,kjd->kgtj", qs.view(n, Hk, G, D), keys.to(acc)) * scale
+        hidden = torch.ones(n, keys.shape[1], dtype=torch.bool, device=q.device).triu(keys.shape[1] - n + 1)
+        w = torch.softmax(w.masked_fill(hidden, -math.inf), -1)
+        o[s:e] = torch.einsum("kgtj,kjd->tkgd", w, values.to(acc)).reshape(n, H, D).to(o.dtype)
+        if mass is not None:
+            mass[slot, :, first:have] = 0
+            mass[slot, :, :have] += w.sum((1, 2))[:, keys.shape[1] - have:].to(mass.dtype)
+            held[slot, :, first:have] = torch.arange(pos, pos + n, dtype=held.dtype, device=held.device)
+    return o.view(q.shape)
+
+
+@torch.no_grad()
+def cache_evict(k_cache, v_cache, mass, held, lengths, seen, keep, recent=0, slots=None):
+    """``ops.cache_evict`` head by head."""
+    S, Hk, M, _ = k_cache.shape
+    rows, at = lengths.tolist(), seen.tolist()
+    for slot in range(S) if slots is None else slots.tolist():
+        if not 0 <= slot < S or not keep < rows[slot] <= M:
+            continue
+        n = rows[slot]
+        gathered = mass[slot, :, :n]
+        low = torch.isnan(gathered) | (gathered == -math.inf)
+        rank = torch.where(held[slot, :, :n].long() >= at[slot] - recent, math.inf,
+                           torch.where(low, -math.inf, gathered.clamp(max=torch.finfo(gathered.dtype).max)))
+        order = torch.sort(rank, dim=-1, descending=True, stable=True).indices
+        kept = torch.zeros(rank.shape, dtype=torch.bool, device=rank.device).scatter_(-1, order[:, :keep], True)
+        h, hole = torch.nonzero(~kept[:, :keep], as_tuple=True)
+        row = torch.nonzero(kept[:, keep:], as_tuple=True)[1] + keep
+        for t in (k_cache, v_cache, mass, held):
+            t[slot, h, hole] = t[slot, h, row]
+
+
+def _score_rows(logits, temperature):
+    """Scores below their row's largest, and the rows in which there is one."""
+    x = torch.where(torch.isnan(logits), -math.inf, logits).clamp(max=torch.finfo(torch.float32).max)
+    top = x.max(1, keepdim=True).values
+    some = top > -math.inf
+    return (x - torch.where(some, top, 0.0)) / temperature, some
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, temperature):
+        ctx.save_for_backward(logits, tokens)
+        ctx.temperature = temperature
+        d, some = _score_rows(logits.to(_acc_dtype(logits)), temperature)
+        p = torch.exp(d)
+        total = p.sum(1, keepdim=True)
+        logp = torch.where(some, d - torch.log(total), -math.inf)
+        given = (tokens >= 0) & (tokens < logits.shape[1])
+        lp = torch.where(given, logp.gather(1, torch.where(given, tokens, 0)[:, None])[:, 0], 0.0)
+        entropy = -torch.where(p > 0, p / total * logp, 0.0).sum(1)
+        return lp, entropy
+
+    @staticmethod
+    def backward(ctx, g, ge):
+        logits, tokens = ctx.saved_tensors
+        d, some = _score_rows(logits.to(_acc_dtype(logits)), ctx.temperature)
+        p = torch.exp(d)
+        total = p.sum(1, keepdim=True)
+        p, logp = p / total, torch.where(p > 0, d - torch.log(total), 0.0)
+        entropy = -(p * logp).sum(1, keepdim=True)
+        given = (tokens >= 0) & (tokens < logits.shape[1])
+        g = torch.where(given, g, 0.0)[:, None].to(p.dtype)
+        dx = -p * (g + ge[:, None].to(p.dtype) * (logp + entropy))
+        dx.scatter_add_(1, torch.where(given, tokens, 0)[:, None], g)
+        # tokens without probability stay without gradient, the given one among them
+        dx = torch.where((d > -math.inf) & some, dx, 0.0) / ctx.temperature
+        return dx.to(logits.dtype), None, None
+
+
+def token_logprobs(logits, tokens, top: int = 0, temperature: float = 1.0):
+    """``ops.token_logprobs`` from whole rows (the alternatives by sorting)."""
+    lp, entropy = _TokenLogprobs.apply(logits, tokens, temperature)
+    if not top:
+        return lp, entropy
+    with torch.no_grad():
+        d, some = _score_rows(logits.to(_acc_dtype(logits)), temperature)
+        best, index = torch.sort(d, dim=1, descending=True, stable=True)
+        best, index = best[:, :top], index[:, :top]
+        best = torch.where(some, best - torch.log(torch.exp(d).sum(1, keepdim=True)), -math.inf)
+        index = torch.where(best > -math.inf, index, -1)
+    return lp, entropy, index, best
+
+
 def newton_schulz3(g: Tensor, steps: int = 3, eps: float = 1e-4) -> Tensor:
     """Reference Muon orthogonalisation (reference `optimizer.py:53-77`)."""
     if g.ndim == 3:

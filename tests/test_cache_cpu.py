@@ -1,0 +1,130 @@
+"""The plain forms of the cache operators against definitions in 64 bits, and the refusals that need no GPU."""
+import math
+
+import pytest
+import torch
+
+from atomic_ai_hybrid_b200 import ops
+from _cache import BF, F32, F64, attention_inputs, check_attention, copied, evict_truth, gen, score_truth
+
+CPU = torch.device("cpu")
+
+
+@pytest.mark.parametrize("dtype", [F32, F64, BF])
+@pytest.mark.parametrize("lens,had,heads,prefix", [
+    ([1], [0], (2, 2, 8), None), ([3, 1, 5], [4, 0, 9], (4, 2, 8), None), ([1, 1, 1], [7, 2, 0], (6, 2, 16), ([5], [0, 0, 0])),
+    ([2, 4, 0, 1, 3], [0, 3, 5, 1, 2], (3, 1, 8), ([6, 2], [0, 1, 1, -1, 0]))])
+def test_plain_attention(dtype, lens, had, heads, prefix):
+    a = attention_inputs(lens, had, *heads, dtype, CPU, prefix=prefix, tracked=True)
+    check_attention(ops.cached_attention, a, torch.finfo(dtype).eps / 2 if dtype == BF else 0.0)
+
+
+def test_plain_attention_forms():
+    a = attention_inputs([2, 2, 2], [3, 0, 1], 2, 1, 8, F32, CPU)
+    y, _ = check_attention(ops.cached_attention, a, 0.0)
+    b = {**copied(a), "cu_seqlens": None, **{n: a[n].view(3, 2, -1) for n in ("q", "k", "v")}}
+    y3, _ = check_attention(ops.cached_attention, b, 0.0)
+    assert torch.equal(y.view(3, 2, -1), y3)
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        ops.cached_attention(**{**b, "cu_seqlens": a["cu_seqlens"]})
+    one = attention_inputs([1, 1], [3, 2], 2, 2, 8, F32, CPU)
+    check_attention(ops.cached_attention, {**one, "cu_seqlens": None}, 0.0)
+    check_attention(ops.cached_attention, {**one, "cos": None, "sin": None, "sm_scale": 0.3}, 0.0)
+    check_attention(ops.cached_attention, {**one, "seen": one["lengths"] * 0 + 1}, 0.0)
+
+
+def test_plain_attention_padding():
+    """Sequences that cannot run give zeros and write nothing."""
+    a = attention_inputs([2, 2, 2, 2], [3, 0, 1, 2], 2, 2, 8, F32, CPU, prefix=([4], [0, 0, 0, 0]), tracked=True)
+    S = a["k_cache"].shape[0]
+    for slot in (-1, S, 2 ** 31 - 1):
+        b = copied(a)
+        b["slots"][1] = slot
+        y, _ = check_attention(ops.cached_attention, b, 0.0)
+        assert (y[2:4] == 0).all() and (y[:2] != 0).any()
+    for name, value in (("lengths", -1), ("lengths", a["k_cache"].shape[2] - 1), ("lengths", 2 ** 31 - 1), ("seen", -1),
+                        ("seen", a["cos"].shape[0] - 1), ("seen", 2 ** 31 - 1)):
+        b = copied(a)
+        b["seen"] = b["lengths"] + 4
+        b[name][b["slots"][2]] = value
+        y, _ = check_attention(ops.cached_attention, b, 0.0)
+        assert (y[4:6] == 0).all() and (y[6:] != 0).any()
+    for value in (-1, S, a["k_cache"].shape[2] + 1):  # no prefix, or one whose length makes no sense
+        b = copied(a)
+        if value > S:
+            b["lengths"][b["prefix"][0]] = value
+        else:
+            b["prefix"][:] = value
+        check_attention(ops.cached_attention, b, 0.0)
+
+
+@pytest.mark.parametrize("keep,recent,n", [(1, 0, 2), (4, 2, 9), (4, 4, 5), (6, 1, 6), (3, 0, 12)])
+def test_plain_evict(keep, recent, n):
+    g = gen(keep, CPU)
+    S, Hk, M, D = 4, 3, 13, 4
+    kc, vc = torch.randn(S, Hk, M, D, generator=g), torch.randn(S, Hk, M, D, generator=g)
+    mass = torch.randint(0, 4, (S, Hk, M), generator=g).float()
+    mass[0, 0, :3] = torch.tensor([math.nan, math.inf, -math.inf])
+    held = torch.rand(S, Hk, M, generator=g).argsort(-1).to(torch.int32)
+    lengths = torch.tensor([n, n, max(0, n - 2), M + 1], dtype=torch.int32)
+    seen = torch.full((S,), M, dtype=torch.int32)
+    for slots in (None, torch.tensor([2, 0, -1, S], dtype=torch.int32)):
+        args = [t.clone() for t in (kc, vc, mass, held)]
+        want = evict_truth(kc, vc, mass, held, lengths, seen, keep, recent, slots)
+        assert ops.cache_evict(*args, lengths, seen, keep, recent=recent, slots=slots) is None
+        for x, y in zip(args, want):
+            assert torch.equal(x.nan_to_num(99.0), y.nan_to_num(99.0))
+
+
+@pytest.mark.parametrize("keep,recent", [(0, 0), (3, 4), (3, -1)])
+def test_evict_refuses(keep, recent):
+    z = torch.zeros(1, 1, 4, 8)
+    with pytest.raises(ValueError, match="cache_evict: keep"):
+        ops.cache_evict(z, z.clone(), z[..., 0], z[..., 0].int(), torch.tensor([4], dtype=torch.int32),
+                        torch.tensor([4], dtype=torch.int32), keep, recent=recent)
+
+
+def _scores(R, V, dtype, seed=0):
+    g = gen(seed, CPU)
+    x = (torch.randn(R, V, generator=g) * 3).to(dtype)
+    y = torch.randint(0, V, (R,), generator=g)
+    return x, y
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.5, 3.0])
+def test_plain_logprobs_and_gradient(temperature):
+    x, y = _scores(9, 17, F64)
+    y[2], y[5] = -100, 17
+    x[0, :5] = -math.inf
+    x[1] = -math.inf
+    x[3, 4] = math.nan
+    x[4] = math.nan
+    x[6, y[6]] = -math.inf
+    x[7] = 0.25
+    x.requires_grad_()
+    out = ops.token_logprobs(x, y, top=6, temperature=temperature)
+    want = score_truth(x.detach(), y, 6, temperature)
+    for got, w in zip(out, want):
+        assert (got == w).all() if not got.dtype.is_floating_point else torch.allclose(got, w, rtol=1e-12, atol=1e-12)
+    assert out[0][1] == -math.inf and out[1][1] == 0 and (out[2][1] == -1).all() and out[0][2] == 0 and out[0][5] == 0
+    assert out[2][7].tolist() == [0, 1, 2, 3, 4, 5]
+    g, ge = torch.randn(9, dtype=F64, generator=gen(1, CPU)), torch.randn(9, dtype=F64, generator=gen(2, CPU))
+    dx, = torch.autograd.grad(out[:2], [x], [g, ge])
+    assert torch.allclose(dx, score_truth(x.detach(), y, 0, temperature, g, ge)[-1], rtol=1e-12, atol=1e-12)
+    assert (dx[1] == 0).all() and (dx[4] == 0).all() and dx.isfinite().all()
+
+
+def test_logprobs_gradient_by_differences():
+    x, y = _scores(4, 7, F64, seed=3)
+    y[1] = -100
+    assert torch.autograd.gradcheck(lambda t: ops.token_logprobs(t, y, temperature=0.7), [x.requires_grad_()])
+
+
+def test_logprobs_refuses():
+    x, y = _scores(3, 5, F32)
+    for match, args, kw in [("one int64 token", (x, y[:2]), {}), ("one int64 token", (x, y.int()), {}),
+                            ("one int64 token", (x[0], y), {}), ("top", (x, y), dict(top=6)), ("top", (x, y), dict(top=-1)),
+                            ("top", (torch.zeros(3, 100), y), dict(top=65)), ("temperature", (x, y), dict(temperature=0.0)),
+                            ("temperature", (x, y), dict(temperature=math.inf)), ("temperature", (x, y), dict(temperature=math.nan))]:
+        with pytest.raises(ValueError, match=match):
+            ops.token_logprobs(*args, **kw)
