@@ -51,6 +51,7 @@ def compute_weights(model):
     return model
 
 
+SCORE_LOGITS = 1 << 28  # logits that ``Generator.score`` makes at a time (half a GB in bf16)
 MAX_GRAPHS = 8  # captured token steps that a Generator keeps, one per batch size; a capture launches the step twice
 
 
@@ -59,14 +60,17 @@ class Generator:
 
     ``model`` stays as it is, in training mode or not and owned by a trainer or not: its weights are read where they
     are at every token, matrices of another dtype than the compute dtype are rounded on the way (``compute_weights``
-    keeps them rounded).  ``max_len`` bounds prompt plus answer for models with MLA layers.  On a GPU, models without
-    MLA whose sizes all have kernels replay the token step from one CUDA graph per batch size; others launch it."""
+    keeps them rounded).  ``max_len`` bounds prompt plus answer for models with MLA layers, a common prefix apart; with
+    ``kv_budget`` longer conversations go on up to ``max_positions`` tokens, with that many rows a head once the rows run out:
+    the ``kv_recent`` newest and those that got most attention (``DecodeState``).  On a GPU, models whose sizes all have
+    kernels replay the token step from one CUDA graph per batch size; others launch it."""
 
-    def __init__(self, model, max_sequences: int, max_len: int = 0, cuda_graph: bool = True):
+    def __init__(self, model, max_sequences: int, max_len: int = 0, cuda_graph: bool = True, max_positions: int = 0,
+                 kv_budget: int = 0, kv_recent: Optional[int] = None):
         self.model = model
         p = next(model.parameters())
         self.device = p.device
-        self.state = DecodeState(model, max_sequences, max_len)
+        self.state = DecodeState(model, max_sequences, max_len, max_positions, kv_budget, kv_recent)
         self.cuda_graph = cuda_graph
         self._graphs, self._captured, self._rows = {}, None, None
 
@@ -78,6 +82,11 @@ class Generator:
     def prefill(self, prompts: Sequence[Sequence[int]], slots: List[int], fresh: bool = True) -> torch.Tensor:
         """Reads ``prompts`` into ``slots`` (``fresh``: as new conversations) and returns the logits
         ``(prompts, vocabulary)`` after their last tokens."""
+        h, last = self._read(prompts, slots, fresh)
+        return self._logits(h[last])
+
+    def _read(self, prompts: Sequence[Sequence[int]], slots: List[int], fresh: bool):
+        """The hidden rows of ``prompts``, packed, and where each one's last row is."""
         lens = [len(p) for p in prompts]
         ids = torch.cat([torch.as_tensor(p, dtype=torch.long) for p in prompts])
         if ids.numel() and not 0 <= int(ids.min()) <= int(ids.max()) < self.model.cfg.vocab_size:
@@ -86,7 +95,11 @@ class Generator:
         with serving(self.state, slots, lens, fresh=fresh) as call:
             h, _ = self.model(ids[None])
             last = call.cu[1:].long() - 1
-        return self._logits(h[0, last])
+        return h[0], last
+
+    def fork(self, source: int, slots: List[int]) -> None:
+        """Makes the conversations in ``slots`` new ones that go on from the one in ``source`` (``DecodeState.fork``)."""
+        self.state.fork(source, slots)
 
     @torch.no_grad()
     def step(self, tokens: torch.Tensor, slots: List[int]) -> torch.Tensor:
@@ -101,7 +114,7 @@ class Generator:
         if where != self._captured:  # a graph reads the weights by address: they have moved since
             self._graphs.clear()
             self._captured = where
-        key = tuple(slots)
+        key = tuple(slots), tuple(self.state.prefix[s] for s in slots)
         if key not in self._graphs:
             while len(self._graphs) >= MAX_GRAPHS:  # the one that was used least recently
                 self._graphs.pop(next(iter(self._graphs)))
@@ -114,18 +127,24 @@ class Generator:
                 # one stream, of the model's device, for every capture: the allocator keeps a stream's memory for it
                 self._pool, self._side = torch.cuda.graph_pool_handle(), torch.cuda.Stream(device=dev)
             buf = {name: t[:B] for name, t in self._rows.items()}
-            buf["slots"] = torch.tensor(slots, dtype=torch.int32, device=dev)
+            buf["slots"], buf["prefix"] = (torch.tensor(s, dtype=torch.int32, device=dev) for s in key)
+            if max(key[1]) < 0:
+                buf["prefix"] = None
 
             def run():
-                with serving(self.state, slots, slots_dev=buf["slots"]):
+                with serving(self.state, slots, slots_dev=buf["slots"], prefix_dev=buf["prefix"]):
                     h, _ = self.model(buf["tokens"][None])
                 t, lp = ops.sample(self._logits(h[0]), buf["noise"], buf["temperature"], buf["top_k"], buf["top_p"], buf["min_p"])
                 buf["tokens"].copy_(t.clamp(min=0))
                 return t, lp
 
             # warm up and capture on a copy of what the step changes
-            kept = [{n: c[n].clone() for n in ("conv", "state")} for c in self.state.layers.values()]
-            lengths = list(self.state.lengths)
+            st = self.state
+            st.cut_back(st.check_room(slots, [1] * B))  # outside the graph: the step itself then finds room
+            changed = [c[n] for c in st.layers.values() for n in ("conv", "state", "mass", "held") if n in c]
+            changed += [st.rows_dev, st.seen_dev] if st.has_mla else []
+            kept = [t.clone() for t in changed]
+            lengths, rows = list(st.lengths), list(st.rows)
             side = self._side
             side.wait_stream(torch.cuda.current_stream(dev))
             graph = torch.cuda.CUDAGraph()
@@ -137,38 +156,85 @@ class Generator:
                     buf["out"] = run()
             finally:
                 torch.cuda.current_stream(dev).wait_stream(side)
-                for c, k in zip(self.state.layers.values(), kept):
-                    for n, t in k.items():
-                        c[n].copy_(t)
-                self.state.lengths = lengths
+                for t, k in zip(changed, kept):
+                    t.copy_(k)
+                st.lengths, st.rows = lengths, rows
         else:
             graph, buf = self._graphs.pop(key)
         self._graphs[key] = graph, buf
         return graph, buf
 
+    # ------------------------------------------------------------ scores
+    def _check_prompts(self, prompts, prefix) -> None:
+        room = self.state.slots - (prefix is not None)
+        if not 1 <= len(prompts) <= room:
+            raise ValueError(f"{len(prompts)} prompts, room for {room}")
+        if any(len(p) == 0 for p in prompts) or prefix is not None and len(prefix) == 0:
+            raise ValueError("a prompt needs at least one token")
+
+    def _read_prefix(self, prefix: Sequence[int], B: int) -> torch.Tensor:
+        """Reads ``prefix`` into slot ``B`` and forks slots 0 to ``B - 1`` from it; returns its last hidden row."""
+        self.state.reset(list(range(B + 1)))
+        h, last = self._read([prefix], [B], True)
+        self.state.fork(B, list(range(B)))
+        return h[last]
+
+    @torch.no_grad()
+    def score(self, sequences: Sequence[Sequence[int]], top: int = 0, temperature: float = 1.0,
+              prefix: Optional[Sequence[int]] = None):
+        """How likely the model finds ``sequences`` (lists of token ids, at most ``max_sequences`` non-empty ones): a dict of
+        lists, one per sequence, with an entry for each of its tokens but the first (with ``prefix``, ids before every sequence
+        that are read once for all: for the first too): ``logprobs`` of the tokens, ``entropy`` of the distributions that they are
+        drawn from, and with ``top`` the likeliest ``top_tokens`` and their ``top_logprobs`` (``ops.token_logprobs``).  Slots 0
+        to ``len(sequences) - 1`` (the next one too with ``prefix``) hold new conversations afterwards."""
+        self._check_prompts(sequences, prefix)
+        B, slots, first = len(sequences), list(range(len(sequences))), None
+        if prefix is not None:
+            first = self._read_prefix(prefix, B)
+        h, _ = self._read(sequences, slots, prefix is None)
+        # row t of a sequence answers for its token t + 1, the prefix's last row for the first ones
+        rows, tokens, counts, at = [], [], [], 0
+        for s in sequences:
+            n = len(s)
+            rows += ([-1] if first is not None else []) + list(range(at, at + n - 1))
+            tokens += list(s if first is not None else s[1:])
+            counts.append(len(tokens))
+            at += n
+        rows, tokens = torch.tensor(rows, dtype=torch.long).to(self.device), torch.tensor(tokens, dtype=torch.long).to(self.device)
+        if first is not None:
+            h = torch.cat([h, first])  # row -1
+        step, parts = max(1, SCORE_LOGITS // self.model.cfg.vocab_size), []
+        for a in range(0, max(1, len(rows)), step):
+            logits = self._logits(h[rows[a:a + step]])
+            parts.append([t.tolist() for t in ops.token_logprobs(logits, tokens[a:a + step], top=top, temperature=temperature)])
+        names = ("logprobs", "entropy", "top_tokens", "top_logprobs")[:len(parts[0])]
+        flat = [sum(p, []) for p in zip(*parts)]
+        return {name: [v[a:e] for a, e in zip([0] + counts[:-1], counts)] for name, v in zip(names, flat)}
+
     # ------------------------------------------------------------ generation
     @torch.no_grad()
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int, temperature=1.0, top_k=0, top_p=1.0,
-                 min_p=0.0, stop_token: Optional[int] = None, generator: Optional[torch.Generator] = None):
+                 min_p=0.0, stop_token: Optional[int] = None, generator: Optional[torch.Generator] = None,
+                 prefix: Optional[Sequence[int]] = None):
         """Answers to ``prompts`` (lists of token ids, at most ``max_sequences`` non-empty ones): returns
         ``(tokens, logprobs)``, one list per prompt, each at most ``max_new_tokens`` long and ending with
         ``stop_token`` where it was drawn.  The settings are numbers or one value per prompt;
         ``generator`` (on the model's device) makes the noise.  The prompts are new conversations in slots 0 to
         ``len(prompts) - 1``, which later hold every token that was run, those after a stop among them: conversations of
-        ``prefill`` and ``step`` belong in other slots or another ``Generator``."""
+        ``prefill`` and ``step`` belong in other slots or another ``Generator``.  ``prefix`` (token ids) comes before every
+        prompt and is read once for all, in slot ``len(prompts)``, where it stays."""
         B = len(prompts)
-        if not 1 <= B <= self.state.slots:
-            raise ValueError(f"{B} prompts, room for {self.state.slots}")
-        if any(len(p) == 0 for p in prompts):
-            raise ValueError("a prompt needs at least one token")
+        self._check_prompts(prompts, prefix)
         if max_new_tokens < 1:
             return [[] for _ in prompts], [[] for _ in prompts]
         slots = list(range(B))
+        if prefix is not None:
+            self._read_prefix(prefix, B)
         V, dev = self.model.cfg.vocab_size, self.device
         row = lambda v, dt: torch.as_tensor(v, dtype=dt).expand(B).contiguous().to(dev)  # noqa: E731
         rules = (row(temperature, torch.float32), row(top_k, torch.int32), row(top_p, torch.float32), row(min_p, torch.float32))
         noise = lambda out: out.exponential_(generator=generator)  # noqa: E731
-        t, lp = ops.sample(self.prefill(prompts, slots), noise(torch.empty(B, V, device=dev)), *rules)
+        t, lp = ops.sample(self.prefill(prompts, slots, fresh=prefix is None), noise(torch.empty(B, V, device=dev)), *rules)
         steps = [(t, lp)]
         done = (t < 0) | (t == stop_token) if stop_token is not None else t < 0
         replay = self.cuda_graph and max_new_tokens > 1 and self.state.on_device()
@@ -181,11 +247,13 @@ class Generator:
             if i % 16 == 0 and bool(done.all()):  # the host waits for the device every 16 tokens only
                 break
             if replay:
+                self.state.cut_back(self.state.check_room(slots, [1] * B))
                 noise(buf["noise"])
                 graph.replay()
                 t, lp = (o.clone() for o in buf["out"])
                 for s in slots:
                     self.state.lengths[s] += 1
+                    self.state.rows[s] += 1
             else:
                 t, lp = ops.sample(self.step(t.clamp(min=0), slots), noise(torch.empty(B, V, device=dev)), *rules)
             steps.append((t, lp))

@@ -3,12 +3,12 @@
 The reference trains only; its layers see whole sequences.  Here every layer keeps, for each of
 ``slots`` conversations, what its next token needs: the recurrent layers a convolution window of three
 rows and a fp32 state of fixed size (``ops.selective_scan``, ``ops.gdn2_recurrent``), MLA its rotated keys
-and values.  Inside ``serving(...)`` a model's ``forward`` takes ``(1, T)`` packed tokens of several
+and values (``ops.cached_attention``).  Conversations may start as copies of another one (``fork``): recurrent state is
+copied, MLA rows are shared and read once for all of them.  Inside ``serving(...)`` a model's ``forward`` takes ``(1, T)`` packed tokens of several
 conversations and its mixers run on this state; everything else in the model is per token already."""
 from __future__ import annotations
 
 import contextlib
-import math
 from typing import Dict, List, Optional
 
 import torch
@@ -37,10 +37,12 @@ GDN_CHUNKED_FROM, GDN_CHUNKED_HEADS = 768, 64
 
 class DecodeState:
     """State of ``slots`` conversations for every mixer of ``model`` (on its device, convolution
-    windows and keys in its compute dtype).  ``max_len`` bounds a conversation's tokens and is needed for
-    models with MLA layers only."""
+    windows and keys in its compute dtype).  The rest is for models with MLA layers only: ``max_len`` (needed there) bounds the
+    rows that a conversation keeps of its own, ``max_positions`` (default ``2 * max_len``) its tokens, those of a conversation
+    that it was forked from included.  With ``budget``, a conversation whose rows run out is cut back to that
+    many a head (``ops.cache_evict``): its ``recent`` newest tokens (default half of it) and those that got most attention."""
 
-    def __init__(self, model, slots: int, max_len: int = 0):
+    def __init__(self, model, slots: int, max_len: int = 0, max_positions: int = 0, budget: int = 0, recent: Optional[int] = None):
         if get_tp() is not None or get_cp() is not None:
             raise ValueError("serving runs on one rank's whole model: tensor and context parallelism are for training")
         if any(isinstance(m, MoE) and m.ep_world > 1 for m in model.modules()):
@@ -49,7 +51,12 @@ class DecodeState:
         self.model = model
         p = next(model.parameters())
         self.device, self.dtype, self.slots, self.max_len = p.device, model.compute_dtype, slots, max_len
-        self.lengths = [0] * slots
+        # tokens of a conversation, rows of its own that MLA layers keep, the slot that it was forked from (-1: none)
+        self.lengths, self.rows, self.prefix = [0] * slots, [0] * slots, [-1] * slots
+        self.max_positions, self.budget = max_positions or 2 * max_len, budget
+        self.recent = budget // 2 if recent is None else recent
+        if budget and not 0 <= self.recent <= budget < max_len:
+            raise ValueError(f"budget must be below max_len={max_len} and recent at most budget, got budget={budget}, recent={self.recent}")
         self.layers: Dict[torch.nn.Module, dict] = {}
         kw = dict(device=self.device, dtype=self.dtype)
         f32 = dict(device=self.device, dtype=torch.float32)
@@ -65,9 +72,14 @@ class DecodeState:
                 if max_len <= 0:
                     raise ValueError("a model with MLA layers keeps keys and values: max_len must be given")
                 H, D = m.n_heads, m.cfg.d_model // m.cfg.n_heads
-                if "cos" not in self.__dict__:
-                    self.cos, self.sin = R.rope_cos_sin(max_len, D, device=self.device)
-                self.layers[m] = dict(k=torch.zeros(slots, max_len, H, D, **kw), v=torch.zeros(slots, max_len, H, D, **kw))
+                if "cos" not in self.__dict__:  # rounded as the training forward's, which multiplies in the compute dtype
+                    self.cos, self.sin = (t.to(self.dtype).float() for t in R.rope_cos_sin(self.max_positions, D, device=self.device))
+                    # rows and lengths again, where the layers read them
+                    self.rows_dev, self.seen_dev = (torch.zeros(slots, dtype=torch.int32, device=self.device) for _ in range(2))
+                c = self.layers[m] = dict(k=torch.zeros(slots, H, max_len, D, **kw), v=torch.zeros(slots, H, max_len, D, **kw))
+                if budget:
+                    c.update(mass=torch.zeros(slots, H, max_len, **f32),
+                             held=torch.zeros(slots, H, max_len, dtype=torch.int32, device=self.device))
 
     @property
     def has_mla(self) -> bool:
@@ -76,10 +88,13 @@ class DecodeState:
     def on_device(self) -> bool:
         """Whether a token step runs without a host read, as a CUDA graph needs it: every layer's sizes have kernels."""
         from ..ops import kernels as K
-        if self.device.type != "cuda" or ops.get_impl() != "cuda" or self.has_mla:
+        if self.device.type != "cuda" or ops.get_impl() != "cuda":
+            return False
+        if self.has_mla and self.dtype != torch.bfloat16:
             return False
         return all((not isinstance(m, Mamba2) or m.cfg.d_state in K.SCAN_STATES)
                    and (not isinstance(m, GatedDeltaNet2) or m.d_head in K.RECURRENT_HEADS)
+                   and (not isinstance(m, MLA) or m.cfg.d_model // m.cfg.n_heads in K.ATTENTION_HEADS)
                    and (not isinstance(m, MoE) or m.has_kernels(self.dtype)) for m in self.model.modules())
 
     def nbytes(self) -> int:
@@ -92,19 +107,88 @@ class DecodeState:
     def reset(self, slots: List[int]) -> None:
         """Makes the conversations in ``slots`` new ones."""
         self.check_slots(slots)
-        idx = torch.tensor(slots, device=self.device)
+        self._check_unshared(slots, besides=slots)
+        idx = torch.tensor(slots, dtype=torch.long, device=self.device)
         for cache in self.layers.values():
             for name in ("conv", "state"):
                 if name in cache:
                     cache[name][idx] = 0
         for s in slots:
-            self.lengths[s] = 0
+            self.lengths[s], self.rows[s], self.prefix[s] = 0, 0, -1
+        self._rows_to_device(slots)
+
+    def _rows_to_device(self, slots: List[int]) -> None:
+        if self.has_mla and slots:
+            now = torch.tensor([[s, self.rows[s], self.lengths[s]] for s in slots], dtype=torch.int32).to(self.device)
+            idx = now[:, 0].long()
+            self.rows_dev[idx], self.seen_dev[idx] = now[:, 1], now[:, 2]
+
+    def _check_unshared(self, slots: List[int], besides: List[int] = ()) -> None:
+        """A conversation whose rows others read stays as it is while they do."""
+        mine, free = set(slots), set(besides)
+        by = {p: s for s, p in enumerate(self.prefix) if p in mine and s not in free}
+        if by:
+            raise ValueError(f"slot {min(by)} is shared: the conversation in slot {by[min(by)]} was forked from it and reads its rows")
+
+    def fork(self, source: int, slots: List[int]) -> None:
+        """Makes the conversations in ``slots`` new ones that go on from the one in ``source``.  Recurrent layers' state is
+        copied; MLA layers' rows are not: as long as these conversations live, ``source`` adds no tokens, and it must not have been
+        forked from another one itself."""
+        self.check_slots(slots)
+        self.check_slots([source])
+        if source in slots:
+            raise ValueError(f"slot {source} cannot be forked into itself")
+        if self.has_mla and self.prefix[source] >= 0:
+            raise ValueError(f"the conversation in slot {source} was forked from slot {self.prefix[source]}: its rows are not all its own")
+        self.reset(slots)
+        idx = torch.tensor(slots, dtype=torch.long, device=self.device)
+        for cache in self.layers.values():
+            for name in ("conv", "state"):
+                if name in cache:
+                    cache[name][idx] = cache[name][source].clone()
+        for s in slots:
+            self.lengths[s] = self.lengths[source]
+            self.prefix[s] = source if self.has_mla else -1
+        self._rows_to_device(slots)
+
+    def check_room(self, slots: List[int], lens: List[int], fresh: bool = False) -> List[int]:
+        """Raises where MLA layers cannot hold ``lens`` more tokens; returns the slots that are to be cut back for them."""
+        if not self.has_mla:
+            return []
+        if not fresh:
+            self._check_unshared(slots)
+        cut = []
+        for s, n in zip(slots, lens):
+            if (0 if fresh else self.lengths[s]) + n > self.max_positions:
+                raise ValueError(f"a conversation would grow past max_positions={self.max_positions}")
+            if (0 if fresh else self.rows[s]) + n > self.max_len:
+                if not self.budget or fresh or min(self.rows[s], self.budget) + n > self.max_len:
+                    raise ValueError(f"a conversation would grow past max_len={self.max_len}")
+                cut.append(s)
+        return cut
+
+    def cut_back(self, slots: List[int]) -> None:
+        """Cuts the MLA rows of the conversations in ``slots`` back to ``budget`` a head."""
+        if not slots:
+            return
+        self.check_slots(slots)
+        self._check_unshared(slots)
+        if not self.budget:
+            raise ValueError("cutting back needs a budget")
+        which = torch.tensor(slots, dtype=torch.int32, device=self.device)
+        for c in self.layers.values():
+            if "mass" in c:
+                ops.cache_evict(c["k"], c["v"], c["mass"], c["held"], self.rows_dev, self.seen_dev, self.budget, recent=self.recent,
+                                slots=which)
+        for s in slots:
+            self.rows[s] = min(self.rows[s], self.budget)
+        self._rows_to_device(slots)
 
 
 class _Call:
     """One forward over packed tokens: sequence ``i`` adds ``lens[i]`` tokens to slot ``slots[i]``."""
 
-    def __init__(self, state: DecodeState, slots: List[int], lens: Optional[List[int]], slots_dev=None):
+    def __init__(self, state: DecodeState, slots: List[int], lens: Optional[List[int]], slots_dev=None, prefix_dev=None):
         self.state, self.slots, self.lens = state, slots, lens
         dev = state.device
         self.slots_dev = slots_dev if slots_dev is not None else torch.tensor(slots, dtype=torch.int32, device=dev)
@@ -115,6 +199,9 @@ class _Call:
                 ends.append(ends[-1] + n)
             self.starts = ends
             self.cu = torch.tensor(ends, dtype=torch.int32, device=dev)
+        self.prefix_dev = prefix_dev
+        if prefix_dev is None and any(state.prefix[s] >= 0 for s in slots):
+            self.prefix_dev = torch.tensor([state.prefix[s] for s in slots], dtype=torch.int32).to(dev)
         self._pad = self._rates = None
 
     def _check_rows(self, x: torch.Tensor) -> None:
@@ -206,54 +293,46 @@ class _Call:
 
     # ------------------------------------------------------------ MLA
     def mla(self, mod: MLA, x: torch.Tensor) -> torch.Tensor:
-        """Keys and values kept rotated per slot; the products are PyTorch's attention, as under
-        context parallelism."""
         self._check_rows(x)
         st, c = self.state, self.state.layers[mod]
-        H, D = mod.n_heads, mod.cfg.d_model // mod.cfg.n_heads
-        lens = self.lens or [1] * len(self.slots)
-        pos = torch.cat([torch.arange(st.lengths[s], st.lengths[s] + n) for s, n in zip(self.slots, lens)]).to(x.device)
-        which = torch.repeat_interleave(torch.tensor(self.slots), torch.tensor(lens)).to(x.device)
-        cos, sin = st.cos[pos][:, None], st.sin[pos][:, None]
         q, lat = mod.W_q(x)[0], mod.W_kv_down(x)
-        q = R.apply_rope(q.view(-1, H, D), cos, sin)
-        k = R.apply_rope(mod.W_k_up(lat)[0].view(-1, H, D), cos, sin)
-        v = mod.W_v_up(lat)[0].view(-1, H, D)
-        q, k, v = (R.sanitize(t, 1e3) for t in (q, k, v))
-        c["k"][which, pos], c["v"][which, pos] = k, v
-        out, at = [], 0
-        for s, n in zip(self.slots, lens):
-            end = st.lengths[s] + n
-            keep = torch.arange(end, device=x.device)[None] <= pos[at:at + n, None]
-            out.append(F.scaled_dot_product_attention(q[at:at + n].transpose(0, 1)[None], c["k"][s, :end].transpose(0, 1)[None],
-                                                      c["v"][s, :end].transpose(0, 1)[None], attn_mask=keep,
-                                                      scale=1.0 / math.sqrt(D))[0].transpose(0, 1))
-            at += n
-        o = torch.cat(out).reshape(1, -1, H * D)
-        return mod.W_o(mod.attn_out_norm(o))
+        o = ops.cached_attention(q, mod.W_k_up(lat)[0], mod.W_v_up(lat)[0], c["k"], c["v"], st.rows_dev, cos=st.cos, sin=st.sin,
+                                 cu_seqlens=self.cu, slots=self.slots_dev, prefix=self.prefix_dev, seen=st.seen_dev,
+                                 mass=c.get("mass"), held=c.get("held"))
+        return mod.W_o(mod.attn_out_norm(o[None]))
+
+    def advance(self) -> None:
+        """Moves the conversations past this call's tokens."""
+        st = self.state
+        for s, n in zip(self.slots, self.lens or [1] * len(self.slots)):
+            st.lengths[s] += n
+            st.rows[s] += n
+        if st.has_mla:
+            n = torch.ones_like(self.slots_dev) if self.cu is None else self.cu[1:] - self.cu[:-1]
+            st.rows_dev.index_add_(0, self.slots_dev, n)
+            st.seen_dev.index_add_(0, self.slots_dev, n)
 
 
 @contextlib.contextmanager
-def serving(state: DecodeState, slots: List[int], lens: Optional[List[int]] = None, slots_dev=None, fresh: bool = False):
+def serving(state: DecodeState, slots: List[int], lens: Optional[List[int]] = None, slots_dev=None, fresh: bool = False,
+            prefix_dev=None):
     """Runs a model's forwards on ``state``: ``(1, T)`` tokens of ``len(slots)`` conversations packed one
     after another, ``lens[i]`` of them each (None: one each; ``fresh``: as new conversations).  ``slots_dev`` is
-    ``slots`` as an int32 tensor on the device, where the caller has it.  It holds for the thread that enters it; a
+    ``slots`` as an int32 tensor on the device, where the caller has it, ``prefix_dev`` the slots that they were forked from.  It holds for the thread that enters it; a
     state serves one call at a time."""
     if get_serving() is not None:
         raise RuntimeError("serving(...) is not nested")
     state.check_slots(slots)
     if lens is not None and (len(lens) != len(slots) or min(lens, default=1) < 1):
         raise ValueError("every sequence of a call adds at least one token")
-    if state.has_mla and any((0 if fresh else state.lengths[s]) + n > state.max_len
-                             for s, n in zip(slots, lens or [1] * len(slots))):
-        raise ValueError(f"a conversation would grow past max_len={state.max_len}")
+    cut = state.check_room(slots, lens or [1] * len(slots), fresh)
     if fresh:
         state.reset(slots)
-    call = _Call(state, slots, lens, slots_dev)
+    state.cut_back(cut)
+    call = _Call(state, slots, lens, slots_dev, prefix_dev)
     token = serving_call.enter(call)
     try:
         yield call
-        for s, n in zip(slots, lens or [1] * len(slots)):
-            state.lengths[s] += n
+        call.advance()
     finally:
         serving_call.leave(token)
