@@ -481,6 +481,17 @@ torch::Tensor& err_word() {
   return e;
 }
 
+// the error word of kernels that run on any device: err_word() on its own one
+torch::Tensor& err_word_on(const torch::Device& device) {
+  static std::mutex m;
+  static std::map<int, torch::Tensor> words;
+  std::lock_guard<std::mutex> lock(m);
+  torch::Tensor& e = words[device.index()];
+  if (!e.defined())
+    e = err_word().device() == device ? err_word() : torch::zeros({1}, torch::dtype(torch::kInt32).device(device));
+  return e;
+}
+
 int64_t gemm_error() { return err_word().item<int>(); }
 void gemm_error_reset() { err_word().zero_(); }
 
@@ -1912,6 +1923,7 @@ torch::Tensor cached_attention(const torch::Tensor& q, const torch::Tensor& k, c
   a.D = (int)D;
   a.scale2 = (float)(scale * 1.4426950408889634);
   a.o = (ahb::cattn::bf16*)o.data_ptr();
+  a.err = err_word_on(q.device()).data_ptr<int>();
   auto work = new_output({ahb_cached_attention_bytes(a)}, at::kByte, q);
   const int rc = ahb_cached_attention(a, work.data_ptr(), cur_stream());
   TORCH_CHECK(rc == 0, op, ": failed with code ", rc, " for head dim ", D);

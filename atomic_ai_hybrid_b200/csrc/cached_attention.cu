@@ -9,8 +9,7 @@
 // Kernels: ca_append rotates the new rows and writes the cache (one block a token row; one more block lays the
 // work out as units of 16 cache rows); ca_rows gives every warp the same number of units, one after another;
 // ca_join joins what several warps or the prefix contributed; ca_mass adds up what every cache row was given.
-#include "cached_attention.h"
-#include "common.cuh"
+#include "cached_attention.cuh"
 #include "launchers.h"
 #include "mma.cuh"
 #include "packed.cuh"
@@ -20,11 +19,7 @@ using namespace ahb::cattn;
 
 namespace {
 
-constexpr int KU = 16;        // cache rows of a unit
-constexpr int RT = 16;        // query rows of an item
-constexpr int RW = 4;         // warps of a block of ca_rows
-constexpr float CLIP = 1e3f;
-constexpr float SLACK = 8.f;  // the running maximum moves when a score passes it by more than 2^8: p <= 256, and no sum nears overflow
+constexpr int RW = 4, RB = 3; // warps of a block of ca_rows, its blocks on an SM (168 registers a thread)
 
 struct Seq {
   int row0, n, slot, have, pos, pre, pre_rows;  // n = 0: padding or no token
@@ -57,12 +52,6 @@ AHB_DEVICE Seq load_seq(const Args& a, int i) {
   return s;
 }
 
-AHB_DEVICE int ceil_div(int a, int b) { return (a + b - 1) / b; }
-AHB_DEVICE int row_tiles(const Args& a, int tokens) { return ceil_div(tokens * (a.H / a.Hk), RT); }
-AHB_DEVICE int64_t group_units(const Args& a, const Group& g) {
-  return (int64_t)a.Hk * row_tiles(a, g.tokens) * ceil_div(g.keys, KU);
-}
-
 // ----------------------------------------------------------------------------- new rows and the plan
 constexpr int AT = 256, PT = 256;
 
@@ -89,11 +78,11 @@ AHB_DEVICE int64_t block_scan(int64_t v, int64_t* sh, F f) {
   return v;
 }
 
+// One block lays the work out: the groups, and the first unit of each in the kernel that takes it.
 AHB_DEVICE void make_plan(const Args& a) {
-  __shared__ int64_t sh[4][PT / 32];
-  __shared__ int64_t carry[4];
-  if (threadIdx.x < 4) carry[threadIdx.x] = threadIdx.x == 3 ? -1 : 0;
-  int64_t *own = a.units, *runs = own + a.B + 1, *mass = runs + a.B + 1;
+  __shared__ int64_t sh[PT / 32];
+  __shared__ int64_t carry[2 * KINDS + 1];  // sums so far, of own rows and of runs; the last run's start
+  if (threadIdx.x <= 2 * KINDS) carry[threadIdx.x] = threadIdx.x == 2 * KINDS ? -1 : 0;
   for (int base = 0; base < a.B; base += PT) {
     const int i = base + (int)threadIdx.x;
     Seq s{0, 0, 0, 0, 0, -1, 0};
@@ -111,43 +100,48 @@ AHB_DEVICE void make_plan(const Args& a) {
         }
       }
     }
-    const bool live = s.n > 0;
-    const bool starts = live && s.pre >= 0 && before != s.pre, ends = live && s.pre >= 0 && after != s.pre;
-    const Group g{s.row0, live ? s.n : 0, s.slot, live ? s.have + s.n : 0, s.have};
-    const int64_t u_own = group_units(a, g), u_mass = a.mass ? (int64_t)a.Hk * ceil_div(g.keys, KU) : 0;
-    __syncthreads();
-    const int64_t c_own = carry[0], c_runs = carry[1], c_mass = carry[2], c_start = carry[3];
-    const int64_t i_own = c_own + block_scan(u_own, sh[0], Sum64());
-    const int64_t i_mass = c_mass + block_scan(u_mass, sh[1], Sum64());
-    const int64_t first = Max64()(c_start, block_scan(starts ? i : -1, sh[2], Max64()));
-    Group r{0, 0, 0, 0, 0};
-    if (ends) {
-      const int row0 = a.cu ? min(max(a.cu[first], 0), a.T) : (int)first * a.L;
-      r = Group{row0, s.row0 + s.n - row0, s.pre, s.pre_rows, s.pre_rows};
-      a.run_end[first] = i;
+    const bool live = s.n > 0, starts = live && s.pre >= 0 && before != s.pre, ends = live && s.pre >= 0 && after != s.pre;
+    const Group own{s.row0, live ? s.n : 0, s.slot, live ? s.have + s.n : 0, s.have};
+    Group run{0, 0, 0, 0, 0};
+    if (a.prefix) {
+      __syncthreads();
+      const int64_t c = carry[2 * KINDS];
+      const int64_t first = Max64()(c, block_scan(starts ? i : -1, sh, Max64()));
+      if (ends) {
+        const int row0 = a.cu ? min(max(a.cu[first], 0), a.T) : (int)first * a.L;
+        run = Group{row0, s.row0 + s.n - row0, s.pre, s.pre_rows, s.pre_rows};
+        a.run_end[first] = i;
+      }
+      if (i < a.B) a.run_start[i] = live && s.pre >= 0 ? (int)first : -1;
+      if (threadIdx.x == PT - 1) carry[2 * KINDS] = first;
     }
-    const int64_t u_runs = group_units(a, r);
-    const int64_t i_runs = c_runs + block_scan(u_runs, sh[3], Sum64());
     if (i < a.B) {
-      a.groups[i] = g;
-      a.groups[a.B + i] = r;
-      own[i] = i_own - u_own;
-      runs[i] = i_runs - u_runs;
-      mass[i] = i_mass - u_mass;
-      a.run_start[i] = live && s.pre >= 0 ? (int)first : -1;
+      a.groups[i] = own;
+      a.groups[a.B + i] = run;
     }
-    if (threadIdx.x == PT - 1) {
-      carry[0] = i_own;
-      carry[1] = i_runs;
-      carry[2] = i_mass;
-      carry[3] = first;
+    for (int x = 0; x < (a.prefix ? 2 : 1); ++x) {
+      const Group& g = x ? run : own;
+      int64_t units[KINDS] = {0, 0, 0, 0};
+      if (g.tokens > 0 && !is_tiles(a, g)) units[ROWS] = (int64_t)a.Hk * row_units(g);
+      if (g.tokens > 0 && is_tiles(a, g)) {
+        const int n = row_tiles(a, g);
+        for (int rt = 0; rt < n; ++rt) units[TILES] += tile_item(a, g, rt).units;
+        units[TILES] *= a.Hk;
+      }
+      if (a.mass && !x && g.tokens > 0) units[is_tiles(a, g) ? TILES_MASS : ROWS_MASS] = (int64_t)a.Hk * row_units(g);
+      for (int k = 0; k < (x || !a.mass ? 2 : KINDS); ++k) {
+        __syncthreads();
+        const int64_t c = carry[KINDS * x + k];
+        const int64_t upto = c + block_scan(units[k], sh, Sum64());
+        if (i < a.B) a.sums[k][x * (a.B + 1) + i] = upto - units[k];
+        if (threadIdx.x == PT - 1) carry[KINDS * x + k] = upto;
+      }
     }
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    own[a.B] = carry[0];
-    runs[a.B] = carry[1];
-    mass[a.B] = carry[2];
+  if (threadIdx.x < KINDS && (threadIdx.x < 2 || a.mass)) {
+    a.sums[threadIdx.x][a.B] = carry[threadIdx.x];
+    if (threadIdx.x < 2) a.sums[threadIdx.x][2 * a.B + 1] = carry[KINDS + threadIdx.x];
   }
 }
 
@@ -168,12 +162,14 @@ AHB_DEVICE void load8(const bf16* p, float* v) {
     for (int i = 0; i < 8; ++i) v[i] = __bfloat162float(p[i]);
   }
 }
-AHB_DEVICE void store8(bf16* p, const float* v) {
-  uint4 u;
-  uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+// ... to p, and what their rounding leaves of them to `rest` (null: nowhere)
+AHB_DEVICE void store8(bf16* p, bf16* rest, const float* v) {
+  uint4 u, x;
+  uint32_t *w = reinterpret_cast<uint32_t*>(&u), *y = reinterpret_cast<uint32_t*>(&x);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = pack2(sanitize(v[2 * i], CLIP), sanitize(v[2 * i + 1], CLIP));
+  for (int i = 0; i < 4; ++i) split2(make_float2(sanitize(v[2 * i], CLIP), sanitize(v[2 * i + 1], CLIP)), w[i], y[i]);
   *reinterpret_cast<uint4*>(p) = u;
+  if (rest) *reinterpret_cast<uint4*>(rest) = x;
 }
 
 // Block 0 makes the plan; every other block rotates, clips and places one token row.
@@ -217,11 +213,12 @@ __global__ void __launch_bounds__(AT) ca_append(const Args a) {
   for (int x = threadIdx.x; x < heads * per; x += AT) {
     const int h = x / per, c = (x - h * per) << 3;
     const bf16* src;
-    bf16* dst;
+    bf16 *dst, *rest = nullptr;
     bool turn = cs != nullptr;
     if (h < a.H) {
       src = a.q + (int64_t)t * a.qs + h * a.D;
-      dst = a.qw + ((int64_t)t * a.H + h) * a.D;
+      dst = a.qw + ((int64_t)t * a.H + h) * 2 * a.D;
+      rest = dst + a.D;
     } else {
       const int hk = h < a.H + a.Hk ? h - a.H : h - a.H - a.Hk;
       const int64_t at = (((int64_t)s.slot * a.Hk + hk) * a.M + row) * a.D;
@@ -245,8 +242,12 @@ __global__ void __launch_bounds__(AT) ca_append(const Args a) {
         hi[i] = x2 * cs[c + half + i] + x1 * sn[c + half + i];
       }
     }
-    store8(dst + c, lo);
-    store8(dst + c + half, hi);
+    if (rest && a.negate) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) lo[i] = -lo[i], hi[i] = -hi[i];
+    }
+    store8(dst + c, rest ? rest + c : nullptr, lo);
+    store8(dst + c + half, rest ? rest + c + half : nullptr, hi);
   }
   if (a.mass)
     for (int h = threadIdx.x; h < a.Hk; h += AT) {
@@ -257,45 +258,24 @@ __global__ void __launch_bounds__(AT) ca_append(const Args a) {
 }
 
 // ----------------------------------------------------------------------------- rows against cache rows
-// The group whose units hold unit u: the last i with sums[i] <= u (one probe a lane, 32 ways a step).
-AHB_DEVICE int find_group(const int64_t* sums, int n, int64_t u) {
-  const int lane = threadIdx.x & 31;
-  int lo = 0, hi = n;  // sums[lo] <= u < sums[hi]
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) >> 5;
-    const int at = lo + (lane + 1) * step;
-    const bool in = at < hi && sums[at] <= u;
-    const int k = __popc(__ballot_sync(0xffffffffu, in));
-    lo += k * step;
-    hi = min(hi, lo + step);
-  }
-  return lo;
-}
-
-// Units a warp: equal shares of all units.
-AHB_DEVICE int64_t warp_share(int64_t units, int warps) { return (units + warps - 1) / warps; }
-
-// Channels of a lane in 32-channel (scores) and 64-channel (values) pieces of a head.  A lane loads 16
-// bytes of a cache row at once; which channel a fragment's position means is free, as long as both operands agree.
+// A unit's products on m16n8k16 tiles.  Scores: A is the queries, eight rows as rounded to bf16 and, in the
+// tile's other eight rows, what the rounding left of them: the sum of the two halves is the score of the
+// query in 32 bits, at no further product.  Values: A is the values' transpose, B the weights as rounded and, in a second product,
+// what that left of them, so no row of the tile is idle and eight rows of O take D / 4 registers.
+// Lane (g, t4) loads 16 bytes of a cache row at once: which channel a fragment's position means is free, as long as both
+// operands agree.
 template <int D>
-struct Frag {
-  static constexpr int KJ = D / 32;            // 32-channel pieces: two k steps each
-  static constexpr int VC = (D + 63) / 64;     // 64-channel pieces; the last one of 96 channels has 32
-  static constexpr int NT = D / 8;             // n tiles of O
-};
-
-template <int D>
-AHB_DEVICE void load_q(uint32_t (&qa)[D / 16][4], const bf16* g0, const bf16* g1, int t4) {
+AHB_DEVICE void load_q(uint32_t (&qa)[D / 16][4], const bf16* p, int t4) {
 #pragma unroll
   for (int j = 0; j < D / 32; ++j) {
-    const uint4 x = g0 ? *reinterpret_cast<const uint4*>(g0 + 32 * j + 8 * t4) : make_uint4(0, 0, 0, 0);
-    const uint4 y = g1 ? *reinterpret_cast<const uint4*>(g1 + 32 * j + 8 * t4) : make_uint4(0, 0, 0, 0);
+    const uint4 x = p ? *reinterpret_cast<const uint4*>(p + 32 * j + 8 * t4) : make_uint4(0, 0, 0, 0);
+    const uint4 y = p ? *reinterpret_cast<const uint4*>(p + D + 32 * j + 8 * t4) : make_uint4(0, 0, 0, 0);
     qa[2 * j][0] = x.x, qa[2 * j][2] = x.y, qa[2 * j + 1][0] = x.z, qa[2 * j + 1][2] = x.w;
     qa[2 * j][1] = y.x, qa[2 * j][3] = y.y, qa[2 * j + 1][1] = y.z, qa[2 * j + 1][3] = y.w;
   }
 }
 
-// The 16 rows of a unit as operands of the scores: lane (g, t4) holds channels 32 j + 8 t4 .. + 8 of rows g and g + 8.
+// Channels 32 j + 8 t4 .. + 8 of rows g and g + 8 of the unit.
 template <int D>
 AHB_DEVICE void load_keys(uint4 (&kr)[2][D / 32], const bf16* base, int j0, int keys, int g, int t4) {
 #pragma unroll
@@ -307,23 +287,25 @@ AHB_DEVICE void load_keys(uint4 (&kr)[2][D / 32], const bf16* base, int j0, int 
                      : make_uint4(0, 0, 0, 0);
 }
 
+// s[x][e]: query row g, cache row 8 x + 2 t4 + e
 template <int D>
-AHB_DEVICE void scores(float (&s)[2][4], const uint32_t (&qa)[D / 16][4], const uint4 (&kr)[2][D / 32]) {
+AHB_DEVICE void scores(float (&s)[2][2], const uint32_t (&qa)[D / 16][4], const uint4 (&kr)[2][D / 32]) {
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
+    float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
       const uint32_t b0[2] = {kr[x][j].x, kr[x][j].y}, b1[2] = {kr[x][j].z, kr[x][j].w};
-      mma16816(s[x], qa[2 * j], b0);
-      mma16816(s[x], qa[2 * j + 1], b1);
+      mma16816(c, qa[2 * j], b0);
+      mma16816(c, qa[2 * j + 1], b1);
     }
+    s[x][0] = c[0] + c[2];
+    s[x][1] = c[1] + c[3];
   }
 }
 
-// The same rows as operands of p v: lane (g, t4) holds channels 64 c + 8 g .. + 8 (a last piece of 32
-// channels: 64 c + 4 g .. + 4) of rows 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9.  Rows at or past `keys` are zero: what the
-// cache holds there may be infinite, and 0 times that is no zero.
+// Channels 64 c + 8 g .. + 8 (a last piece of 32 channels: 64 c + 4 g .. + 4) of rows 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9.
+// Rows at or past `keys` are zero: what the cache holds there may be infinite, and 0 times that is no zero.
 template <int D>
 AHB_DEVICE void load_values(uint4 (&vr)[4][(D + 63) / 64], const bf16* base, int j0, int keys, int g, int t4) {
 #pragma unroll
@@ -346,36 +328,31 @@ AHB_DEVICE void load_values(uint4 (&vr)[4][(D + 63) / 64], const bf16* base, int
   }
 }
 
-// channel e (0 .. 7) of rows a and b as one operand register
-AHB_DEVICE uint32_t pair(const uint4& a, const uint4& b, int e) {
-  const uint32_t x = (&a.x)[e >> 1], y = (&b.x)[e >> 1];
-  return (e & 1) ? __byte_perm(x, y, 0x7632) : __byte_perm(x, y, 0x5410);
-}
-
+// o[4 c + j][0, 1]: channel 64 c + 8 g + 2 j (a last piece of 32: 4 g + 2 j) of query rows 2 t4 and 2 t4 + 1; [2, 3]: the next channel
 template <int D>
-AHB_DEVICE void add_values(float (&o)[D / 8][4], const uint32_t (&pa)[4], const uint4 (&vr)[4][(D + 63) / 64]) {
+AHB_DEVICE void add_values(float (&o)[D / 16][4], const uint32_t (&ph)[2], const uint32_t (&pl)[2],
+                           const uint4 (&vr)[4][(D + 63) / 64]) {
 #pragma unroll
   for (int c = 0; c < (D + 63) / 64; ++c) {
-    const int nt = 64 * c + 64 <= D ? 8 : 4;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (e >= nt) break;
-      const uint32_t b[2] = {pair(vr[0][c], vr[1][c], e), pair(vr[2][c], vr[3][c], e)};
-      mma16816(o[8 * c + e], pa, b);
+    for (int j = 0; j < 4; ++j) {
+      if (64 * c + 16 * j >= D) break;
+      const uint32_t w0 = (&vr[0][c].x)[j], w1 = (&vr[1][c].x)[j], w2 = (&vr[2][c].x)[j], w3 = (&vr[3][c].x)[j];
+      const uint32_t va[4] = {__byte_perm(w0, w1, 0x5410), __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x5410),
+                              __byte_perm(w2, w3, 0x7632)};
+      mma16816(o[4 * c + j], va, ph);
+      mma16816(o[4 * c + j], va, pl);
     }
   }
 }
 
-// First channel of the run of channels that n tiles 8 c .. hold in a lane, in order: column 2 t4 of tiles e = 0, 1, ..
-// and then column 2 t4 + 1 of them.
-AHB_DEVICE int lane_channel(int c, int t4, int width) { return 64 * c + 2 * width * t4; }
-
 template <int D>
-__global__ void __launch_bounds__(RW * 32) ca_rows(const Args a) {
+__global__ void __launch_bounds__(RW * 32, RB) ca_rows(const Args a) {
+  constexpr int MT = D / 16, VC = (D + 63) / 64;
   const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const int w = blockIdx.x * RW + (threadIdx.x >> 5);
-  const int64_t *own = a.units, *runs = own + a.B + 1;
-  const int64_t n_own = own[a.B], all = n_own + runs[a.B], share = warp_share(all, a.warps);
+  const int64_t *own = a.sums[ROWS], *runs = own + a.B + 1;
+  const int64_t n_own = own[a.B], all = n_own + runs[a.B], share = share_of(all, a.warps);
   int64_t u = (int64_t)w * share;
   const int64_t u_first = u, u_end = min(u + share, all);
   const int G = a.H / a.Hk;
@@ -383,228 +360,235 @@ __global__ void __launch_bounds__(RW * 32) ca_rows(const Args a) {
     const bool pre = u >= n_own;
     const int i = pre ? find_group(runs, a.B, u - n_own) : find_group(own, a.B, u);
     const Group gr = a.groups[pre ? a.B + i : i];
-    const int per_item = ceil_div(gr.keys, KU), tiles = row_tiles(a, gr.tokens);
+    const int per_head = row_units(gr);
     const int64_t u0 = pre ? n_own + runs[i] : own[i];
-    const int64_t item = (u - u0) / per_item;
-    const int64_t first = u0 + item * per_item;       // the item's units
-    const int ks = (int)(u - first), ke = (int)min((int64_t)per_item, u_end - first);
-    const int h = (int)(item / tiles), r0 = (int)(item - (int64_t)h * tiles) * RT;
+    const int h = (int)((u - u0) / per_head);
+    const int64_t first = u0 + (int64_t)h * per_head;  // the head's units
+    const int ks = (int)(u - first), ke = (int)min((int64_t)per_head, u_end - first);
     u = first + ke;
     const bf16* kb = a.kc + ((int64_t)gr.slot * a.Hk + h) * a.M * D;
     const bf16* vb = a.vc + ((int64_t)gr.slot * a.Hk + h) * a.M * D;
-    // rows of this lane: g and g + 8 of the tile; row r is token r / G, query head h G + r % G
-    const int rows = gr.tokens * G;
-    const bf16* qp[2];
-    int64_t out[2];
-    int last[2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int r = r0 + g + 8 * x, tt = r / G;
-      out[x] = r < rows ? (int64_t)(gr.row0 + tt) * a.H + h * G + (r - tt * G) : -1;
-      qp[x] = out[x] >= 0 ? a.qw + out[x] * D : nullptr;
-      last[x] = min(gr.keys - 1, pre ? gr.keys : gr.before + tt);
-    }
-    uint32_t qa[D / 16][4];
-    load_q<D>(qa, qp[0], qp[1], t4);
-    float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    zero_acc<D / 8>(o);
-    uint4 kr[2][D / 32], vr[4][(D + 63) / 64];
+    uint4 kr[2][D / 32], vr[4][VC];
     load_keys<D>(kr, kb, ks * KU, gr.keys, g, t4);
     load_values<D>(vr, vb, ks * KU, gr.keys, g, t4);
+    // this lane's row: row g is token g / G, query head h G + g % G
+    const int tt = g / G;
+    const int64_t out = g < gr.tokens * G ? (int64_t)(gr.row0 + tt) * a.H + h * G + (g - tt * G) : -1;
+    const int last = min(gr.keys - 1, pre ? gr.keys : gr.before + tt);
+    uint32_t qa[D / 16][4];
+    load_q<D>(qa, out >= 0 ? a.qw + out * 2 * D : nullptr, t4);
+    float o[MT][4], m = -INFINITY, l = 0.f;
+    zero_acc<MT>(o);
     for (int c = ks; c < ke; ++c) {
-      float s[2][4];
+      float s[2][2];
       scores<D>(s, qa, kr);
       if (c + 1 < ke) load_keys<D>(kr, kb, (c + 1) * KU, gr.keys, g, t4);
-      float mx[2] = {-INFINITY, -INFINITY};
+      float mx = -INFINITY;
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = c * KU + 8 * x + 2 * t4 + (e & 1);
-          s[x][e] = j <= last[e >> 1] ? s[x][e] * a.scale2 : -INFINITY;
-          mx[e >> 1] = fmaxf(mx[e >> 1], s[x][e]);
+        for (int e = 0; e < 2; ++e) {
+          s[x][e] = c * KU + 8 * x + 2 * t4 + e <= last ? s[x][e] * a.scale2 : -INFINITY;
+          mx = fmaxf(mx, s[x][e]);
         }
-      if (__any_sync(0xffffffffu, mx[0] > m[0] + SLACK || mx[1] > m[1] + SLACK)) {
+      if (__any_sync(0xffffffffu, mx > m + SLACK)) {
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : ex2(m - mn);
+        m = mn;
+        l *= f;
+        const float f0 = __shfl_sync(0xffffffffu, f, 8 * t4), f1 = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
-          mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
-          const float mn = fmaxf(m[x], mx[x]);
-          const float f = m[x] == -INFINITY ? 0.f : ex2(m[x] - mn);
-          m[x] = mn;
-          l[x] *= f;
-#pragma unroll
-          for (int j = 0; j < D / 8; ++j) {
-            o[j][2 * x] *= f;
-            o[j][2 * x + 1] *= f;
-          }
+        for (int j = 0; j < MT; ++j) {
+          o[j][0] *= f0, o[j][1] *= f1;
+          o[j][2] *= f0, o[j][3] *= f1;
         }
       }
-      // p rounded to bf16 for its product with the values (relative 2^-9 each, averaging out); l sums what was not rounded
-      uint32_t pa[4];
+      const float mr = m == -INFINITY ? 0.f : m;
+      uint32_t ph[2], pl[2];
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float mr = m[r] == -INFINITY ? 0.f : m[r];
-          const float p0 = ex2(s[x][2 * r] - mr), p1 = ex2(s[x][2 * r + 1] - mr);
-          l[r] += p0 + p1;
-          pa[2 * x + r] = pack2(p0, p1);
-        }
-      add_values<D>(o, pa, vr);
+      for (int x = 0; x < 2; ++x) {
+        const float2 p = make_float2(ex2(s[x][0] - mr), ex2(s[x][1] - mr));
+        l += p.x + p.y;
+        split2(p, ph[x], pl[x]);
+      }
+      add_values<D>(o, ph, pl, vr);
       if (c + 1 < ke) load_values<D>(vr, vb, (c + 1) * KU, gr.keys, g, t4);
     }
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    const bool whole = ks == 0 && ke == per_head, final = whole && !a.full;
+    float* part = a.part + (2 * (int64_t)w + (first >= u_first ? 1 : 0)) * RT * (D + 2);
+    float* full = whole && a.full ? a.full + (int64_t)(pre ? a.T : 0) * a.H * (D + 2) : nullptr;
+    const float inv = final ? 1.f / l : 1.f;
+    if (t4 == 0 && out >= 0) {
+      if (!final)
+        *reinterpret_cast<float2*>((full ? full + out * (D + 2) : part + g * (D + 2)) + D) = make_float2(m, l);
+      else if (a.lse)
+        a.lse[out] = m + log2f(l);
     }
-    const bool whole = ks == 0 && ke == per_item;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      if (out[x] < 0) continue;
-      if (whole && !a.full) {  // final
-        const float inv = 1.f / l[x];
-        bf16* y = a.o + out[x] * D;
+    for (int b = 0; b < 2; ++b) {  // rows 2 t4 and 2 t4 + 1
+      const int64_t row = __shfl_sync(0xffffffffu, out, 8 * t4 + 4 * b);
+      const float f = __shfl_sync(0xffffffffu, inv, 8 * t4 + 4 * b);
+      if (row < 0) continue;
+      float* y = full ? full + row * (D + 2) : part + (2 * t4 + b) * (D + 2);
 #pragma unroll
-        for (int c = 0; c < (D + 63) / 64; ++c) {
-          const int nt = 64 * c + 64 <= D ? 8 : 4;
-          bf16* p = y + lane_channel(c, t4, nt);
+      for (int c = 0; c < VC; ++c) {
+        const int at = 64 * c + (64 * c + 64 <= D ? 8 : 4) * g;
 #pragma unroll
-          for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int e = 0; e < 8; e += 2)
-              if (e < nt)
-                *reinterpret_cast<uint32_t*>(p + b * nt + e) =
-                    pack2(o[8 * c + e][2 * x + b] * inv, o[8 * c + e + 1][2 * x + b] * inv);
+        for (int j = 0; j < 4; ++j) {
+          if (64 * c + 16 * j >= D) break;
+          const float x0 = o[4 * c + j][b], x1 = o[4 * c + j][2 + b];
+          if (final) *reinterpret_cast<uint32_t*>(a.o + row * D + at + 2 * j) = pack2(x0 * f, x1 * f);
+          else *reinterpret_cast<float2*>(y + at + 2 * j) = make_float2(x0, x1);
         }
-        if (a.lse && t4 == 0) a.lse[out[x]] = m[x] + log2f(l[x]);
-      } else {
-        float* y = whole ? a.full + ((int64_t)(pre ? a.T : 0) * a.H + out[x]) * (D + 2)
-                         : a.part + ((2 * (int64_t)w + (first >= u_first ? 1 : 0)) * RT + g + 8 * x) * (D + 2);
-#pragma unroll
-        for (int c = 0; c < (D + 63) / 64; ++c) {
-          const int nt = 64 * c + 64 <= D ? 8 : 4;
-          float* p = y + lane_channel(c, t4, nt);
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int e = 0; e < 8; e += 2)
-              if (e < nt)
-                *reinterpret_cast<float2*>(p + b * nt + e) =
-                    make_float2(o[8 * c + e][2 * x + b], o[8 * c + e + 1][2 * x + b]);
-        }
-        if (t4 == 0) *reinterpret_cast<float2*>(y + D) = make_float2(m[x], l[x]);
       }
     }
   }
 }
 
 // ----------------------------------------------------------------------------- joining
-// One warp for each row and query head.  Zeros for rows of no sequence; nothing for what ca_rows has finished.
+// One block for each token row, a query head for each warp in turn.  Zeros for rows of no sequence; nothing for what
+// is final already.
 template <int D>
 __global__ void __launch_bounds__(128) ca_join(const Args a) {
   constexpr int PL = (D + 63) / 64;  // channel pairs of a lane
-  const int lane = threadIdx.x & 31;
-  const int64_t out = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (out >= (int64_t)a.T * a.H) return;
-  const int t = (int)(out / a.H), hq = (int)(out - (int64_t)t * a.H), G = a.H / a.Hk, h = hq / G;
+  const int lane = threadIdx.x & 31, t = blockIdx.x, G = a.H / a.Hk;
   const int i = a.row_seq[t];
   if (i < 0) {
-#pragma unroll
-    for (int c = 0; c < PL; ++c)
-      if (64 * c + 2 * lane < D) *reinterpret_cast<uint32_t*>(a.o + out * D + 64 * c + 2 * lane) = 0u;
+    for (int x = threadIdx.x; x < a.H * D / 8; x += 128)
+      reinterpret_cast<uint4*>(a.o + (int64_t)t * a.H * D)[x] = make_uint4(0, 0, 0, 0);
     return;
   }
-  const int64_t *own = a.units, *runs = own + a.B + 1;
-  const int64_t n_own = own[a.B], share = warp_share(n_own + runs[a.B], a.warps);
-  float m = -INFINITY, l = 0.f;
-  float2 o[PL];
+  // the group of the sequence's own rows, and that of its prefix run
+  Group gr[2];
+  int at[2], n = 1;
+  at[0] = i;
+  gr[0] = a.groups[i];
+  const int start = a.full ? a.run_start[i] : -1;
+  if (start >= 0) {
+    at[1] = a.run_end[start];
+    gr[1] = a.groups[a.B + at[1]];
+    n = 2;
+  }
+  for (int hq = threadIdx.x >> 5; hq < a.H; hq += 4) {
+    const int h = hq / G;
+    const int64_t out = (int64_t)t * a.H + hq;
+    float m = -INFINITY, l = 0.f;
+    float2 o[PL];
 #pragma unroll
-  for (int c = 0; c < PL; ++c) o[c] = make_float2(0.f, 0.f);
-  auto add = [&](const float* y) {
-    const float2 ml = *reinterpret_cast<const float2*>(y + D);
-    const float mn = fmaxf(m, ml.x);
-    const float f = m == -INFINITY ? 0.f : ex2(m - mn), e = ml.x == -INFINITY ? 0.f : ex2(ml.x - mn);
-    m = mn;
-    l = l * f + ml.y * e;
+    for (int c = 0; c < PL; ++c) o[c] = make_float2(0.f, 0.f);
+    // `count` partial results, `stride` apart: eight at a time, so that their loads travel together
+    auto add = [&](const float* y, int64_t stride, int count) {
+      for (int k0 = 0; k0 < count; k0 += 8) {
+        float2 ml[8], v[8][PL];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (k0 + k >= count) break;
+          const float* p = y + (k0 + k) * stride;
+          ml[k] = *reinterpret_cast<const float2*>(p + D);
+#pragma unroll
+          for (int c = 0; c < PL; ++c)
+            if (64 * c + 2 * lane < D) v[k][c] = *reinterpret_cast<const float2*>(p + 64 * c + 2 * lane);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (k0 + k >= count || ml[k].x == -INFINITY) continue;
+          const float mn = fmaxf(m, ml[k].x), f = ex2(m - mn), e = ex2(ml[k].x - mn);
+          m = mn;
+          l = l * f + ml[k].y * e;
+#pragma unroll
+          for (int c = 0; c < PL; ++c) {
+            o[c].x = o[c].x * f + v[k][c].x * e;
+            o[c].y = o[c].y * f + v[k][c].y * e;
+          }
+        }
+      }
+    };
+    bool done = false;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      if (x >= n) break;
+      const Group& g = gr[x];
+      const bool tiles = is_tiles(a, g);
+      const int64_t* own = a.sums[tiles ? TILES : ROWS];
+      const int64_t* runs = own + a.B + 1;
+      const int64_t n_own = own[a.B], share = share_of(n_own + runs[a.B], tiles ? a.blocks : a.warps);
+      const int r = (t - g.row0) * G + hq - h * G;  // the row within the group and key head
+      int64_t first = x ? n_own + runs[at[1]] : own[at[0]];
+      int units, row = r, rows = RT;
+      if (tiles) {
+        const int nt = row_tiles(a, g), rt = r / (2 * TQ);
+        int before = 0, per_head = 0;
+        for (int k = lane; k < nt; k += 32) {
+          const int q = tile_item(a, g, k).units;
+          before += k < rt ? q : 0;
+          per_head += q;
+        }
+        before = __reduce_add_sync(0xffffffffu, before);
+        per_head = __reduce_add_sync(0xffffffffu, per_head);
+        first += (int64_t)h * per_head + before;
+        units = tile_item(a, g, rt).units;
+        row = r - rt * 2 * TQ;
+        rows = 2 * TQ;
+      } else {
+        units = row_units(g);
+        first += (int64_t)h * units;
+      }
+      const int64_t w0 = first / share, w1 = (first + units - 1) / share;
+      if (w0 == w1) {
+        done = !a.full;
+        if (!done) add(a.full + ((int64_t)x * a.T * a.H + out) * (D + 2), 0, 1);
+      } else {
+        const float* part = (tiles ? a.tile_part : a.part) + (int64_t)row * (D + 2);
+        const int64_t slot = (int64_t)rows * (D + 2);
+        add(part + (2 * w0 + (first >= w0 * share ? 1 : 0)) * slot, 0, 1);
+        add(part + 2 * (w0 + 1) * slot, 2 * slot, (int)(w1 - w0));  // the others began before their worker's units
+      }
+    }
+    if (done) continue;
+    const float inv = 1.f / l;
 #pragma unroll
     for (int c = 0; c < PL; ++c)
-      if (64 * c + 2 * lane < D) {
-        const float2 v = *reinterpret_cast<const float2*>(y + 64 * c + 2 * lane);
-        o[c].x = o[c].x * f + v.x * e;
-        o[c].y = o[c].y * f + v.y * e;
-      }
-  };
-  for (int src = 0; src < (a.full ? 2 : 1); ++src) {
-    int j = i;
-    if (src == 1) {  // the run that this sequence is in
-      const int start = a.run_start[i];
-      if (start < 0) break;
-      j = a.run_end[start];
-    }
-    const Group gr = a.groups[src * a.B + j];
-    const int r = (t - gr.row0) * G + hq - h * G, per_item = ceil_div(gr.keys, KU);
-    const int64_t first =
-        (src ? n_own + runs[j] : own[j]) + ((int64_t)h * row_tiles(a, gr.tokens) + r / RT) * per_item;
-    const int64_t w0 = first / share, w1 = (first + per_item - 1) / share;
-    if (w0 == w1) {
-      if (!a.full) return;  // final already
-      add(a.full + ((int64_t)src * a.T * a.H + out) * (D + 2));
-    } else {
-      for (int64_t w = w0; w <= w1; ++w)
-        add(a.part + ((2 * w + (first >= w * share ? 1 : 0)) * RT + r % RT) * (D + 2));
-    }
+      if (64 * c + 2 * lane < D)
+        *reinterpret_cast<uint32_t*>(a.o + out * D + 64 * c + 2 * lane) = pack2(o[c].x * inv, o[c].y * inv);
+    if (a.lse && lane == 0) a.lse[out] = m + log2f(l);
   }
-  const float inv = 1.f / l;
-#pragma unroll
-  for (int c = 0; c < PL; ++c)
-    if (64 * c + 2 * lane < D)
-      *reinterpret_cast<uint32_t*>(a.o + out * D + 64 * c + 2 * lane) = pack2(o[c].x * inv, o[c].y * inv);
-  if (a.lse && lane == 0) a.lse[out] = m + log2f(l);
 }
 
 // ----------------------------------------------------------------------------- what every cache row was given
 // A warp holds 16 cache rows and goes over the query rows that see them: sum_t 2^(s_tj - lse_t).
 template <int D>
-__global__ void __launch_bounds__(RW * 32) ca_mass(const Args a) {
+__global__ void __launch_bounds__(RW * 32) ca_mass(const Args a, int kind) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  const int64_t* units = a.units + 2 * (a.B + 1);
+  const int64_t* units = a.sums[kind];
   const int64_t all = units[a.B];
   const int G = a.H / a.Hk;
   for (int64_t u = (int64_t)blockIdx.x * RW + (threadIdx.x >> 5); u < all; u += (int64_t)gridDim.x * RW) {
     const int i = find_group(units, a.B, u);
     const Group gr = a.groups[i];
-    const int per_head = ceil_div(gr.keys, KU), h = (int)((u - units[i]) / per_head);
+    const int per_head = row_units(gr), h = (int)((u - units[i]) / per_head);
     const int j0 = (int)(u - units[i] - (int64_t)h * per_head) * KU;
     uint4 kr[2][D / 32];
     load_keys<D>(kr, a.kc + ((int64_t)gr.slot * a.Hk + h) * a.M * D, j0, gr.keys, g, t4);
     float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
     const int rows = gr.tokens * G;
-    // the first token that sees row j0
+    // from the first token that sees row j0
     for (int r0 = max(0, j0 - gr.before) * G / RT * RT; r0 < rows; r0 += RT) {
-      const bf16* qp[2];
-      float lse[2];
-      int last[2];
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int r = r0 + g + 8 * x, tt = r / G;
-        const int64_t out = (int64_t)(gr.row0 + tt) * a.H + h * G + (r - tt * G);
-        qp[x] = r < rows ? a.qw + out * D : nullptr;
-        lse[x] = r < rows ? a.lse[out] : 0.f;
-        last[x] = r < rows ? gr.before + tt : -1;
-      }
+      const int r = r0 + g, tt = r / G;
+      const int64_t out = (int64_t)(gr.row0 + tt) * a.H + h * G + (r - tt * G);
+      const float lse = r < rows ? a.lse[out] : 0.f;
+      const int last = r < rows ? gr.before + tt : -1;
       uint32_t qa[D / 16][4];
-      load_q<D>(qa, qp[0], qp[1], t4);
-      float s[2][4];
+      load_q<D>(qa, r < rows ? a.qw + out * 2 * D : nullptr, t4);
+      float s[2][2];
       scores<D>(s, qa, kr);
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = j0 + 8 * x + 2 * t4 + (e & 1);
-          if (j <= last[e >> 1]) sum[x][e & 1] += ex2(s[x][e] * a.scale2 - lse[e >> 1]);
-        }
+        for (int e = 0; e < 2; ++e)
+          if (j0 + 8 * x + 2 * t4 + e <= last) sum[x][e] += ex2(s[x][e] * a.scale2 - lse);
     }
 #pragma unroll
     for (int x = 0; x < 2; ++x)
@@ -636,44 +620,57 @@ int64_t lay_out(Args& a, char* base) {
     return p;
   };
   const int64_t rows = (int64_t)a.T * a.H;
-  a.warps = sm_count() * 4 * RW;
-  a.qw = (bf16*)place(rows * a.D * 2);
+  const int sms = sm_count(), G = a.H / a.Hk;
+  a.warps = sms * RB * RW;
+  // no group takes tiles if there is no run and every sequence has few rows
+  a.blocks = a.prefix || a.cu || a.L * G > RT ? sms : 0;
+  a.qw = (bf16*)place(rows * a.D * 4);
   a.row_seq = (int*)place((int64_t)a.T * 4);
   a.groups = (Group*)place((int64_t)2 * a.B * sizeof(Group));
   a.run_start = (int*)place((int64_t)a.B * 4);
   a.run_end = (int*)place((int64_t)a.B * 4);
-  a.units = (int64_t*)place((int64_t)3 * (a.B + 1) * 8);
+  for (int k = 0; k < (a.mass ? KINDS : 2); ++k) a.sums[k] = (int64_t*)place((int64_t)2 * (a.B + 1) * 8);
   a.lse = a.mass ? (float*)place(rows * 4) : nullptr;
   a.part = (float*)place((int64_t)2 * a.warps * RT * (a.D + 2) * 4);
+  a.tile_part = (float*)place((int64_t)2 * a.blocks * 2 * TQ * (a.D + 2) * 4);
   a.full = a.prefix ? (float*)place(2 * rows * (a.D + 2) * 4) : nullptr;
   return at;
 }
 
 template <int D>
-void launch(const Args& a, cudaStream_t st) {
+int launch(const Args& a, cudaStream_t st) {
+  if (a.blocks) {
+    const int rc = launch_tiles(a, st);
+    if (rc) return rc;
+  }
   ca_rows<D><<<a.warps / RW, RW * 32, 0, st>>>(a);
-  ca_join<D><<<(unsigned)(((int64_t)a.T * a.H + 3) / 4), 128, 0, st>>>(a);
-  if (a.mass) ca_mass<D><<<a.warps / RW, RW * 32, 0, st>>>(a);
+  ca_join<D><<<a.T, 128, 0, st>>>(a);
+  if (a.mass) {
+    ca_mass<D><<<a.warps / RW, RW * 32, 0, st>>>(a, ROWS_MASS);
+    if (a.blocks) ca_mass<D><<<a.warps / RW, RW * 32, 0, st>>>(a, TILES_MASS);
+  }
+  return 0;
 }
 
 }  // namespace
 
-int64_t ahb_cached_attention_bytes(const ahb::cattn::Args& args) {
+int64_t ahb_cached_attention_bytes(const Args& args) {
   Args a = args;
   return lay_out(a, nullptr);
 }
 
-int ahb_cached_attention(const ahb::cattn::Args& args, void* work, cudaStream_t st) {
+int ahb_cached_attention(const Args& args, void* work, cudaStream_t st) {
   Args a = args;
+  a.negate = a.scale2 < 0.f;  // the queries take the scale's sign: the largest product is then the largest score
+  a.scale2 = a.scale2 < 0.f ? -a.scale2 : a.scale2;
   lay_out(a, (char*)work);
   const bool vec = (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0 && ((a.qs | a.ks | a.vs) & 7) == 0;
   if (vec) ca_append<true><<<a.T + 1, AT, 0, st>>>(a);
   else ca_append<false><<<a.T + 1, AT, 0, st>>>(a);
   switch (a.D) {
-    case 64: launch<64>(a, st); break;
-    case 96: launch<96>(a, st); break;
-    case 128: launch<128>(a, st); break;
+    case 64: return launch<64>(a, st);
+    case 96: return launch<96>(a, st);
+    case 128: return launch<128>(a, st);
     default: return -1;
   }
-  return 0;
 }

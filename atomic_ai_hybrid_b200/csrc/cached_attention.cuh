@@ -1,0 +1,59 @@
+// Device code that the kernels of cached attention share: how work is numbered and found.
+#pragma once
+#include "cached_attention.h"
+#include "common.cuh"
+
+namespace ahb {
+namespace cattn {
+
+constexpr int KU = 16;    // row kernel: cache rows of a unit
+constexpr int RT = 8;     // ... and the query rows that it takes
+constexpr int TK = 128;   // tile kernel: cache rows of a block
+constexpr int TQ = 128;   // ... query rows of a tensor-core tile; an item has one or two of them
+constexpr float CLIP = 1e3f;
+constexpr float SLACK = 8.f;  // the running maximum moves when a score passes it by more than 2^8: p <= 256, and no sum nears overflow
+
+AHB_DEVICE int ceil_div(int a, int b) { return (a + b - 1) / b; }
+AHB_DEVICE int query_rows(const Args& a, const Group& g) { return g.tokens * (a.H / a.Hk); }
+
+// Which kernel takes a group: up to eight query rows leave a 128-row tile idle and need no tile to be read once.
+AHB_DEVICE bool is_tiles(const Args& a, const Group& g) { return query_rows(a, g) > RT; }
+
+// Units of the row kernel: 16 cache rows for all query rows of one key head.
+AHB_DEVICE int row_units(const Group& g) { return ceil_div(g.keys, KU); }
+
+// Units of the tile kernel for query rows 256 rt ..: 128 cache rows against two tiles, or 256 against one.
+struct TileItem {
+  int rows, blocks, units;  // valid query rows, blocks of cache rows that any of them sees, units
+};
+AHB_DEVICE TileItem tile_item(const Args& a, const Group& g, int rt) {
+  const int G = a.H / a.Hk;
+  TileItem t;
+  t.rows = min(2 * TQ, g.tokens * G - 2 * TQ * rt);
+  const int last = (2 * TQ * rt + t.rows - 1) / G;  // the last token
+  t.blocks = ceil_div((int)min((int64_t)g.keys, (int64_t)g.before + last + 1), TK);
+  t.units = t.rows > TQ ? t.blocks : (t.blocks + 1) >> 1;
+  return t;
+}
+AHB_DEVICE int row_tiles(const Args& a, const Group& g) { return ceil_div(query_rows(a, g), 2 * TQ); }
+
+// The group whose units hold unit u: the last i with sums[i] <= u (one probe a lane, 32 ways a step).
+AHB_DEVICE int find_group(const int64_t* sums, int n, int64_t u) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = n;  // sums[lo] <= u < sums[hi]
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) >> 5;
+    const int at = lo + (lane + 1) * step;
+    const bool in = at < hi && sums[at] <= u;
+    const int k = __popc(__ballot_sync(0xffffffffu, in));
+    lo += k * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+
+// Units of each of n workers: equal shares of all.
+AHB_DEVICE int64_t share_of(int64_t units, int n) { return (units + n - 1) / n; }
+
+}  // namespace cattn
+}  // namespace ahb

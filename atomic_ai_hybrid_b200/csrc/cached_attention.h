@@ -9,13 +9,17 @@ namespace cattn {
 
 using bf16 = __nv_bfloat16;
 
-// One block of query rows and the cache rows that it sees: a sequence's own rows, or the rows of a prefix for
+// A block of query rows and the cache rows that they see: a sequence's own rows, or the rows of a prefix for
 // the sequences of a run that share it.
 struct Group {
   int row0, tokens;  // packed token rows row0 .. row0 + tokens (tokens 0: nothing to do)
   int slot, keys;    // cache slot, rows of it that any token sees
-  int before;        // token t sees rows j <= before + t (a prefix: all of them)
+  int before;        // token t sees rows j < min(keys, before + t + 1) (a prefix: before = keys)
 };
+
+// Groups [0, B) are the sequences' own rows, [B, 2 B) the prefix runs, each at its last sequence.  Each group is worked on by one of
+// two kernels; a kernel's units are numbered through the groups, and sums[kind][g] is group g's first one.
+enum Kind { ROWS = 0, TILES = 1, ROWS_MASS = 2, TILES_MASS = 3, KINDS = 4 };
 
 struct Args {
   const bf16 *q, *k, *v;
@@ -27,19 +31,25 @@ struct Args {
   int B, L, T, S, M, H, Hk, D;
   float* mass;
   int* held;
-  float scale2;                  // sm_scale log2(e)
+  float scale2;                  // sm_scale log2(e), without its sign
+  bool negate;                   // the sign: the rotated queries are negated
   bf16* o;                       // (T, H, D)
   // workspace
-  bf16* qw;                      // (T, H, D) rotated queries
+  bf16* qw;                      // (T, H, 2, D) rotated queries rounded to bf16, and what the rounding left of them
   int* row_seq;                  // (T) sequence of a row, -1: none
-  Group* groups;                 // [0, B) own rows, [B, 2 B) prefix runs at their last sequence
+  Group* groups;                 // (2 B)
   int *run_start, *run_end;      // a sequence's run: its first sequence (-1: no prefix), and that one's last
-  int64_t* units;                // exclusive sums of the groups' units: own (B + 1), runs (B + 1), mass (B + 1)
+  int64_t* sums[KINDS];          // (2 B + 1) each
   float* lse;                    // (T, H) log2 of the softmax's denominators, for mass
   float* part;                   // partial results of items that several warps share, two a warp
+  float* tile_part;              // ... of items that several blocks share, two a block
   float* full;                   // (2, T, H, D + 2) whole results of own rows and of prefix rows, if there is a prefix
-  int warps;                     // warps of the row kernel
+  int warps, blocks;             // warps of the row kernel, blocks of the tile kernel (0: it is not launched)
+  int* err;                      // error word of waits that ran out
 };
+
+// The tile kernel (cached_attention_tc.cu).
+int launch_tiles(const Args& a, cudaStream_t st);
 
 }  // namespace cattn
 }  // namespace ahb
