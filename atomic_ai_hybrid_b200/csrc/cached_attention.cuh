@@ -8,7 +8,7 @@ namespace cattn {
 
 constexpr int KU = 16;    // row kernel: cache rows of a unit
 constexpr int RT = 8;     // ... and the query rows that it takes
-constexpr int TK = 128;   // tile kernel: cache rows of a block
+constexpr int TK = 64;    // tile kernel: cache rows of a block
 constexpr int TQ = 128;   // ... query rows of a tensor-core tile; an item has one or two of them
 constexpr float CLIP = 1e3f;
 constexpr float SLACK = 8.f;  // the running maximum moves when a score passes it by more than 2^8: p <= 256, and no sum nears overflow
@@ -22,7 +22,7 @@ AHB_DEVICE bool is_tiles(const Args& a, const Group& g) { return query_rows(a, g
 // Units of the row kernel: 16 cache rows for all query rows of one key head.
 AHB_DEVICE int row_units(const Group& g) { return ceil_div(g.keys, KU); }
 
-// Units of the tile kernel for query rows 256 rt ..: 128 cache rows against two tiles, or 256 against one.
+// Units of the tile kernel for query rows 256 rt ..: 64 cache rows against two tiles, or 128 against one.
 struct TileItem {
   int rows, blocks, units;  // valid query rows, blocks of cache rows that any of them sees, units
 };

@@ -2,14 +2,17 @@
 // that share it.
 //
 // An item is up to 256 query rows of one key head (two 128-row tiles) and the cache rows that they see, in blocks of
-// 128; every thread block gets the same number of units (128 cache rows against both tiles) and goes through them item
+// 64; every thread block gets the same number of units (64 cache rows against both tiles) and goes through them item
 // by item.  Per block of cache rows and tile:
-//   S = Q K^T (128 x 128, TMEM)  ->  P = 2^(S c - m), rounded to bf16 into the columns S came from  ->  O += P V (TMEM)
+//   S = Q K^T (128 x 64, TMEM)  ->  P = 2^(S c - m), rounded to bf16 into the columns S came from  ->  O += P V (TMEM)
 // A thread owns a query row: maximum and sum need no exchange, and O is scaled only when a row's maximum has moved
-// by more than 2^8.  The two tiles take turns: while one's softmax runs, the other's products do.  Where an item has
+// by more than 2^8.  Each tile has two S buffers: the products P V and the next S of one run while the softmax works
+// on the other, and the two tiles' softmaxes share the exponential unit between them.  Where an item has
 // one tile only (a prefix under few tokens), the two sides take every other block of cache rows, and join at the end.
 //
-// Warps: 0 loads K and V by TMA into a ring of 32 KB buffers, 1 issues the products, 4-7 and 8-11 are the two sides.
+// Warps: 0 loads K and V by TMA into a ring of 16 KB buffers, 1 and 2 issue the two sides' products (one thread for
+// both spent as long on its waits and commits as the tensor cores on the products: a prompt of 8192 tokens 780 us), 4-7 and 8-11 are
+// the sides' softmaxes.
 // With `mass` the queries' rounding remainder multiplies too (S += Qlo K^T), as sums of weights are kept in 32 bits; without it the
 // query is rounded to bf16 as P is, each by at most 2^-8, in no common direction.
 #include <cuda.h>
@@ -33,13 +36,14 @@ using sm100::tc_fence_before;
 namespace {
 
 constexpr int NTHR = 384;
-constexpr uint32_t BUF = 32 * 1024;  // one block of K or V (or a tile of queries), two 64-channel slabs of 128 rows
-constexpr int COL_O = 256;           // TMEM columns: S and P of the sides at 0 and 128, O at 256 and 384
+constexpr uint32_t QBUF = 32 * 1024;  // a tile of queries: two 64-channel slabs of 128 rows
+constexpr uint32_t BUF = 16 * 1024;   // a block of K or V: two 64-channel slabs of 64 rows
+constexpr int COL_O = 256;            // TMEM columns: side w's S and P buffer b at 128 w + 64 b, its O at 256 + 128 w
 
 template <bool EXACT>
-constexpr int ring() { return EXACT ? 3 : 5; }
+constexpr int ring() { return EXACT ? 6 : 10; }
 template <bool EXACT>
-constexpr size_t smem_bytes() { return (size_t)BUF * (ring<EXACT>() + (EXACT ? 4 : 2)) + 1024 + 2048; }
+constexpr size_t smem_bytes() { return (size_t)BUF * ring<EXACT>() + QBUF * (EXACT ? 4 : 2) + 1024 + 2048; }
 
 struct Item {
   int pre, h, r0, rows, blocks, ks, ke;  // units ks .. ke of the item
@@ -51,48 +55,80 @@ struct Item {
   AHB_DEVICE int block(int w, int j) const { return two ? ks + j : 2 * (ks + j) + w; }
 };
 
-// The item that holds unit u, as far as this block's units go; moves u behind it.
-AHB_DEVICE Item next_item(const Args& a, int64_t& u, int64_t u_first, int64_t u_end) {
+// Where a thread block is in its units.
+struct Place {
+  int64_t u, u_first, u_end;
+  int x, h, rt, at;  // group, key head, 256-row tile and the unit within it; x < 0: not looked up yet
+};
+
+// The next item, as far as this block's units go; moves the place behind it.  A whole warp calls it.
+AHB_DEVICE Item next_item(const Args& a, Place& p) {
   const int64_t *own = a.sums[TILES], *runs = own + a.B + 1;
   const int64_t n_own = own[a.B];
   Item it;
-  it.pre = u >= n_own;
-  const int64_t* sums = it.pre ? runs : own;
-  const int64_t v = it.pre ? u - n_own : u;
-  const int i = find_group(sums, a.B, v);
-  it.g = a.groups[it.pre ? a.B + i : i];
-  const int64_t base = sums[i], per_head = (sums[i + 1] - base) / a.Hk;
-  it.h = (int)((v - base) / per_head);
-  int rest = (int)(v - base - it.h * per_head), rt = 0;
-  TileItem t = tile_item(a, it.g, 0);
-  while (rest >= t.units) {
-    rest -= t.units;
-    t = tile_item(a, it.g, ++rt);
+  TileItem t;
+  bool found = false;
+  if (p.x >= 0) {  // on from the last one: its next tile, its next head
+    it.g = a.groups[p.x];
+    if (++p.rt == row_tiles(a, it.g)) p.rt = 0, ++p.h;
+    p.at = 0;
+    found = p.h < a.Hk;
   }
-  it.r0 = rt * 2 * TQ;
+  if (!found) {
+    const bool pre = p.u >= n_own;
+    const int64_t *sums = pre ? runs : own, v = pre ? p.u - n_own : p.u;
+    const int i = find_group(sums, a.B, v), lane = threadIdx.x & 31;
+    p.x = pre ? a.B + i : i;
+    it.g = a.groups[p.x];
+    const int64_t base = sums[i], per_head = (sums[i + 1] - base) / a.Hk;
+    p.h = (int)((v - base) / per_head);
+    int64_t rest = v - base - p.h * per_head;
+    const int tiles = row_tiles(a, it.g);
+    for (p.rt = 0;; p.rt += 32) {  // 32 tiles at a time
+      const int64_t mine = p.rt + lane < tiles ? tile_item(a, it.g, p.rt + lane).units : 0;
+      int64_t upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      const uint32_t behind = __ballot_sync(0xffffffffu, upto > rest);
+      if (behind) {
+        const int k = __ffs(behind) - 1;
+        rest -= __shfl_sync(0xffffffffu, upto - mine, k);
+        p.rt += k;
+        break;
+      }
+      rest -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    p.at = (int)rest;
+  }
+  t = tile_item(a, it.g, p.rt);
+  it.pre = p.x >= a.B;
+  it.h = p.h;
+  it.r0 = p.rt * 2 * TQ;
   it.rows = t.rows;
   it.blocks = t.blocks;
   it.two = t.rows > TQ;
-  it.ks = rest;
-  it.ke = (int)min((int64_t)t.units, rest + (u_end - u));
+  it.ks = p.at;
+  it.ke = (int)min((int64_t)t.units, p.at + (p.u_end - p.u));
   it.whole = it.ks == 0 && it.ke == t.units;
-  it.late = u - rest < u_first;
-  u += it.ke - it.ks;
+  it.late = p.u - p.at < p.u_first;
+  p.u += it.ke - it.ks;
   return it;
 }
 
-// The order in which blocks of K and V go through the ring: the sides' first K, then for every step and side V and the next
-// step's K.  With two tiles both sides read the same ones.  f(is V, side, step).
+// The order in which blocks of K and V go through the ring: the sides' first two K, then for every step and side V and the
+// K of two steps on.  With two tiles both sides read the same ones.  f(is V, side, step).
 template <class F>
 AHB_DEVICE void in_order(const Item& it, F&& f) {
   const int n0 = it.count(0), n1 = it.two ? 0 : it.count(1);
-  f(false, 0, 0);
-  if (n1 > 0) f(false, 1, 0);
-  for (int j = 0; j < n0; ++j) {
-    f(true, 0, j);
-    if (j + 1 < n0) f(false, 0, j + 1);
-    if (j < n1) f(true, 1, j);
-    if (j + 1 < n1) f(false, 1, j + 1);
+#pragma unroll 1
+  for (int j = -2; j < n0; ++j) {
+    if (j >= 0) f(true, 0, j);
+    if (j + 2 < n0) f(false, 0, j + 2);
+    if (j >= 0 && j < n1) f(true, 1, j);
+    if (j + 2 < n1) f(false, 1, j + 2);
   }
 }
 
@@ -132,13 +168,6 @@ AHB_DEVICE void tmem_put32(uint32_t addr, const uint32_t* r) {
       "r"(r[31])
       : "memory");
 }
-AHB_DEVICE void tmem_put16(uint32_t addr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
 AHB_DEVICE void tmem_put_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // named barriers of the softmax warps: 1 both sides
@@ -152,46 +181,47 @@ __global__ void __launch_bounds__(NTHR, 1)
   extern __shared__ unsigned char raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* qs = smem;                               // tiles of queries (EXACT: rounded ones, then remainders)
-  unsigned char* kv = smem + BUF * (EXACT ? 4 : 2);       // the ring
+  unsigned char* kv = smem + QBUF * (EXACT ? 4 : 2);      // the ring
   uint64_t* bars = reinterpret_cast<uint64_t*>(kv + BUF * NB);
-  uint64_t *kv_full = bars, *kv_empty = bars + NB, *q_full = bars + 2 * NB, *s_full = q_full + 2, *p_full = s_full + 2,
-           *o_full = p_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  // side w's buffer b at 2 w + b: its S is there, its P is, and its P V is done
+  uint64_t *kv_full = bars, *kv_empty = bars + NB, *q_full = bars + 2 * NB, *s_full = q_full + 2, *p_full = s_full + 4,
+           *pv_done = p_full + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float2* other = reinterpret_cast<float2*>(tmem_slot + 4);  // the second side's maximum and sum, row by row
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t* sums = a.sums[TILES];
   const int64_t all = sums[a.B] + sums[2 * a.B + 1], share = share_of(all, a.blocks);
-  const int64_t u_first = (int64_t)blockIdx.x * share, u_end = min(u_first + share, all);
-  if (u_first >= u_end) return;
+  Place at;
+  at.u_first = at.u = (int64_t)blockIdx.x * share;
+  at.u_end = min(at.u_first + share, all);
+  at.x = -1;
+  if (at.u >= at.u_end) return;
   if (threadIdx.x == 0) {
     for (int i = 0; i < NB; ++i) {
       mbar_init(kv_full + i, 1);
-      mbar_init(kv_empty + i, 1);
+      mbar_init(kv_empty + i, 2);  // both sides'
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(q_full + i, 128);
+    for (int i = 0; i < 4; ++i) {
       mbar_init(s_full + i, 1);
       mbar_init(p_full + i, 128);
-      mbar_init(o_full + i, 1);
+      mbar_init(pv_done + i, 1);
     }
+    for (int i = 0; i < 2; ++i) mbar_init(q_full + i, 128);
     *abort_flag = 0;
     sm100::fence_barrier_init();
   }
-  if (warp == 2) sm100::tmem_alloc(tmem_slot, 512);
+  if (warp == 3) sm100::tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  int64_t u = u_first;
-  // registers: 3 x 168 at the launch = 88 + 2 x 208
-  if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+
   if (warp == 0) {  // ------------------------------------------------ loads
     uint32_t n = 0;
     bool ok = true;
-    while (u < u_end && ok) {
-      const Item it = next_item(a, u, u_first, u_end);
+    while (at.u < at.u_end && ok) {
+      const Item it = next_item(a, at);
       if (lane == 0) {
         const int plane = it.g.slot * a.Hk + it.h;
         in_order(it, [&](bool is_v, int w, int j) {
@@ -213,125 +243,131 @@ __global__ void __launch_bounds__(NTHR, 1)
     }
     if (lane == 0)  // copies in flight end before the block does
       for (uint32_t i = n > NB ? n - NB : 0; i < n; ++i) umma::wait_bar(kv_full + i % NB, (i / NB) & 1, a.err, 62);
-  } else if (warp == 1) {  // ----------------------------------------- products
+  } else if (warp < 3) {  // ------------------------------------------ products of side w
     constexpr uint32_t ID_S = sm100::idesc_bf16(TQ, TK, false, false), ID_O = sm100::idesc_bf16(TQ, D, false, true);
-    uint32_t n = 0, np[2] = {0, 0}, nq[2] = {0, 0};
+    const int w = warp - 1;
+    uint32_t n = 0, np = 0, items = 0, twos = 0;  // buffers through the ring, steps of this side, items, those of two tiles
     bool ok = true;
-    while (u < u_end && ok) {
-      const Item it = next_item(a, u, u_first, u_end);
+    while (at.u < at.u_end && ok) {
+      const Item it = next_item(a, at);
       if (lane == 0) {
-        const int cnt[2] = {it.count(0), it.count(1)};
-        // the buffer that comes next in the ring, once it is filled
+        const int n0 = it.count(0), n1 = it.count(1), cnt = w ? n1 : n0;
+        // Both sides go through the whole ring in order, so that neither mistakes one filling of a buffer for another: what a
+        // side does not use it gives back at once.
         auto next = [&]() {
           const uint32_t b = n % NB;
           ok = ok && mbar_wait(kv_full + b, (n / NB) & 1, abort_flag, a.err, 63);
           ++n;
           return b;
         };
-        auto wait_q = [&](int w) {
-          ok = ok && mbar_wait(q_full + w, nq[w] & 1, abort_flag, a.err, 64);
-          ++nq[w];
+        auto pass = [&]() {
+          const uint32_t b = next();
+          if (ok) mbar_arrive(kv_empty + b);
         };
-        auto score = [&](int w, uint32_t b) {
+        // a step uses S buffer (steps before this item + step) & 1
+        auto score = [&](int j) {
+          const uint32_t kb = next(), sb = (np + j) & 1;
           if (!ok) return;
-          const uint32_t q = smem_u32(qs) + (it.two ? w : 0) * BUF, k = smem_u32(kv) + b * BUF;
+          uint32_t q = smem_u32(qs) + (it.two ? w : 0) * QBUF, k = smem_u32(kv) + kb * BUF;
+          asm volatile("" : "+r"(q), "+r"(k));  // descriptors made here, not kept over the loop in registers
           tc_fence_after();
 #pragma unroll
           for (int s = 0; s < D / 16; ++s)
-            sm100::umma_bf16(tmem + 128 * w, umma::kdesc(q, TQ, s), umma::kdesc(k, TK, s), ID_S, s > 0);
+            sm100::umma_bf16(tmem + 128 * w + 64 * sb, umma::kdesc(q, TQ, s), umma::kdesc(k, TK, s), ID_S, s > 0);
           if (EXACT) {
 #pragma unroll
             for (int s = 0; s < D / 16; ++s)
-              sm100::umma_bf16(tmem + 128 * w, umma::kdesc(q + 2 * BUF, TQ, s), umma::kdesc(k, TK, s), ID_S, 1);
+              sm100::umma_bf16(tmem + 128 * w + 64 * sb, umma::kdesc(q + 2 * QBUF, TQ, s), umma::kdesc(k, TK, s), ID_S, 1);
           }
-          sm100::umma_commit(s_full + w);
+          sm100::umma_commit(s_full + 2 * w + sb);
+          sm100::umma_commit(kv_empty + kb);
         };
-        wait_q(0);
-        if (it.two) wait_q(1);
-        uint32_t kb = next();
-        score(0, kb);
-        if (!it.two) sm100::umma_commit(kv_empty + kb);
-        if (cnt[1] > 0) {
-          if (!it.two) kb = next();
-          score(1, kb);
-          sm100::umma_commit(kv_empty + kb);
-        } else if (it.two) {
-          sm100::umma_commit(kv_empty + kb);
-        }
-        for (int j = 0; j < cnt[0] && ok; ++j) {
-          uint32_t vb = 0;
+        auto value = [&](int j) {
+          const uint32_t vb = next(), step = np + j, sb = step & 1;
+          ok = ok && mbar_wait(p_full + 2 * w + sb, (step >> 1) & 1, abort_flag, a.err, 65);
+          if (!ok) return;
+          tc_fence_after();
+          uint32_t v = smem_u32(kv) + vb * BUF;
+          asm volatile("" : "+r"(v));
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            if (j >= cnt[w] || !ok) continue;
-            if (w == 0 || !it.two) vb = next();
-            ok = ok && mbar_wait(p_full + w, np[w] & 1, abort_flag, a.err, 65);
-            ++np[w];
-            if (!ok) continue;
-            tc_fence_after();
-            const uint32_t v = smem_u32(kv) + vb * BUF;
-#pragma unroll
-            for (int s = 0; s < TK / 16; ++s)
-              umma_ts(tmem + COL_O + 128 * w, tmem + 128 * w + 8 * s, umma::mndesc(v, TK, s), ID_O, j > 0 || s > 0);
-            if (w == 1 || !it.two) sm100::umma_commit(kv_empty + vb);
-            if (j + 1 < cnt[w]) {
-              if (w == 0 || !it.two) kb = next();
-              score(w, kb);
-              if (ok && (w == 1 || !it.two)) sm100::umma_commit(kv_empty + kb);
-            } else {
-              sm100::umma_commit(o_full + w);
-            }
+          for (int s = 0; s < TK / 16; ++s)
+            umma_ts(tmem + COL_O + 128 * w, tmem + 128 * w + 64 * sb + 8 * s, umma::mndesc(v, TK, s), ID_O, j > 0 || s > 0);
+          sm100::umma_commit(pv_done + 2 * w + sb);
+          sm100::umma_commit(kv_empty + vb);
+        };
+        ok = ok && mbar_wait(q_full, items & 1, abort_flag, a.err, 64);
+        if (it.two && w == 1) ok = ok && mbar_wait(q_full + 1, twos & 1, abort_flag, a.err, 64);
+        ++items;
+        twos += it.two;
+        for (int j = -2; j < n0 && ok; ++j) {  // the order of the ring
+          if (!it.two && w == 1) {
+            if (j >= 0) pass();
+            if (j + 2 < n0) pass();
+          }
+          if (j >= 0 && j < cnt) value(j);
+          if (j + 2 < cnt) score(j + 2);
+          if (!it.two && w == 0) {
+            if (j >= 0 && j < n1) pass();
+            if (j + 2 < n1) pass();
           }
         }
+        np += cnt;
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0);
     }
-  }
-  } else {  // ------------------------------------------ softmax: side w, a row a thread
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+  } else if (warp >= 4) {  // ------------------------------------------ softmax: side w, a row a thread
     const int w = (warp - 4) >> 2, quarter = warp & 3, row = 32 * quarter + lane, G = a.H / a.Hk;
     const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
     const uint32_t t_s = tmem + lanes + 128 * w, t_o = tmem + lanes + COL_O + 128 * w;
-    uint32_t n = 0, ns = 0, no = 0;  // buffers through the ring, scores and results seen
+    uint32_t n = 0, ns = 0;  // buffers through the ring, steps of this side
     bool ok = true;
     // a whole warp's wait; after one that ran out the items are only counted, so that both sides meet at their barriers
     auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
       return (bool)__all_sync(0xffffffffu, mbar_wait(bar, phase & 1, abort_flag, a.err, code));
     };
-    while (u < u_end) {
-      const Item it = next_item(a, u, u_first, u_end);
-      const int r = it.r0 + row + (it.two ? TQ * w : 0), tt = r / G;
-      const bool mine = r < it.r0 + it.rows;
-      const int64_t out = mine ? (int64_t)(it.g.row0 + tt) * a.H + it.h * G + (r - tt * G) : -1;
+    const float2 scale = both(a.scale2);
+    while (at.u < at.u_end) {
+      const Item it = next_item(a, at);
+      const int r_tile = it.r0 + (it.two ? TQ * w : 0);
       if (w == 0 || it.two) {  // the tile of queries; its last readers have been waited for
-        const uint4* src = reinterpret_cast<const uint4*>(a.qw + out * 2 * D);
-        const uint32_t dst = smem_u32(qs) + w * BUF;
+        const uint32_t dst = smem_u32(qs) + w * QBUF;
+        constexpr int C8 = D / 8;
+#pragma unroll 4
+        for (int c = 0; c < C8; ++c) {
+          const int x = c * 128 + (threadIdx.x & 127), qr = x / C8, ch = 8 * (x - qr * C8), r = r_tile + qr, tt = r / G;
+          const bool in = r < it.r0 + it.rows;
+          const bf16* src = a.qw + (((int64_t)(it.g.row0 + tt) * a.H + it.h * G + (r - tt * G)) * 2) * D + ch;
 #pragma unroll
-        for (int x = 0; x < (EXACT ? 2 : 1); ++x)
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c) {
-            const uint4 q = mine ? src[x * (D / 8) + c] : make_uint4(0, 0, 0, 0);
-            umma::st_shared16(dst + 2 * x * BUF + umma::sw_off16(TQ, row, 8 * c), q.x, q.y, q.z, q.w);
+          for (int e = 0; e < (EXACT ? 2 : 1); ++e) {
+            const uint4 q = in ? *reinterpret_cast<const uint4*>(src + e * D) : make_uint4(0, 0, 0, 0);
+            umma::st_shared16(dst + 2 * e * QBUF + umma::sw_off16(TQ, qr, ch), q.x, q.y, q.z, q.w);
           }
+        }
         umma::fence_async_smem();
         mbar_arrive(q_full + w);
       }
+      const int r = r_tile + row, tt = r / G;
+      const bool mine = r < it.r0 + it.rows;
+      const int64_t out = mine ? (int64_t)(it.g.row0 + tt) * a.H + it.h * G + (r - tt * G) : -1;
       const int cnt = it.count(w), last = min(it.g.keys - 1, it.g.before + (mine ? tt : 0));
-      // Cache rows behind the last one are made zero among the last block's values, as 0 times infinity is none; that
-      // block is a side's last one, and its values are last or last but one in the ring's order
+      // Cache rows behind the last one are made zero among the last block's values, as 0 times infinity is none (by both
+      // sides where both read them, each before its own products); that block is a side's last one, and its values are
+      // last or last but one in the ring's order
       const int n0 = it.count(0), n1 = it.two ? 0 : it.count(1);
       n += 2 * (n0 + n1);
-      const bool tail = cnt > 0 && (it.block(w, cnt - 1) + 1) * TK > it.g.keys && !(it.two && w == 1);
+      const bool tail = cnt > 0 && (it.block(w, cnt - 1) + 1) * TK > it.g.keys;
       const uint32_t tail_buf = n - (it.two || (n1 == n0) == (w == 1) ? 1 : 2);
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < cnt && ok; ++j) {
+#pragma unroll 1
+      for (int j = 0; j < cnt && ok; ++j, ++ns) {
         const int k0 = it.block(w, j) * TK;
-        ok = wait(s_full + w, ns, 66);
-        ++ns;
+        const uint32_t sb = ns & 1, t_b = t_s + 64 * sb;
+        ok = wait(s_full + 2 * w + sb, ns >> 1, 66);
         if (!ok) break;
         tc_fence_after();
         float s[TK];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_get32(t_s + 32 * c, s + 32 * c);
+        tmem_get32(t_b, s);
+        tmem_get32(t_b + 32, s + 32);
         tmem_wait();
         arrived<TK>(s);
         if (__any_sync(0xffffffffu, k0 + TK - 1 > last)) {
@@ -349,6 +385,8 @@ __global__ void __launch_bounds__(NTHR, 1)
           m = mn;
           l *= f;
           if (j > 0) {
+            ok = wait(pv_done + 2 * w + (sb ^ 1), (ns - 1) >> 1, 67);
+            tc_fence_after();
 #pragma unroll
             for (int c = 0; c < DC; ++c) {
               float o[32];
@@ -361,39 +399,36 @@ __global__ void __launch_bounds__(NTHR, 1)
             }
           }
         }
-        const float2 neg = both(m == -INFINITY ? 0.f : -m), scale = both(a.scale2);
-        float2 sum = both(0.f);
+        const float2 neg = both(m == -INFINITY ? 0.f : -m);
+        float2 sum[2] = {both(0.f), both(0.f)};
+        uint32_t p[TK / 2];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t p[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float2 x = fma2(make_float2(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), scale, neg);
-            const float2 y = make_float2(ex2(x.x), ex2(x.y));
-            sum = add2(sum, y);
-            p[e] = umma::pack_bf2(y.x, y.y);
-          }
-          tmem_put16(t_s + 16 * c, p);
+        for (int e = 0; e < TK / 2; ++e) {
+          const float2 x = fma2(make_float2(s[2 * e], s[2 * e + 1]), scale, neg);
+          const float2 y = make_float2(ex2(x.x), ex2(x.y));
+          sum[e & 1] = add2(sum[e & 1], y);
+          p[e] = umma::pack_bf2(y.x, y.y);
         }
-        l += sum.x + sum.y;
+        tmem_put32(t_b, p);
+        sum[0] = add2(sum[0], sum[1]);
+        l += sum[0].x + sum[0].y;
         tmem_put_wait();
         if (tail && j == cnt - 1) {
-          ok = wait(kv_full + tail_buf % NB, tail_buf / NB, 67);
-          if (k0 + row >= it.g.keys) {
-            const uint32_t at = smem_u32(kv) + (tail_buf % NB) * BUF + row * 128;
+          ok = wait(kv_full + tail_buf % NB, tail_buf / NB, 68) && ok;
+          if (row < TK && k0 + row >= it.g.keys) {
+            const uint32_t z = smem_u32(kv) + (tail_buf % NB) * BUF + row * 128;
 #pragma unroll
             for (int x = 0; x < SLABS; ++x)
 #pragma unroll
-              for (int c = 0; c < 8; ++c) umma::st_shared16(at + x * SLAB + 16 * c, 0, 0, 0, 0);
+              for (int c = 0; c < 8; ++c) umma::st_shared16(z + x * SLAB + 16 * c, 0, 0, 0, 0);
           }
           umma::fence_async_smem();
         }
         tc_fence_before();
-        mbar_arrive(p_full + w);
+        mbar_arrive(p_full + 2 * w + sb);
       }
       if (cnt > 0 && ok) {
-        ok = wait(o_full + w, no, 68);
-        ++no;
+        ok = wait(pv_done + 2 * w + ((ns - 1) & 1), (ns - 1) >> 1, 69);
         tc_fence_after();
       }
       // every thread comes to the barriers, whatever its waits said
@@ -461,7 +496,7 @@ __global__ void __launch_bounds__(NTHR, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 2) sm100::tmem_dealloc(tmem, 512);
+  if (warp == 3) sm100::tmem_dealloc(tmem, 512);
 }
 
 // bf16 caches (S Hk, M, D): boxes of 64 channels and 128 rows of one slot's head, rows past M as zeros
