@@ -1865,6 +1865,7 @@ torch::Tensor cached_attention(const torch::Tensor& q, const torch::Tensor& k, c
               " channels shared evenly by ", Hk, " key heads");
   const int64_t H = q.size(1) / D;
   TORCH_CHECK(T < (1ll << 30) && H < (1ll << 15) && T * H < (1ll << 31), op, ": sizes out of range");
+  TORCH_CHECK(H <= 128 * Hk, op, ": at most 128 query heads can share a key head, got ", H / Hk);
   TORCH_CHECK(std::isfinite(scale), op, ": sm_scale must be finite, got ", scale);
   check_rows(q, q, T, H * D, op, "q");
   check_rows(k, q, T, Hk * D, op, "k");

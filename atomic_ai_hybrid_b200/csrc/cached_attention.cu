@@ -172,89 +172,105 @@ AHB_DEVICE void store8(bf16* p, bf16* rest, const float* v) {
   if (rest) *reinterpret_cast<uint4*>(rest) = x;
 }
 
-// Block 0 makes the plan; every other block rotates, clips and places one token row.
+// Block 0 makes the plan; the others rotate, clip and place `per` token rows each, and make rows of no sequence zero.
 template <bool VEC>
-__global__ void __launch_bounds__(AT) ca_append(const Args a) {
+__global__ void __launch_bounds__(AT) ca_append(const Args a, int per) {
   if (blockIdx.x == 0) {
     make_plan(a);
     return;
   }
   __shared__ Seq s_sh;
-  __shared__ int i_sh;
-  const int t = blockIdx.x - 1;
-  if (threadIdx.x == 0) {
-    int i = -1;
-    if (a.cu) {  // the last sequence that starts at or before the row
-      int lo = 0, hi = a.B;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (a.cu[mid] <= t) lo = mid + 1;
-        else hi = mid;
-      }
-      i = lo - 1;
-    } else {
-      i = t / a.L;
-    }
-    Seq s{0, 0, 0, 0, 0, -1, 0};
-    if (i >= 0) s = load_seq(a, i);
-    if (t < s.row0 || t >= s.row0 + s.n) i = -1;
-    a.row_seq[t] = i;
-    i_sh = i;
-    s_sh = s;
-  }
-  __syncthreads();
-  if (i_sh < 0) return;
-  const Seq s = s_sh;
-  const int tt = t - s.row0, half = a.D >> 1, per = half >> 3;
-  const int64_t row = (int64_t)s.have + tt;
-  const float* cs = a.table >= 0 ? a.cos + (int64_t)(s.pos + tt) * a.D : nullptr;
-  const float* sn = a.table >= 0 ? a.sin + (int64_t)(s.pos + tt) * a.D : nullptr;
-  const int heads = a.H + 2 * a.Hk;
-  for (int x = threadIdx.x; x < heads * per; x += AT) {
-    const int h = x / per, c = (x - h * per) << 3;
-    const bf16* src;
-    bf16 *dst, *rest = nullptr;
-    bool turn = cs != nullptr;
-    if (h < a.H) {
-      src = a.q + (int64_t)t * a.qs + h * a.D;
-      dst = a.qw + ((int64_t)t * a.H + h) * 2 * a.D;
-      rest = dst + a.D;
-    } else {
-      const int hk = h < a.H + a.Hk ? h - a.H : h - a.H - a.Hk;
-      const int64_t at = (((int64_t)s.slot * a.Hk + hk) * a.M + row) * a.D;
-      if (h < a.H + a.Hk) {
-        src = a.k + (int64_t)t * a.ks + hk * a.D;
-        dst = a.kc + at;
+  __shared__ int i_sh, end_sh;
+  const int t_end = min(a.T, (int)blockIdx.x * per), half = a.D >> 1, pc = half >> 3, heads = a.H + 2 * a.Hk, G = a.H / a.Hk;
+  for (int t = (blockIdx.x - 1) * per; t < t_end;) {
+    __syncthreads();
+    if (threadIdx.x == 0) {  // the rows from t on that are of one sequence, or of none
+      int i = -1, end = t_end;
+      if (a.cu) {  // the last sequence that starts at or before the row
+        int lo = 0, hi = a.B;
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (a.cu[mid] <= t) lo = mid + 1;
+          else hi = mid;
+        }
+        i = lo - 1;
+        if (lo < a.B) end = min(end, a.cu[lo]);
       } else {
-        src = a.v + (int64_t)t * a.vs + hk * a.D;
-        dst = a.vc + at;
-        turn = false;
+        i = t / a.L;
+        end = min(end, (i + 1) * a.L);
       }
+      Seq s{0, 0, 0, 0, 0, -1, 0};
+      if (i >= 0) s = load_seq(a, i);
+      if (t < s.row0 || t >= s.row0 + s.n) i = -1;
+      else end = min(end, s.row0 + s.n);
+      i_sh = i;
+      s_sh = s;
+      end_sh = end;
     }
-    float lo[8], hi[8];
-    load8<VEC>(src + c, lo);
-    load8<VEC>(src + c + half, hi);
-    if (turn) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x1 = lo[i], x2 = hi[i];
-        lo[i] = x1 * cs[c + i] - x2 * sn[c + i];
-        hi[i] = x2 * cs[c + half + i] + x1 * sn[c + half + i];
+    __syncthreads();
+    const int i = i_sh, n = end_sh - t;
+    const Seq s = s_sh;
+    for (int x = threadIdx.x; x < n; x += AT) a.row_seq[t + x] = i;
+    if (i < 0) {
+      for (int64_t x = threadIdx.x; x < (int64_t)n * a.H * a.D / 8; x += AT)
+        reinterpret_cast<uint4*>(a.o + (int64_t)t * a.H * a.D)[x] = make_uint4(0, 0, 0, 0);
+      t = end_sh;
+      continue;
+    }
+    const bool exact = a.mass || s.n * G <= RT;  // some kernel multiplies the rounding remainders too
+    const int64_t row0 = (int64_t)s.have + t - s.row0;
+    const int pos0 = s.pos + t - s.row0;
+#pragma unroll 2
+    for (int x = threadIdx.x; x < n * heads * pc; x += AT) {
+      const int y = x / (heads * pc), z = x - y * heads * pc, h = z / pc, c = (z - h * pc) << 3;
+      const int64_t row = row0 + y;
+      const bf16* src;
+      bf16 *dst, *rest = nullptr;
+      bool turn = a.table >= 0;
+      if (h < a.H) {
+        src = a.q + (t + y) * a.qs + h * a.D;
+        dst = a.qw + ((int64_t)(t + y) * a.H + h) * 2 * a.D;
+        rest = exact ? dst + a.D : nullptr;
+      } else {
+        const int hk = h < a.H + a.Hk ? h - a.H : h - a.H - a.Hk;
+        const int64_t at = (((int64_t)s.slot * a.Hk + hk) * a.M + row) * a.D;
+        if (h < a.H + a.Hk) {
+          src = a.k + (t + y) * a.ks + hk * a.D;
+          dst = a.kc + at;
+        } else {
+          src = a.v + (t + y) * a.vs + hk * a.D;
+          dst = a.vc + at;
+          turn = false;
+        }
       }
-    }
-    if (rest && a.negate) {
+      float lo[8], hi[8];
+      load8<VEC>(src + c, lo);
+      load8<VEC>(src + c + half, hi);
+      if (turn) {
+        const float *cs = a.cos + (int64_t)(pos0 + y) * a.D + c, *sn = a.sin + (int64_t)(pos0 + y) * a.D + c;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) lo[i] = -lo[i], hi[i] = -hi[i];
+        for (int e = 0; e < 8; ++e) {
+          const float x1 = lo[e], x2 = hi[e];
+          lo[e] = x1 * cs[e] - x2 * sn[e];
+          hi[e] = x2 * cs[half + e] + x1 * sn[half + e];
+        }
+      }
+      if (h < a.H && a.negate) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) lo[e] = -lo[e], hi[e] = -hi[e];
+      }
+      store8(dst + c, rest ? rest + c : nullptr, lo);
+      store8(dst + c + half, rest ? rest + c + half : nullptr, hi);
     }
-    store8(dst + c, rest ? rest + c : nullptr, lo);
-    store8(dst + c + half, rest ? rest + c + half : nullptr, hi);
+    if (a.mass)
+      for (int x = threadIdx.x; x < n * a.Hk; x += AT) {
+        const int y = x / a.Hk, h = x - y * a.Hk;
+        const int64_t at = ((int64_t)s.slot * a.Hk + h) * a.M + row0 + y;
+        a.mass[at] = 0.f;
+        a.held[at] = pos0 + y;
+      }
+    t = end_sh;
   }
-  if (a.mass)
-    for (int h = threadIdx.x; h < a.Hk; h += AT) {
-      const int64_t at = ((int64_t)s.slot * a.Hk + h) * a.M + row;
-      a.mass[at] = 0.f;
-      a.held[at] = s.pos + tt;
-    }
 }
 
 // ----------------------------------------------------------------------------- rows against cache rows
@@ -362,7 +378,7 @@ __global__ void __launch_bounds__(RW * 32, RB) ca_rows(const Args a) {
     const Group gr = a.groups[pre ? a.B + i : i];
     const int per_head = row_units(gr);
     const int64_t u0 = pre ? n_own + runs[i] : own[i];
-    const int h = (int)((u - u0) / per_head);
+    const int h = (int)div64(u - u0, per_head);
     const int64_t first = u0 + (int64_t)h * per_head;  // the head's units
     const int ks = (int)(u - first), ke = (int)min((int64_t)per_head, u_end - first);
     u = first + ke;
@@ -418,12 +434,12 @@ __global__ void __launch_bounds__(RW * 32, RB) ca_rows(const Args a) {
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     const bool whole = ks == 0 && ke == per_head, final = whole && !a.full;
-    float* part = a.part + (2 * (int64_t)w + (first >= u_first ? 1 : 0)) * RT * (D + 2);
-    float* full = whole && a.full ? a.full + (int64_t)(pre ? a.T : 0) * a.H * (D + 2) : nullptr;
+    float* part = a.part + (2 * (int64_t)w + (first >= u_first ? 1 : 0)) * RT * (D + 4);
+    float* full = whole && a.full ? a.full + (int64_t)(pre ? a.T : 0) * a.H * (D + 4) : nullptr;
     const float inv = final ? 1.f / l : 1.f;
     if (t4 == 0 && out >= 0) {
       if (!final)
-        *reinterpret_cast<float2*>((full ? full + out * (D + 2) : part + g * (D + 2)) + D) = make_float2(m, l);
+        *reinterpret_cast<float2*>((full ? full + out * (D + 4) : part + g * (D + 4)) + D) = make_float2(m, l);
       else if (a.lse)
         a.lse[out] = m + log2f(l);
     }
@@ -432,7 +448,7 @@ __global__ void __launch_bounds__(RW * 32, RB) ca_rows(const Args a) {
       const int64_t row = __shfl_sync(0xffffffffu, out, 8 * t4 + 4 * b);
       const float f = __shfl_sync(0xffffffffu, inv, 8 * t4 + 4 * b);
       if (row < 0) continue;
-      float* y = full ? full + row * (D + 2) : part + (2 * t4 + b) * (D + 2);
+      float* y = full ? full + row * (D + 4) : part + (2 * t4 + b) * (D + 4);
 #pragma unroll
       for (int c = 0; c < VC; ++c) {
         const int at = 64 * c + (64 * c + 64 <= D ? 8 : 4) * g;
@@ -449,111 +465,170 @@ __global__ void __launch_bounds__(RW * 32, RB) ca_rows(const Args a) {
 }
 
 // ----------------------------------------------------------------------------- joining
-// One block for each token row, a query head for each warp in turn.  Zeros for rows of no sequence; nothing for what
-// is final already.
+// Partial results of one query row, a lane's channel pairs of them.
 template <int D>
-__global__ void __launch_bounds__(128) ca_join(const Args a) {
-  constexpr int PL = (D + 63) / 64;  // channel pairs of a lane
-  const int lane = threadIdx.x & 31, t = blockIdx.x, G = a.H / a.Hk;
-  const int i = a.row_seq[t];
-  if (i < 0) {
-    for (int x = threadIdx.x; x < a.H * D / 8; x += 128)
-      reinterpret_cast<uint4*>(a.o + (int64_t)t * a.H * D)[x] = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  // the group of the sequence's own rows, and that of its prefix run
-  Group gr[2];
-  int at[2], n = 1;
-  at[0] = i;
-  gr[0] = a.groups[i];
-  const int start = a.full ? a.run_start[i] : -1;
-  if (start >= 0) {
-    at[1] = a.run_end[start];
-    gr[1] = a.groups[a.B + at[1]];
-    n = 2;
-  }
-  for (int hq = threadIdx.x >> 5; hq < a.H; hq += 4) {
-    const int h = hq / G;
-    const int64_t out = (int64_t)t * a.H + hq;
-    float m = -INFINITY, l = 0.f;
-    float2 o[PL];
+struct Joined {
+  static constexpr int PL = (D + 63) / 64;
+  float m = -INFINITY, l = 0.f;
+  float2 o[PL];
+  AHB_DEVICE Joined() {
 #pragma unroll
     for (int c = 0; c < PL; ++c) o[c] = make_float2(0.f, 0.f);
-    // `count` partial results, `stride` apart: eight at a time, so that their loads travel together
-    auto add = [&](const float* y, int64_t stride, int count) {
-      for (int k0 = 0; k0 < count; k0 += 8) {
-        float2 ml[8], v[8][PL];
+  }
+  AHB_DEVICE void one(float2 ml, const float2* v) {
+    if (ml.x == -INFINITY) return;
+    const float mn = fmaxf(m, ml.x), f = ex2(m - mn), e = ex2(ml.x - mn);
+    m = mn;
+    l = l * f + ml.y * e;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (k0 + k >= count) break;
-          const float* p = y + (k0 + k) * stride;
-          ml[k] = *reinterpret_cast<const float2*>(p + D);
-#pragma unroll
-          for (int c = 0; c < PL; ++c)
-            if (64 * c + 2 * lane < D) v[k][c] = *reinterpret_cast<const float2*>(p + 64 * c + 2 * lane);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (k0 + k >= count || ml[k].x == -INFINITY) continue;
-          const float mn = fmaxf(m, ml[k].x), f = ex2(m - mn), e = ex2(ml[k].x - mn);
-          m = mn;
-          l = l * f + ml[k].y * e;
-#pragma unroll
-          for (int c = 0; c < PL; ++c) {
-            o[c].x = o[c].x * f + v[k][c].x * e;
-            o[c].y = o[c].y * f + v[k][c].y * e;
-          }
-        }
-      }
-    };
-    bool done = false;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      if (x >= n) break;
-      const Group& g = gr[x];
-      const bool tiles = is_tiles(a, g);
-      const int64_t* own = a.sums[tiles ? TILES : ROWS];
-      const int64_t* runs = own + a.B + 1;
-      const int64_t n_own = own[a.B], share = share_of(n_own + runs[a.B], tiles ? a.blocks : a.warps);
-      const int r = (t - g.row0) * G + hq - h * G;  // the row within the group and key head
-      int64_t first = x ? n_own + runs[at[1]] : own[at[0]];
-      int units, row = r, rows = RT;
-      if (tiles) {
-        const int nt = row_tiles(a, g), rt = r / (2 * TQ);
-        int before = 0, per_head = 0;
-        for (int k = lane; k < nt; k += 32) {
-          const int q = tile_item(a, g, k).units;
-          before += k < rt ? q : 0;
-          per_head += q;
-        }
-        before = __reduce_add_sync(0xffffffffu, before);
-        per_head = __reduce_add_sync(0xffffffffu, per_head);
-        first += (int64_t)h * per_head + before;
-        units = tile_item(a, g, rt).units;
-        row = r - rt * 2 * TQ;
-        rows = 2 * TQ;
-      } else {
-        units = row_units(g);
-        first += (int64_t)h * units;
-      }
-      const int64_t w0 = first / share, w1 = (first + units - 1) / share;
-      if (w0 == w1) {
-        done = !a.full;
-        if (!done) add(a.full + ((int64_t)x * a.T * a.H + out) * (D + 2), 0, 1);
-      } else {
-        const float* part = (tiles ? a.tile_part : a.part) + (int64_t)row * (D + 2);
-        const int64_t slot = (int64_t)rows * (D + 2);
-        add(part + (2 * w0 + (first >= w0 * share ? 1 : 0)) * slot, 0, 1);
-        add(part + 2 * (w0 + 1) * slot, 2 * slot, (int)(w1 - w0));  // the others began before their worker's units
-      }
+    for (int c = 0; c < PL; ++c) {
+      o[c].x = o[c].x * f + v[c].x * e;
+      o[c].y = o[c].y * f + v[c].y * e;
     }
-    if (done) continue;
+  }
+  // `count` results, `stride` apart: eight at a time, so that their loads travel together
+  AHB_DEVICE void add(const float* y, int64_t stride, int count) {
+    const int lane = threadIdx.x & 31;
+    for (int k0 = 0; k0 < count; k0 += 8) {
+      float2 ml[8], v[8][PL];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (k0 + k >= count) break;
+        const float* p = y + (k0 + k) * stride;
+        ml[k] = *reinterpret_cast<const float2*>(p + D);
+#pragma unroll
+        for (int c = 0; c < PL; ++c)
+          if (64 * c + 2 * lane < D) v[k][c] = *reinterpret_cast<const float2*>(p + 64 * c + 2 * lane);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k0 + k < count) one(ml[k], v[k]);
+    }
+  }
+  AHB_DEVICE void finish(const Args& a, int64_t out) const {
+    const int lane = threadIdx.x & 31;
     const float inv = 1.f / l;
 #pragma unroll
     for (int c = 0; c < PL; ++c)
       if (64 * c + 2 * lane < D)
         *reinterpret_cast<uint32_t*>(a.o + out * D + 64 * c + 2 * lane) = pack2(o[c].x * inv, o[c].y * inv);
     if (a.lse && lane == 0) a.lse[out] = m + log2f(l);
+  }
+};
+
+constexpr int JW = 8;  // warps of a block
+
+// A block takes a token row and JW query heads (WIDE: one head, its partial results spread over the warps: where rows are
+// few, every one is cut into many).  Nothing is done for what is final already.
+template <int D, bool WIDE>
+__global__ void __launch_bounds__(JW * 32) ca_join(const Args a) {
+  const int warp = threadIdx.x >> 5, t = blockIdx.x, G = a.H / a.Hk;
+  const int hq = WIDE ? blockIdx.y : blockIdx.y * JW + warp, h = hq / G;
+  const int i = a.row_seq[t];
+  if (i < 0) return;
+  // the group of the sequence's own rows, and that of its prefix run
+  Group gr[2];
+  int at[2], n = 1;
+  at[0] = i;
+  gr[0] = a.groups[i];
+  if (!a.full && is_tiles(a, gr[0])) return;  // ca_join_tiles
+  const int start = a.full ? a.run_start[i] : -1;
+  if (start >= 0) {
+    at[1] = a.run_end[start];
+    gr[1] = a.groups[a.B + at[1]];
+    n = 2;
+  }
+  if (hq >= a.H) return;
+  const int64_t out = (int64_t)t * a.H + hq;
+  Joined<D> sum;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    if (x >= n) break;
+    const Group& g = gr[x];
+    const bool tiles = is_tiles(a, g);
+    const int64_t* own = a.sums[tiles ? TILES : ROWS];
+    const int64_t* runs = own + a.B + 1;
+    const int64_t n_own = own[a.B], share = share_of(n_own + runs[a.B], tiles ? a.blocks : a.warps);
+    int64_t first = x ? n_own + runs[at[1]] : own[at[0]];
+    int units, row = (t - g.row0) * G + hq - h * G, rows = RT;  // the row within the group and key head
+    if (tiles) {
+      const int rt = row / (2 * a.tile_rows);
+      const int64_t per_head = div64(x ? runs[at[1] + 1] - runs[at[1]] : own[at[0] + 1] - own[at[0]], a.Hk);
+      int before = 0;
+      for (int k = threadIdx.x & 31; k < rt; k += 32) before += tile_item(a, g, k).units;
+      first += h * per_head + __reduce_add_sync(0xffffffffu, before);
+      units = tile_item(a, g, rt).units;
+      row -= rt * 2 * a.tile_rows;
+      rows = 2 * TQ;
+    } else {
+      units = row_units(g);
+      first += (int64_t)h * units;
+    }
+    const int64_t w0 = div64(first, share), w1 = div64(first + units - 1, share);
+    if (w0 == w1) {
+      if (!a.full) return;
+      if (!WIDE || warp == 0) sum.add(a.full + ((int64_t)x * a.T * a.H + out) * (D + 4), 0, 1);
+    } else {
+      const float* part = (tiles ? a.tile_part : a.part) + (int64_t)row * (D + 4);
+      const int64_t slot = (int64_t)rows * (D + 4);
+      if (!WIDE || warp == 0) sum.add(part + (2 * w0 + (first >= w0 * share ? 1 : 0)) * slot, 0, 1);
+      const int more = (int)(w1 - w0);  // the others began before their worker's units
+      if (WIDE) {
+        const int each = (more + JW - 1) / JW, k0 = warp * each;
+        if (k0 < more) sum.add(part + 2 * (w0 + 1 + k0) * slot, 2 * slot, min(each, more - k0));
+      } else {
+        sum.add(part + 2 * (w0 + 1) * slot, 2 * slot, more);
+      }
+    }
+  }
+  if (WIDE) {
+    constexpr int PL = Joined<D>::PL;
+    __shared__ float2 sh[JW][PL + 1][32];
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int c = 0; c < PL; ++c) sh[warp][c][lane] = sum.o[c];
+    sh[warp][PL][lane] = make_float2(sum.m, sum.l);
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int k = 1; k < JW; ++k) {
+      float2 v[PL];
+#pragma unroll
+      for (int c = 0; c < PL; ++c) v[c] = sh[k][c][lane];
+      sum.one(sh[k][PL][lane], v);
+    }
+  }
+  sum.finish(a, out);
+}
+
+// Without a prefix only items of the tile kernel that several of its blocks share are left to join.  Block (b, y) takes
+// rows 32 y .. of the item that began among block b's units and goes on behind them.
+template <int D>
+__global__ void __launch_bounds__(JW * 32) ca_join_tiles(const Args a) {
+  const int64_t* own = a.sums[TILES];
+  const int64_t all = own[a.B], share = share_of(all, a.blocks);
+  const int64_t u_first = blockIdx.x * share, u_end = u_first + share;
+  if (u_end >= all) return;
+  const int i = find_group(own, a.B, u_end - 1), G = a.H / a.Hk;
+  const Group g = a.groups[i];
+  const int64_t per_head = div64(own[i + 1] - own[i], a.Hk), v = u_end - 1 - own[i];
+  const int h = (int)div64(v, per_head);
+  int64_t first = own[i] + h * per_head;
+  int rt = 0;
+  TileItem it = tile_item(a, g, 0);
+  while (first + it.units < u_end) {
+    first += it.units;
+    it = tile_item(a, g, ++rt);
+  }
+  if (first < u_first || first + it.units <= u_end) return;
+  const int64_t w1 = div64(first + it.units - 1, share), slot = 2 * TQ * (D + 4);
+  for (int row = 32 * blockIdx.y + (threadIdx.x >> 5); row < min(it.rows, 32 * (int)blockIdx.y + 32); row += JW) {
+    const int r = 2 * a.tile_rows * rt + row, tt = r / G;
+    const float* part = a.tile_part + (int64_t)row * (D + 4);
+    Joined<D> sum;
+    sum.add(part + (2 * (int64_t)blockIdx.x + 1) * slot, 0, 1);
+    sum.add(part + 2 * ((int64_t)blockIdx.x + 1) * slot, 2 * slot, (int)(w1 - blockIdx.x));
+    sum.finish(a, (int64_t)(g.row0 + tt) * a.H + h * G + (r - tt * G));
   }
 }
 
@@ -568,7 +643,7 @@ __global__ void __launch_bounds__(RW * 32) ca_mass(const Args a, int kind) {
   for (int64_t u = (int64_t)blockIdx.x * RW + (threadIdx.x >> 5); u < all; u += (int64_t)gridDim.x * RW) {
     const int i = find_group(units, a.B, u);
     const Group gr = a.groups[i];
-    const int per_head = row_units(gr), h = (int)((u - units[i]) / per_head);
+    const int per_head = row_units(gr), h = (int)div64(u - units[i], per_head);
     const int j0 = (int)(u - units[i] - (int64_t)h * per_head) * KU;
     uint4 kr[2][D / 32];
     load_keys<D>(kr, a.kc + ((int64_t)gr.slot * a.Hk + h) * a.M * D, j0, gr.keys, g, t4);
@@ -621,6 +696,7 @@ int64_t lay_out(Args& a, char* base) {
   };
   const int64_t rows = (int64_t)a.T * a.H;
   const int sms = sm_count(), G = a.H / a.Hk;
+  a.tile_rows = TQ / G * G;
   a.warps = sms * RB * RW;
   // no group takes tiles if there is no run and every sequence has few rows
   a.blocks = a.prefix || a.cu || a.L * G > RT ? sms : 0;
@@ -631,9 +707,9 @@ int64_t lay_out(Args& a, char* base) {
   a.run_end = (int*)place((int64_t)a.B * 4);
   for (int k = 0; k < (a.mass ? KINDS : 2); ++k) a.sums[k] = (int64_t*)place((int64_t)2 * (a.B + 1) * 8);
   a.lse = a.mass ? (float*)place(rows * 4) : nullptr;
-  a.part = (float*)place((int64_t)2 * a.warps * RT * (a.D + 2) * 4);
-  a.tile_part = (float*)place((int64_t)2 * a.blocks * 2 * TQ * (a.D + 2) * 4);
-  a.full = a.prefix ? (float*)place(2 * rows * (a.D + 2) * 4) : nullptr;
+  a.part = (float*)place((int64_t)2 * a.warps * RT * (a.D + 4) * 4);
+  a.tile_part = (float*)place((int64_t)2 * a.blocks * 2 * TQ * (a.D + 4) * 4);
+  a.full = a.prefix ? (float*)place(2 * rows * (a.D + 4) * 4) : nullptr;
   return at;
 }
 
@@ -644,7 +720,9 @@ int launch(const Args& a, cudaStream_t st) {
     if (rc) return rc;
   }
   ca_rows<D><<<a.warps / RW, RW * 32, 0, st>>>(a);
-  ca_join<D><<<a.T, 128, 0, st>>>(a);
+  if (a.blocks && !a.full) ca_join_tiles<D><<<dim3(a.blocks, 2 * TQ / 32), JW * 32, 0, st>>>(a);
+  if ((int64_t)a.T * a.H <= 4 * a.warps / (RB * RW)) ca_join<D, true><<<dim3(a.T, a.H), JW * 32, 0, st>>>(a);
+  else ca_join<D, false><<<dim3(a.T, (a.H + JW - 1) / JW), JW * 32, 0, st>>>(a);
   if (a.mass) {
     ca_mass<D><<<a.warps / RW, RW * 32, 0, st>>>(a, ROWS_MASS);
     if (a.blocks) ca_mass<D><<<a.warps / RW, RW * 32, 0, st>>>(a, TILES_MASS);
@@ -665,8 +743,9 @@ int ahb_cached_attention(const Args& args, void* work, cudaStream_t st) {
   a.scale2 = a.scale2 < 0.f ? -a.scale2 : a.scale2;
   lay_out(a, (char*)work);
   const bool vec = (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0 && ((a.qs | a.ks | a.vs) & 7) == 0;
-  if (vec) ca_append<true><<<a.T + 1, AT, 0, st>>>(a);
-  else ca_append<false><<<a.T + 1, AT, 0, st>>>(a);
+  const int per = 1 + (a.T - 1) / (8 * sm_count()), blocks = 1 + (a.T + per - 1) / per;  // eight blocks an SM at most
+  if (vec) ca_append<true><<<blocks, AT, 0, st>>>(a, per);
+  else ca_append<false><<<blocks, AT, 0, st>>>(a, per);
   switch (a.D) {
     case 64: return launch<64>(a, st);
     case 96: return launch<96>(a, st);

@@ -43,7 +43,8 @@ struct Args {
   float* lse;                    // (T, H) log2 of the softmax's denominators, for mass
   float* part;                   // partial results of items that several warps share, two a warp
   float* tile_part;              // ... of items that several blocks share, two a block
-  float* full;                   // (2, T, H, D + 2) whole results of own rows and of prefix rows, if there is a prefix
+  float* full;                   // (2, T, H, D + 4) whole results of own rows and of prefix rows, if there is a prefix
+  int tile_rows;                 // query rows of a tile: as many tokens as fit into 128 rows, with their heads
   int warps, blocks;             // warps of the row kernel, blocks of the tile kernel (0: it is not launched)
   int* err;                      // error word of waits that ran out
 };

@@ -10,7 +10,7 @@
 // on the other, and the two tiles' softmaxes share the exponential unit between them.  Where an item has
 // one tile only (a prefix under few tokens), the two sides take every other block of cache rows, and join at the end.
 //
-// Warps: 0 loads K and V by TMA into a ring of 16 KB buffers, 1 and 2 issue the two sides' products (one thread for
+// Warps: 0 loads K and V by TMA into a ring of 16 KB buffers, 3 the tiles of queries, 1 and 2 issue the two sides' products (one thread for
 // both spent as long on its waits and commits as the tensor cores on the products: a prompt of 8192 tokens 780 us), 4-7 and 8-11 are
 // the sides' softmaxes.
 // With `mass` the queries' rounding remainder multiplies too (S += Qlo K^T), as sums of weights are kept in 32 bits; without it the
@@ -40,10 +40,12 @@ constexpr uint32_t QBUF = 32 * 1024;  // a tile of queries: two 64-channel slabs
 constexpr uint32_t BUF = 16 * 1024;   // a block of K or V: two 64-channel slabs of 64 rows
 constexpr int COL_O = 256;            // TMEM columns: side w's S and P buffer b at 128 w + 64 b, its O at 256 + 128 w
 
+constexpr uint32_t STAGE = 4 * 1024;  // a softmax warp's results on their way out
+
 template <bool EXACT>
-constexpr int ring() { return EXACT ? 6 : 10; }
+constexpr int ring() { return EXACT ? 4 : 8; }
 template <bool EXACT>
-constexpr size_t smem_bytes() { return (size_t)BUF * ring<EXACT>() + QBUF * (EXACT ? 4 : 2) + 1024 + 2048; }
+constexpr size_t smem_bytes() { return (size_t)BUF * ring<EXACT>() + QBUF * (EXACT ? 4 : 2) + 8 * STAGE + 1024 + 2048; }
 
 struct Item {
   int pre, h, r0, rows, blocks, ks, ke;  // units ks .. ke of the item
@@ -80,8 +82,8 @@ AHB_DEVICE Item next_item(const Args& a, Place& p) {
     const int i = find_group(sums, a.B, v), lane = threadIdx.x & 31;
     p.x = pre ? a.B + i : i;
     it.g = a.groups[p.x];
-    const int64_t base = sums[i], per_head = (sums[i + 1] - base) / a.Hk;
-    p.h = (int)((v - base) / per_head);
+    const int64_t base = sums[i], per_head = div64(sums[i + 1] - base, a.Hk);
+    p.h = (int)div64(v - base, per_head);
     int64_t rest = v - base - p.h * per_head;
     const int tiles = row_tiles(a, it.g);
     for (p.rt = 0;; p.rt += 32) {  // 32 tiles at a time
@@ -106,10 +108,10 @@ AHB_DEVICE Item next_item(const Args& a, Place& p) {
   t = tile_item(a, it.g, p.rt);
   it.pre = p.x >= a.B;
   it.h = p.h;
-  it.r0 = p.rt * 2 * TQ;
+  it.r0 = p.rt * 2 * a.tile_rows;
   it.rows = t.rows;
   it.blocks = t.blocks;
-  it.two = t.rows > TQ;
+  it.two = t.rows > a.tile_rows;
   it.ks = p.at;
   it.ke = (int)min((int64_t)t.units, p.at + (p.u_end - p.u));
   it.whole = it.ks == 0 && it.ke == t.units;
@@ -170,21 +172,51 @@ AHB_DEVICE void tmem_put32(uint32_t addr, const uint32_t* r) {
 }
 AHB_DEVICE void tmem_put_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// 4-D TMA tile load (no multicast)
+AHB_DEVICE void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// A warp's 32 rows of B bytes (64 or 128), a row a thread, through shared memory, so that every row leaves in whole
+// 32-byte sectors.  dst(row): where a row goes, null for nowhere.
+template <int B, class F>
+AHB_DEVICE void rows_out(unsigned char* stage, const uint4* v, F&& dst) {
+  constexpr int C = B / 16, R = 32 / C;  // chunks a row, rows at a time
+  const int lane = threadIdx.x & 31;
+  auto at = [&](int row, int c) { return row * B + ((B == 128 ? c ^ (row & 7) : c ^ ((row >> 1) & 3)) << 4); };
+#pragma unroll
+  for (int c = 0; c < C; ++c) *reinterpret_cast<uint4*>(stage + at(lane, c)) = v[c];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const int row = i * R + lane / C, c = lane % C;
+    unsigned char* p = dst(row);
+    if (p) *reinterpret_cast<uint4*>(p + 16 * c) = *reinterpret_cast<const uint4*>(stage + at(row, c));
+  }
+  __syncwarp();
+}
+
 // named barriers of the softmax warps: 1 both sides
 AHB_DEVICE void sides_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 template <int D, bool EXACT>
 __global__ void __launch_bounds__(NTHR, 1)
-    ca_tiles(const Args a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
+    ca_tiles(const Args a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+             const __grid_constant__ CUtensorMap mq) {
   constexpr int NB = ring<EXACT>(), SLABS = (D + 63) / 64, DC = (D + 31) / 32;
   constexpr uint32_t SLAB = TK * 128, LOAD = SLABS * SLAB;
   extern __shared__ unsigned char raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* qs = smem;                               // tiles of queries (EXACT: rounded ones, then remainders)
   unsigned char* kv = smem + QBUF * (EXACT ? 4 : 2);      // the ring
-  uint64_t* bars = reinterpret_cast<uint64_t*>(kv + BUF * NB);
+  unsigned char* stage = kv + BUF * NB;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(stage + 8 * STAGE);
   // side w's buffer b at 2 w + b: its S is there, its P is, and its P V is done
-  uint64_t *kv_full = bars, *kv_empty = bars + NB, *q_full = bars + 2 * NB, *s_full = q_full + 2, *p_full = s_full + 4,
+  uint64_t *kv_full = bars, *kv_empty = bars + NB, *q_full = bars + 2 * NB, *q_empty = q_full + 2, *s_full = q_empty + 2, *p_full = s_full + 4,
            *pv_done = p_full + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -207,7 +239,10 @@ __global__ void __launch_bounds__(NTHR, 1)
       mbar_init(p_full + i, 128);
       mbar_init(pv_done + i, 1);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(q_full + i, 128);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + i, 1);
+      mbar_init(q_empty + i, 2);  // both sides' (a second tile: its side's twice)
+    }
     *abort_flag = 0;
     sm100::fence_barrier_init();
   }
@@ -281,6 +316,7 @@ __global__ void __launch_bounds__(NTHR, 1)
           }
           sm100::umma_commit(s_full + 2 * w + sb);
           sm100::umma_commit(kv_empty + kb);
+          if (j + 1 == cnt) sm100::umma_commit(q_empty + (it.two ? w : 0));
         };
         auto value = [&](int j) {
           const uint32_t vb = next(), step = np + j, sb = step & 1;
@@ -299,6 +335,9 @@ __global__ void __launch_bounds__(NTHR, 1)
         if (it.two && w == 1) ok = ok && mbar_wait(q_full + 1, twos & 1, abort_flag, a.err, 64);
         ++items;
         twos += it.two;
+        // the tiles of queries that this side does not read, or does not read after its last score
+        if (w == 1 && ok && (it.two || cnt == 0)) mbar_arrive(q_empty);
+        if (w == 0 && ok && it.two) mbar_arrive(q_empty + 1);
         for (int j = -2; j < n0 && ok; ++j) {  // the order of the ring
           if (!it.two && w == 1) {
             if (j >= 0) pass();
@@ -315,7 +354,35 @@ __global__ void __launch_bounds__(NTHR, 1)
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0);
     }
-  } else if (warp >= 4) {  // ------------------------------------------ softmax: side w, a row a thread
+  } else if (warp == 3) {  // ----------------------------------------- tiles of queries
+    uint32_t n[2] = {0, 0};
+    bool ok = true;
+    const int G = a.H / a.Hk;
+    const uint32_t bytes = a.tile_rows * 128 * SLABS * (EXACT ? 2 : 1);
+    while (at.u < at.u_end && ok) {
+      const Item it = next_item(a, at);
+      if (lane == 0) {
+        const int t0 = it.g.row0 + per_group(it.r0, G), tokens = per_group(a.tile_rows, G);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (x && !it.two) break;
+          if (n[x] > 0) ok = ok && mbar_wait(q_empty + x, (n[x] & 1) ^ 1, abort_flag, a.err, 70);
+          if (!ok) break;
+          mbar_expect_tx(q_full + x, bytes);
+#pragma unroll
+          for (int e = 0; e < (EXACT ? 2 : 1); ++e)
+#pragma unroll
+            for (int s = 0; s < SLABS; ++s)
+              tma_load_4d(qs + (x + 2 * e) * QBUF + s * TQ * 128, &mq, q_full + x, 64 * s, e, it.h * G, t0 + x * tokens);
+          ++n[x];
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+    }
+    if (lane == 0)
+      for (int x = 0; x < 2; ++x)
+        if (n[x] > 0) umma::wait_bar(q_full + x, (n[x] & 1) ^ 1, a.err, 71);
+  } else {  // --------------------------------------------------------- softmax: side w, a row a thread
     const int w = (warp - 4) >> 2, quarter = warp & 3, row = 32 * quarter + lane, G = a.H / a.Hk;
     const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
     const uint32_t t_s = tmem + lanes + 128 * w, t_o = tmem + lanes + COL_O + 128 * w;
@@ -328,26 +395,9 @@ __global__ void __launch_bounds__(NTHR, 1)
     const float2 scale = both(a.scale2);
     while (at.u < at.u_end) {
       const Item it = next_item(a, at);
-      const int r_tile = it.r0 + (it.two ? TQ * w : 0);
-      if (w == 0 || it.two) {  // the tile of queries; its last readers have been waited for
-        const uint32_t dst = smem_u32(qs) + w * QBUF;
-        constexpr int C8 = D / 8;
-#pragma unroll 4
-        for (int c = 0; c < C8; ++c) {
-          const int x = c * 128 + (threadIdx.x & 127), qr = x / C8, ch = 8 * (x - qr * C8), r = r_tile + qr, tt = r / G;
-          const bool in = r < it.r0 + it.rows;
-          const bf16* src = a.qw + (((int64_t)(it.g.row0 + tt) * a.H + it.h * G + (r - tt * G)) * 2) * D + ch;
-#pragma unroll
-          for (int e = 0; e < (EXACT ? 2 : 1); ++e) {
-            const uint4 q = in ? *reinterpret_cast<const uint4*>(src + e * D) : make_uint4(0, 0, 0, 0);
-            umma::st_shared16(dst + 2 * e * QBUF + umma::sw_off16(TQ, qr, ch), q.x, q.y, q.z, q.w);
-          }
-        }
-        umma::fence_async_smem();
-        mbar_arrive(q_full + w);
-      }
-      const int r = r_tile + row, tt = r / G;
-      const bool mine = r < it.r0 + it.rows;
+      const int r_tile = it.r0 + (it.two ? a.tile_rows * w : 0);
+      const int r = r_tile + row, tt = per_group(r, G);
+      const bool mine = row < a.tile_rows && r < it.r0 + it.rows;
       const int64_t out = mine ? (int64_t)(it.g.row0 + tt) * a.H + it.h * G + (r - tt * G) : -1;
       const int cnt = it.count(w), last = min(it.g.keys - 1, it.g.before + (mine ? tt : 0));
       // Cache rows behind the last one are made zero among the last block's values, as 0 times infinity is none (by both
@@ -450,10 +500,11 @@ __global__ void __launch_bounds__(NTHR, 1)
       if (ok && (w == 0 || it.two)) {
         const bool final = it.whole && !a.full, join = !it.two && it.count(1) > 0;
         const float inv = final ? 1.f / l : 1.f;
-        float* y = nullptr;
-        if (!final)
-          y = it.whole ? a.full + ((int64_t)(it.pre ? a.T : 0) * a.H + out) * (D + 2)
-                       : a.tile_part + ((2 * (int64_t)blockIdx.x + (it.late ? 0 : 1)) * 2 * TQ + r - it.r0) * (D + 2);
+        unsigned char* st = stage + (warp - 4) * STAGE;
+        // a row's place among whole results, or among this block's partial ones
+        const int64_t place = !mine ? -1 : final ? out : it.whole ? (int64_t)(it.pre ? a.T : 0) * a.H + out
+                                                                  : (2 * (int64_t)blockIdx.x + (it.late ? 0 : 1)) * 2 * TQ + r - it.r0;
+        float* y = it.whole ? a.full : a.tile_part;
 #pragma unroll
         for (int c = 0; c < DC; ++c) {
           float o[32];
@@ -470,22 +521,28 @@ __global__ void __launch_bounds__(NTHR, 1)
             tmem_wait();
             arrived<32>(o);
           }
-          if (mine && final) {
+          if (final) {
+            uint4 v[4];
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
+            for (int e = 0; e < 4; ++e) {
               float x[8];
 #pragma unroll
-              for (int k = 0; k < 8; ++k) x[k] = o[e + k] * inv;
-              *reinterpret_cast<uint4*>(a.o + out * D + 32 * c + e) = umma::pack8(x);
+              for (int k = 0; k < 8; ++k) x[k] = o[8 * e + k] * inv;
+              v[e] = umma::pack8(x);
             }
-          } else if (mine) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) *reinterpret_cast<float2*>(y + 32 * c + e) = make_float2(o[e], o[e + 1]);
+            rows_out<64>(st, v, [&](int k) {
+              const int64_t p = __shfl_sync(0xffffffffu, place, k);
+              return p < 0 ? nullptr : reinterpret_cast<unsigned char*>(a.o + p * D + 32 * c);
+            });
+          } else {
+            rows_out<128>(st, reinterpret_cast<const uint4*>(o), [&](int k) {
+              const int64_t p = __shfl_sync(0xffffffffu, place, k);
+              return p < 0 ? nullptr : reinterpret_cast<unsigned char*>(y + p * (D + 4) + 32 * c);
+            });
           }
-          __syncwarp();
         }
         if (mine) {
-          if (!final) *reinterpret_cast<float2*>(y + D) = make_float2(m, l);
+          if (!final) *reinterpret_cast<float2*>(y + place * (D + 4) + D) = make_float2(m, l);
           else if (a.lse) a.lse[out] = m + log2f(l);
         }
       }
@@ -512,27 +569,41 @@ int map_cache(CUtensorMap* m, const void* p, const Args& a) {
              : -2;
 }
 
+// the queries (T, H, 2, D): boxes of 64 channels of one half, for the query heads of a key head and as many tokens as a tile has
+int map_queries(CUtensorMap* m, const Args& a) {
+  TmapEncodeFn fn = tmap_encode_fn();
+  if (!fn) return -1;
+  const cuuint32_t G = a.H / a.Hk;
+  cuuint64_t dims[4] = {(cuuint64_t)a.D, 2, (cuuint64_t)a.H, (cuuint64_t)a.T};
+  cuuint64_t strides[3] = {(cuuint64_t)a.D * 2, (cuuint64_t)a.D * 4, (cuuint64_t)a.H * a.D * 4};
+  cuuint32_t box[4] = {64, 1, G, a.tile_rows / G}, es[4] = {1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, a.qw, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? 0
+             : -2;
+}
+
 template <int D, bool EXACT>
-int launch_one(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
+int launch_one(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, cudaStream_t st) {
   constexpr int bytes = (int)smem_bytes<EXACT>();
   if (cudaFuncSetAttribute(ca_tiles<D, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -3;
-  ca_tiles<D, EXACT><<<a.blocks, NTHR, bytes, st>>>(a, mk, mv);
+  ca_tiles<D, EXACT><<<a.blocks, NTHR, bytes, st>>>(a, mk, mv, mq);
   return 0;
 }
 
 template <int D>
-int launch_dim(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
-  return a.mass ? launch_one<D, true>(a, mk, mv, st) : launch_one<D, false>(a, mk, mv, st);
+int launch_dim(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, cudaStream_t st) {
+  return a.mass ? launch_one<D, true>(a, mk, mv, mq, st) : launch_one<D, false>(a, mk, mv, mq, st);
 }
 
 }  // namespace
 
 int ahb::cattn::launch_tiles(const Args& a, cudaStream_t st) {
-  CUtensorMap mk, mv;
-  if (map_cache(&mk, a.kc, a) || map_cache(&mv, a.vc, a)) return -2;
+  CUtensorMap mk, mv, mq;
+  if (map_cache(&mk, a.kc, a) || map_cache(&mv, a.vc, a) || map_queries(&mq, a)) return -2;
   switch (a.D) {
-    case 64: return launch_dim<64>(a, mk, mv, st);
-    case 96: return launch_dim<96>(a, mk, mv, st);
-    default: return launch_dim<128>(a, mk, mv, st);
+    case 64: return launch_dim<64>(a, mk, mv, mq, st);
+    case 96: return launch_dim<96>(a, mk, mv, mq, st);
+    default: return launch_dim<128>(a, mk, mv, mq, st);
   }
 }
