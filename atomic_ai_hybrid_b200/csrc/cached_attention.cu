@@ -557,7 +557,8 @@ __global__ void __launch_bounds__(JW * 32) ca_join(const Args a) {
       int before = 0;
       for (int k = threadIdx.x & 31; k < rt; k += 32) before += tile_item(a, g, k).units;
       first += h * per_head + __reduce_add_sync(0xffffffffu, before);
-      units = tile_item(a, g, rt).units;
+      first += ITEM_COST;
+      units = tile_item(a, g, rt).units - ITEM_COST;
       row -= rt * 2 * a.tile_rows;
       rows = 2 * TQ;
     } else {
@@ -620,7 +621,7 @@ __global__ void __launch_bounds__(JW * 32) ca_join_tiles(const Args a) {
     first += it.units;
     it = tile_item(a, g, ++rt);
   }
-  if (first < u_first || first + it.units <= u_end) return;
+  if (first + ITEM_COST < u_first || first + ITEM_COST >= u_end || first + it.units <= u_end) return;
   const int64_t w1 = div64(first + it.units - 1, share), slot = 2 * TQ * (D + 4);
   for (int row = 32 * blockIdx.y + (threadIdx.x >> 5); row < min(it.rows, 32 * (int)blockIdx.y + 32); row += JW) {
     const int r = 2 * a.tile_rows * rt + row, tt = r / G;

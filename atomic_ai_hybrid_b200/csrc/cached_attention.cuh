@@ -29,8 +29,11 @@ AHB_DEVICE bool is_tiles(const Args& a, const Group& g) { return query_rows(a, g
 AHB_DEVICE int row_units(const Group& g) { return ceil_div(g.keys, KU); }
 
 // Units of the tile kernel for the rt-th pair of tiles: 64 cache rows against two tiles, or 128 against one.
+// An item's first ITEM_COST units stand for its beginning and end, which take as long as that many blocks, and hold no block:
+// thread blocks with many short items get as much to do as those with one long one.
+constexpr int ITEM_COST = 4;
 struct TileItem {
-  int rows, blocks, units;  // valid query rows, blocks of cache rows that any of them sees, units
+  int rows, blocks, units;  // valid query rows, blocks of cache rows that any of them sees, units with ITEM_COST
 };
 AHB_DEVICE TileItem tile_item(const Args& a, const Group& g, int rt) {
   const int G = a.H / a.Hk;
@@ -38,7 +41,7 @@ AHB_DEVICE TileItem tile_item(const Args& a, const Group& g, int rt) {
   t.rows = min(2 * a.tile_rows, g.tokens * G - 2 * a.tile_rows * rt);
   const int last = per_group(2 * a.tile_rows * rt + t.rows - 1, G);  // the last token
   t.blocks = ceil_div((int)min((int64_t)g.keys, (int64_t)g.before + last + 1), TK);
-  t.units = t.rows > a.tile_rows ? t.blocks : (t.blocks + 1) >> 1;
+  t.units = ITEM_COST + (t.rows > a.tile_rows ? t.blocks : (t.blocks + 1) >> 1);
   return t;
 }
 AHB_DEVICE int row_tiles(const Args& a, const Group& g) { return ceil_div(query_rows(a, g), 2 * a.tile_rows); }

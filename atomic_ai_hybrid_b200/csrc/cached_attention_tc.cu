@@ -38,7 +38,7 @@ namespace {
 constexpr int NTHR = 384;
 constexpr uint32_t QBUF = 32 * 1024;  // a tile of queries: two 64-channel slabs of 128 rows
 constexpr uint32_t BUF = 16 * 1024;   // a block of K or V: two 64-channel slabs of 64 rows
-constexpr int COL_O = 256;            // TMEM columns: side w's S and P buffer b at 128 w + 64 b, its O at 256 + 128 w
+constexpr int COL_P = 64, COL_O = 256;  // TMEM columns: side w's S at 128 w, its P buffer b at 128 w + 64 + 32 b, its O at 256 + 128 w
 
 constexpr uint32_t STAGE = 4 * 1024;  // a softmax warp's results on their way out
 
@@ -50,7 +50,7 @@ constexpr size_t smem_bytes() { return (size_t)BUF * ring<EXACT>() + QBUF * (EXA
 struct Item {
   int pre, h, r0, rows, blocks, ks, ke;  // units ks .. ke of the item
   bool two, whole;                       // two tiles; all of the item's units
-  bool late;                             // the item began before this block's units
+  bool late;                             // its first block of cache rows came before this thread block's units
   Group g;
   // blocks of cache rows of side w in these units, and the j-th of them
   AHB_DEVICE int count(int w) const { return (two ? ke : min(ke, (blocks - w + 1) >> 1)) - ks; }
@@ -63,7 +63,8 @@ struct Place {
   int x, h, rt, at;  // group, key head, 256-row tile and the unit within it; x < 0: not looked up yet
 };
 
-// The next item, as far as this block's units go; moves the place behind it.  A whole warp calls it.
+// The next item, as far as this block's units go (the last one may be without a block of cache rows: ke <= ks); moves the
+// place behind it.  A whole warp calls it.
 AHB_DEVICE Item next_item(const Args& a, Place& p) {
   const int64_t *own = a.sums[TILES], *runs = own + a.B + 1;
   const int64_t n_own = own[a.B];
@@ -112,11 +113,12 @@ AHB_DEVICE Item next_item(const Args& a, Place& p) {
   it.rows = t.rows;
   it.blocks = t.blocks;
   it.two = t.rows > a.tile_rows;
-  it.ks = p.at;
-  it.ke = (int)min((int64_t)t.units, p.at + (p.u_end - p.u));
-  it.whole = it.ks == 0 && it.ke == t.units;
-  it.late = p.u - p.at < p.u_first;
-  p.u += it.ke - it.ks;
+  const int to = (int)min((int64_t)t.units, p.at + (p.u_end - p.u));
+  it.ks = max(p.at - ITEM_COST, 0);
+  it.ke = to - ITEM_COST;
+  it.whole = it.ks == 0 && to == t.units;
+  it.late = p.u - p.at + ITEM_COST < p.u_first;
+  p.u += to - p.at;
   return it;
 }
 
@@ -182,23 +184,30 @@ AHB_DEVICE void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, in
 }
 
 // A warp's 32 rows of B bytes (64 or 128), a row a thread, through shared memory, so that every row leaves in whole
-// 32-byte sectors.  dst(row): where a row goes, null for nowhere.
-template <int B, class F>
-AHB_DEVICE void rows_out(unsigned char* stage, const uint4* v, F&& dst) {
-  constexpr int C = B / 16, R = 32 / C;  // chunks a row, rows at a time
-  const int lane = threadIdx.x & 31;
-  auto at = [&](int row, int c) { return row * B + ((B == 128 ? c ^ (row & 7) : c ^ ((row >> 1) & 3)) << 4); };
+// 32-byte sectors: thread `lane` hands out chunk lane % C of rows lane / C, lane / C + R, ..  place[i]: which row of `out`,
+// `stride` bytes apart, the i-th of those is; negative for none.
+template <int B>
+struct RowsOut {
+  static constexpr int C = B / 16, R = 32 / C;  // chunks a row, rows at a time
+  int place[C];
+  AHB_DEVICE RowsOut(int mine) {
 #pragma unroll
-  for (int c = 0; c < C; ++c) *reinterpret_cast<uint4*>(stage + at(lane, c)) = v[c];
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < C; ++i) {
-    const int row = i * R + lane / C, c = lane % C;
-    unsigned char* p = dst(row);
-    if (p) *reinterpret_cast<uint4*>(p + 16 * c) = *reinterpret_cast<const uint4*>(stage + at(row, c));
+    for (int i = 0; i < C; ++i) place[i] = __shfl_sync(0xffffffffu, mine, i * R + (threadIdx.x & 31) / C);
   }
-  __syncwarp();
-}
+  static AHB_DEVICE int at(int row, int c) { return row * B + ((B == 128 ? c ^ (row & 7) : c ^ ((row >> 1) & 3)) << 4); }
+  AHB_DEVICE void write(unsigned char* stage, const uint4* v, unsigned char* out, int stride) const {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int c = 0; c < C; ++c) *reinterpret_cast<uint4*>(stage + at(lane, c)) = v[c];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (place[i] >= 0)
+        *reinterpret_cast<uint4*>(out + (int64_t)place[i] * stride + 16 * (lane % C)) =
+            *reinterpret_cast<const uint4*>(stage + at(i * R + lane / C, lane % C));
+    __syncwarp();
+  }
+};
 
 // named barriers of the softmax warps: 1 both sides
 AHB_DEVICE void sides_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
@@ -215,9 +224,9 @@ __global__ void __launch_bounds__(NTHR, 1)
   unsigned char* kv = smem + QBUF * (EXACT ? 4 : 2);      // the ring
   unsigned char* stage = kv + BUF * NB;
   uint64_t* bars = reinterpret_cast<uint64_t*>(stage + 8 * STAGE);
-  // side w's buffer b at 2 w + b: its S is there, its P is, and its P V is done
-  uint64_t *kv_full = bars, *kv_empty = bars + NB, *q_full = bars + 2 * NB, *q_empty = q_full + 2, *s_full = q_empty + 2, *p_full = s_full + 4,
-           *pv_done = p_full + 4;
+  // side w's S is there, and in registers; its P buffer b (at 2 w + b) is there, and its product done
+  uint64_t *kv_full = bars, *kv_empty = bars + NB, *q_full = bars + 2 * NB, *q_empty = q_full + 2, *s_full = q_empty + 2, *s_free = s_full + 2,
+           *p_full = s_free + 2, *pv_done = p_full + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float2* other = reinterpret_cast<float2*>(tmem_slot + 4);  // the second side's maximum and sum, row by row
@@ -235,11 +244,12 @@ __global__ void __launch_bounds__(NTHR, 1)
       mbar_init(kv_empty + i, 2);  // both sides'
     }
     for (int i = 0; i < 4; ++i) {
-      mbar_init(s_full + i, 1);
       mbar_init(p_full + i, 128);
       mbar_init(pv_done + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 1);
+      mbar_init(s_free + i, 128);
       mbar_init(q_full + i, 1);
       mbar_init(q_empty + i, 2);  // both sides' (a second tile: its side's twice)
     }
@@ -252,11 +262,15 @@ __global__ void __launch_bounds__(NTHR, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  // registers: 3 x 168 at the launch = 88 + 2 x 208
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 0) {  // ------------------------------------------------ loads
     uint32_t n = 0;
     bool ok = true;
     while (at.u < at.u_end && ok) {
       const Item it = next_item(a, at);
+      if (it.ke <= it.ks) break;
       if (lane == 0) {
         const int plane = it.g.slot * a.Hk + it.h;
         in_order(it, [&](bool is_v, int w, int j) {
@@ -285,6 +299,7 @@ __global__ void __launch_bounds__(NTHR, 1)
     bool ok = true;
     while (at.u < at.u_end && ok) {
       const Item it = next_item(a, at);
+      if (it.ke <= it.ks) break;
       if (lane == 0) {
         const int n0 = it.count(0), n1 = it.count(1), cnt = w ? n1 : n0;
         // Both sides go through the whole ring in order, so that neither mistakes one filling of a buffer for another: what a
@@ -299,22 +314,22 @@ __global__ void __launch_bounds__(NTHR, 1)
           const uint32_t b = next();
           if (ok) mbar_arrive(kv_empty + b);
         };
-        // a step uses S buffer (steps before this item + step) & 1
         auto score = [&](int j) {
-          const uint32_t kb = next(), sb = (np + j) & 1;
+          const uint32_t kb = next();
+          if (np + j > 0) ok = ok && mbar_wait(s_free + w, (np + j - 1) & 1, abort_flag, a.err, 72);
           if (!ok) return;
           uint32_t q = smem_u32(qs) + (it.two ? w : 0) * QBUF, k = smem_u32(kv) + kb * BUF;
           asm volatile("" : "+r"(q), "+r"(k));  // descriptors made here, not kept over the loop in registers
           tc_fence_after();
 #pragma unroll
           for (int s = 0; s < D / 16; ++s)
-            sm100::umma_bf16(tmem + 128 * w + 64 * sb, umma::kdesc(q, TQ, s), umma::kdesc(k, TK, s), ID_S, s > 0);
+            sm100::umma_bf16(tmem + 128 * w, umma::kdesc(q, TQ, s), umma::kdesc(k, TK, s), ID_S, s > 0);
           if (EXACT) {
 #pragma unroll
             for (int s = 0; s < D / 16; ++s)
-              sm100::umma_bf16(tmem + 128 * w + 64 * sb, umma::kdesc(q + 2 * QBUF, TQ, s), umma::kdesc(k, TK, s), ID_S, 1);
+              sm100::umma_bf16(tmem + 128 * w, umma::kdesc(q + 2 * QBUF, TQ, s), umma::kdesc(k, TK, s), ID_S, 1);
           }
-          sm100::umma_commit(s_full + 2 * w + sb);
+          sm100::umma_commit(s_full + w);
           sm100::umma_commit(kv_empty + kb);
           if (j + 1 == cnt) sm100::umma_commit(q_empty + (it.two ? w : 0));
         };
@@ -327,7 +342,7 @@ __global__ void __launch_bounds__(NTHR, 1)
           asm volatile("" : "+r"(v));
 #pragma unroll
           for (int s = 0; s < TK / 16; ++s)
-            umma_ts(tmem + COL_O + 128 * w, tmem + 128 * w + 64 * sb + 8 * s, umma::mndesc(v, TK, s), ID_O, j > 0 || s > 0);
+            umma_ts(tmem + COL_O + 128 * w, tmem + 128 * w + COL_P + 32 * sb + 8 * s, umma::mndesc(v, TK, s), ID_O, j > 0 || s > 0);
           sm100::umma_commit(pv_done + 2 * w + sb);
           sm100::umma_commit(kv_empty + vb);
         };
@@ -361,6 +376,7 @@ __global__ void __launch_bounds__(NTHR, 1)
     const uint32_t bytes = a.tile_rows * 128 * SLABS * (EXACT ? 2 : 1);
     while (at.u < at.u_end && ok) {
       const Item it = next_item(a, at);
+      if (it.ke <= it.ks) break;
       if (lane == 0) {
         const int t0 = it.g.row0 + per_group(it.r0, G), tokens = per_group(a.tile_rows, G);
 #pragma unroll
@@ -382,7 +398,9 @@ __global__ void __launch_bounds__(NTHR, 1)
     if (lane == 0)
       for (int x = 0; x < 2; ++x)
         if (n[x] > 0) umma::wait_bar(q_full + x, (n[x] & 1) ^ 1, a.err, 71);
+  }
   } else {  // --------------------------------------------------------- softmax: side w, a row a thread
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int w = (warp - 4) >> 2, quarter = warp & 3, row = 32 * quarter + lane, G = a.H / a.Hk;
     const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
     const uint32_t t_s = tmem + lanes + 128 * w, t_o = tmem + lanes + COL_O + 128 * w;
@@ -395,6 +413,7 @@ __global__ void __launch_bounds__(NTHR, 1)
     const float2 scale = both(a.scale2);
     while (at.u < at.u_end) {
       const Item it = next_item(a, at);
+      if (it.ke <= it.ks) break;
       const int r_tile = it.r0 + (it.two ? a.tile_rows * w : 0);
       const int r = r_tile + row, tt = per_group(r, G);
       const bool mine = row < a.tile_rows && r < it.r0 + it.rows;
@@ -411,15 +430,17 @@ __global__ void __launch_bounds__(NTHR, 1)
 #pragma unroll 1
       for (int j = 0; j < cnt && ok; ++j, ++ns) {
         const int k0 = it.block(w, j) * TK;
-        const uint32_t sb = ns & 1, t_b = t_s + 64 * sb;
-        ok = wait(s_full + 2 * w + sb, ns >> 1, 66);
+        const uint32_t pb = ns & 1;
+        ok = wait(s_full + w, ns, 66);
         if (!ok) break;
         tc_fence_after();
         float s[TK];
-        tmem_get32(t_b, s);
-        tmem_get32(t_b + 32, s + 32);
+        tmem_get32(t_s, s);
+        tmem_get32(t_s + 32, s + 32);
         tmem_wait();
         arrived<TK>(s);
+        tc_fence_before();
+        mbar_arrive(s_free + w);  // the next S may come
         if (__any_sync(0xffffffffu, k0 + TK - 1 > last)) {
 #pragma unroll
           for (int c = 0; c < TK; ++c) s[c] = k0 + c <= last ? s[c] : -INFINITY;
@@ -435,7 +456,7 @@ __global__ void __launch_bounds__(NTHR, 1)
           m = mn;
           l *= f;
           if (j > 0) {
-            ok = wait(pv_done + 2 * w + (sb ^ 1), (ns - 1) >> 1, 67);
+            ok = wait(pv_done + 2 * w + (pb ^ 1), (ns - 1) >> 1, 67);
             tc_fence_after();
 #pragma unroll
             for (int c = 0; c < DC; ++c) {
@@ -459,7 +480,11 @@ __global__ void __launch_bounds__(NTHR, 1)
           sum[e & 1] = add2(sum[e & 1], y);
           p[e] = umma::pack_bf2(y.x, y.y);
         }
-        tmem_put32(t_b, p);
+        if (ns >= 2) {  // the buffer's last product
+          ok = wait(pv_done + 2 * w + pb, (ns >> 1) - 1, 73) && ok;
+          tc_fence_after();
+        }
+        tmem_put32(t_s + COL_P + 32 * pb, p);
         sum[0] = add2(sum[0], sum[1]);
         l += sum[0].x + sum[0].y;
         tmem_put_wait();
@@ -475,7 +500,7 @@ __global__ void __launch_bounds__(NTHR, 1)
           umma::fence_async_smem();
         }
         tc_fence_before();
-        mbar_arrive(p_full + 2 * w + sb);
+        mbar_arrive(p_full + 2 * w + pb);
       }
       if (cnt > 0 && ok) {
         ok = wait(pv_done + 2 * w + ((ns - 1) & 1), (ns - 1) >> 1, 69);
@@ -499,15 +524,8 @@ __global__ void __launch_bounds__(NTHR, 1)
       }
       if (ok && (w == 0 || it.two)) {
         const bool final = it.whole && !a.full, join = !it.two && it.count(1) > 0;
-        const float inv = final ? 1.f / l : 1.f;
         unsigned char* st = stage + (warp - 4) * STAGE;
-        // a row's place among whole results, or among this block's partial ones
-        const int64_t place = !mine ? -1 : final ? out : it.whole ? (int64_t)(it.pre ? a.T : 0) * a.H + out
-                                                                  : (2 * (int64_t)blockIdx.x + (it.late ? 0 : 1)) * 2 * TQ + r - it.r0;
-        float* y = it.whole ? a.full : a.tile_part;
-#pragma unroll
-        for (int c = 0; c < DC; ++c) {
-          float o[32];
+        auto result = [&](int c, float* o) {  // 32 channels of the row
           tmem_get32(t_o + 32 * c, o);
           if (join) {
             float b[32];
@@ -521,7 +539,14 @@ __global__ void __launch_bounds__(NTHR, 1)
             tmem_wait();
             arrived<32>(o);
           }
-          if (final) {
+        };
+        if (final) {
+          const RowsOut<64> rows((int)out);
+          const float inv = 1.f / l;
+#pragma unroll
+          for (int c = 0; c < DC; ++c) {
+            float o[32];
+            result(c, o);
             uint4 v[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -530,20 +555,22 @@ __global__ void __launch_bounds__(NTHR, 1)
               for (int k = 0; k < 8; ++k) x[k] = o[8 * e + k] * inv;
               v[e] = umma::pack8(x);
             }
-            rows_out<64>(st, v, [&](int k) {
-              const int64_t p = __shfl_sync(0xffffffffu, place, k);
-              return p < 0 ? nullptr : reinterpret_cast<unsigned char*>(a.o + p * D + 32 * c);
-            });
-          } else {
-            rows_out<128>(st, reinterpret_cast<const uint4*>(o), [&](int k) {
-              const int64_t p = __shfl_sync(0xffffffffu, place, k);
-              return p < 0 ? nullptr : reinterpret_cast<unsigned char*>(y + p * (D + 4) + 32 * c);
-            });
+            rows.write(st, v, reinterpret_cast<unsigned char*>(a.o + 32 * c), D * 2);
           }
-        }
-        if (mine) {
-          if (!final) *reinterpret_cast<float2*>(y + place * (D + 4) + D) = make_float2(m, l);
-          else if (a.lse) a.lse[out] = m + log2f(l);
+          if (mine && a.lse) a.lse[out] = m + log2f(l);
+        } else {
+          // among whole results, or among this block's partial ones
+          float* y = it.whole ? a.full + (int64_t)(it.pre ? a.T : 0) * a.H * (D + 4)
+                              : a.tile_part + (2 * (int64_t)blockIdx.x + (it.late ? 0 : 1)) * 2 * TQ * (D + 4);
+          const int place = !mine ? -1 : it.whole ? (int)out : r - it.r0;
+          const RowsOut<128> rows(place);
+#pragma unroll
+          for (int c = 0; c < DC; ++c) {
+            float o[32];
+            result(c, o);
+            rows.write(st, reinterpret_cast<const uint4*>(o), reinterpret_cast<unsigned char*>(y + 32 * c), (D + 4) * 4);
+          }
+          if (mine) *reinterpret_cast<float2*>(y + (int64_t)place * (D + 4) + D) = make_float2(m, l);
         }
       }
       tc_fence_before();
