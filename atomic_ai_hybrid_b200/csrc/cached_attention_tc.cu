@@ -37,13 +37,14 @@ namespace {
 
 constexpr int NTHR = 384;
 constexpr uint32_t QBUF = 32 * 1024;  // a tile of queries: two 64-channel slabs of 128 rows
-constexpr uint32_t BUF = 16 * 1024;   // a block of K or V: two 64-channel slabs of 64 rows
+constexpr uint32_t HALF = 16 * 1024;  // a block of K or V: two 64-channel slabs of 64 rows
+constexpr uint32_t BUF = 2 * HALF;    // what a step multiplies: the K of its S, the V of its P
 constexpr int COL_P = 64, COL_O = 256;  // TMEM columns: side w's S at 128 w, its P buffer b at 128 w + 64 + 32 b, its O at 256 + 128 w
 
 constexpr uint32_t STAGE = 4 * 1024;  // a softmax warp's results on their way out
 
 template <bool EXACT>
-constexpr int ring() { return EXACT ? 4 : 8; }
+constexpr int ring() { return EXACT ? 2 : 4; }
 template <bool EXACT>
 constexpr size_t smem_bytes() { return (size_t)BUF * ring<EXACT>() + QBUF * (EXACT ? 4 : 2) + 8 * STAGE + 1024 + 2048; }
 
@@ -122,19 +123,11 @@ AHB_DEVICE Item next_item(const Args& a, Place& p) {
   return it;
 }
 
-// The order in which blocks of K and V go through the ring: the sides' first two K, then for every step and side V and the
-// K of two steps on.  With two tiles both sides read the same ones.  f(is V, side, step).
-template <class F>
-AHB_DEVICE void in_order(const Item& it, F&& f) {
-  const int n0 = it.count(0), n1 = it.two ? 0 : it.count(1);
-#pragma unroll 1
-  for (int j = -2; j < n0; ++j) {
-    if (j >= 0) f(true, 0, j);
-    if (j + 2 < n0) f(false, 0, j + 2);
-    if (j >= 0 && j < n1) f(true, 1, j);
-    if (j + 2 < n1) f(false, 1, j + 2);
-  }
-}
+// A side's steps are j = -2 .. n - 1 for n blocks: step j makes S(j + 2) and multiplies P(j) V(j), where there are such, once
+// the softmax has taken S(j + 1) into registers, with P(j) behind it.  What a step reads is one filling of the ring: K(j + 2)
+// and V(j); with two tiles both sides read the same one, else side 0's and side 1's take turns.
+AHB_DEVICE bool has_step(int j, int n) { return (j >= 0 && j < n) || (j < 0 && j + 2 < n); }
+AHB_DEVICE int fillings(int n) { return n > 1 ? n + 2 : 2 * n; }
 
 AHB_DEVICE void umma_ts(uint32_t d, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -224,10 +217,9 @@ __global__ void __launch_bounds__(NTHR, 1)
   unsigned char* kv = smem + QBUF * (EXACT ? 4 : 2);      // the ring
   unsigned char* stage = kv + BUF * NB;
   uint64_t* bars = reinterpret_cast<uint64_t*>(stage + 8 * STAGE);
-  // side w's S is there, and in registers; its P buffer b (at 2 w + b) is there, and its product done
-  uint64_t *kv_full = bars, *kv_empty = bars + NB, *q_full = bars + 2 * NB, *q_empty = q_full + 2, *s_full = q_empty + 2, *s_free = s_full + 2,
-           *p_full = s_free + 2, *pv_done = p_full + 4;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 4);
+  // of side w: its steps are done (at 2 w, by turns); the softmax has taken a step's S, with the P before it
+  uint64_t *kv_full = bars, *kv_empty = bars + NB, *q_full = bars + 2 * NB, *q_empty = q_full + 2, *done = q_empty + 2, *taken = done + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(taken + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float2* other = reinterpret_cast<float2*>(tmem_slot + 4);  // the second side's maximum and sum, row by row
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -243,13 +235,9 @@ __global__ void __launch_bounds__(NTHR, 1)
       mbar_init(kv_full + i, 1);
       mbar_init(kv_empty + i, 2);  // both sides'
     }
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(p_full + i, 128);
-      mbar_init(pv_done + i, 1);
-    }
+    for (int i = 0; i < 4; ++i) mbar_init(done + i, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full + i, 1);
-      mbar_init(s_free + i, 128);
+      mbar_init(taken + i, 4);  // a side's warps
       mbar_init(q_full + i, 1);
       mbar_init(q_empty + i, 2);  // both sides' (a second tile: its side's twice)
     }
@@ -273,20 +261,26 @@ __global__ void __launch_bounds__(NTHR, 1)
       if (it.ke <= it.ks) break;
       if (lane == 0) {
         const int plane = it.g.slot * a.Hk + it.h;
-        in_order(it, [&](bool is_v, int w, int j) {
-          if (!ok) return;
-          const uint32_t b = n % NB;
-          if (n >= NB && !mbar_wait(kv_empty + b, ((n / NB) & 1) ^ 1, abort_flag, a.err, 61)) {
-            ok = false;
-            return;
-          }
-          mbar_expect_tx(kv_full + b, LOAD);
-          const int row = it.block(w, j) * TK;
+        const int n0 = it.count(0), n1 = it.two ? 0 : it.count(1);
+        for (int j = -2; j < n0; ++j)
 #pragma unroll
-          for (int s = 0; s < SLABS; ++s)
-            umma::tma_load_3d(kv + b * BUF + s * SLAB, is_v ? &mv : &mk, kv_full + b, 64 * s, row, plane);
-          ++n;
-        });
+          for (int w = 0; w < 2; ++w) {
+            const int cnt = w ? n1 : n0;
+            if (!has_step(j, cnt) || !ok) continue;
+            const uint32_t b = n % NB;
+            if (n >= NB && !mbar_wait(kv_empty + b, ((n / NB) & 1) ^ 1, abort_flag, a.err, 61)) {
+              ok = false;
+              continue;
+            }
+            const bool k = j + 2 < cnt, v = j >= 0;
+            mbar_expect_tx(kv_full + b, (k ? LOAD : 0) + (v ? LOAD : 0));
+#pragma unroll
+            for (int s = 0; s < SLABS; ++s) {
+              if (v) umma::tma_load_3d(kv + b * BUF + HALF + s * SLAB, &mv, kv_full + b, 64 * s, it.block(w, j) * TK, plane);
+              if (k) umma::tma_load_3d(kv + b * BUF + s * SLAB, &mk, kv_full + b, 64 * s, it.block(w, j + 2) * TK, plane);
+            }
+            ++n;
+          }
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0);
     }
@@ -295,56 +289,20 @@ __global__ void __launch_bounds__(NTHR, 1)
   } else if (warp < 3) {  // ------------------------------------------ products of side w
     constexpr uint32_t ID_S = sm100::idesc_bf16(TQ, TK, false, false), ID_O = sm100::idesc_bf16(TQ, D, false, true);
     const int w = warp - 1;
-    uint32_t n = 0, np = 0, items = 0, twos = 0;  // buffers through the ring, steps of this side, items, those of two tiles
+    uint32_t n = 0, nd = 0, nt = 0, items = 0, twos = 0;  // fillings, steps, S taken, items, those of two tiles
     bool ok = true;
     while (at.u < at.u_end && ok) {
       const Item it = next_item(a, at);
       if (it.ke <= it.ks) break;
       if (lane == 0) {
-        const int n0 = it.count(0), n1 = it.count(1), cnt = w ? n1 : n0;
+        const int n0 = it.count(0), n1 = it.count(1), cnt = w ? n1 : n0, others = it.two ? 0 : w ? n0 : n1;
         // Both sides go through the whole ring in order, so that neither mistakes one filling of a buffer for another: what a
         // side does not use it gives back at once.
-        auto next = [&]() {
-          const uint32_t b = n % NB;
-          ok = ok && mbar_wait(kv_full + b, (n / NB) & 1, abort_flag, a.err, 63);
+        auto pass = [&](int j) {
+          if (!has_step(j, others)) return;
+          ok = ok && mbar_wait(kv_full + n % NB, (n / NB) & 1, abort_flag, a.err, 63);
+          if (ok) mbar_arrive(kv_empty + n % NB);
           ++n;
-          return b;
-        };
-        auto pass = [&]() {
-          const uint32_t b = next();
-          if (ok) mbar_arrive(kv_empty + b);
-        };
-        auto score = [&](int j) {
-          const uint32_t kb = next();
-          if (np + j > 0) ok = ok && mbar_wait(s_free + w, (np + j - 1) & 1, abort_flag, a.err, 72);
-          if (!ok) return;
-          uint32_t q = smem_u32(qs) + (it.two ? w : 0) * QBUF, k = smem_u32(kv) + kb * BUF;
-          asm volatile("" : "+r"(q), "+r"(k));  // descriptors made here, not kept over the loop in registers
-          tc_fence_after();
-#pragma unroll
-          for (int s = 0; s < D / 16; ++s)
-            sm100::umma_bf16(tmem + 128 * w, umma::kdesc(q, TQ, s), umma::kdesc(k, TK, s), ID_S, s > 0);
-          if (EXACT) {
-#pragma unroll
-            for (int s = 0; s < D / 16; ++s)
-              sm100::umma_bf16(tmem + 128 * w, umma::kdesc(q + 2 * QBUF, TQ, s), umma::kdesc(k, TK, s), ID_S, 1);
-          }
-          sm100::umma_commit(s_full + w);
-          sm100::umma_commit(kv_empty + kb);
-          if (j + 1 == cnt) sm100::umma_commit(q_empty + (it.two ? w : 0));
-        };
-        auto value = [&](int j) {
-          const uint32_t vb = next(), step = np + j, sb = step & 1;
-          ok = ok && mbar_wait(p_full + 2 * w + sb, (step >> 1) & 1, abort_flag, a.err, 65);
-          if (!ok) return;
-          tc_fence_after();
-          uint32_t v = smem_u32(kv) + vb * BUF;
-          asm volatile("" : "+r"(v));
-#pragma unroll
-          for (int s = 0; s < TK / 16; ++s)
-            umma_ts(tmem + COL_O + 128 * w, tmem + 128 * w + COL_P + 32 * sb + 8 * s, umma::mndesc(v, TK, s), ID_O, j > 0 || s > 0);
-          sm100::umma_commit(pv_done + 2 * w + sb);
-          sm100::umma_commit(kv_empty + vb);
         };
         ok = ok && mbar_wait(q_full, items & 1, abort_flag, a.err, 64);
         if (it.two && w == 1) ok = ok && mbar_wait(q_full + 1, twos & 1, abort_flag, a.err, 64);
@@ -353,19 +311,43 @@ __global__ void __launch_bounds__(NTHR, 1)
         // the tiles of queries that this side does not read, or does not read after its last score
         if (w == 1 && ok && (it.two || cnt == 0)) mbar_arrive(q_empty);
         if (w == 0 && ok && it.two) mbar_arrive(q_empty + 1);
-        for (int j = -2; j < n0 && ok; ++j) {  // the order of the ring
-          if (!it.two && w == 1) {
-            if (j >= 0) pass();
-            if (j + 2 < n0) pass();
+        for (int j = -2; j < n0 && ok; ++j) {
+          if (w == 1) pass(j);
+          if (j < cnt && cnt > 0) {
+            const bool some = has_step(j, cnt);
+            const uint32_t b = n % NB, t_w = tmem + 128 * w;
+            if (some) ok = ok && mbar_wait(kv_full + b, (n / NB) & 1, abort_flag, a.err, 63);
+            if (j >= -1) {
+              ok = ok && mbar_wait(taken + w, nt & 1, abort_flag, a.err, 65);
+              ++nt;
+            }
+            if (!ok) break;
+            uint32_t q = smem_u32(qs) + (it.two ? w : 0) * QBUF, k = smem_u32(kv) + b * BUF;
+            asm volatile("" : "+r"(q), "+r"(k));  // descriptors made here, not kept over the loop in registers
+            tc_fence_after();
+            if (j + 2 < cnt) {
+#pragma unroll
+              for (int s = 0; s < D / 16; ++s) sm100::umma_bf16(t_w, umma::kdesc(q, TQ, s), umma::kdesc(k, TK, s), ID_S, s > 0);
+              if (EXACT) {
+#pragma unroll
+                for (int s = 0; s < D / 16; ++s)
+                  sm100::umma_bf16(t_w, umma::kdesc(q + 2 * QBUF, TQ, s), umma::kdesc(k, TK, s), ID_S, 1);
+              }
+            }
+            if (j >= 0) {
+              const uint32_t t_p = t_w + COL_P + 32 * (j & 1);
+#pragma unroll
+              for (int s = 0; s < TK / 16; ++s)
+                umma_ts(tmem + COL_O + 128 * w, t_p + 8 * s, umma::mndesc(k + HALF, TK, s), ID_O, j > 0 || s > 0);
+            }
+            sm100::umma_commit(done + 2 * w + ((nd + j) & 1));
+            if (some) sm100::umma_commit(kv_empty + b);
+            if (j + 3 == cnt) sm100::umma_commit(q_empty + (it.two ? w : 0));
+            n += some;
           }
-          if (j >= 0 && j < cnt) value(j);
-          if (j + 2 < cnt) score(j + 2);
-          if (!it.two && w == 0) {
-            if (j >= 0 && j < n1) pass();
-            if (j + 2 < n1) pass();
-          }
+          if (w == 0) pass(j);
         }
-        np += cnt;
+        if (cnt > 0) nd += cnt + 2;
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0);
     }
@@ -404,7 +386,7 @@ __global__ void __launch_bounds__(NTHR, 1)
     const int w = (warp - 4) >> 2, quarter = warp & 3, row = 32 * quarter + lane, G = a.H / a.Hk;
     const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
     const uint32_t t_s = tmem + lanes + 128 * w, t_o = tmem + lanes + COL_O + 128 * w;
-    uint32_t n = 0, ns = 0;  // buffers through the ring, steps of this side
+    uint32_t n = 0, nd = 0;  // fillings of the ring, steps of this side
     bool ok = true;
     // a whole warp's wait; after one that ran out the items are only counted, so that both sides meet at their barriers
     auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
@@ -420,18 +402,17 @@ __global__ void __launch_bounds__(NTHR, 1)
       const int64_t out = mine ? (int64_t)(it.g.row0 + tt) * a.H + it.h * G + (r - tt * G) : -1;
       const int cnt = it.count(w), last = min(it.g.keys - 1, it.g.before + (mine ? tt : 0));
       // Cache rows behind the last one are made zero among the last block's values, as 0 times infinity is none (by both
-      // sides where both read them, each before its own products); that block is a side's last one, and its values are
-      // last or last but one in the ring's order
+      // sides where both read them, each before its own products); that block is a side's last one, in the ring's last
+      // filling, or the last but one if the other side's comes behind it
       const int n0 = it.count(0), n1 = it.two ? 0 : it.count(1);
-      n += 2 * (n0 + n1);
+      n += fillings(n0) + fillings(n1);
       const bool tail = cnt > 0 && (it.block(w, cnt - 1) + 1) * TK > it.g.keys;
       const uint32_t tail_buf = n - (it.two || (n1 == n0) == (w == 1) ? 1 : 2);
       float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-      for (int j = 0; j < cnt && ok; ++j, ++ns) {
+      for (int j = 0; j < cnt && ok; ++j) {
         const int k0 = it.block(w, j) * TK;
-        const uint32_t pb = ns & 1;
-        ok = wait(s_full + w, ns, 66);
+        ok = wait(done + 2 * w + ((nd + j) & 1), (nd + j) >> 1, 66);  // step j - 2: S(j) is there, P(j)'s place is free
         if (!ok) break;
         tc_fence_after();
         float s[TK];
@@ -440,7 +421,8 @@ __global__ void __launch_bounds__(NTHR, 1)
         tmem_wait();
         arrived<TK>(s);
         tc_fence_before();
-        mbar_arrive(s_free + w);  // the next S may come
+        __syncwarp();
+        if (lane == 0) mbar_arrive(taken + w);
         if (__any_sync(0xffffffffu, k0 + TK - 1 > last)) {
 #pragma unroll
           for (int c = 0; c < TK; ++c) s[c] = k0 + c <= last ? s[c] : -INFINITY;
@@ -456,7 +438,7 @@ __global__ void __launch_bounds__(NTHR, 1)
           m = mn;
           l *= f;
           if (j > 0) {
-            ok = wait(pv_done + 2 * w + (pb ^ 1), (ns - 1) >> 1, 67);
+            ok = wait(done + 2 * w + ((nd + j + 1) & 1), (nd + j + 1) >> 1, 67);  // step j - 1: O has all before this block
             tc_fence_after();
 #pragma unroll
             for (int c = 0; c < DC; ++c) {
@@ -480,18 +462,19 @@ __global__ void __launch_bounds__(NTHR, 1)
           sum[e & 1] = add2(sum[e & 1], y);
           p[e] = umma::pack_bf2(y.x, y.y);
         }
-        if (ns >= 2) {  // the buffer's last product
-          ok = wait(pv_done + 2 * w + pb, (ns >> 1) - 1, 73) && ok;
-          tc_fence_after();
-        }
-        tmem_put32(t_s + COL_P + 32 * pb, p);
+        tmem_put32(t_s + COL_P + 32 * (j & 1), p);
         sum[0] = add2(sum[0], sum[1]);
         l += sum[0].x + sum[0].y;
         tmem_put_wait();
-        if (tail && j == cnt - 1) {
-          ok = wait(kv_full + tail_buf % NB, tail_buf / NB, 68) && ok;
-          if (row < TK && k0 + row >= it.g.keys) {
-            const uint32_t z = smem_u32(kv) + (tail_buf % NB) * BUF + row * 128;
+      }
+      if (cnt > 0) {
+        // the last step but one: it has seen that the last S is taken, so that the last P is a new phase of that barrier; and what
+        // filled the tail's buffer before has come and gone
+        ok = ok && wait(done + 2 * w + ((nd + cnt) & 1), (nd + cnt) >> 1, 68);
+        if (tail) {
+          ok = ok && wait(kv_full + tail_buf % NB, tail_buf / NB, 68);
+          if (row < TK && it.block(w, cnt - 1) * TK + row >= it.g.keys) {
+            const uint32_t z = smem_u32(kv) + (tail_buf % NB) * BUF + HALF + row * 128;
 #pragma unroll
             for (int x = 0; x < SLABS; ++x)
 #pragma unroll
@@ -500,11 +483,11 @@ __global__ void __launch_bounds__(NTHR, 1)
           umma::fence_async_smem();
         }
         tc_fence_before();
-        mbar_arrive(p_full + 2 * w + pb);
-      }
-      if (cnt > 0 && ok) {
-        ok = wait(pv_done + 2 * w + ((ns - 1) & 1), (ns - 1) >> 1, 69);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(taken + w);  // the last P
+        ok = ok && wait(done + 2 * w + ((nd + cnt + 1) & 1), (nd + cnt + 1) >> 1, 69);  // the last step
         tc_fence_after();
+        nd += cnt + 2;
       }
       // every thread comes to the barriers, whatever its waits said
       float f0 = 1.f, f1 = 0.f;
