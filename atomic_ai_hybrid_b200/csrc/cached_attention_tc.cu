@@ -217,8 +217,9 @@ __global__ void __launch_bounds__(NTHR, 1)
   unsigned char* kv = smem + QBUF * (EXACT ? 4 : 2);      // the ring
   unsigned char* stage = kv + BUF * NB;
   uint64_t* bars = reinterpret_cast<uint64_t*>(stage + 8 * STAGE);
-  // of side w: its steps are done (at 2 w, by turns); the softmax has taken a step's S, with the P before it
-  uint64_t *kv_full = bars, *kv_empty = bars + NB, *q_full = bars + 2 * NB, *q_empty = q_full + 2, *done = q_empty + 2, *taken = done + 4;
+  // of side w: its steps are done (at 2 w, by turns), S is there, the softmax has taken it, with the P before it
+  uint64_t *kv_full = bars, *kv_empty = bars + NB, *q_full = bars + 2 * NB, *q_empty = q_full + 2, *done = q_empty + 2, *s_full = done + 4,
+           *taken = s_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(taken + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float2* other = reinterpret_cast<float2*>(tmem_slot + 4);  // the second side's maximum and sum, row by row
@@ -237,6 +238,7 @@ __global__ void __launch_bounds__(NTHR, 1)
     }
     for (int i = 0; i < 4; ++i) mbar_init(done + i, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 1);
       mbar_init(taken + i, 4);  // a side's warps
       mbar_init(q_full + i, 1);
       mbar_init(q_empty + i, 2);  // both sides' (a second tile: its side's twice)
@@ -333,6 +335,7 @@ __global__ void __launch_bounds__(NTHR, 1)
                 for (int s = 0; s < D / 16; ++s)
                   sm100::umma_bf16(t_w, umma::kdesc(q + 2 * QBUF, TQ, s), umma::kdesc(k, TK, s), ID_S, 1);
               }
+              sm100::umma_commit(s_full + w);  // a completion is seen 500 cycles later: S is not to wait for P V
             }
             if (j >= 0) {
               const uint32_t t_p = t_w + COL_P + 32 * (j & 1);
@@ -386,7 +389,7 @@ __global__ void __launch_bounds__(NTHR, 1)
     const int w = (warp - 4) >> 2, quarter = warp & 3, row = 32 * quarter + lane, G = a.H / a.Hk;
     const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
     const uint32_t t_s = tmem + lanes + 128 * w, t_o = tmem + lanes + COL_O + 128 * w;
-    uint32_t n = 0, nd = 0;  // fillings of the ring, steps of this side
+    uint32_t n = 0, nd = 0, ns = 0;  // fillings of the ring, steps of this side, its S
     bool ok = true;
     // a whole warp's wait; after one that ran out the items are only counted, so that both sides meet at their barriers
     auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
@@ -410,9 +413,9 @@ __global__ void __launch_bounds__(NTHR, 1)
       const uint32_t tail_buf = n - (it.two || (n1 == n0) == (w == 1) ? 1 : 2);
       float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-      for (int j = 0; j < cnt && ok; ++j) {
+      for (int j = 0; j < cnt && ok; ++j, ++ns) {
         const int k0 = it.block(w, j) * TK;
-        ok = wait(done + 2 * w + ((nd + j) & 1), (nd + j) >> 1, 66);  // step j - 2: S(j) is there, P(j)'s place is free
+        ok = wait(s_full + w, ns, 66);
         if (!ok) break;
         tc_fence_after();
         float s[TK];
@@ -462,6 +465,8 @@ __global__ void __launch_bounds__(NTHR, 1)
           sum[e & 1] = add2(sum[e & 1], y);
           p[e] = umma::pack_bf2(y.x, y.y);
         }
+        ok = wait(done + 2 * w + ((nd + j) & 1), (nd + j) >> 1, 67) && ok;  // step j - 2: P(j)'s place is free
+        tc_fence_after();
         tmem_put32(t_s + COL_P + 32 * (j & 1), p);
         sum[0] = add2(sum[0], sum[1]);
         l += sum[0].x + sum[0].y;
