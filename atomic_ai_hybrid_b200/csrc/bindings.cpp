@@ -1982,11 +1982,12 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Te
   auto lp = new_output({R}, at::kFloat, logits), entropy = new_output({R}, at::kFloat, logits);
   auto stats = new_output({R, 4}, at::kFloat, logits);
   auto top_tok = new_output({R, top}, at::kLong, logits), top_lp = new_output({R, top}, at::kFloat, logits);
-  ahb_token_logprobs_fwd(logits.data_ptr(), logits.stride(0), dt_code(logits), tokens.data_ptr<int64_t>(), R, (int)V,
+  const int rc = ahb_token_logprobs_fwd(logits.data_ptr(), logits.stride(0), dt_code(logits), tokens.data_ptr<int64_t>(), R, (int)V,
                          (int)top, (float)temperature, lp.data_ptr<float>(), entropy.data_ptr<float>(), stats.data_ptr(),
                          top > 0 ? top_tok.data_ptr<int64_t>() : nullptr, top > 0 ? top_lp.data_ptr<float>() : nullptr,
                          cur_stream());
   check_launch(op);
+  TORCH_CHECK(rc == 0, op, ": failed with code ", rc);
   return {lp, entropy, stats, top_tok, top_lp};
 }
 

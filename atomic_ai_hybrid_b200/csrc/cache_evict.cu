@@ -14,7 +14,7 @@ using namespace ahb;
 
 namespace {
 
-constexpr int NT = 512;
+constexpr int NT = 256;
 
 AHB_DEVICE uint32_t rank_key(float mass, int held, int64_t newest) {
   if (held >= newest) return 0xffffffffu;
@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(NT) evict_kernel(char* __restrict__ kc, char* 
   uint32_t prefix = 0, mask = 0;
   int left = keep;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
+    hist[tid] = 0;
     __syncthreads();
     for (int i = tid; i < n; i += NT) {
       const uint32_t k = key(i);
@@ -137,12 +137,26 @@ __global__ void __launch_bounds__(NT) evict_kernel(char* __restrict__ kc, char* 
   const int chunks = row_bytes >> 4;
   uint4* kr = reinterpret_cast<uint4*>(kc) + base * chunks;
   uint4* vr = reinterpret_cast<uint4*>(vc) + base * chunks;
-  for (int x = tid; x < moves * chunks; x += NT) {
-    const int r = x / chunks, c = x - r * chunks;
-    const int64_t src = (int64_t)from[r] * chunks + c, dst = (int64_t)to[r] * chunks + c;
-    const uint4 k = kr[src], v = vr[src];
-    kr[dst] = k;
-    vr[dst] = v;
+  constexpr int UN = 4;  // pieces of 16 bytes of k and of v that a thread has on their way
+  for (int x0 = tid; x0 < moves * chunks; x0 += NT * UN) {
+    uint4 k[UN], v[UN];
+    int64_t dst[UN];
+#pragma unroll
+    for (int j = 0; j < UN; ++j) {
+      const int x = x0 + j * NT;
+      if (x >= moves * chunks) break;
+      const int r = x / chunks, c = x - r * chunks;
+      const int64_t src = (int64_t)from[r] * chunks + c;
+      dst[j] = (int64_t)to[r] * chunks + c;
+      k[j] = kr[src];
+      v[j] = vr[src];
+    }
+#pragma unroll
+    for (int j = 0; j < UN; ++j) {
+      if (x0 + j * NT >= moves * chunks) break;
+      kr[dst[j]] = k[j];
+      vr[dst[j]] = v[j];
+    }
   }
 }
 

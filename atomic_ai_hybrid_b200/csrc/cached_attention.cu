@@ -162,6 +162,16 @@ AHB_DEVICE void load8(const bf16* p, float* v) {
     for (int i = 0; i < 8; ++i) v[i] = __bfloat162float(p[i]);
   }
 }
+template <bool VEC>
+AHB_DEVICE void load8(const float* p, float* v) {
+  if (VEC) {
+    *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p);
+    *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(p + 4);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = p[i];
+  }
+}
 // ... to p, and what their rounding leaves of them to `rest` (null: nowhere)
 AHB_DEVICE void store8(bf16* p, bf16* rest, const float* v) {
   uint4 u, x;
@@ -243,16 +253,18 @@ __global__ void __launch_bounds__(AT) ca_append(const Args a, int per) {
           turn = false;
         }
       }
-      float lo[8], hi[8];
+      alignas(16) float lo[8], hi[8];
       load8<VEC>(src + c, lo);
       load8<VEC>(src + c + half, hi);
       if (turn) {
-        const float *cs = a.cos + (int64_t)(pos0 + y) * a.D + c, *sn = a.sin + (int64_t)(pos0 + y) * a.D + c;
+        alignas(16) float cs[8], sn[8];
+        load8<VEC>(a.cos + (int64_t)(pos0 + y) * a.D + c, cs);
+        load8<VEC>(a.sin + (int64_t)(pos0 + y) * a.D + c, sn);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float x1 = lo[e], x2 = hi[e];
           lo[e] = x1 * cs[e] - x2 * sn[e];
-          hi[e] = x2 * cs[half + e] + x1 * sn[half + e];
+          hi[e] = x2 * cs[e] + x1 * sn[e];
         }
       }
       if (h < a.H && a.negate) {
@@ -486,13 +498,13 @@ struct Joined {
       o[c].y = o[c].y * f + v[c].y * e;
     }
   }
-  // `count` results, `stride` apart: eight at a time, so that their loads travel together
+  // `count` results, `stride` apart: four at a time, so that their loads travel together
   AHB_DEVICE void add(const float* y, int64_t stride, int count) {
     const int lane = threadIdx.x & 31;
-    for (int k0 = 0; k0 < count; k0 += 8) {
-      float2 ml[8], v[8][PL];
+    for (int k0 = 0; k0 < count; k0 += 4) {
+      float2 ml[4], v[4][PL];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 4; ++k) {
         if (k0 + k >= count) break;
         const float* p = y + (k0 + k) * stride;
         ml[k] = *reinterpret_cast<const float2*>(p + D);
@@ -501,7 +513,7 @@ struct Joined {
           if (64 * c + 2 * lane < D) v[k][c] = *reinterpret_cast<const float2*>(p + 64 * c + 2 * lane);
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
+      for (int k = 0; k < 4; ++k)
         if (k0 + k < count) one(ml[k], v[k]);
     }
   }
@@ -518,118 +530,130 @@ struct Joined {
 
 constexpr int JW = 8;  // warps of a block
 
-// A block takes a token row and JW query heads (WIDE: one head, its partial results spread over the warps: where rows are
-// few, every one is cut into many).  Nothing is done for what is final already.
+// Where the results of a token row lie: of its own rows and of its prefix's, the same for all its query heads but for `first`.
+struct Source {
+  bool tiles;
+  int row, rows;                       // the row within a worker's partial results (of query head 0), rows of those
+  int64_t base, per_head, units, share;  // key head h's first unit is base + h per_head
+};
+AHB_DEVICE Source source(const Args& a, const Group& g, int x, int at, int t) {
+  Source s;
+  s.tiles = is_tiles(a, g);
+  const int64_t* own = a.sums[s.tiles ? TILES : ROWS];
+  const int64_t* runs = own + a.B + 1;
+  const int64_t n_own = own[a.B], all = n_own + runs[a.B];
+  const int64_t u0 = x ? runs[at] : own[at], u1 = x ? runs[at + 1] : own[at + 1];
+  s.share = share_of(all, s.tiles ? a.blocks : a.warps);
+  s.base = (x ? n_own : 0) + u0;
+  s.row = (t - g.row0) * (a.H / a.Hk);
+  s.rows = RT;
+  s.per_head = div64(u1 - u0, a.Hk);
+  s.units = s.per_head;
+  if (s.tiles) {  // a token's rows are of one item
+    const int rt = s.row / (2 * a.tile_rows);
+    int before = 0;
+    for (int k = threadIdx.x & 31; k < rt; k += 32) before += tile_item(a, g, k).units;
+    s.base += __reduce_add_sync(0xffffffffu, before) + ITEM_COST;
+    s.units = tile_item(a, g, rt).units - ITEM_COST;
+    s.row -= rt * 2 * a.tile_rows;
+    s.rows = 2 * TQ;
+  }
+  return s;
+}
+
+// A token row and query heads h0, h0 + step .. below h1, one a warp (WIDE: head h0, its partial results spread over the
+// block's warps: where rows are few, every one is cut into many).  Nothing is done for what is final already.
 template <int D, bool WIDE>
-__global__ void __launch_bounds__(JW * 32) ca_join(const Args a) {
-  const int warp = threadIdx.x >> 5, t = blockIdx.x, G = a.H / a.Hk;
-  const int hq = WIDE ? blockIdx.y : blockIdx.y * JW + warp, h = hq / G;
+AHB_DEVICE void join_row(const Args& a, int t, int h0, int h1, int step) {
+  const int warp = threadIdx.x >> 5, G = a.H / a.Hk;
   const int i = a.row_seq[t];
   if (i < 0) return;
-  // the group of the sequence's own rows, and that of its prefix run
-  Group gr[2];
-  int at[2], n = 1;
-  at[0] = i;
-  gr[0] = a.groups[i];
-  if (!a.full && is_tiles(a, gr[0])) return;  // ca_join_tiles
-  const int start = a.full ? a.run_start[i] : -1;
-  if (start >= 0) {
-    at[1] = a.run_end[start];
-    gr[1] = a.groups[a.B + at[1]];
-    n = 2;
+  const Group own = a.groups[i];
+  if (!a.full && is_tiles(a, own)) return;  // ca_join_tiles
+  const int start = a.full ? a.run_start[i] : -1, n = start >= 0 ? 2 : 1;
+  Source src[2];
+  src[0] = source(a, own, 0, i, t);
+  if (n == 2) {
+    const int end = a.run_end[start];
+    src[1] = source(a, a.groups[a.B + end], 1, end, t);
   }
-  if (hq >= a.H) return;
-  const int64_t out = (int64_t)t * a.H + hq;
-  Joined<D> sum;
+  for (int hq = h0; hq < h1; hq += step) {
+    const int h = per_group(hq, G);
+    const int64_t out = (int64_t)t * a.H + hq;
+    Joined<D> sum;
+    bool done = false;
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    if (x >= n) break;
-    const Group& g = gr[x];
-    const bool tiles = is_tiles(a, g);
-    const int64_t* own = a.sums[tiles ? TILES : ROWS];
-    const int64_t* runs = own + a.B + 1;
-    const int64_t n_own = own[a.B], share = share_of(n_own + runs[a.B], tiles ? a.blocks : a.warps);
-    int64_t first = x ? n_own + runs[at[1]] : own[at[0]];
-    int units, row = (t - g.row0) * G + hq - h * G, rows = RT;  // the row within the group and key head
-    if (tiles) {
-      const int rt = row / (2 * a.tile_rows);
-      const int64_t per_head = div64(x ? runs[at[1] + 1] - runs[at[1]] : own[at[0] + 1] - own[at[0]], a.Hk);
-      int before = 0;
-      for (int k = threadIdx.x & 31; k < rt; k += 32) before += tile_item(a, g, k).units;
-      first += h * per_head + __reduce_add_sync(0xffffffffu, before);
-      first += ITEM_COST;
-      units = tile_item(a, g, rt).units - ITEM_COST;
-      row -= rt * 2 * a.tile_rows;
-      rows = 2 * TQ;
-    } else {
-      units = row_units(g);
-      first += (int64_t)h * units;
-    }
-    const int64_t w0 = div64(first, share), w1 = div64(first + units - 1, share);
-    if (w0 == w1) {
-      if (!a.full) return;
-      if (!WIDE || warp == 0) sum.add(a.full + ((int64_t)x * a.T * a.H + out) * (D + 4), 0, 1);
-    } else {
-      const float* part = (tiles ? a.tile_part : a.part) + (int64_t)row * (D + 4);
-      const int64_t slot = (int64_t)rows * (D + 4);
-      if (!WIDE || warp == 0) sum.add(part + (2 * w0 + (first >= w0 * share ? 1 : 0)) * slot, 0, 1);
-      const int more = (int)(w1 - w0);  // the others began before their worker's units
-      if (WIDE) {
-        const int each = (more + JW - 1) / JW, k0 = warp * each;
-        if (k0 < more) sum.add(part + 2 * (w0 + 1 + k0) * slot, 2 * slot, min(each, more - k0));
+    for (int x = 0; x < 2; ++x) {
+      if (x >= n) break;
+      const Source& s = src[x];
+      const int64_t first = s.base + h * s.per_head;
+      const int64_t w0 = div64(first, s.share), w1 = div64(first + s.units - 1, s.share);
+      if (w0 == w1) {
+        done = !a.full;
+        if (!done && (!WIDE || warp == 0)) sum.add(a.full + ((int64_t)x * a.T * a.H + out) * (D + 4), 0, 1);
       } else {
-        sum.add(part + 2 * (w0 + 1) * slot, 2 * slot, more);
+        const int64_t slot = (int64_t)s.rows * (D + 4);
+        const float* part = (s.tiles ? a.tile_part : a.part) + (int64_t)(s.row + hq - h * G) * (D + 4);
+        if (!WIDE || warp == 0) sum.add(part + (2 * w0 + (first >= w0 * s.share ? 1 : 0)) * slot, 0, 1);
+        const int more = (int)(w1 - w0);  // the others began before their worker's units
+        if (WIDE) {
+          const int each = (more + JW - 1) / JW, k0 = warp * each;
+          if (k0 < more) sum.add(part + 2 * (w0 + 1 + k0) * slot, 2 * slot, min(each, more - k0));
+        } else {
+          sum.add(part + 2 * (w0 + 1) * slot, 2 * slot, more);
+        }
       }
     }
-  }
-  if (WIDE) {
-    constexpr int PL = Joined<D>::PL;
-    __shared__ float2 sh[JW][PL + 1][32];
-    const int lane = threadIdx.x & 31;
+    if (done) continue;
+    if (WIDE) {
+      constexpr int PL = Joined<D>::PL;
+      __shared__ float2 sh[JW][PL + 1][32];
+      const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int c = 0; c < PL; ++c) sh[warp][c][lane] = sum.o[c];
-    sh[warp][PL][lane] = make_float2(sum.m, sum.l);
-    __syncthreads();
-    if (warp > 0) return;
+      for (int c = 0; c < PL; ++c) sh[warp][c][lane] = sum.o[c];
+      sh[warp][PL][lane] = make_float2(sum.m, sum.l);
+      __syncthreads();
+      if (warp > 0) return;
 #pragma unroll
-    for (int k = 1; k < JW; ++k) {
-      float2 v[PL];
+      for (int k = 1; k < JW; ++k) {
+        float2 v[PL];
 #pragma unroll
-      for (int c = 0; c < PL; ++c) v[c] = sh[k][c][lane];
-      sum.one(sh[k][PL][lane], v);
+        for (int c = 0; c < PL; ++c) v[c] = sh[k][c][lane];
+        sum.one(sh[k][PL][lane], v);
+      }
     }
+    sum.finish(a, out);
   }
-  sum.finish(a, out);
+}
+template <int D>
+__global__ void __launch_bounds__(JW * 32) ca_join_wide(const Args a) {
+  join_row<D, true>(a, blockIdx.x, blockIdx.y, blockIdx.y + 1, 1);
+}
+// `heads` query heads a block
+template <int D>
+__global__ void __launch_bounds__(JW * 32, 3) ca_join(const Args a, int heads) {
+  if (!a.full && a.sums[ROWS][a.B] == 0) return;  // all is the tile kernel's
+  const int per = (a.H + heads - 1) / heads;
+  for (int64_t x = blockIdx.x; x < (int64_t)a.T * per; x += gridDim.x) {
+    const int t = (int)div64(x, per), h0 = (int)(x - (int64_t)t * per) * heads;
+    join_row<D, false>(a, t, h0 + (threadIdx.x >> 5), min(a.H, h0 + heads), JW);
+  }
 }
 
 // Without a prefix only items of the tile kernel that several of its blocks share are left to join.  Block (b, y) takes
-// rows 32 y .. of the item that began among block b's units and goes on behind them.
+// rows 32 y .. of the item that began among block b's units and goes on behind them, as block b has noted it.
 template <int D>
 __global__ void __launch_bounds__(JW * 32) ca_join_tiles(const Args a) {
-  const int64_t* own = a.sums[TILES];
-  const int64_t all = own[a.B], share = share_of(all, a.blocks);
-  const int64_t u_first = blockIdx.x * share, u_end = u_first + share;
-  if (u_end >= all) return;
-  const int i = find_group(own, a.B, u_end - 1), G = a.H / a.Hk;
-  const Group g = a.groups[i];
-  const int64_t per_head = div64(own[i + 1] - own[i], a.Hk), v = u_end - 1 - own[i];
-  const int h = (int)div64(v, per_head);
-  int64_t first = own[i] + h * per_head;
-  int rt = 0;
-  TileItem it = tile_item(a, g, 0);
-  while (first + it.units < u_end) {
-    first += it.units;
-    it = tile_item(a, g, ++rt);
-  }
-  if (first + ITEM_COST < u_first || first + ITEM_COST >= u_end || first + it.units <= u_end) return;
-  const int64_t w1 = div64(first + it.units - 1, share), slot = 2 * TQ * (D + 4);
+  const SharedItem it = a.shared_items[blockIdx.x];
+  const int G = a.H / a.Hk;
+  const int64_t slot = 2 * TQ * (D + 4);
   for (int row = 32 * blockIdx.y + (threadIdx.x >> 5); row < min(it.rows, 32 * (int)blockIdx.y + 32); row += JW) {
-    const int r = 2 * a.tile_rows * rt + row, tt = r / G;
+    const int r = it.r0 + row, tt = per_group(r, G);
     const float* part = a.tile_part + (int64_t)row * (D + 4);
     Joined<D> sum;
-    sum.add(part + (2 * (int64_t)blockIdx.x + 1) * slot, 0, 1);
-    sum.add(part + 2 * ((int64_t)blockIdx.x + 1) * slot, 2 * slot, (int)(w1 - blockIdx.x));
-    sum.finish(a, (int64_t)(g.row0 + tt) * a.H + h * G + (r - tt * G));
+    sum.add(part + (2 * (int64_t)blockIdx.x + 1) * slot, slot, 2);  // and the next block's, right behind it
+    sum.add(part + 2 * ((int64_t)blockIdx.x + 2) * slot, 2 * slot, it.last - (int)blockIdx.x - 1);
+    sum.finish(a, (int64_t)(it.row0 + tt) * a.H + it.h * G + (r - tt * G));
   }
 }
 
@@ -710,6 +734,7 @@ int64_t lay_out(Args& a, char* base) {
   a.lse = a.mass ? (float*)place(rows * 4) : nullptr;
   a.part = (float*)place((int64_t)2 * a.warps * RT * (a.D + 4) * 4);
   a.tile_part = (float*)place((int64_t)2 * a.blocks * 2 * TQ * (a.D + 4) * 4);
+  a.shared_items = (SharedItem*)place((int64_t)a.blocks * sizeof(SharedItem));
   a.full = a.prefix ? (float*)place(2 * rows * (a.D + 4) * 4) : nullptr;
   return at;
 }
@@ -722,8 +747,12 @@ int launch(const Args& a, cudaStream_t st) {
   }
   ca_rows<D><<<a.warps / RW, RW * 32, 0, st>>>(a);
   if (a.blocks && !a.full) ca_join_tiles<D><<<dim3(a.blocks, 2 * TQ / 32), JW * 32, 0, st>>>(a);
-  if ((int64_t)a.T * a.H <= 4 * a.warps / (RB * RW)) ca_join<D, true><<<dim3(a.T, a.H), JW * 32, 0, st>>>(a);
-  else ca_join<D, false><<<dim3(a.T, (a.H + JW - 1) / JW), JW * 32, 0, st>>>(a);
+  const int sms = a.warps / (RB * RW);
+  // a block a row where there are rows enough: what its heads share is looked up once
+  const int heads = a.T > 4 * sms ? a.H : JW;
+  const int64_t rows = (int64_t)a.T * ((a.H + heads - 1) / heads);
+  if ((int64_t)a.T * a.H <= 4 * sms) ca_join_wide<D><<<dim3(a.T, a.H), JW * 32, 0, st>>>(a);
+  else ca_join<D><<<(unsigned)(rows < 16 * sms ? rows : 16 * sms), JW * 32, 0, st>>>(a, heads);
   if (a.mass) {
     ca_mass<D><<<a.warps / RW, RW * 32, 0, st>>>(a, ROWS_MASS);
     if (a.blocks) ca_mass<D><<<a.warps / RW, RW * 32, 0, st>>>(a, TILES_MASS);
@@ -743,7 +772,7 @@ int ahb_cached_attention(const Args& args, void* work, cudaStream_t st) {
   a.negate = a.scale2 < 0.f;  // the queries take the scale's sign: the largest product is then the largest score
   a.scale2 = a.scale2 < 0.f ? -a.scale2 : a.scale2;
   lay_out(a, (char*)work);
-  const bool vec = (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0 && ((a.qs | a.ks | a.vs) & 7) == 0;
+  const bool vec = (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.cos | (uintptr_t)a.sin) & 15) == 0 && ((a.qs | a.ks | a.vs) & 7) == 0;
   const int per = 1 + (a.T - 1) / (8 * sm_count()), blocks = 1 + (a.T + per - 1) / per;  // eight blocks an SM at most
   if (vec) ca_append<true><<<blocks, AT, 0, st>>>(a, per);
   else ca_append<false><<<blocks, AT, 0, st>>>(a, per);

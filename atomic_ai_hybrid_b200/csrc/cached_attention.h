@@ -21,6 +21,11 @@ struct Group {
 // two kernels; a kernel's units are numbered through the groups, and sums[kind][g] is group g's first one.
 enum Kind { ROWS = 0, TILES = 1, ROWS_MASS = 2, TILES_MASS = 3, KINDS = 4 };
 
+// What a block of the tile kernel began and others go on with (rows 0: nothing), up to block `last`.
+struct SharedItem {
+  int row0, r0, rows, h, last;
+};
+
 struct Args {
   const bf16 *q, *k, *v;
   int64_t qs, ks, vs;            // row strides
@@ -43,6 +48,7 @@ struct Args {
   float* lse;                    // (T, H) log2 of the softmax's denominators, for mass
   float* part;                   // partial results of items that several warps share, two a warp
   float* tile_part;              // ... of items that several blocks share, two a block
+  SharedItem* shared_items;      // (blocks)
   float* full;                   // (2, T, H, D + 4) whole results of own rows and of prefix rows, if there is a prefix
   int tile_rows;                 // query rows of a tile: as many tokens as fit into 128 rows, with their heads
   int warps, blocks;             // warps of the row kernel, blocks of the tile kernel (0: it is not launched)

@@ -51,6 +51,7 @@ constexpr size_t smem_bytes() { return (size_t)BUF * ring<EXACT>() + QBUF * (EXA
 struct Item {
   int pre, h, r0, rows, blocks, ks, ke;  // units ks .. ke of the item
   bool two, whole;                       // two tiles; all of the item's units
+  int64_t u_last;                        // the item's last unit
   bool late;                             // its first block of cache rows came before this thread block's units
   Group g;
   // blocks of cache rows of side w in these units, and the j-th of them
@@ -119,6 +120,7 @@ AHB_DEVICE Item next_item(const Args& a, Place& p) {
   it.ke = to - ITEM_COST;
   it.whole = it.ks == 0 && to == t.units;
   it.late = p.u - p.at + ITEM_COST < p.u_first;
+  it.u_last = p.u - p.at + t.units - 1;
   p.u += to - p.at;
   return it;
 }
@@ -230,6 +232,7 @@ __global__ void __launch_bounds__(NTHR, 1)
   at.u_first = at.u = (int64_t)blockIdx.x * share;
   at.u_end = min(at.u_first + share, all);
   at.x = -1;
+  if (threadIdx.x == 0) a.shared_items[blockIdx.x].rows = 0;
   if (at.u >= at.u_end) return;
   if (threadIdx.x == 0) {
     for (int i = 0; i < NB; ++i) {
@@ -559,6 +562,8 @@ __global__ void __launch_bounds__(NTHR, 1)
             rows.write(st, reinterpret_cast<const uint4*>(o), reinterpret_cast<unsigned char*>(y + 32 * c), (D + 4) * 4);
           }
           if (mine) *reinterpret_cast<float2*>(y + (int64_t)place * (D + 4) + D) = make_float2(m, l);
+          if (!it.whole && !it.late && threadIdx.x == 128)
+            a.shared_items[blockIdx.x] = SharedItem{it.g.row0, it.r0, it.rows, it.h, (int)div64(it.u_last, share)};
         }
       }
       tc_fence_before();

@@ -281,10 +281,10 @@ int64_t ahb_cache_evict_bytes(int n_slots, int Hk, int M, int keep);
 int ahb_cache_evict(void* kc, void* vc, float* mass, int* held, const int* lengths, const int* seen, const int* slots,
                     int n_slots, int S, int Hk, int M, int row_bytes, int keep, int recent, void* work, cudaStream_t st);
 // token_logprobs.cu: logits (R, V) of `dtype` with row stride ls; stats (R, 4) carries a row's maximum, log2 of its sum
-// and entropy to the backward; top_tok, top_lp (R, top), top <= 64; dx (R, V) contiguous
-void ahb_token_logprobs_fwd(const void* logits, int64_t ls, int dtype, const int64_t* tokens, int64_t R, int V, int top,
-                            float temperature, float* lp, float* entropy, void* stats, int64_t* top_tok, float* top_lp,
-                            cudaStream_t st);
+// and entropy to the backward; top_tok, top_lp (R, top), top <= 64; dx (R, V) contiguous.  0, or a launch that failed.
+int ahb_token_logprobs_fwd(const void* logits, int64_t ls, int dtype, const int64_t* tokens, int64_t R, int V, int top,
+                           float temperature, float* lp, float* entropy, void* stats, int64_t* top_tok, float* top_lp,
+                           cudaStream_t st);
 void ahb_token_logprobs_bwd(const void* logits, int64_t ls, int dtype, const int64_t* tokens, const void* stats,
                             const float* g, const float* ge, int64_t R, int V, float temperature, void* dx,
                             cudaStream_t st);

@@ -3,12 +3,14 @@
 //   d_v = (x_v - max x) / T,  S = sum e^{d_v},  log p_v = d_v - log S,  H = log S - sum e^{d_v} d_v / S
 //   dx_v = (g ([v = y] - p_v) - gH p_v (log p_v + H)) / T
 //
-// Sums run over differences from the running maximum, in which nothing is lost to the size of the logits.
+// Sums run over differences from the running maximum, in which nothing is lost to the size of the logits.  Two values
+// at a time where the GPU has instructions for it: a bf16 logit costs five, where the copy's rate leaves time for ten.
 //
-// Forward: one block a row, one pass over it.  Every thread keeps its largest logit (the lowest index where equal).
-// The k-th largest of the 64 eight-lane groups' best is a bound that at least k logits reach, and only a thread
-// whose own best reaches it can hold one of them: those few read their share of the row again, and what reaches the
-// bound is ranked by counting.
+// Forward: one pass over a row, by one block or, where rows are few, by a cluster of up to eight.  Every thread keeps
+// its largest logit (the lowest index where equal).  The k-th largest of 64 groups' best is a bound that at least k
+// logits reach, and only a thread whose own best reaches it can hold one of them: the shares of those few are read again,
+// by all threads, and what reaches the bound is ranked by counting.
+#include <cooperative_groups.h>
 #include "common.cuh"
 #include "launchers.h"
 #include "packed.cuh"
@@ -18,7 +20,7 @@ using bf16 = __nv_bfloat16;
 
 namespace {
 
-constexpr int NT = 512, CAND = 1024;
+constexpr int NT = 256, CAND = 512, MAX_TOP = 64;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, BIG = 3.4028234663852886e38f;
 constexpr float FLOOR = -200.f;  // 2^-200 is 0 in fp32, and 0 times -200 is 0 where 0 times -inf is NaN
 
@@ -55,19 +57,17 @@ AHB_DEVICE float logit_of(uint64_t r) {
 }
 
 struct Sums {
-  float m, s, z;  // maximum, sum 2^d, sum 2^d d with d = (x - m) c
+  float m, s, z;  // maximum, sum 2^d, sum 2^d d with d = (x - m) c, c = log2(e) / T
   AHB_DEVICE void move(float mn, float c) {
-    if (m == -INFINITY) {
-      m = mn;
-      return;
+    if (m != -INFINITY) {
+      const float d = fmaxf((m - mn) * c, FLOOR), f = ex2(d);
+      z = f * (z + s * d);
+      s *= f;
     }
-    const float d = fmaxf((m - mn) * c, FLOOR), f = ex2(d);
-    z = f * (z + s * d);
-    s *= f;
     m = mn;
   }
   AHB_DEVICE void add(float x, float c) {
-    const float d = fminf(fmaxf((x - m) * c, FLOOR), 0.f), e = ex2(d);  // NaN: no mass; +inf: as the largest
+    const float d = fmaxf((x - m) * c, FLOOR), e = ex2(d);
     s += e;
     z += e * d;
   }
@@ -82,6 +82,16 @@ struct Sums {
   }
 };
 
+// The largest of a vector; NaN is passed over.
+AHB_DEVICE float vec_max(const uint4& u, const float (&x)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);
+  const __nv_bfloat162 a = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  const float2 f = __bfloat1622float2(a);
+  return fmaxf(f.x, f.y);
+}
+AHB_DEVICE float vec_max(const uint4&, const float (&x)[4]) { return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])); }
+
 // A row's elements as this thread sees them: f(x, v) in rising v, in vectors where the row is aligned.
 template <typename T>
 struct Row {
@@ -95,18 +105,27 @@ struct Row {
   AHB_DEVICE uint4 vec(int i) const { return reinterpret_cast<const uint4*>(p + head)[i]; }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(NT) logprobs_fwd(const T* __restrict__ logits, int64_t ls, const int64_t* __restrict__ tokens,
-                                                   int V, int top, float c, float* __restrict__ lp, float* __restrict__ entropy,
-                                                   float4* __restrict__ stats, int64_t* __restrict__ top_tok,
-                                                   float* __restrict__ top_lp) {
-  constexpr int N = Vec<T>::N, UN = 4;
+// C: blocks of a row's cluster, each with a part of it
+template <typename T, int C>
+__global__ void __launch_bounds__(NT, 4) logprobs_fwd(const T* __restrict__ logits, int64_t ls, const int64_t* __restrict__ tokens,
+                                                      int V, int top, float c, float* __restrict__ lp, float* __restrict__ entropy,
+                                                      float4* __restrict__ stats, int64_t* __restrict__ top_tok,
+                                                      float* __restrict__ top_lp) {
+  constexpr int N = Vec<T>::N, UN = 4, GL = NT / 64;  // GL: lanes of a group
   __shared__ Sums sums[NT / 32];
   __shared__ uint64_t best_sh[64], cand[CAND], bound_sh;
-  __shared__ int count;
-  const int64_t r = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const Row<T> row(logits + r * ls, V);
+  __shared__ int count, who[NT], n_who;
+  struct Part {
+    Sums sums;
+    uint64_t best[MAX_TOP];
+  };
+  __shared__ Part part;  // what the cluster's first block reads
+  const int64_t r = blockIdx.x / C;
+  const int rank = blockIdx.x % C, tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const T* p = logits + r * ls;
+  // parts of whole 64-element pieces
+  const int each = C == 1 ? V : ((V + C - 1) / C + 63) & ~63, v0 = min(V, rank * each), v1 = min(V, v0 + each);
+  const Row<T> row(p + v0, v1 - v0);
   Sums a{-INFINITY, 0.f, 0.f};
   uint64_t best = 0;
   auto one = [&](int v) {  // the few elements outside the vectors
@@ -114,11 +133,11 @@ __global__ void __launch_bounds__(NT) logprobs_fwd(const T* __restrict__ logits,
     if (x == -INFINITY) return;
     if (x > a.m) a.move(x, c);
     a.add(x, c);
-    const uint64_t k = rank_of(x, v);
+    const uint64_t k = rank_of(x, v0 + v);
     best = k > best ? k : best;
   };
   if (tid < row.head) one(tid);
-  if (row.tail() + tid < V) one(row.tail() + tid);
+  if (row.tail() + tid < row.V) one(row.tail() + tid);
   float top_x = -INFINITY;
   int top_v = 0;
   for (int i0 = tid; i0 < row.vecs; i0 += NT * UN) {
@@ -131,22 +150,31 @@ __global__ void __launch_bounds__(NT) logprobs_fwd(const T* __restrict__ logits,
       if (i0 + j * NT >= row.vecs) break;
       float x[N];
       unpack(u[j], x);
-      float mx = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < N; ++e) mx = fmaxf(mx, x[e]);  // NaN is passed over
+      const float mx = vec_max(u[j], x);
       if (mx > top_x) {  // seldom, but for a thread's first vectors
-        mx = fminf(mx, BIG);
-        if (mx > a.m) a.move(mx, c);
-        if (mx > top_x) {
-          top_x = mx;
+        const float xx = fminf(mx, BIG);
+        if (xx > a.m) a.move(xx, c);
+        if (xx > top_x) {
+          top_x = xx;
 #pragma unroll
           for (int e = N - 1; e >= 0; --e)
-            if (clean(x[e]) == mx) top_v = row.head + (i0 + j * NT) * N + e;
+            if (clean(x[e]) == xx) top_v = v0 + row.head + (i0 + j * NT) * N + e;
         }
       }
-      if (a.m > -INFINITY) {
+      if (mx == INFINITY) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) a.add(x[e], c);
+        for (int e = 0; e < N; ++e) a.add(clean(x[e]), c);
+      } else if (a.m > -INFINITY) {
+        float2 s2 = both(0.f), z2 = both(0.f);
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+          const float2 d = max2(mul2(add2(make_float2(x[e], x[e + 1]), both(-a.m)), both(c)), FLOOR);  // NaN: no mass
+          const float2 q = make_float2(ex2(d.x), ex2(d.y));
+          s2 = add2(s2, q);
+          z2 = fma2(q, d, z2);
+        }
+        a.s += s2.x + s2.y;
+        a.z += z2.x + z2.y;
       }
     }
   }
@@ -157,107 +185,135 @@ __global__ void __launch_bounds__(NT) logprobs_fwd(const T* __restrict__ logits,
   const uint64_t mine = best;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    Sums b{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.z, o)};
+    const Sums b{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.z, o)};
     a.join(b, c);
   }
   if (lane == 0) sums[w] = a;
   if (top > 0) {
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
+    for (int o = 1; o < GL; o <<= 1) {
       const uint64_t b = __shfl_xor_sync(0xffffffffu, best, o);
       best = b > best ? b : best;
     }
-    if ((lane & 7) == 0) best_sh[tid >> 3] = best;
-    if (tid == 0) count = 0;
+    if (tid % GL == 0) best_sh[tid / GL] = best;
+    if (tid == 0) count = n_who = 0;
   }
   __syncthreads();
   a = sums[0];
 #pragma unroll
   for (int i = 1; i < NT / 32; ++i) a.join(sums[i], c);
-  const bool some = a.m > -INFINITY;
-  const float log2s = some ? log2f(a.s) : 0.f;
-  auto logprob = [&](float x) { return x == -INFINITY || !some ? -INFINITY : ((x - a.m) * c - log2s) * LN2; };
-  if (tid == 0) {
-    const int64_t y = tokens[r];
-    lp[r] = y >= 0 && y < V ? logprob(clean(to_f(row.p[y]))) : 0.f;
-    const float H = some ? (log2s - a.z / a.s) * LN2 : 0.f;
-    entropy[r] = H;
-    stats[r] = make_float4(a.m, log2s, H, 0.f);
-  }
-  if (top == 0) return;
-  if (tid < 64) {
-    const uint64_t b = best_sh[tid];
-    int above = 0;
-    for (int i = 0; i < 64; ++i) above += best_sh[i] > b || (best_sh[i] == b && i < tid);
-    if (above == top - 1) bound_sh = b;
-  }
-  __syncthreads();
-  const uint64_t bound = bound_sh > 0 ? bound_sh : 1;
-  auto take = [&](float x, int v) {
-    const uint64_t k = rank_of(x, v);
-    if (k < bound) return;
-    const int at = atomicAdd(&count, 1);
-    if (at < CAND) cand[at] = k;
-  };
-  if (mine >= bound) {
-    const float least = logit_of(bound);
-    if (tid < row.head) take(clean(to_f(row.p[tid])), tid);
-    if (row.tail() + tid < V) take(clean(to_f(row.p[row.tail() + tid])), row.tail() + tid);
-    for (int i0 = tid; i0 < row.vecs; i0 += NT * UN) {
+  int n = 0;  // candidates for the row's likeliest, in `cand`
+  if (top > 0) {
+    if (tid < 64) {
+      const uint64_t b = best_sh[tid];
+      int above = 0;
+      for (int i = 0; i < 64; ++i) above += best_sh[i] > b || (best_sh[i] == b && i < tid);
+      if (above == top - 1) bound_sh = b;
+    }
+    __syncthreads();
+    const uint64_t bound = bound_sh > 0 ? bound_sh : 1;
+    auto take = [&](float x, int v) {
+      const uint64_t k = rank_of(x, v);
+      if (k < bound) return;
+      const int at = atomicAdd(&count, 1);
+      if (at < CAND) cand[at] = k;
+    };
+    if (mine >= bound) {
+      if (tid < row.head) take(clean(to_f(row.p[tid])), v0 + tid);
+      if (row.tail() + tid < row.V) take(clean(to_f(row.p[row.tail() + tid])), v0 + row.tail() + tid);
+      who[atomicAdd(&n_who, 1)] = tid;
+    }
+    __syncthreads();
+    const int turns = (row.vecs + NT - 1) / NT, all = n_who * turns;
+    const float least = bound == 1 ? -INFINITY : logit_of(bound);
+    for (int x0 = tid; x0 < all; x0 += NT * UN) {
       uint4 u[UN];
-#pragma unroll
-      for (int j = 0; j < UN; ++j)
-        if (i0 + j * NT < row.vecs) u[j] = row.vec(i0 + j * NT);
+      int i[UN];
 #pragma unroll
       for (int j = 0; j < UN; ++j) {
-        if (i0 + j * NT >= row.vecs) break;
+        const int x = x0 + j * NT;
+        i[j] = x < all ? who[x / turns] + (x % turns) * NT : row.vecs;
+        if (i[j] < row.vecs) u[j] = row.vec(i[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < UN; ++j) {
+        if (i[j] >= row.vecs) continue;
         float x[N];
         unpack(u[j], x);
 #pragma unroll
         for (int e = 0; e < N; ++e)
-          if (bound == 1 || x[e] >= least) take(clean(x[e]), row.head + (i0 + j * NT) * N + e);
+          if (x[e] >= least) take(clean(x[e]), v0 + row.head + i[j] * N + e);
       }
     }
-  }
-  __syncthreads();
-  int n = count;
-  if (n > CAND) {  // logits in an order that puts the largest into few threads: one pass for each alternative
-    uint64_t last = ~0ull;
-    for (int k = 0; k < top; ++k) {
-      uint64_t b = 0;
-      for (int v = tid; v < V; v += NT) {
-        const uint64_t q = rank_of(clean(to_f(row.p[v])), v);
-        if (q < last && q > b) b = q;
-      }
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t q = __shfl_xor_sync(0xffffffffu, b, o);
-        b = q > b ? q : b;
-      }
-      __syncthreads();
-      if (lane == 0) best_sh[w] = b;
-      __syncthreads();
-      for (int i = 0; i < NT / 32; ++i) b = best_sh[i] > b ? best_sh[i] : b;
-      last = b;
-      if (tid == 0) cand[k] = b;
-    }
-    n = top;
     __syncthreads();
+    n = count;
+    if (n > CAND) {  // logits in an order that puts the largest into few threads: one pass for each alternative
+      uint64_t last = ~0ull;
+      for (int k = 0; k < top; ++k) {
+        uint64_t b = 0;
+        for (int v = tid; v < row.V; v += NT) {
+          const uint64_t q = rank_of(clean(to_f(row.p[v])), v0 + v);
+          if (q < last && q > b) b = q;
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint64_t q = __shfl_xor_sync(0xffffffffu, b, o);
+          b = q > b ? q : b;
+        }
+        __syncthreads();
+        if (lane == 0) best_sh[w] = b;
+        __syncthreads();
+        for (int i = 0; i < NT / 32; ++i) b = best_sh[i] > b ? best_sh[i] : b;
+        last = b;
+        if (tid == 0) cand[k] = b;
+      }
+      n = top;
+      __syncthreads();
+    }
   }
+  if (C > 1) {  // the parts meet in the cluster's first block: sums, and each one's likeliest in order
+    namespace cg = cooperative_groups;
+    auto cluster = cg::this_cluster();
+    if (tid == 0) part.sums = a;
+    for (int i = tid; i < top; i += NT)
+      if (i >= n) part.best[i] = 0;
+    for (int i = tid; i < n; i += NT) {
+      int above = 0;
+      for (int j = 0; j < n; ++j) above += cand[j] > cand[i];
+      if (above < top) part.best[above] = cand[i];
+    }
+    cluster.sync();
+    if (rank == 0) {
+      for (int k = 1; k < C; ++k) a.join(cluster.map_shared_rank(&part, k)->sums, c);
+      for (int i = tid; i < C * top; i += NT) cand[i] = cluster.map_shared_rank(&part, i / top)->best[i % top];
+      n = C * top;
+    }
+    cluster.sync();  // no part leaves before it has been read
+    if (rank != 0) return;
+  }
+  const bool some = a.m > -INFINITY;
+  const float log2s = some ? log2f(a.s) : 0.f;
+  // without the floor: a logit however far below has a log-probability
+  auto logprob = [&](float x) { return x == -INFINITY || !some ? -INFINITY : ((x - a.m) * c - log2s) * LN2; };
+  if (tid == 0) {
+    const int64_t y = tokens[r];
+    lp[r] = y >= 0 && y < V ? logprob(clean(to_f(p[y]))) : 0.f;
+    const float H = some ? (log2s - a.z / a.s) * LN2 : 0.f;
+    entropy[r] = H;
+    stats[r] = make_float4(a.m, log2s, H, 0.f);
+  }
+  auto place = [&](int at, uint64_t b) {
+    const float q = b ? logprob(logit_of(b)) : -INFINITY;
+    top_tok[r * top + at] = q > -INFINITY ? index_of(b) : -1;
+    top_lp[r * top + at] = q;
+  };
   for (int i = tid; i < n; i += NT) {
     const uint64_t b = cand[i];
     int above = 0;
-    for (int j = 0; j < n; ++j) above += cand[j] > b;
-    if (above < top) {
-      const float p = b ? logprob(logit_of(b)) : -INFINITY;
-      top_tok[r * top + above] = p > -INFINITY ? index_of(b) : -1;
-      top_lp[r * top + above] = p;
-    }
+    for (int j = 0; j < n; ++j) above += cand[j] > b || (cand[j] == b && j < i);
+    if (above < top) place(above, b);
   }
-  for (int i = n + tid; i < top; i += NT) {  // fewer logits with a probability than asked for
-    top_tok[r * top + i] = -1;
-    top_lp[r * top + i] = -INFINITY;
-  }
+  for (int i = n + tid; i < top; i += NT) place(i, 0);  // fewer logits with a probability than asked for
 }
 
 // Elementwise over the row's part; logits and gradient in vectors where both lie alike.
@@ -273,27 +329,45 @@ __global__ void __launch_bounds__(256) logprobs_bwd(const T* __restrict__ logits
   const float4 st = stats[r];
   const int64_t y64 = tokens[r];
   const int y = y64 >= 0 && y64 < V ? (int)y64 : -1;
-  const bool some = st.x > -INFINITY;
+  const bool some = st.x > -INFINITY, plain = some && st.x < BIG;
   const float gy = y >= 0 ? g[r] * inv_t : 0.f, gh = ge[r] * inv_t;
   auto grad = [&](float v, int i) {
     v = clean(v);
     if (v == -INFINITY || !some) return 0.f;
-    const float q = fmaxf((v - st.x) * c - st.y, -1e30f), p = ex2(q);
+    const float q = fmaxf((v - st.x) * c - st.y, FLOOR), p = ex2(q);
     return (i == y ? gy : 0.f) - p * (gy + gh * (q * LN2 + st.z));
   };
   const int b = blockIdx.x * part, e = min(V, b + part);
   const Row<T> row(x + b, e - b);
   const bool alike = ((reinterpret_cast<uintptr_t>(x + b) ^ reinterpret_cast<uintptr_t>(d + b)) & 15) == 0;
   if (alike) {
-    for (int i = threadIdx.x; i < row.vecs; i += 256) {
-      const uint4 u = row.vec(i);
-      float v[N];
-      unpack(u, v);
-      const int at = b + row.head + i * N;
-      alignas(16) T o[N];
+    constexpr int UN = 4;
+    for (int i0 = threadIdx.x; i0 < row.vecs; i0 += 256 * UN) {
+      uint4 u[UN];
 #pragma unroll
-      for (int k = 0; k < N; ++k) o[k] = from_f<T>(grad(v[k], at + k));
-      *reinterpret_cast<uint4*>(d + at) = *reinterpret_cast<uint4*>(o);
+      for (int j = 0; j < UN; ++j)
+        if (i0 + j * 256 < row.vecs) u[j] = row.vec(i0 + j * 256);
+#pragma unroll
+      for (int j = 0; j < UN; ++j) {
+        if (i0 + j * 256 >= row.vecs) break;
+        float v[N];
+        unpack(u[j], v);
+        const int at = b + row.head + (i0 + j * 256) * N;
+        alignas(16) T o[N];
+        if ((y >= at && y < at + N) || !plain) {  // the given token's, or an unusual row
+#pragma unroll
+          for (int k = 0; k < N; ++k) o[k] = from_f<T>(grad(v[k], at + k));
+        } else {
+#pragma unroll
+          for (int k = 0; k < N; k += 2) {
+            const float2 q = max2(fma2(add2(make_float2(v[k], v[k + 1]), both(-st.x)), both(c), both(-st.y)), FLOOR);
+            const float2 g2 = mul2(make_float2(ex2(q.x), ex2(q.y)), fma2(q, both(-gh * LN2), both(-gy - gh * st.z)));
+            o[k] = from_f<T>(g2.x);
+            o[k + 1] = from_f<T>(g2.y);
+          }
+        }
+        *reinterpret_cast<uint4*>(d + at) = *reinterpret_cast<uint4*>(o);
+      }
     }
     if ((int)threadIdx.x < row.head) d[b + threadIdx.x] = from_f<T>(grad(to_f(x[b + threadIdx.x]), b + threadIdx.x));
     const int t = b + row.tail() + threadIdx.x;
@@ -303,19 +377,44 @@ __global__ void __launch_bounds__(256) logprobs_bwd(const T* __restrict__ logits
   }
 }
 
+// Few rows are cut for as many blocks as two an SM: a row alone on a block takes its 10 us however few there are (64 rows of
+// 50304 logits: 15.6 us whole, with four blocks a row less).  A part keeps 4096 logits at least.
+template <typename T>
+int launch_fwd(const T* logits, int64_t ls, const int64_t* tokens, int64_t R, int V, int top, float c, float* lp, float* entropy,
+               float4* stats, int64_t* top_tok, float* top_lp, cudaStream_t st) {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -1;
+  int C = 1;
+  while (C < 8 && R * 2 * C <= 2 * sms && V / (2 * C) >= 4096) C *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(R * C));
+  cfg.blockDim = dim3(NT);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {(unsigned)C, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  auto go = [&](auto kernel) {
+    return cudaLaunchKernelEx(&cfg, kernel, logits, ls, tokens, V, top, c, lp, entropy, stats, top_tok, top_lp) == cudaSuccess ? 0 : -2;
+  };
+  switch (C) {
+    case 8: return go(logprobs_fwd<T, 8>);
+    case 4: return go(logprobs_fwd<T, 4>);
+    case 2: return go(logprobs_fwd<T, 2>);
+    default: return go(logprobs_fwd<T, 1>);
+  }
+}
+
 }  // namespace
 
-void ahb_token_logprobs_fwd(const void* logits, int64_t ls, int dtype, const int64_t* tokens, int64_t R, int V, int top,
-                            float temperature, float* lp, float* entropy, void* stats, int64_t* top_tok, float* top_lp,
-                            cudaStream_t st) {
-  if (R == 0) return;
+int ahb_token_logprobs_fwd(const void* logits, int64_t ls, int dtype, const int64_t* tokens, int64_t R, int V, int top,
+                           float temperature, float* lp, float* entropy, void* stats, int64_t* top_tok, float* top_lp,
+                           cudaStream_t st) {
+  if (R == 0) return 0;
   const float c = LOG2E / temperature;
-  if (dtype == AHB_BF16)
-    logprobs_fwd<<<(unsigned)R, NT, 0, st>>>((const bf16*)logits, ls, tokens, V, top, c, lp, entropy, (float4*)stats, top_tok,
-                                             top_lp);
-  else
-    logprobs_fwd<<<(unsigned)R, NT, 0, st>>>((const float*)logits, ls, tokens, V, top, c, lp, entropy, (float4*)stats, top_tok,
-                                             top_lp);
+  return dtype == AHB_BF16 ? launch_fwd((const bf16*)logits, ls, tokens, R, V, top, c, lp, entropy, (float4*)stats, top_tok, top_lp, st)
+                           : launch_fwd((const float*)logits, ls, tokens, R, V, top, c, lp, entropy, (float4*)stats, top_tok, top_lp, st);
 }
 
 void ahb_token_logprobs_bwd(const void* logits, int64_t ls, int dtype, const int64_t* tokens, const void* stats,
