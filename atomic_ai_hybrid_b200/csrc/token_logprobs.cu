@@ -6,10 +6,11 @@
 // Sums run over differences from the running maximum, in which nothing is lost to the size of the logits.  Two values
 // at a time where the GPU has instructions for it: a bf16 logit costs five, where the copy's rate leaves time for ten.
 //
-// Forward: one pass over a row, by one block or, where rows are few, by a cluster of up to eight.  Every thread keeps
-// its largest logit (the lowest index where equal).  The k-th largest of 64 groups' best is a bound that at least k
-// logits reach, and only a thread whose own best reaches it can hold one of them: the shares of those few are read again,
-// by all threads, and what reaches the bound is ranked by counting.
+// Forward: one pass over a row, by one block or, where rows are few, by a cluster of up to eight.  A warp's sums refer
+// to its own running maximum, which moves a handful of times (with one for each thread some lane of a warp had a new one at
+// almost every step: 2048 x 128256 logits 156 to 191 us).  Every thread keeps its largest logit: the k-th largest of 64
+// groups' is a bound that at least k logits reach, and only a thread whose own reaches it can hold one of them: the
+// shares of those few are read again, by all threads, and what reaches the bound is ranked by counting.
 #include <cooperative_groups.h>
 #include "common.cuh"
 #include "launchers.h"
@@ -20,7 +21,7 @@ using bf16 = __nv_bfloat16;
 
 namespace {
 
-constexpr int NT = 256, CAND = 512, MAX_TOP = 64;
+constexpr int NT = 256, CAND = 1024, MAX_TOP = 64;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, BIG = 3.4028234663852886e38f;
 constexpr float FLOOR = -200.f;  // 2^-200 is 0 in fp32, and 0 times -200 is 0 where 0 times -inf is NaN
 
@@ -82,15 +83,26 @@ struct Sums {
   }
 };
 
-// The largest of a vector; NaN is passed over.
-AHB_DEVICE float vec_max(const uint4& u, const float (&x)[8]) {
+// A vector's elements with NaN and what lies below LOW as LOW, and the largest of them.
+constexpr float LOW = -1e30f;
+AHB_DEVICE float unpack_low(const uint4& u, float (&x)[8]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);
-  const __nv_bfloat162 a = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-  const float2 f = __bfloat1622float2(a);
+  const __nv_bfloat162* in = reinterpret_cast<const __nv_bfloat162*>(w);
+  const __nv_bfloat162 low = __float2bfloat162_rn(LOW);
+  uint4 v;
+  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __hmax2(in[i], low);
+  const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+  unpack(v, x);
   return fmaxf(f.x, f.y);
 }
-AHB_DEVICE float vec_max(const uint4&, const float (&x)[4]) { return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])); }
+AHB_DEVICE float unpack_low(const uint4& u, float (&x)[4]) {
+  unpack(u, x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = fmaxf(x[i], LOW);
+  return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+}
 
 // A row's elements as this thread sees them: f(x, v) in rising v, in vectors where the row is aligned.
 template <typename T>
@@ -113,7 +125,8 @@ __global__ void __launch_bounds__(NT, 4) logprobs_fwd(const T* __restrict__ logi
                                                       float* __restrict__ top_lp) {
   constexpr int N = Vec<T>::N, UN = 4, GL = NT / 64;  // GL: lanes of a group
   __shared__ Sums sums[NT / 32];
-  __shared__ uint64_t best_sh[64], cand[CAND], bound_sh;
+  __shared__ uint64_t best_sh[NT / 32], cand[CAND];
+  __shared__ float group_max[64], bound_sh;
   __shared__ int count, who[NT], n_who;
   struct Part {
     Sums sums;
@@ -127,75 +140,70 @@ __global__ void __launch_bounds__(NT, 4) logprobs_fwd(const T* __restrict__ logi
   const int each = C == 1 ? V : ((V + C - 1) / C + 63) & ~63, v0 = min(V, rank * each), v1 = min(V, v0 + each);
   const Row<T> row(p + v0, v1 - v0);
   Sums a{-INFINITY, 0.f, 0.f};
-  uint64_t best = 0;
-  auto one = [&](int v) {  // the few elements outside the vectors
-    const float x = clean(to_f(row.p[v]));
-    if (x == -INFINITY) return;
-    if (x > a.m) a.move(x, c);
-    a.add(x, c);
-    const uint64_t k = rank_of(x, v0 + v);
-    best = k > best ? k : best;
+  float best = -INFINITY;  // this thread's largest, where it is above LOW
+  auto one = [&](int v) {  // the few elements outside the vectors, and all where the maximum is infinite or below LOW
+    const float x = clean(v < row.V ? to_f(row.p[v]) : -INFINITY);
+    const float mx = warp_max(x);
+    best = fmaxf(best, x);
+    if (mx > a.m) a.move(mx, c);
+    if (x > -INFINITY) a.add(x, c);
   };
-  if (tid < row.head) one(tid);
-  if (row.tail() + tid < row.V) one(row.tail() + tid);
-  float top_x = -INFINITY;
-  int top_v = 0;
-  for (int i0 = tid; i0 < row.vecs; i0 += NT * UN) {
+  if (w == 0) one(lane < row.head ? lane : row.V);
+  if (w == 1) one(row.tail() + lane);
+  auto vec = [&](const uint4& u, int i) {
+    float x[N];
+    const bool in = i < row.vecs;
+    const float mx = in ? unpack_low(u, x) : -INFINITY;
+    if (__any_sync(0xffffffffu, mx > a.m)) {
+      float y[N], top_y = -INFINITY;
+      unpack(u, y);
+#pragma unroll
+      for (int e = 0; e < N; ++e) top_y = fmaxf(top_y, clean(y[e]));
+      top_y = warp_max(in ? top_y : -INFINITY);
+      if (top_y > a.m) a.move(top_y, c);
+    }
+    if (!in) return;
+    best = fmaxf(best, mx);
+    if (!(a.m > 0.1f * LOW && a.m < BIG)) {
+      unpack(u, x);
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (clean(x[e]) > -INFINITY) a.add(clean(x[e]), c);
+      return;
+    }
+    const float2 neg = both(-a.m), cc = both(c);
+    float2 s2 = both(0.f), z2 = both(0.f);
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const float2 d = mul2(add2(make_float2(x[e], x[e + 1]), neg), cc);
+      const float2 q = make_float2(ex2(d.x), ex2(d.y));
+      s2 = add2(s2, q);
+      z2 = fma2(q, d, z2);
+    }
+    a.s += s2.x + s2.y;
+    a.z += z2.x + z2.y;
+  };
+  int i0 = tid;
+  for (; i0 - lane + 31 + (UN - 1) * NT < row.vecs; i0 += NT * UN) {  // whole warps
     uint4 u[UN];
 #pragma unroll
-    for (int j = 0; j < UN; ++j)
-      if (i0 + j * NT < row.vecs) u[j] = row.vec(i0 + j * NT);
+    for (int j = 0; j < UN; ++j) u[j] = row.vec(i0 + j * NT);
 #pragma unroll
-    for (int j = 0; j < UN; ++j) {
-      if (i0 + j * NT >= row.vecs) break;
-      float x[N];
-      unpack(u[j], x);
-      const float mx = vec_max(u[j], x);
-      if (mx > top_x) {  // seldom, but for a thread's first vectors
-        const float xx = fminf(mx, BIG);
-        if (xx > a.m) a.move(xx, c);
-        if (xx > top_x) {
-          top_x = xx;
-#pragma unroll
-          for (int e = N - 1; e >= 0; --e)
-            if (clean(x[e]) == xx) top_v = v0 + row.head + (i0 + j * NT) * N + e;
-        }
-      }
-      if (mx == INFINITY) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) a.add(clean(x[e]), c);
-      } else if (a.m > -INFINITY) {
-        float2 s2 = both(0.f), z2 = both(0.f);
-#pragma unroll
-        for (int e = 0; e < N; e += 2) {
-          const float2 d = max2(mul2(add2(make_float2(x[e], x[e + 1]), both(-a.m)), both(c)), FLOOR);  // NaN: no mass
-          const float2 q = make_float2(ex2(d.x), ex2(d.y));
-          s2 = add2(s2, q);
-          z2 = fma2(q, d, z2);
-        }
-        a.s += s2.x + s2.y;
-        a.z += z2.x + z2.y;
-      }
-    }
+    for (int j = 0; j < UN; ++j) vec(u[j], i0 + j * NT);
   }
-  {
-    const uint64_t k = rank_of(top_x, top_v);
-    best = k > best ? k : best;
-  }
-  const uint64_t mine = best;
+  for (; i0 - lane < row.vecs; i0 += NT) vec(i0 < row.vecs ? row.vec(i0) : make_uint4(0, 0, 0, 0), i0);
+  best = fminf(best, BIG);
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const Sums b{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.z, o)};
-    a.join(b, c);
+  for (int o = 1; o < 32; o <<= 1) {  // the maximum is the warp's already
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    a.z += __shfl_xor_sync(0xffffffffu, a.z, o);
   }
   if (lane == 0) sums[w] = a;
   if (top > 0) {
+    float b = best;
 #pragma unroll
-    for (int o = 1; o < GL; o <<= 1) {
-      const uint64_t b = __shfl_xor_sync(0xffffffffu, best, o);
-      best = b > best ? b : best;
-    }
-    if (tid % GL == 0) best_sh[tid / GL] = best;
+    for (int o = 1; o < GL; o <<= 1) b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, o));
+    if (tid % GL == 0) group_max[tid / GL] = b;
     if (tid == 0) count = n_who = 0;
   }
   __syncthreads();
@@ -205,27 +213,24 @@ __global__ void __launch_bounds__(NT, 4) logprobs_fwd(const T* __restrict__ logi
   int n = 0;  // candidates for the row's likeliest, in `cand`
   if (top > 0) {
     if (tid < 64) {
-      const uint64_t b = best_sh[tid];
+      const float b = group_max[tid];
       int above = 0;
-      for (int i = 0; i < 64; ++i) above += best_sh[i] > b || (best_sh[i] == b && i < tid);
+      for (int i = 0; i < 64; ++i) above += group_max[i] > b || (group_max[i] == b && i < tid);
       if (above == top - 1) bound_sh = b;
     }
     __syncthreads();
-    const uint64_t bound = bound_sh > 0 ? bound_sh : 1;
+    // a bound that says nothing (few logits above LOW): all with a probability
+    const float bound = bound_sh > LOW ? bound_sh : -INFINITY;
     auto take = [&](float x, int v) {
-      const uint64_t k = rank_of(x, v);
-      if (k < bound) return;
+      if (!(x >= bound) || x == -INFINITY) return;
       const int at = atomicAdd(&count, 1);
-      if (at < CAND) cand[at] = k;
+      if (at < CAND) cand[at] = rank_of(x, v);
     };
-    if (mine >= bound) {
-      if (tid < row.head) take(clean(to_f(row.p[tid])), v0 + tid);
-      if (row.tail() + tid < row.V) take(clean(to_f(row.p[row.tail() + tid])), v0 + row.tail() + tid);
-      who[atomicAdd(&n_who, 1)] = tid;
-    }
+    if (w == 0 && lane < row.head) take(clean(to_f(row.p[lane])), v0 + lane);
+    if (w == 1 && row.tail() + lane < row.V) take(clean(to_f(row.p[row.tail() + lane])), v0 + row.tail() + lane);
+    if (best >= bound) who[atomicAdd(&n_who, 1)] = tid;
     __syncthreads();
     const int turns = (row.vecs + NT - 1) / NT, all = n_who * turns;
-    const float least = bound == 1 ? -INFINITY : logit_of(bound);
     for (int x0 = tid; x0 < all; x0 += NT * UN) {
       uint4 u[UN];
       int i[UN];
@@ -241,13 +246,12 @@ __global__ void __launch_bounds__(NT, 4) logprobs_fwd(const T* __restrict__ logi
         float x[N];
         unpack(u[j], x);
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (x[e] >= least) take(clean(x[e]), v0 + row.head + i[j] * N + e);
+        for (int e = 0; e < N; ++e) take(clean(x[e]), v0 + row.head + i[j] * N + e);
       }
     }
     __syncthreads();
     n = count;
-    if (n > CAND) {  // logits in an order that puts the largest into few threads: one pass for each alternative
+    if (n > CAND) {  // many equal ones, or an order that puts the largest into few threads: one pass for each alternative
       uint64_t last = ~0ull;
       for (int k = 0; k < top; ++k) {
         uint64_t b = 0;
