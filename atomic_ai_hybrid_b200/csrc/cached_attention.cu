@@ -121,14 +121,14 @@ AHB_DEVICE void make_plan(const Args& a) {
     }
     for (int x = 0; x < (a.prefix ? 2 : 1); ++x) {
       const Group& g = x ? run : own;
-      int64_t units[KINDS] = {0, 0, 0, 0};
+      int64_t units[KINDS] = {0, 0, 0};
       if (g.tokens > 0 && !is_tiles(a, g)) units[ROWS] = (int64_t)a.Hk * row_units(g);
       if (g.tokens > 0 && is_tiles(a, g)) {
         const int n = row_tiles(a, g);
         for (int rt = 0; rt < n; ++rt) units[TILES] += tile_item(a, g, rt).units;
         units[TILES] *= a.Hk;
       }
-      if (a.mass && !x && g.tokens > 0) units[is_tiles(a, g) ? TILES_MASS : ROWS_MASS] = (int64_t)a.Hk * row_units(g);
+      if (a.mass && !x && g.tokens > 0) units[TILES_MASS] = is_tiles(a, g) ? (int64_t)a.Hk * ceil_div(g.keys, 4 * KU) : 0;
       for (int k = 0; k < (x || !a.mass ? 2 : KINDS); ++k) {
         __syncthreads();
         const int64_t c = carry[KINDS * x + k];
@@ -419,6 +419,11 @@ __global__ void __launch_bounds__(RW * 32, RB) ca_rows(const Args a) {
           s[x][e] = c * KU + 8 * x + 2 * t4 + e <= last ? s[x][e] * a.scale2 : -INFINITY;
           mx = fmaxf(mx, s[x][e]);
         }
+      if (a.mass && !pre && out >= 0) {  // for ca_mass_rows
+        float* y = a.scores + ((first + c) * RT + g) * KU + 2 * t4;
+        *reinterpret_cast<float2*>(y) = make_float2(s[0][0], s[0][1]);
+        *reinterpret_cast<float2*>(y + 8) = make_float2(s[1][0], s[1][1]);
+      }
       if (__any_sync(0xffffffffu, mx > m + SLACK)) {
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -658,47 +663,96 @@ __global__ void __launch_bounds__(JW * 32) ca_join_tiles(const Args a) {
 }
 
 // ----------------------------------------------------------------------------- what every cache row was given
-// A warp holds 16 cache rows and goes over the query rows that see them: sum_t 2^(s_tj - lse_t).
+// Of the row kernel's groups, from the scores that it has kept (1/16 of the cache's bytes at most; made again from the
+// keys they took as long as the row kernel itself).  A warp goes through its share of the units; lane 4 r + k has query row r
+// and cache rows 4 k .. + 4.
+constexpr int MB = 12;  // blocks of ca_mass_rows on an SM
+__global__ void __launch_bounds__(RW * 32, MB) ca_mass_rows(const Args a, int warps) {
+  const int lane = threadIdx.x & 31, G = a.H / a.Hk, r = lane >> 2, tt = per_group(r, G), k0 = 4 * (lane & 3);
+  const int64_t* units = a.sums[ROWS];
+  const int64_t all = units[a.B], share = share_of(all, warps);
+  int64_t u = ((int64_t)blockIdx.x * RW + (threadIdx.x >> 5)) * share;
+  const int64_t u_end = min(u + share, all);
+  while (u < u_end) {
+    const int i = find_group(units, a.B, u);
+    const Group gr = a.groups[i];
+    const int per_head = row_units(gr), h = (int)div64(u - units[i], per_head), c0 = (int)(u - units[i] - (int64_t)h * per_head);
+    const int n = (int)min((int64_t)(per_head - c0), u_end - u);
+    const bool in = r < gr.tokens * G;
+    const float lse = in ? a.lse[(int64_t)(gr.row0 + tt) * a.H + h * G + r - tt * G] : 0.f;
+    float* m = a.mass + ((int64_t)gr.slot * a.Hk + h) * a.M;
+#pragma unroll 4
+    for (int c = 0; c < n; ++c) {
+      float4 p = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (in) {
+        const float4 s = *reinterpret_cast<const float4*>(a.scores + (u + c) * RT * KU + lane * 4);
+        p = make_float4(ex2(s.x - lse), ex2(s.y - lse), ex2(s.z - lse), ex2(s.w - lse));
+      }
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        p.x += __shfl_xor_sync(0xffffffffu, p.x, o);
+        p.y += __shfl_xor_sync(0xffffffffu, p.y, o);
+        p.z += __shfl_xor_sync(0xffffffffu, p.z, o);
+        p.w += __shfl_xor_sync(0xffffffffu, p.w, o);
+      }
+      const int x = lane >> 2, j = (c0 + c) * KU + k0 + x;  // lanes 0 .. 15: a cache row each
+      const float mine = x == 0 ? p.x : x == 1 ? p.y : x == 2 ? p.z : p.w;
+      if (x < 4 && j < gr.keys) m[j] += mine;
+    }
+    u += n;
+  }
+}
+
+// Of the tile kernel's: a warp holds 64 cache rows and goes over the query rows that see them, eight at a time:
+// sum_t 2^(s_tj - lse_t).
+constexpr int KM = 4;  // units of 16 cache rows that a warp holds
 template <int D>
-__global__ void __launch_bounds__(RW * 32) ca_mass(const Args a, int kind) {
+__global__ void __launch_bounds__(RW * 32, 2) ca_mass(const Args a) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  const int64_t* units = a.sums[kind];
+  const int64_t* units = a.sums[TILES_MASS];
   const int64_t all = units[a.B];
   const int G = a.H / a.Hk;
   for (int64_t u = (int64_t)blockIdx.x * RW + (threadIdx.x >> 5); u < all; u += (int64_t)gridDim.x * RW) {
     const int i = find_group(units, a.B, u);
     const Group gr = a.groups[i];
-    const int per_head = row_units(gr), h = (int)div64(u - units[i], per_head);
-    const int j0 = (int)(u - units[i] - (int64_t)h * per_head) * KU;
-    uint4 kr[2][D / 32];
-    load_keys<D>(kr, a.kc + ((int64_t)gr.slot * a.Hk + h) * a.M * D, j0, gr.keys, g, t4);
-    float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+    const int per_head = ceil_div(gr.keys, KM * KU), h = (int)div64(u - units[i], per_head);
+    const int j0 = (int)(u - units[i] - (int64_t)h * per_head) * KM * KU;
+    uint4 kr[KM][2][D / 32];
+#pragma unroll
+    for (int y = 0; y < KM; ++y) load_keys<D>(kr[y], a.kc + ((int64_t)gr.slot * a.Hk + h) * a.M * D, j0 + y * KU, gr.keys, g, t4);
+    float sum[KM][2][2] = {};
     const int rows = gr.tokens * G;
     // from the first token that sees row j0
     for (int r0 = max(0, j0 - gr.before) * G / RT * RT; r0 < rows; r0 += RT) {
-      const int r = r0 + g, tt = r / G;
+      const int r = r0 + g, tt = per_group(r, G);
       const int64_t out = (int64_t)(gr.row0 + tt) * a.H + h * G + (r - tt * G);
       const float lse = r < rows ? a.lse[out] : 0.f;
       const int last = r < rows ? gr.before + tt : -1;
       uint32_t qa[D / 16][4];
       load_q<D>(qa, r < rows ? a.qw + out * 2 * D : nullptr, t4);
-      float s[2][2];
-      scores<D>(s, qa, kr);
+#pragma unroll
+      for (int y = 0; y < KM; ++y) {
+        float s[2][2];
+        scores<D>(s, qa, kr[y]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (j0 + y * KU + 8 * x + 2 * t4 + e <= last) sum[y][x][e] += ex2(s[x][e] * a.scale2 - lse);
+      }
+    }
+#pragma unroll
+    for (int y = 0; y < KM; ++y)
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (j0 + 8 * x + 2 * t4 + e <= last) sum[x][e] += ex2(s[x][e] * a.scale2 - lse);
-    }
+        for (int e = 0; e < 2; ++e) {
+          float v = sum[y][x][e];
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) sum[x][e] += __shfl_xor_sync(0xffffffffu, sum[x][e], o);
-        const int j = j0 + 8 * x + 2 * t4 + e;
-        if (g == 0 && j < gr.keys) a.mass[((int64_t)gr.slot * a.Hk + h) * a.M + j] += sum[x][e];
-      }
+          for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+          const int j = j0 + y * KU + 8 * x + 2 * t4 + e;
+          if (g == 0 && j < gr.keys) a.mass[((int64_t)gr.slot * a.Hk + h) * a.M + j] += v;
+        }
   }
 }
 
@@ -731,6 +785,7 @@ int64_t lay_out(Args& a, char* base) {
   a.run_start = (int*)place((int64_t)a.B * 4);
   a.run_end = (int*)place((int64_t)a.B * 4);
   for (int k = 0; k < (a.mass ? KINDS : 2); ++k) a.sums[k] = (int64_t*)place((int64_t)2 * (a.B + 1) * 8);
+  a.scores = a.mass ? (float*)place((int64_t)a.B * a.Hk * ((a.M + KU - 1) / KU) * RT * KU * 4) : nullptr;
   a.lse = a.mass ? (float*)place(rows * 4) : nullptr;
   a.part = (float*)place((int64_t)2 * a.warps * RT * (a.D + 4) * 4);
   a.tile_part = (float*)place((int64_t)2 * a.blocks * 2 * TQ * (a.D + 4) * 4);
@@ -754,8 +809,8 @@ int launch(const Args& a, cudaStream_t st) {
   if ((int64_t)a.T * a.H <= 4 * sms) ca_join_wide<D><<<dim3(a.T, a.H), JW * 32, 0, st>>>(a);
   else ca_join<D><<<(unsigned)(rows < 16 * sms ? rows : 16 * sms), JW * 32, 0, st>>>(a, heads);
   if (a.mass) {
-    ca_mass<D><<<a.warps / RW, RW * 32, 0, st>>>(a, ROWS_MASS);
-    if (a.blocks) ca_mass<D><<<a.warps / RW, RW * 32, 0, st>>>(a, TILES_MASS);
+    ca_mass_rows<<<sms * MB, RW * 32, 0, st>>>(a, sms * MB * RW);
+    if (a.blocks) ca_mass<D><<<sms * 2, RW * 32, 0, st>>>(a);
   }
   return 0;
 }

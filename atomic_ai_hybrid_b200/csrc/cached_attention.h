@@ -19,7 +19,7 @@ struct Group {
 
 // Groups [0, B) are the sequences' own rows, [B, 2 B) the prefix runs, each at its last sequence.  Each group is worked on by one of
 // two kernels; a kernel's units are numbered through the groups, and sums[kind][g] is group g's first one.
-enum Kind { ROWS = 0, TILES = 1, ROWS_MASS = 2, TILES_MASS = 3, KINDS = 4 };
+enum Kind { ROWS = 0, TILES = 1, TILES_MASS = 2, KINDS = 3 };
 
 // What a block of the tile kernel began and others go on with (rows 0: nothing), up to block `last`.
 struct SharedItem {
@@ -45,6 +45,7 @@ struct Args {
   Group* groups;                 // (2 B)
   int *run_start, *run_end;      // a sequence's run: its first sequence (-1: no prefix), and that one's last
   int64_t* sums[KINDS];          // (2 B + 1) each
+  float* scores;                 // the row kernel's, unit by unit (8 query rows of 16 cache rows), for mass
   float* lse;                    // (T, H) log2 of the softmax's denominators, for mass
   float* part;                   // partial results of items that several warps share, two a warp
   float* tile_part;              // ... of items that several blocks share, two a block
