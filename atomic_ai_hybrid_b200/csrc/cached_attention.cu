@@ -185,6 +185,7 @@ AHB_DEVICE void store8(bf16* p, bf16* rest, const float* v) {
 // Block 0 makes the plan; the others rotate, clip and place `per` token rows each, and make rows of no sequence zero.
 template <bool VEC>
 __global__ void __launch_bounds__(AT) ca_append(const Args a, int per) {
+  next_may_start();
   if (blockIdx.x == 0) {
     make_plan(a);
     return;
@@ -376,6 +377,8 @@ AHB_DEVICE void add_values(float (&o)[D / 16][4], const uint32_t (&ph)[2], const
 
 template <int D>
 __global__ void __launch_bounds__(RW * 32, RB) ca_rows(const Args a) {
+  next_may_start();
+  after_previous();
   constexpr int MT = D / 16, VC = (D + 63) / 64;
   const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const int w = blockIdx.x * RW + (threadIdx.x >> 5);
@@ -632,11 +635,15 @@ AHB_DEVICE void join_row(const Args& a, int t, int h0, int h1, int step) {
 }
 template <int D>
 __global__ void __launch_bounds__(JW * 32) ca_join_wide(const Args a) {
+  next_may_start();
+  after_previous();
   join_row<D, true>(a, blockIdx.x, blockIdx.y, blockIdx.y + 1, 1);
 }
 // `heads` query heads a block
 template <int D>
 __global__ void __launch_bounds__(JW * 32, 3) ca_join(const Args a, int heads) {
+  next_may_start();
+  after_previous();
   if (!a.full && a.sums[ROWS][a.B] == 0) return;  // all is the tile kernel's
   const int per = (a.H + heads - 1) / heads;
   for (int64_t x = blockIdx.x; x < (int64_t)a.T * per; x += gridDim.x) {
@@ -649,6 +656,8 @@ __global__ void __launch_bounds__(JW * 32, 3) ca_join(const Args a, int heads) {
 // rows 32 y .. of the item that began among block b's units and goes on behind them, as block b has noted it.
 template <int D>
 __global__ void __launch_bounds__(JW * 32) ca_join_tiles(const Args a) {
+  next_may_start();
+  after_previous();
   const SharedItem it = a.shared_items[blockIdx.x];
   const int G = a.H / a.Hk;
   const int64_t slot = 2 * TQ * (D + 4);
@@ -668,6 +677,8 @@ __global__ void __launch_bounds__(JW * 32) ca_join_tiles(const Args a) {
 // and cache rows 4 k .. + 4.
 constexpr int MB = 12;  // blocks of ca_mass_rows on an SM
 __global__ void __launch_bounds__(RW * 32, MB) ca_mass_rows(const Args a, int warps) {
+  next_may_start();
+  after_previous();
   const int lane = threadIdx.x & 31, G = a.H / a.Hk, r = lane >> 2, tt = per_group(r, G), k0 = 4 * (lane & 3);
   const int64_t* units = a.sums[ROWS];
   const int64_t all = units[a.B], share = share_of(all, warps);
@@ -708,6 +719,8 @@ __global__ void __launch_bounds__(RW * 32, MB) ca_mass_rows(const Args a, int wa
 constexpr int KM = 4;  // units of 16 cache rows that a warp holds
 template <int D>
 __global__ void __launch_bounds__(RW * 32, 2) ca_mass(const Args a) {
+  next_may_start();
+  after_previous();
   const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const int64_t* units = a.sums[TILES_MASS];
   const int64_t all = units[a.B];
@@ -800,18 +813,24 @@ int launch(const Args& a, cudaStream_t st) {
     const int rc = launch_tiles(a, st);
     if (rc) return rc;
   }
-  ca_rows<D><<<a.warps / RW, RW * 32, 0, st>>>(a);
-  if (a.blocks && !a.full) ca_join_tiles<D><<<dim3(a.blocks, 2 * TQ / 32), JW * 32, 0, st>>>(a);
+  cudaError_t e = cudaSuccess;
+  // behind the tile kernel not before it has ended: its waiting blocks would sit on the SMs that the first of them leave
+  // (one token of 64 conversations on a prefix 99 us, so 88)
+  if (a.blocks) ca_rows<D><<<a.warps / RW, RW * 32, 0, st>>>(a);
+  else e = launch_after(ca_rows<D>, a.warps / RW, RW * 32, 0, st, a);
   const int sms = a.warps / (RB * RW);
   // a block a row where there are rows enough: what its heads share is looked up once
   const int heads = a.T > 4 * sms ? a.H : JW;
   const int64_t rows = (int64_t)a.T * ((a.H + heads - 1) / heads);
-  if ((int64_t)a.T * a.H <= 4 * sms) ca_join_wide<D><<<dim3(a.T, a.H), JW * 32, 0, st>>>(a);
-  else ca_join<D><<<(unsigned)(rows < 16 * sms ? rows : 16 * sms), JW * 32, 0, st>>>(a, heads);
+  auto then = [&](cudaError_t next) { e = e == cudaSuccess ? next : e; };
+  if (a.blocks && !a.full) then(launch_after(ca_join_tiles<D>, dim3(a.blocks, 2 * TQ / 32), JW * 32, 0, st, a));
+  if ((int64_t)a.T * a.H <= 4 * sms) then(launch_after(ca_join_wide<D>, dim3(a.T, a.H), JW * 32, 0, st, a));
+  else then(launch_after(ca_join<D>, (unsigned)(rows < 16 * sms ? rows : 16 * sms), JW * 32, 0, st, a, heads));
   if (a.mass) {
-    ca_mass_rows<<<sms * MB, RW * 32, 0, st>>>(a, sms * MB * RW);
-    if (a.blocks) ca_mass<D><<<sms * 2, RW * 32, 0, st>>>(a);
+    then(launch_after(ca_mass_rows, sms * MB, RW * 32, 0, st, a, sms * MB * RW));
+    if (a.blocks) then(launch_after(ca_mass<D>, sms * 2, RW * 32, 0, st, a));
   }
+  if (e != cudaSuccess) return -4;
   return 0;
 }
 

@@ -6,6 +6,25 @@
 namespace ahb {
 namespace cattn {
 
+// The kernels of a call follow one another closely: each lets the next one start while it runs (its blocks take the places
+// that become free), and waits for the one before, whole and with all that it wrote, before it reads anything.
+AHB_DEVICE void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+AHB_DEVICE void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <class... P, class... A>
+inline cudaError_t launch_after(void (*kernel)(P...), dim3 grid, int block, int smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 constexpr int KU = 16;    // row kernel: cache rows of a unit
 constexpr int RT = 8;     // ... and the query rows that it takes
 constexpr int TK = 64;    // tile kernel: cache rows of a block

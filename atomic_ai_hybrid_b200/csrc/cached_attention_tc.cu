@@ -211,6 +211,8 @@ template <int D, bool EXACT>
 __global__ void __launch_bounds__(NTHR, 1)
     ca_tiles(const Args a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
              const __grid_constant__ CUtensorMap mq) {
+  next_may_start();
+  after_previous();
   constexpr int NB = ring<EXACT>(), SLABS = (D + 63) / 64, DC = (D + 31) / 32;
   constexpr uint32_t SLAB = TK * 128, LOAD = SLABS * SLAB;
   extern __shared__ unsigned char raw[];
@@ -607,8 +609,7 @@ template <int D, bool EXACT>
 int launch_one(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, cudaStream_t st) {
   constexpr int bytes = (int)smem_bytes<EXACT>();
   if (cudaFuncSetAttribute(ca_tiles<D, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -3;
-  ca_tiles<D, EXACT><<<a.blocks, NTHR, bytes, st>>>(a, mk, mv, mq);
-  return 0;
+  return launch_after(ca_tiles<D, EXACT>, a.blocks, NTHR, bytes, st, a, mk, mv, mq) == cudaSuccess ? 0 : -4;
 }
 
 template <int D>
