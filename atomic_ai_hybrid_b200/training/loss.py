@@ -58,3 +58,24 @@ def compute_loss(model, batch: Dict[str, torch.Tensor], deterministic: bool = Fa
         "assignment_frac": _stack(stats, "assignment_frac"),
     }
     return total, info
+
+
+def token_scores(model, batch: Dict[str, torch.Tensor], temperature: float = 1.0, chunk: int = 2048):
+    """``(logprobs, entropy)``, fp32 and shaped like ``batch["labels"]``: the log-probability of every label under the model and the entropy of
+    the distribution that it is drawn from, with gradients (``ops.token_logprobs``), for objectives on the answers themselves
+    (preference pairs, policy gradients).  Labels of -100 have log-probability 0 and no gradient.  As in ``compute_loss`` the logits are made
+    ``chunk`` tokens at a time and again in the backward; they are rounded to the hidden states' type."""
+    import torch.utils.checkpoint as ckpt
+
+    hidden, _ = model(batch["input_ids"], return_hidden=True)
+    labels = model.token_shard(batch["labels"]) if hasattr(model, "token_shard") else batch["labels"]
+    w = model.lm_weight()
+
+    def piece(h, y, w):
+        return ops.token_logprobs(h @ w.to(h.dtype).t(), y, temperature=temperature)
+
+    h, y = hidden.reshape(-1, hidden.shape[-1]), labels.reshape(-1)
+    parts = [ckpt.checkpoint(piece, h[s:s + chunk], y[s:s + chunk], w, use_reentrant=False) if torch.is_grad_enabled() else
+             piece(h[s:s + chunk], y[s:s + chunk], w) for s in range(0, h.shape[0], chunk)]
+    lp, entropy = (torch.cat(t).view(labels.shape) for t in zip(*parts))
+    return lp, entropy

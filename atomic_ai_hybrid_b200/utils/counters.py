@@ -11,10 +11,23 @@ def _scan_kernels(a, k):
     return ext()._mod.selective_scan_kernels(a[0], a[8], a[9], a[10])
 
 
+def _attention_kernels(a, k):
+    """``cached_attention(q, k, v, k_cache, .., tokens a row [8], cu_seqlens, slots, prefix, seen, mass, ..)``: the new rows, the row
+    kernel and the join; the tile kernel where a sequence or a run may have more than eight query rows, with a join of its
+    own where there is no prefix; what rows gather."""
+    q, cache, cu, prefix, mass = a[0], a[3], a[9], a[11], a[13]
+    if q.shape[0] == 0 or (cu is not None and cu.numel() == 1):
+        return 0
+    group = q.shape[1] // (cache.shape[1] * cache.shape[3])
+    tiles = prefix is not None or cu is not None or a[8] * group > 8
+    return 3 + tiles + (tiles and prefix is None) + (0 if mass is None else 1 + tiles)
+
+
 class LaunchCounter:
     MULTI = {"gdn_fwd": 2, "gdn_fwd_train": 2, "gdn_bwd": 4, "gdn_bwd_saved": 2, "ssd_fwd": 2, "ssd_fwd_train": 2,
              "ssd_bwd": 4, "moe_fwd": 7, "moe_bwd": 8, "ce_online_fwd": 2, "add_rmsnorm_bwd": 2,
              "norm_gate_bwd": 2, "selective_scan": _scan_kernels,
+             "cached_attention": _attention_kernels,
              # three GEMMs per row chunk: ce_online_bwd(h, W, labels, lse, ls, g, dW_acc, chunk_rows)
              "ce_online_bwd": lambda a, k: 3 * -(-a[0].shape[0] // a[7])}
 

@@ -128,3 +128,58 @@ def test_logprobs_refuses():
                             ("temperature", (x, y), dict(temperature=math.inf)), ("temperature", (x, y), dict(temperature=math.nan))]:
         with pytest.raises(ValueError, match=match):
             ops.token_logprobs(*args, **kw)
+
+
+def test_token_scores_of_a_model():
+    """Log-probabilities and entropies of labels through a model, and their gradients against the log-softmax's."""
+    from atomic_ai_hybrid_b200.config import get_preset
+    from atomic_ai_hybrid_b200.models import HybridMoEModel
+    from atomic_ai_hybrid_b200.training.loss import token_scores
+
+    torch.manual_seed(0)
+    cfg = get_preset("tiny", num_layers=2, vocab_size=300)
+    model = HybridMoEModel(cfg, compute_dtype=F32)
+    ids = torch.randint(0, 300, (2, 65), generator=gen(1, CPU))
+    batch = {"input_ids": ids[:, :-1], "labels": ids[:, 1:].clone()}
+    batch["labels"][0, :10] = -100
+
+    def grads(f):
+        model.zero_grad()
+        lp, entropy = f()
+        (lp.sum() * 0.1 + 0.01 * entropy.sum()).backward()
+        return lp.detach(), entropy.detach(), {n: p.grad.clone() for n, p in model.named_parameters() if p.grad is not None}
+
+    def plain():
+        h, _ = model(batch["input_ids"])
+        logp = torch.log_softmax(h @ model.lm_weight().t(), -1)
+        given = batch["labels"] >= 0
+        lp = logp.gather(2, batch["labels"].clamp(min=0)[..., None])[..., 0] * given
+        return lp, -(logp.exp() * logp).sum(-1)
+
+    a, b = grads(lambda: token_scores(model, batch, chunk=50)), grads(plain)
+    assert a[0].shape == batch["labels"].shape and (a[0][0, :10] == 0).all()
+    for x, y in zip(a[:2], b[:2]):
+        assert torch.allclose(x, y, rtol=1e-4, atol=1e-4)
+    assert set(a[2]) == set(b[2])
+    for n in a[2]:
+        assert (a[2][n] - b[2][n]).norm() <= 1e-3 * b[2][n].norm() + 1e-6, n
+    with torch.no_grad():
+        assert torch.allclose(token_scores(model, batch)[0], a[0], atol=1e-5)
+
+
+def test_launches_counted():
+    from atomic_ai_hybrid_b200.utils.counters import LaunchCounter
+
+    c = LaunchCounter()
+    c.enable()
+    q, cache = torch.zeros(4, 128), torch.zeros(4, 1, 8, 64)
+
+    def count(L=1, cu=None, prefix=None, mass=None, rows=4):
+        c.reset()
+        c.add("cached_attention", (q[:rows], None, None, cache, cache, None, None, None, L, cu, None, prefix, None, mass, None, 1.0))
+        return c.count
+
+    some = torch.zeros(3, dtype=torch.int32)
+    assert count() == 3 and count(L=4) == 3 and count(L=5) == 5 and count(cu=some) == 5 and count(prefix=some) == 4
+    assert count(mass=some) == 4 and count(cu=some, mass=some) == 7 and count(prefix=some, mass=some) == 6
+    assert count(rows=0) == 0 and count(cu=some[:1]) == 0
