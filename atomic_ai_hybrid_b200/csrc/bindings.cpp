@@ -1976,8 +1976,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Te
   check_logits(logits, tokens, op);
   const int64_t R = logits.size(0), V = logits.size(1);
   TORCH_CHECK(top >= 0 && top <= 64 && top <= V, op, ": top must lie between 0 and 64 and the vocabulary, got ", top);
-  TORCH_CHECK(temperature > 0 && (float)temperature > 0.f && std::isfinite(1.f / (float)temperature) && std::isfinite((float)temperature),
-              op, ": temperature must be positive, with a finite reciprocal, got ", temperature);
+  TORCH_CHECK(temperature >= 1e-37 && temperature <= 1e37, op, ": temperature must lie between 1e-37 and 1e37, got ", temperature);
   const c10::cuda::CUDAGuard guard(logits.device());
   auto lp = new_output({R}, at::kFloat, logits), entropy = new_output({R}, at::kFloat, logits);
   auto stats = new_output({R, 4}, at::kFloat, logits);

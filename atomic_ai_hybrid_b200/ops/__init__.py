@@ -288,8 +288,8 @@ def token_logprobs(logits, tokens, top: int = 0, temperature: float = 1.0):
                          f"for {tuple(logits.shape)}")
     if not 0 <= top <= min(MAX_ALTERNATIVES, logits.shape[1]):
         raise ValueError(f"token_logprobs: top must lie between 0 and {min(MAX_ALTERNATIVES, logits.shape[1])}, got {top}")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"token_logprobs: temperature must be positive and finite, got {temperature}")
+    if not 1e-37 <= temperature <= 1e37:
+        raise ValueError(f"token_logprobs: temperature must lie between 1e-37 and 1e37, got {temperature}")
     if logits.is_cuda and _IMPL == "cuda":
         return _k().token_logprobs(logits, tokens, top, temperature)
     return R.token_logprobs(logits, tokens, top, temperature)

@@ -195,3 +195,15 @@ def score_truth(logits, tokens, top=0, temperature=1.0, g=None, ge=None):
         dx = g.double()[:, None] * (one - p * given[:, None]) - ge.double()[:, None] * (torch.xlogy(p, p) + p * entropy[:, None])
         out.append(torch.where(logp > -math.inf, dx, 0.0) / temperature)
     return out
+
+
+def extreme_scores(dtype, device):
+    """Logits with masked places, and logits near the type's largest: (logits, tokens, temperatures)."""
+    x = torch.randn(4, 5003, generator=torch.Generator().manual_seed(3)) * 3
+    x[0, :100] = -math.inf
+    x[1, ::7] = math.nan
+    x[2, 5:] = torch.finfo(dtype).min
+    y = torch.tensor([4000, 4001, 3, -100])
+    huge = torch.linspace(0, 2.9e38, 1000).roll(300)[None]
+    return [(x.to(dtype).to(device), y.to(device), T) for T in (1e-3, 1e-9, 1e-12)] + \
+        [(huge.to(dtype).to(device), y[2:3].to(device), T) for T in (1.0, 1e30, 1e37)]

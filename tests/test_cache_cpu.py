@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from atomic_ai_hybrid_b200 import ops
-from _cache import BF, F32, F64, attention_inputs, check_attention, copied, evict_truth, gen, score_truth
+from _cache import BF, F32, F64, attention_inputs, check_attention, copied, evict_truth, extreme_scores, gen, score_truth
 
 CPU = torch.device("cpu")
 
@@ -183,3 +183,15 @@ def test_launches_counted():
     assert count() == 3 and count(L=4) == 3 and count(L=5) == 5 and count(cu=some) == 5 and count(prefix=some) == 4
     assert count(mass=some) == 4 and count(cu=some, mass=some) == 7 and count(prefix=some, mass=some) == 6
     assert count(rows=0) == 0 and count(cu=some[:1]) == 0
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_plain_logprobs_extremes(dtype):
+    for x, y, T in extreme_scores(dtype, CPU):
+        out, want = ops.token_logprobs(x, y, top=3, temperature=T), score_truth(x, y, 3, T)
+        for i in (0, 1, 3):
+            assert torch.allclose(out[i].double(), want[i].clamp(min=torch.finfo(F32).min), rtol=3e-5, atol=3e-5), (T, i)
+        assert torch.equal(out[2], want[2])
+    for T in (1e-38, 1e38, -1.0):
+        with pytest.raises(ValueError, match="temperature"):
+            ops.token_logprobs(x, y, temperature=T)

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from atomic_ai_hybrid_b200 import ops
-from _cache import BF, F32, attention_inputs, check_attention, copied, evict_truth, gen, offsets, score_truth
+from _cache import BF, F32, attention_inputs, check_attention, copied, evict_truth, extreme_scores, gen, offsets, score_truth
 
 pytestmark = pytest.mark.gpu
 dev = "cuda"
@@ -552,3 +552,13 @@ def test_logprobs_refusals():
                             ("tokens", (x, y.cpu()), {}), ("unit channel stride", (x.repeat(1, 2)[:, ::2], y), {})]:
         with pytest.raises((RuntimeError, ValueError), match=match):
             ops.token_logprobs(*args, **kw)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_logprobs_extremes(dtype):
+    """Temperatures so small that a masked place's exponent would be infinite, and logits so large."""
+    for x, y, T in extreme_scores(dtype, dev):
+        _check_scores(x, y, 3, T, grad=False)
+        out = ops.token_logprobs(x.requires_grad_(), y, temperature=T)
+        dx, = torch.autograd.grad(out[0].sum() + out[1].sum(), [x])
+        assert dx.isfinite().all()
