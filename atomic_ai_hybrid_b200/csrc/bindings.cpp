@@ -1866,7 +1866,7 @@ torch::Tensor cached_attention(const torch::Tensor& q, const torch::Tensor& k, c
   const int64_t H = q.size(1) / D;
   TORCH_CHECK(T < (1ll << 30) && H < (1ll << 15) && T * H < (1ll << 31), op, ": sizes out of range");
   TORCH_CHECK(H <= 128 * Hk, op, ": at most 128 query heads can share a key head, got ", H / Hk);
-  TORCH_CHECK(std::isfinite(scale), op, ": sm_scale must be finite, got ", scale);
+  TORCH_CHECK(std::abs(scale) <= 1e28, op, ": sm_scale must lie between -1e28 and 1e28, got ", scale);
   check_rows(q, q, T, H * D, op, "q");
   check_rows(k, q, T, Hk * D, op, "k");
   check_rows(v, q, T, Hk * D, op, "v");
@@ -1951,6 +1951,7 @@ void cache_evict(const torch::Tensor& k_cache, const torch::Tensor& v_cache, con
     check_flat(*slots, k_cache, at::kInt, n, op, "slots");
   }
   TORCH_CHECK(n <= 65535, op, ": at most 65535 slots in one call, got ", n);
+  TORCH_CHECK(std::min(keep, M) * (row_bytes / 16) < (1ll << 30), op, ": a head's kept rows must lie below 16 GiB");
   if (keep >= M || n == 0) return;  // nothing holds more
   const c10::cuda::CUDAGuard guard(k_cache.device());
   auto work = new_output({ahb_cache_evict_bytes((int)n, (int)Hk, (int)M, (int)keep)}, at::kByte, k_cache);

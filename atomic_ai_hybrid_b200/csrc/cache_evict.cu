@@ -60,6 +60,11 @@ __global__ void __launch_bounds__(NT) evict_kernel(char* __restrict__ kc, char* 
   if ((unsigned)slot >= (unsigned)S) return;
   const int n = lengths[slot];
   if (n <= keep || n > M) return;
+  if (slots) {  // one given twice is the first one's
+    bool twice = false;
+    for (int i = tid; i < b; i += NT) twice |= slots[i] == slot;
+    if (__syncthreads_or(twice)) return;
+  }
   const int64_t newest = (int64_t)seen[slot] - recent, base = ((int64_t)slot * Hk + h) * M;
   float* ms = mass + base;
   int* hd = held + base;

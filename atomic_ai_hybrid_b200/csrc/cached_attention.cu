@@ -672,7 +672,7 @@ __global__ void __launch_bounds__(JW * 32) ca_join_tiles(const Args a) {
 }
 
 // ----------------------------------------------------------------------------- what every cache row was given
-// Of the row kernel's groups, from the scores that it has kept (1/16 of the cache's bytes at most; made again from the
+// Of the row kernel's groups, from the scores that it has kept (32 bytes a cache row, of its 4 D; made again from the
 // keys they took as long as the row kernel itself).  A warp goes through its share of the units; lane 4 r + k has query row r
 // and cache rows 4 k .. + 4.
 constexpr int MB = 12;  // blocks of ca_mass_rows on an SM

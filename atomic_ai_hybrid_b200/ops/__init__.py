@@ -223,7 +223,7 @@ def cached_attention(q, k, v, k_cache, v_cache, lengths, cos=None, sin=None, cu_
                      seen=None, mass=None, held=None, sm_scale: Optional[float] = None) -> torch.Tensor:
     """Attention of new tokens over a kept cache, into which their keys and values go first; no gradient.
 
-    ``q`` has ``H D`` channels, ``k`` and ``v`` have ``Hk D`` (query head ``h`` reads key head ``h // (H // Hk)``),
+    ``q`` has ``H D`` channels, ``k`` and ``v`` have ``Hk D`` (query head ``h`` reads key head ``h // (H // Hk)``; at most 128 share one),
     before rotation; tokens, ``cu_seqlens`` and ``slots`` as in ``selective_scan``.  ``k_cache`` and ``v_cache``
     ``(S, Hk, M, D)`` hold ``lengths[s]`` rows (int32) of slot ``s``.  Sequence ``i`` in slot ``s``::
 
@@ -252,7 +252,7 @@ def cached_attention(q, k, v, k_cache, v_cache, lengths, cos=None, sin=None, cu_
 def cache_evict(k_cache, v_cache, mass, held, lengths, seen, keep: int, recent: int = 0, slots=None) -> None:
     """Thins the cache of ``cached_attention`` out to ``keep`` rows per key head, in place; no gradient.
 
-    Of the ``lengths[s]`` rows of every slot ``s`` in ``slots`` (int32, all different; default all) those are kept whose
+    Of the ``lengths[s]`` rows of every slot ``s`` in ``slots`` (int32, one given twice counts once; default all) those are kept whose
     position ``held`` is at least ``seen[s] - recent`` (``recent <= keep``: the newest ones) and then those with the largest
     ``mass``, up to ``keep`` in all (ties: the lower row; NaN and ``-inf`` last).  Kept rows below ``keep`` stay where they are; the
     others fill the rows below ``keep`` that were given up, in the order of both, with their mass and position.  What

@@ -476,7 +476,7 @@ def cache_evict(k_cache, v_cache, mass, held, lengths, seen, keep, recent=0, slo
     """``ops.cache_evict`` head by head."""
     S, Hk, M, _ = k_cache.shape
     rows, at = lengths.tolist(), seen.tolist()
-    for slot in range(S) if slots is None else slots.tolist():
+    for slot in range(S) if slots is None else dict.fromkeys(slots.tolist()):
         if not 0 <= slot < S or not keep < rows[slot] <= M:
             continue
         n = rows[slot]

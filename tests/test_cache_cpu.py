@@ -195,3 +195,13 @@ def test_plain_logprobs_extremes(dtype):
     for T in (1e-38, 1e38, -1.0):
         with pytest.raises(ValueError, match="temperature"):
             ops.token_logprobs(x, y, temperature=T)
+
+
+def test_evict_slot_given_twice():
+    g = gen(0, CPU)
+    k, v = (torch.randn(3, 2, 40, 8, generator=g) for _ in range(2))
+    mass, held = torch.rand(3, 2, 40, generator=g), torch.arange(40, dtype=torch.int32).expand(3, 2, 40).contiguous()
+    n, seen = torch.full((3,), 40, dtype=torch.int32), torch.full((3,), 40, dtype=torch.int32)
+    want = evict_truth(k, v, mass, held, n, seen, 12, 4, torch.tensor([2, 0]))
+    ops.cache_evict(k, v, mass, held, n, seen, 12, recent=4, slots=torch.tensor([2, 0, 2, -1, 0], dtype=torch.int32))
+    assert all(torch.equal(a, b) for a, b in zip((k, v, mass, held), want))

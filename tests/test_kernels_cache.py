@@ -562,3 +562,38 @@ def test_logprobs_extremes(dtype):
         out = ops.token_logprobs(x.requires_grad_(), y, temperature=T)
         dx, = torch.autograd.grad(out[0].sum() + out[1].sum(), [x])
         assert dx.isfinite().all()
+
+
+@pytest.mark.parametrize("M", [300, 60000])
+def test_evict_slot_given_twice(M):
+    args = _evict_inputs(3, 2, M, 64, levels=40)
+    n, seen = torch.full((3,), M, dtype=torch.int32, device=dev), torch.full((3,), M, dtype=torch.int32, device=dev)
+    want = evict_truth(*args, n, seen, 100, 20, torch.tensor([2, 0]))
+    ops.cache_evict(*args, n, seen, 100, recent=20, slots=torch.tensor([2, 0, 2, 2, -1, 0], dtype=torch.int32, device=dev))
+    assert all(torch.equal(a, b) for a, b in zip(args, want))
+
+
+@pytest.mark.parametrize("D", [64, 96, 128])
+def test_attention_tables_between_boundaries(D):
+    """Rotation tables that start between 16-byte boundaries, for few and for many rows."""
+    a = attention_inputs([1, 40], [30, 20], 4, 2, D, BF, dev)
+    for name in ("cos", "sin"):
+        odd = torch.zeros(a[name].numel() + 1, device=dev)[1:].view(a[name].shape)
+        a[name] = odd.copy_(a[name])
+    check_attention(ops.cached_attention, a, HALF)
+
+
+def test_attention_refuses_too_many_heads():
+    a = attention_inputs([1], [3], 4, 2, 64, BF, dev)
+    a["q"] = torch.zeros(1, 2 * 129 * 64, device=dev, dtype=BF)
+    with pytest.raises((RuntimeError, ValueError), match="128 query heads"):
+        ops.cached_attention(**a)
+    a["q"] = torch.zeros(1, 256, device=dev, dtype=BF)
+    with pytest.raises((RuntimeError, ValueError), match="sm_scale"):
+        ops.cached_attention(**a, sm_scale=1e300)
+
+
+def test_attention_128_heads_share_one():
+    """The most query heads of one key head: single tokens, a prompt, a prefix."""
+    for lens, kept, kw in [([1, 1], [50, 7], {}), ([9], [100], {}), ([1, 3], [5, 6], dict(prefix=([70], [0, 0])))]:
+        check_attention(ops.cached_attention, attention_inputs(lens, kept, 128, 1, 64, BF, dev, **kw), HALF)
