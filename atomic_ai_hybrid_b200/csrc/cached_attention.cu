@@ -506,15 +506,16 @@ struct Joined {
       o[c].y = o[c].y * f + v[c].y * e;
     }
   }
-  // `count` results, `stride` apart: four at a time, so that their loads travel together
-  AHB_DEVICE void add(const float* y, int64_t stride, int count) {
+  // results k0 .. k1 where place(k) says, four at a time, so that their loads travel together
+  template <class F>
+  AHB_DEVICE void add(F place, int k0, int k1) {
     const int lane = threadIdx.x & 31;
-    for (int k0 = 0; k0 < count; k0 += 4) {
+    for (; k0 < k1; k0 += 4) {
       float2 ml[4], v[4][PL];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (k0 + k >= count) break;
-        const float* p = y + (k0 + k) * stride;
+        if (k0 + k >= k1) break;
+        const float* p = place(k0 + k);
         ml[k] = *reinterpret_cast<const float2*>(p + D);
 #pragma unroll
         for (int c = 0; c < PL; ++c)
@@ -522,7 +523,7 @@ struct Joined {
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (k0 + k < count) one(ml[k], v[k]);
+        if (k0 + k < k1) one(ml[k], v[k]);
     }
   }
   AHB_DEVICE void finish(const Args& a, int64_t out) const {
@@ -569,10 +570,10 @@ AHB_DEVICE Source source(const Args& a, const Group& g, int x, int at, int t) {
   return s;
 }
 
-// A token row and query heads h0, h0 + step .. below h1, one a warp (WIDE: head h0, its partial results spread over the
+// A token row and query heads h0 .. h1, by one warp (WIDE: head h0, its partial results spread over the
 // block's warps: where rows are few, every one is cut into many).  Nothing is done for what is final already.
 template <int D, bool WIDE>
-AHB_DEVICE void join_row(const Args& a, int t, int h0, int h1, int step) {
+AHB_DEVICE void join_row(const Args& a, int t, int h0, int h1) {
   const int warp = threadIdx.x >> 5, G = a.H / a.Hk;
   const int i = a.row_seq[t];
   if (i < 0) return;
@@ -585,34 +586,35 @@ AHB_DEVICE void join_row(const Args& a, int t, int h0, int h1, int step) {
     const int end = a.run_end[start];
     src[1] = source(a, a.groups[a.B + end], 1, end, t);
   }
-  for (int hq = h0; hq < h1; hq += step) {
+  for (int hq = h0; hq < h1; ++hq) {
     const int h = per_group(hq, G);
     const int64_t out = (int64_t)t * a.H + hq;
     Joined<D> sum;
-    bool done = false;
+    // the head's results one after another: of own rows, of the prefix's, each whole or from one worker after another
+    const float* from[2] = {nullptr, nullptr};
+    int64_t w0[2] = {0, 0}, slot[2] = {0, 0};
+    int count[2] = {0, 0}, late[2] = {0, 0};
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       if (x >= n) break;
       const Source& s = src[x];
       const int64_t first = s.base + h * s.per_head;
-      const int64_t w0 = div64(first, s.share), w1 = div64(first + s.units - 1, s.share);
-      if (w0 == w1) {
-        done = !a.full;
-        if (!done && (!WIDE || warp == 0)) sum.add(a.full + ((int64_t)x * a.T * a.H + out) * (D + 4), 0, 1);
-      } else {
-        const int64_t slot = (int64_t)s.rows * (D + 4);
-        const float* part = (s.tiles ? a.tile_part : a.part) + (int64_t)(s.row + hq - h * G) * (D + 4);
-        if (!WIDE || warp == 0) sum.add(part + (2 * w0 + (first >= w0 * s.share ? 1 : 0)) * slot, 0, 1);
-        const int more = (int)(w1 - w0);  // the others began before their worker's units
-        if (WIDE) {
-          const int each = (more + JW - 1) / JW, k0 = warp * each;
-          if (k0 < more) sum.add(part + 2 * (w0 + 1 + k0) * slot, 2 * slot, min(each, more - k0));
-        } else {
-          sum.add(part + 2 * (w0 + 1) * slot, 2 * slot, more);
-        }
-      }
+      w0[x] = div64(first, s.share);
+      count[x] = (int)(div64(first + s.units - 1, s.share) - w0[x]) + 1;
+      late[x] = first >= w0[x] * s.share;  // the first one's second result; the others began before their worker's units
+      slot[x] = (int64_t)s.rows * (D + 4);
+      from[x] = count[x] > 1 ? (s.tiles ? a.tile_part : a.part) + (int64_t)(s.row + hq - h * G) * (D + 4)
+                             : a.full + ((int64_t)x * a.T * a.H + out) * (D + 4);
     }
-    if (done) continue;
+    if (!a.full && count[0] == 1) continue;  // done
+    auto place = [&](int k) {
+      const bool x = k >= count[0];
+      const int j = x ? k - count[0] : k;
+      const int64_t at = 2 * ((x ? w0[1] : w0[0]) + j) + (j > 0 ? 0 : x ? late[1] : late[0]);
+      return (x ? from[1] : from[0]) + ((x ? count[1] : count[0]) > 1 ? at * (x ? slot[1] : slot[0]) : 0);
+    };
+    const int all = count[0] + count[1], each = WIDE ? (all + JW - 1) / JW : all, k0 = WIDE ? warp * each : 0;
+    sum.add(place, k0, min(all, k0 + each));
     if (WIDE) {
       constexpr int PL = Joined<D>::PL;
       __shared__ float2 sh[JW][PL + 1][32];
@@ -637,18 +639,19 @@ template <int D>
 __global__ void __launch_bounds__(JW * 32) ca_join_wide(const Args a) {
   next_may_start();
   after_previous();
-  join_row<D, true>(a, blockIdx.x, blockIdx.y, blockIdx.y + 1, 1);
+  join_row<D, true>(a, blockIdx.x, blockIdx.y, blockIdx.y + 1);
 }
-// `heads` query heads a block
+// A warp takes `heads` query heads of a token row: where its results lie costs more to look up than a head to join.
+constexpr int JB = 3;  // blocks on an SM
 template <int D>
-__global__ void __launch_bounds__(JW * 32, 3) ca_join(const Args a, int heads) {
+__global__ void __launch_bounds__(JW * 32, JB) ca_join(const Args a, int heads) {
   next_may_start();
   after_previous();
   if (!a.full && a.sums[ROWS][a.B] == 0) return;  // all is the tile kernel's
   const int per = (a.H + heads - 1) / heads;
-  for (int64_t x = blockIdx.x; x < (int64_t)a.T * per; x += gridDim.x) {
+  for (int64_t x = (int64_t)blockIdx.x * JW + (threadIdx.x >> 5); x < (int64_t)a.T * per; x += (int64_t)gridDim.x * JW) {
     const int t = (int)div64(x, per), h0 = (int)(x - (int64_t)t * per) * heads;
-    join_row<D, false>(a, t, h0 + (threadIdx.x >> 5), min(a.H, h0 + heads), JW);
+    join_row<D, false>(a, t, h0, min(a.H, h0 + heads));
   }
 }
 
@@ -665,8 +668,8 @@ __global__ void __launch_bounds__(JW * 32) ca_join_tiles(const Args a) {
     const int r = it.r0 + row, tt = per_group(r, G);
     const float* part = a.tile_part + (int64_t)row * (D + 4);
     Joined<D> sum;
-    sum.add(part + (2 * (int64_t)blockIdx.x + 1) * slot, slot, 2);  // and the next block's, right behind it
-    sum.add(part + 2 * ((int64_t)blockIdx.x + 2) * slot, 2 * slot, it.last - (int)blockIdx.x - 1);
+    // the block's second result, then the others' first ones
+    sum.add([&](int k) { return part + (2 * ((int64_t)blockIdx.x + k) + (k == 0 ? 1 : 0)) * slot; }, 0, it.last - (int)blockIdx.x + 1);
     sum.finish(a, (int64_t)(it.row0 + tt) * a.H + it.h * G + (r - tt * G));
   }
 }
@@ -819,13 +822,14 @@ int launch(const Args& a, cudaStream_t st) {
   if (a.blocks) ca_rows<D><<<a.warps / RW, RW * 32, 0, st>>>(a);
   else e = launch_after(ca_rows<D>, a.warps / RW, RW * 32, 0, st, a);
   const int sms = a.warps / (RB * RW);
-  // a block a row where there are rows enough: what its heads share is looked up once
-  const int heads = a.T > 4 * sms ? a.H : JW;
-  const int64_t rows = (int64_t)a.T * ((a.H + heads - 1) / heads);
+  // as many heads a warp as make four rounds of warps
+  const int64_t each = ((int64_t)a.T * a.H + 4 * sms * JB * JW - 1) / (4 * sms * JB * JW);
+  const int heads = each < a.H ? (int)each : a.H;
+  const int64_t blocks = ((int64_t)a.T * ((a.H + heads - 1) / heads) + JW - 1) / JW;
   auto then = [&](cudaError_t next) { e = e == cudaSuccess ? next : e; };
   if (a.blocks && !a.full) then(launch_after(ca_join_tiles<D>, dim3(a.blocks, 2 * TQ / 32), JW * 32, 0, st, a));
   if ((int64_t)a.T * a.H <= 4 * sms) then(launch_after(ca_join_wide<D>, dim3(a.T, a.H), JW * 32, 0, st, a));
-  else then(launch_after(ca_join<D>, (unsigned)(rows < 16 * sms ? rows : 16 * sms), JW * 32, 0, st, a, heads));
+  else then(launch_after(ca_join<D>, (unsigned)(blocks < 16 * sms ? blocks : 16 * sms), JW * 32, 0, st, a, heads));
   if (a.mass) {
     then(launch_after(ca_mass_rows, sms * MB, RW * 32, 0, st, a, sms * MB * RW));
     if (a.blocks) then(launch_after(ca_mass<D>, sms * 2, RW * 32, 0, st, a));
