@@ -4,17 +4,25 @@
 // An item is up to 256 query rows of one key head (two 128-row tiles) and the cache rows that they see, in blocks of
 // 64; every thread block gets the same number of units (64 cache rows against both tiles) and goes through them item
 // by item.  Per block of cache rows and tile:
-//   S = Q K^T (128 x 64, TMEM)  ->  P = 2^(S c - m), rounded to bf16 into the columns S came from  ->  O += P V (TMEM)
+//   S = Q K^T (128 x 64, TMEM)  ->  P = 2^(S c - m), rounded to bf16 (TMEM)  ->  O += P V (TMEM)
 // A thread owns a query row: maximum and sum need no exchange, and O is scaled only when a row's maximum has moved
-// by more than 2^8.  Each tile has two S buffers: the products P V and the next S of one run while the softmax works
-// on the other, and the two tiles' softmaxes share the exponential unit between them.  Where an item has
+// by more than 2^8.  The next S is made as soon as the softmax holds the last one in registers, P has two places of its own
+// (products of different shapes do not wait for one another: S must not come to where P V still reads), and the two tiles'
+// softmaxes share the exponential unit between them.  Where an item has
 // one tile only (a prefix under few tokens), the two sides take every other block of cache rows, and join at the end.
 //
-// Warps: 0 loads K and V by TMA into a ring of 16 KB buffers, 3 the tiles of queries, 1 and 2 issue the two sides' products (one thread for
-// both spent as long on its waits and commits as the tensor cores on the products: a prompt of 8192 tokens 780 us), 4-7 and 8-11 are
-// the sides' softmaxes.
-// With `mass` the queries' rounding remainder multiplies too (S += Qlo K^T), as sums of weights are kept in 32 bits; without it the
-// query is rounded to bf16 as P is, each by at most 2^-8, in no common direction.
+// Queries are multiplied as rounded to bf16 and, in as many products more, what the rounding left of them: rounded alone they move
+// every score by up to 2^-8 of its terms, and an output twice as far as its own rounding does (a prompt of 8192 tokens then takes
+// 402 us instead of 502).  P is rounded to bf16, each weight by at most 2^-8 in no common direction, which moves an output
+// about as far as its own rounding; the sums of weights are of those before it, in 32 bits.
+//
+// Warps: 0 loads K and V by TMA into a ring of three 32 KB buffers, 3 the tiles of queries, 1 and 2 issue the two sides' products
+// (one thread for both spent as long on its waits and commits as the tensor cores on the products, so a prompt of 8192 tokens
+// took twice as long), 4-7 and 8-11 are the sides' softmaxes.
+// A step of 64 cache rows and both tiles takes 2700 cycles.  The products need 2080 of them, as S (N = 64) is bound by what a
+// product reads from shared memory, 49 cycles where the tensor cores need 32; the exponentials need 1020.  (8192 tokens of 16 heads
+// of 128: 275 GFLOP in 430 us, the products of the remainders not counted.)  A second S buffer a side, with P in its place
+// and S waiting for P V, was slower (558 us in all): it brings the products into one order with the softmaxes.
 #include <cuda.h>
 #include "cached_attention.cuh"
 #include "launchers.h"
@@ -41,12 +49,9 @@ constexpr uint32_t HALF = 16 * 1024;  // a block of K or V: two 64-channel slabs
 constexpr uint32_t BUF = 2 * HALF;    // what a step multiplies: the K of its S, the V of its P
 constexpr int COL_P = 64, COL_O = 256;  // TMEM columns: side w's S at 128 w, its P buffer b at 128 w + 64 + 32 b, its O at 256 + 128 w
 
-constexpr uint32_t STAGE = 4 * 1024;  // a softmax warp's results on their way out
-
-template <bool EXACT>
-constexpr int ring() { return EXACT ? 2 : 4; }
-template <bool EXACT>
-constexpr size_t smem_bytes() { return (size_t)BUF * ring<EXACT>() + QBUF * (EXACT ? 4 : 2) + 8 * STAGE + 1024 + 2048; }
+constexpr uint32_t STAGE = 4 * 1024;  // a softmax warp's results on their way out, where the queries were
+constexpr int NB = 3;                 // buffers of the ring
+constexpr size_t SMEM_BYTES = (size_t)BUF * NB + QBUF * 4 + 1024 + 2048;  // all that a block can have
 
 struct Item {
   int pre, h, r0, rows, blocks, ks, ke;  // units ks .. ke of the item
@@ -207,20 +212,19 @@ struct RowsOut {
 // named barriers of the softmax warps: 1 both sides
 AHB_DEVICE void sides_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-template <int D, bool EXACT>
+template <int D>
 __global__ void __launch_bounds__(NTHR, 1)
     ca_tiles(const Args a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
              const __grid_constant__ CUtensorMap mq) {
   next_may_start();
   after_previous();
-  constexpr int NB = ring<EXACT>(), SLABS = (D + 63) / 64, DC = (D + 31) / 32;
+  constexpr int SLABS = (D + 63) / 64, DC = (D + 31) / 32;
   constexpr uint32_t SLAB = TK * 128, LOAD = SLABS * SLAB;
   extern __shared__ unsigned char raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  unsigned char* qs = smem;                               // tiles of queries (EXACT: rounded ones, then remainders)
-  unsigned char* kv = smem + QBUF * (EXACT ? 4 : 2);      // the ring
-  unsigned char* stage = kv + BUF * NB;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(stage + 8 * STAGE);
+  unsigned char* qs = smem;             // two tiles of rounded queries, then their remainders
+  unsigned char* kv = smem + QBUF * 4;  // the ring
+  uint64_t* bars = reinterpret_cast<uint64_t*>(kv + BUF * NB);
   // of side w: its steps are done (at 2 w, by turns), S is there, the softmax has taken it, with the P before it
   uint64_t *kv_full = bars, *kv_empty = bars + NB, *q_full = bars + 2 * NB, *q_empty = q_full + 2, *done = q_empty + 2, *s_full = done + 4,
            *taken = s_full + 2;
@@ -246,7 +250,7 @@ __global__ void __launch_bounds__(NTHR, 1)
       mbar_init(s_full + i, 1);
       mbar_init(taken + i, 4);  // a side's warps
       mbar_init(q_full + i, 1);
-      mbar_init(q_empty + i, 2);  // both sides' (a second tile: its side's twice)
+      mbar_init(q_empty + i, 4);  // the warps whose results went through it
     }
     *abort_flag = 0;
     sm100::fence_barrier_init();
@@ -315,9 +319,6 @@ __global__ void __launch_bounds__(NTHR, 1)
         if (it.two && w == 1) ok = ok && mbar_wait(q_full + 1, twos & 1, abort_flag, a.err, 64);
         ++items;
         twos += it.two;
-        // the tiles of queries that this side does not read, or does not read after its last score
-        if (w == 1 && ok && (it.two || cnt == 0)) mbar_arrive(q_empty);
-        if (w == 0 && ok && it.two) mbar_arrive(q_empty + 1);
         for (int j = -2; j < n0 && ok; ++j) {
           if (w == 1) pass(j);
           if (j < cnt && cnt > 0) {
@@ -335,11 +336,9 @@ __global__ void __launch_bounds__(NTHR, 1)
             if (j + 2 < cnt) {
 #pragma unroll
               for (int s = 0; s < D / 16; ++s) sm100::umma_bf16(t_w, umma::kdesc(q, TQ, s), umma::kdesc(k, TK, s), ID_S, s > 0);
-              if (EXACT) {
 #pragma unroll
                 for (int s = 0; s < D / 16; ++s)
                   sm100::umma_bf16(t_w, umma::kdesc(q + 2 * QBUF, TQ, s), umma::kdesc(k, TK, s), ID_S, 1);
-              }
               sm100::umma_commit(s_full + w);  // a completion is seen 500 cycles later: S is not to wait for P V
             }
             if (j >= 0) {
@@ -350,7 +349,6 @@ __global__ void __launch_bounds__(NTHR, 1)
             }
             sm100::umma_commit(done + 2 * w + ((nd + j) & 1));
             if (some) sm100::umma_commit(kv_empty + b);
-            if (j + 3 == cnt) sm100::umma_commit(q_empty + (it.two ? w : 0));
             n += some;
           }
           if (w == 0) pass(j);
@@ -363,7 +361,7 @@ __global__ void __launch_bounds__(NTHR, 1)
     uint32_t n[2] = {0, 0};
     bool ok = true;
     const int G = a.H / a.Hk;
-    const uint32_t bytes = a.tile_rows * 128 * SLABS * (EXACT ? 2 : 1);
+    const uint32_t bytes = a.tile_rows * 128 * SLABS * 2;
     while (at.u < at.u_end && ok) {
       const Item it = next_item(a, at);
       if (it.ke <= it.ks) break;
@@ -376,7 +374,7 @@ __global__ void __launch_bounds__(NTHR, 1)
           if (!ok) break;
           mbar_expect_tx(q_full + x, bytes);
 #pragma unroll
-          for (int e = 0; e < (EXACT ? 2 : 1); ++e)
+          for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int s = 0; s < SLABS; ++s)
               tma_load_4d(qs + (x + 2 * e) * QBUF + s * TQ * 128, &mq, q_full + x, 64 * s, e, it.h * G, t0 + x * tokens);
@@ -517,7 +515,7 @@ __global__ void __launch_bounds__(NTHR, 1)
       }
       if (ok && (w == 0 || it.two)) {
         const bool final = it.whole && !a.full, join = !it.two && it.count(1) > 0;
-        unsigned char* st = stage + (warp - 4) * STAGE;
+        unsigned char* st = qs + (it.two ? w : 0) * QBUF + quarter * STAGE;  // no score of the item is to come
         auto result = [&](int c, float* o) {  // 32 channels of the row
           tmem_get32(t_o + 32 * c, o);
           if (join) {
@@ -568,6 +566,11 @@ __global__ void __launch_bounds__(NTHR, 1)
             a.shared_items[blockIdx.x] = SharedItem{it.g.row0, it.r0, it.rows, it.h, (int)div64(it.u_last, share)};
         }
       }
+      if (w == 0 || it.two) {  // the next queries may come
+        umma::fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_empty + w);
+      }
       tc_fence_before();
       if (!it.two) sides_sync();  // the second side's O has been read
     }
@@ -605,16 +608,10 @@ int map_queries(CUtensorMap* m, const Args& a) {
              : -2;
 }
 
-template <int D, bool EXACT>
-int launch_one(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, cudaStream_t st) {
-  constexpr int bytes = (int)smem_bytes<EXACT>();
-  if (cudaFuncSetAttribute(ca_tiles<D, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -3;
-  return launch_after(ca_tiles<D, EXACT>, a.blocks, NTHR, bytes, st, a, mk, mv, mq) == cudaSuccess ? 0 : -4;
-}
-
 template <int D>
 int launch_dim(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, cudaStream_t st) {
-  return a.mass ? launch_one<D, true>(a, mk, mv, mq, st) : launch_one<D, false>(a, mk, mv, mq, st);
+  if (cudaFuncSetAttribute(ca_tiles<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES) != cudaSuccess) return -3;
+  return launch_after(ca_tiles<D>, a.blocks, NTHR, (int)SMEM_BYTES, st, a, mk, mv, mq) == cudaSuccess ? 0 : -4;
 }
 
 }  // namespace

@@ -11,6 +11,8 @@
 // almost every step: 2048 x 128256 logits 156 to 191 us).  Every thread keeps its largest logit: the k-th largest of 64
 // groups' is a bound that at least k logits reach, and only a thread whose own reaches it can hold one of them: the
 // shares of those few are read again, by all threads, and what reaches the bound is ranked by counting.
+// 2048 x 128256 bf16 logits with 8 alternatives take 138 us, 0.59 of the copy's rate, 62 % of the issue slots; 300 x 151936 fp32
+// 48 us.  Backward: one read and one write, 4096 x 50304 bf16 in 128 us, 0.94 of that rate; fp32 54 us.
 #include <cooperative_groups.h>
 #include "common.cuh"
 #include "launchers.h"
@@ -386,7 +388,7 @@ __global__ void __launch_bounds__(256) logprobs_bwd(const T* __restrict__ logits
 }
 
 // Few rows are cut for as many blocks as two an SM: a row alone on a block takes its 10 us however few there are (64 rows of
-// 50304 logits with 20 alternatives: 15.6 us whole, 12.3 with four blocks a row).  A part keeps 4096 logits at least.
+// 50304 logits with 5 alternatives: 15.6 us whole, 12.3 with four blocks a row).  A part keeps 4096 logits at least.
 template <typename T>
 int launch_fwd(const T* logits, int64_t ls, const int64_t* tokens, int64_t R, int V, int top, float c, float* lp, float* entropy,
                float4* stats, int64_t* top_tok, float* top_lp, cudaStream_t st) {

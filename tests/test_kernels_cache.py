@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from atomic_ai_hybrid_b200 import ops
-from _cache import BF, F32, attention_inputs, check_attention, copied, evict_truth, extreme_scores, gen, offsets, score_truth
+from _cache import BF, F32, attention_inputs, attention_truth, check_attention, copied, evict_truth, extreme_scores, gen, offsets, score_truth
 
 pytestmark = pytest.mark.gpu
 dev = "cuda"
@@ -597,3 +597,15 @@ def test_attention_128_heads_share_one():
     """The most query heads of one key head: single tokens, a prompt, a prefix."""
     for lens, kept, kw in [([1, 1], [50, 7], {}), ([9], [100], {}), ([1, 3], [5, 6], dict(prefix=([70], [0, 0])))]:
         check_attention(ops.cached_attention, attention_inputs(lens, kept, 128, 1, 64, BF, dev, **kw), HALF)
+
+
+@pytest.mark.parametrize("lens,kept,kw", [([900], [300], {}), ([300, 40, 1], [0, 10, 700], dict(prefix=([1500], [0, 0, 0]))),
+                                          ([1, 7], [1000, 1200], {})])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_loses_no_more_than_two_roundings(lens, kept, kw, D):
+    """Values in no common direction: the weights' rounding and the output's, each at most 2^-8 / sqrt(3) of the output on
+    average, add up to sqrt(2 / 3) 2^-8; queries, scores and sums keep 32 bits."""
+    a = attention_inputs(lens, kept, 8, 4, D, BF, dev, **kw)
+    o = attention_truth(**copied(a))[0]
+    y = ops.cached_attention(**copied(a)).double().reshape(o.shape)
+    assert (y - o).norm() <= (2 / 3) ** 0.5 * 2.0 ** -8 * o.norm(), float((y - o).norm() / o.norm())
