@@ -439,7 +439,8 @@ __global__ void __launch_bounds__(NTHR, 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[c + e]);
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale2;
-        if (__any_sync(0xffffffffu, top > m + SLACK)) {
+        // what lies in a tile's rows of no query (its heads times tokens do not fill 128) decides nothing
+        if (__any_sync(0xffffffffu, mine && top > m + SLACK)) {
           const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.f : ex2(m - mn);
           m = mn;
           l *= f;

@@ -609,3 +609,14 @@ def test_attention_loses_no_more_than_two_roundings(lens, kept, kw, D):
     o = attention_truth(**copied(a))[0]
     y = ops.cached_attention(**copied(a)).double().reshape(o.shape)
     assert (y - o).norm() <= (2 / 3) ** 0.5 * 2.0 ** -8 * o.norm(), float((y - o).norm() / o.norm())
+
+
+@pytest.mark.parametrize("H,Hk", [(99, 3), (14, 2), (6, 2), (40, 8)])
+def test_attention_repeats_where_heads_do_not_fill_a_tile(H, Hk):
+    """Rows of a tile that belong to no query hold what was there before: the same call, with other ones between, gives the same bits."""
+    a = attention_inputs([15, 1, 0, 6, 22, 200], [0, 0, 229, 408, 0, 31], H, Hk, 96, BF, dev, prefix=([119, 340], [-1, 1, 1, 0, -1, 1]), std=4.0)
+    b = attention_inputs([700], [100], 16, 4, 128, BF, dev, std=30.0, seed=1)
+    first, _ = check_attention(ops.cached_attention, a, HALF)
+    for _ in range(10):
+        ops.cached_attention(**copied(b))
+        assert torch.equal(ops.cached_attention(**copied(a)), first)
