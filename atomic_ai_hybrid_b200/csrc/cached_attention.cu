@@ -103,33 +103,33 @@ AHB_DEVICE void make_plan(const Args& a) {
       }
     }
     const bool live = s.n > 0, starts = live && s.pre >= 0 && before != s.pre, ends = live && s.pre >= 0 && after != s.pre;
-    const Group own{s.row0, live ? s.n : 0, s.slot, live ? s.have + s.n : 0, s.have};
-    Group run{0, 0, 0, 0, 0};
+    Group own{s.row0, live ? s.n : 0, s.slot, live ? s.have + s.n : 0, s.have, 0};
+    Group run{0, 0, 0, 0, 0, 0};
     if (a.prefix) {
       __syncthreads();
       const int64_t c = carry[2 * KINDS];
       const int64_t first = Max64()(c, block_scan(starts ? i : -1, sh, Max64()));
       if (ends) {
         const int row0 = a.cu ? min(max(a.cu[first], 0), a.T) : (int)first * a.L;
-        run = Group{row0, s.row0 + s.n - row0, s.pre, s.pre_rows, s.pre_rows};
+        run = Group{row0, s.row0 + s.n - row0, s.pre, s.pre_rows, s.pre_rows, 0};
         a.run_end[first] = i;
       }
       if (i < a.B) a.run_start[i] = live && s.pre >= 0 ? (int)first : -1;
       if (threadIdx.x == PT - 1) carry[2 * KINDS] = first;
     }
-    if (i < a.B) {
-      a.groups[i] = own;
-      a.groups[a.B + i] = run;
-    }
     for (int x = 0; x < (a.prefix ? 2 : 1); ++x) {
-      const Group& g = x ? run : own;
+      Group& g = x ? run : own;
       int64_t units[KINDS] = {0, 0, 0};
-      if (g.tokens > 0 && !is_tiles(a, g)) units[ROWS] = (int64_t)a.Hk * row_units(g);
+      if (g.tokens > 0 && !is_tiles(a, g)) {
+        g.per_head = row_units(g);
+        units[ROWS] = a.Hk * g.per_head;
+      }
       if (g.tokens > 0 && is_tiles(a, g)) {
         const int n = row_tiles(a, g);
-        for (int rt = 0; rt < n; ++rt) units[TILES] += tile_item(a, g, rt).units;
-        units[TILES] *= a.Hk;
+        for (int rt = 0; rt < n; ++rt) g.per_head += tile_item(a, g, rt).units;
+        units[TILES] = a.Hk * g.per_head;
       }
+      if (i < a.B) a.groups[x * a.B + i] = g;
       if (a.mass && !x && g.tokens > 0) units[TILES_MASS] = is_tiles(a, g) ? (int64_t)a.Hk * ceil_div(g.keys, 4 * KU) : 0;
       for (int k = 0; k < (x || !a.mass ? 2 : KINDS); ++k) {
         __syncthreads();
@@ -143,7 +143,11 @@ AHB_DEVICE void make_plan(const Args& a) {
   __syncthreads();
   if (threadIdx.x < KINDS && (threadIdx.x < 2 || a.mass)) {
     a.sums[threadIdx.x][a.B] = carry[threadIdx.x];
-    if (threadIdx.x < 2) a.sums[threadIdx.x][2 * a.B + 1] = carry[KINDS + threadIdx.x];
+    if (threadIdx.x < 2) {
+      a.sums[threadIdx.x][2 * a.B + 1] = carry[KINDS + threadIdx.x];
+      const int workers = threadIdx.x == TILES ? a.blocks : a.warps;
+      a.shares[threadIdx.x] = workers ? share_of(carry[threadIdx.x] + carry[KINDS + threadIdx.x], workers) : 0;
+    }
   }
 }
 
@@ -555,13 +559,11 @@ AHB_DEVICE Source source(const Args& a, const Group& g, int x, int at, int t) {
   s.tiles = is_tiles(a, g);
   const int64_t* own = a.sums[s.tiles ? TILES : ROWS];
   const int64_t* runs = own + a.B + 1;
-  const int64_t n_own = own[a.B], all = n_own + runs[a.B];
-  const int64_t u0 = x ? runs[at] : own[at], u1 = x ? runs[at + 1] : own[at + 1];
-  s.share = share_of(all, s.tiles ? a.blocks : a.warps);
-  s.base = (x ? n_own : 0) + u0;
+  s.share = a.shares[s.tiles ? TILES : ROWS];
+  s.base = x ? own[a.B] + runs[at] : own[at];
   s.row = (t - g.row0) * (a.H / a.Hk);
   s.rows = RT;
-  s.per_head = div64(u1 - u0, a.Hk);
+  s.per_head = g.per_head;
   s.units = s.per_head;
   if (s.tiles) {  // a token's rows are of one item
     const int rt = s.row / (2 * a.tile_rows);
@@ -605,7 +607,8 @@ AHB_DEVICE void join_row(const Args& a, int t, int h0, int h1) {
       const Source& s = src[x];
       const int64_t first = s.base + h * s.per_head;
       w0[x] = div64(first, s.share);
-      count[x] = (int)(div64(first + s.units - 1, s.share) - w0[x]) + 1;
+      const int64_t rest = first + s.units - 1 - w0[x] * s.share;  // mostly one or two workers
+      count[x] = rest < s.share ? 1 : rest < 2 * s.share ? 2 : 1 + (int)div64(rest, s.share);
       late[x] = first >= w0[x] * s.share;  // the first one's second result; the others began before their worker's units
       slot[x] = (int64_t)s.rows * (D + 4);
       from[x] = count[x] > 1 ? (s.tiles ? a.tile_part : a.part) + (int64_t)(s.row + hq - h * G) * (D + 4)
@@ -814,6 +817,7 @@ int64_t lay_out(Args& a, char* base) {
   a.lse = a.mass ? (float*)place(rows * 4) : nullptr;
   a.part = (float*)place((int64_t)2 * a.warps * RT * (a.D + 4) * 4);
   a.tile_part = (float*)place((int64_t)2 * a.blocks * 2 * TQ * (a.D + 4) * 4);
+  a.shares = (int64_t*)place(2 * 8);
   a.shared_items = (SharedItem*)place((int64_t)a.blocks * sizeof(SharedItem));
   a.full = a.prefix ? (float*)place(2 * rows * (a.D + 4) * 4) : nullptr;
   return at;

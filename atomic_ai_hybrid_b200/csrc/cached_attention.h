@@ -15,6 +15,7 @@ struct Group {
   int row0, tokens;  // packed token rows row0 .. row0 + tokens (tokens 0: nothing to do)
   int slot, keys;    // cache slot, rows of it that any token sees
   int before;        // token t sees rows j < min(keys, before + t + 1) (a prefix: before = keys)
+  int64_t per_head;  // units of a key head, in the kernel that takes the group
 };
 
 // Groups [0, B) are the sequences' own rows, [B, 2 B) the prefix runs, each at its last sequence.  Each group is worked on by one of
@@ -50,6 +51,7 @@ struct Args {
   float* part;                   // partial results of items that several warps share, two a warp
   float* tile_part;              // ... of items that several blocks share, two a block
   SharedItem* shared_items;      // (blocks)
+  int64_t* shares;               // units of a worker of the row kernel and of the tile kernel
   float* full;                   // (2, T, H, D + 4) whole results of own rows and of prefix rows, if there is a prefix
   int tile_rows;                 // query rows of a tile: as many tokens as fit into 128 rows, with their heads
   int warps, blocks;             // warps of the row kernel, blocks of the tile kernel (0: it is not launched)

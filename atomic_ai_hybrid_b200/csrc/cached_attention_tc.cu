@@ -90,9 +90,9 @@ AHB_DEVICE Item next_item(const Args& a, Place& p) {
     const int i = find_group(sums, a.B, v), lane = threadIdx.x & 31;
     p.x = pre ? a.B + i : i;
     it.g = a.groups[p.x];
-    const int64_t base = sums[i], per_head = div64(sums[i + 1] - base, a.Hk);
-    p.h = (int)div64(v - base, per_head);
-    int64_t rest = v - base - p.h * per_head;
+    const int64_t base = sums[i];
+    p.h = (int)div64(v - base, it.g.per_head);
+    int64_t rest = v - base - p.h * it.g.per_head;
     const int tiles = row_tiles(a, it.g);
     for (p.rt = 0;; p.rt += 32) {  // 32 tiles at a time
       const int64_t mine = p.rt + lane < tiles ? tile_item(a, it.g, p.rt + lane).units : 0;
