@@ -9,7 +9,7 @@
 // Kernels: ca_append rotates the new rows and writes the cache (one more block lays the work out as units of cache
 // rows); ca_tiles (cached_attention_tc.cu) takes groups of more than eight query rows, ca_rows the others; the ca_join kernels
 // join what several workers or the prefix contributed; the ca_mass kernels add up what every cache row was given.
-// A single token of one conversation is bound by three launches that wait for one another (12.3 us with 6 heads and 1000
+// A single token of one conversation is bound by three launches that wait for one another (13.3 us with 6 heads and 1000
 // rows); batches of tokens by the cache's bytes.
 #include "cached_attention.cuh"
 #include "launchers.h"
@@ -650,8 +650,8 @@ __global__ void __launch_bounds__(JW * 32) ca_join_wide(const Args a) {
   join_row<D, true>(a, blockIdx.x, blockIdx.y, blockIdx.y + 1);
 }
 // A warp takes `heads` query heads of a token row: where its results lie costs more to look up than a head to join.  Bound by
-// the latency of these look-ups: 2407 tokens of 16 heads, three or four partial results each, 44 us (a source after the
-// other 62).
+// instructions, 600 a row and head: 2407 tokens of 16 heads, three or four partial results each, 39 us (one result after the other
+// and all looked up by division 62).
 constexpr int JB = 3;  // blocks on an SM
 template <int D>
 __global__ void __launch_bounds__(JW * 32, JB) ca_join(const Args a, int heads) {
@@ -685,7 +685,7 @@ __global__ void __launch_bounds__(JW * 32) ca_join_tiles(const Args a) {
 }
 
 // ----------------------------------------------------------------------------- what every cache row was given
-// Bound by latency and the scores' bytes: 48 tokens of 32 heads over 200 to 4000 rows, 16 us beside the row kernel's 73.
+// Bound by latency and the scores' bytes: 48 tokens of 32 heads over 200 to 4000 rows, 14 us beside the row kernel's 73.
 // Of the row kernel's groups, from the scores that it has kept (32 bytes a cache row, of its 4 D; made again from the
 // keys they took as long as the row kernel itself).  A warp goes through its share of the units; lane 4 r + k has query row r
 // and cache rows 4 k .. + 4.

@@ -13,7 +13,7 @@
 //
 // Queries are multiplied as rounded to bf16 and, in as many products more, what the rounding left of them: rounded alone they move
 // every score by up to 2^-8 of its terms, and an output twice as far as its own rounding does (a prompt of 8192 tokens then takes
-// 402 us instead of 502).  P is rounded to bf16, each weight by at most 2^-8 in no common direction, which moves an output
+// 402 us instead of 508).  P is rounded to bf16, each weight by at most 2^-8 in no common direction, which moves an output
 // about as far as its own rounding; the sums of weights are of those before it, in 32 bits.
 //
 // Warps: 0 loads K and V by TMA into a ring of three 32 KB buffers, 3 the tiles of queries, 1 and 2 issue the two sides' products
@@ -21,7 +21,7 @@
 // took twice as long), 4-7 and 8-11 are the sides' softmaxes.
 // A step of 64 cache rows and both tiles takes 2700 cycles.  The products need 2080 of them, as S (N = 64) is bound by what a
 // product reads from shared memory, 49 cycles where the tensor cores need 32; the exponentials need 1020.  (8192 tokens of 16 heads
-// of 128: 275 GFLOP in 430 us, the products of the remainders not counted.)  A second S buffer a side, with P in its place
+// of 128: 275 GFLOP in 418 us, the products of the remainders not counted.)  A second S buffer a side, with P in its place
 // and S waiting for P V, was slower (558 us in all): it brings the products into one order with the softmaxes.
 #include <cuda.h>
 #include "cached_attention.cuh"
