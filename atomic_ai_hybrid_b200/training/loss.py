@@ -76,6 +76,6 @@ def token_scores(model, batch: Dict[str, torch.Tensor], temperature: float = 1.0
 
     h, y = hidden.reshape(-1, hidden.shape[-1]), labels.reshape(-1)
     parts = [ckpt.checkpoint(piece, h[s:s + chunk], y[s:s + chunk], w, use_reentrant=False) if torch.is_grad_enabled() else
-             piece(h[s:s + chunk], y[s:s + chunk], w) for s in range(0, h.shape[0], chunk)]
+             piece(h[s:s + chunk], y[s:s + chunk], w) for s in range(0, max(1, h.shape[0]), chunk)]
     lp, entropy = (torch.cat(t).view(labels.shape) for t in zip(*parts))
     return lp, entropy

@@ -205,3 +205,17 @@ def test_evict_slot_given_twice():
     want = evict_truth(k, v, mass, held, n, seen, 12, 4, torch.tensor([2, 0]))
     ops.cache_evict(k, v, mass, held, n, seen, 12, recent=4, slots=torch.tensor([2, 0, 2, -1, 0], dtype=torch.int32))
     assert all(torch.equal(a, b) for a, b in zip((k, v, mass, held), want))
+
+
+def test_token_scores_of_no_tokens():
+    from atomic_ai_hybrid_b200.training.loss import token_scores
+
+    class Nothing:
+        def __call__(self, ids, return_hidden):
+            return torch.zeros(*ids.shape, 8), []
+
+        def lm_weight(self):
+            return torch.zeros(30, 8)
+
+    ids = torch.zeros(0, 5, dtype=torch.long)
+    assert [tuple(t.shape) for t in token_scores(Nothing(), {"input_ids": ids, "labels": ids})] == [(0, 5), (0, 5)]
