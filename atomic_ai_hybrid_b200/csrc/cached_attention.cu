@@ -11,6 +11,7 @@
 // join what several workers or the prefix contributed; the ca_mass kernels add up what every cache row was given.
 // A single token of one conversation is bound by three launches that wait for one another (13.3 us with 6 heads and 1000
 // rows); batches of tokens by the cache's bytes.
+#include <cfloat>
 #include "cached_attention.cuh"
 #include "launchers.h"
 #include "mma.cuh"
@@ -861,7 +862,8 @@ int64_t ahb_cached_attention_bytes(const Args& args) {
 int ahb_cached_attention(const Args& args, void* work, cudaStream_t st) {
   Args a = args;
   a.negate = a.scale2 < 0.f;  // the queries take the scale's sign: the largest product is then the largest score
-  a.scale2 = a.scale2 < 0.f ? -a.scale2 : a.scale2;
+  // a masked score is -inf before it is scaled, and -inf times 0 is none: the least normal number gives the same weights
+  a.scale2 = fmaxf(a.scale2 < 0.f ? -a.scale2 : a.scale2, FLT_MIN);
   lay_out(a, (char*)work);
   const bool vec = (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.cos | (uintptr_t)a.sin) & 15) == 0 && ((a.qs | a.ks | a.vs) & 7) == 0;
   const int per = 1 + (a.T - 1) / (8 * sm_count()), blocks = 1 + (a.T + per - 1) / per;  // eight blocks an SM at most
