@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(RW * 32, RB) ca_rows(const Args a) {
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          s[x][e] = c * KU + 8 * x + 2 * t4 + e <= last ? s[x][e] * a.scale2 : -INFINITY;
+          s[x][e] = c * KU + 8 * x + 2 * t4 + e <= last ? __fmul_rn(s[x][e], a.scale2) : -INFINITY;  // rounded once, for the maximum and the weights
           mx = fmaxf(mx, s[x][e]);
         }
       if (a.mass && !pre && out >= 0) {  // for ca_mass_rows

@@ -398,7 +398,6 @@ __global__ void __launch_bounds__(NTHR, 1)
     auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
       return (bool)__all_sync(0xffffffffu, mbar_wait(bar, phase & 1, abort_flag, a.err, code));
     };
-    const float2 scale = both(a.scale2);
     while (at.u < at.u_end) {
       const Item it = next_item(a, at);
       if (it.ke <= it.ks) break;
@@ -418,6 +417,7 @@ __global__ void __launch_bounds__(NTHR, 1)
 #pragma unroll 1
       for (int j = 0; j < cnt && ok; ++j, ++ns) {
         const int k0 = it.block(w, j) * TK;
+        float2 scale = both(a.scale2);
         ok = wait(s_full + w, ns, 66);
         if (!ok) break;
         tc_fence_after();
@@ -460,6 +460,13 @@ __global__ void __launch_bounds__(NTHR, 1)
           }
         }
         const float2 neg = both(m == -INFINITY ? 0.f : -m);
+        // The product s c is exact in the sum and rounded in m: a weight is off by what that rounding took, the same factor in all of a
+        // row's and in their sum.  From |m| = 2^24 on it would be more than 2^1, and soon past 32 bits: there it is rounded before too.
+        if (__any_sync(0xffffffffu, mine && fabsf(neg.x) > 16777216.f)) {
+#pragma unroll
+          for (int c = 0; c < TK; ++c) s[c] = __fmul_rn(s[c], a.scale2);
+          scale = both(1.f);
+        }
         float2 sum[2] = {both(0.f), both(0.f)};
         uint32_t p[TK / 2];
 #pragma unroll

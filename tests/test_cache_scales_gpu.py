@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from atomic_ai_hybrid_b200 import ops
-from _cache import BF, attention_inputs, check_attention
+from _cache import BF, attention_inputs, attention_truth, check_attention, copied, gen
 
 pytestmark = pytest.mark.gpu
 dev = "cuda"
@@ -21,3 +21,31 @@ def test_scales_without_weight(lens, had, prefix, scale):
     a = attention_inputs(lens, had, 4, 2, 64, BF, dev, prefix=prefix, tracked=True)
     y, _ = check_attention(ops.cached_attention, {**a, "sm_scale": scale}, HALF)
     assert y.isfinite().all()
+
+
+def _whole_numbers(lens, had, prefix, seed=0):
+    """Queries and keys of small whole numbers: every score is one too, and exact in whatever order it is summed."""
+    a = attention_inputs(lens, had, 4, 2, 64, BF, dev, prefix=prefix, tracked=True, seed=seed, behind=0.0)
+    g = gen(seed, dev)
+    whole = lambda t: torch.randint(-3, 4, t.shape, generator=g, device=dev).to(BF)  # noqa: E731
+    return {**a, **{n: whole(a[n]) for n in ("q", "k", "k_cache")}, "cos": None, "sin": None}
+
+
+@pytest.mark.parametrize("lens,had,prefix", SHAPES)
+@pytest.mark.parametrize("scale", [1e4, 3e6, 1e9, -1e12, 1e28])
+def test_large_scales(lens, had, prefix, scale):
+    """Weights are one over the number of rows that have the largest score: values are weighed by bf16 numbers of at most half a step off
+    (2^-8), summed in 32 bits, and rounded once."""
+    a = {**_whole_numbers(lens, had, prefix), "sm_scale": scale}
+    o = attention_truth(**copied(a))[0]
+    y = ops.cached_attention(**copied(a)).double()
+    assert y.isfinite().all()
+    assert ((y - o).abs() <= 2 * HALF * (o.abs() + 1e-3)).all(), float((y - o).abs().max())
+
+
+@pytest.mark.parametrize("scale", [1e6, 1e9, 1e12])
+def test_large_scales_of_any_scores(scale):
+    """The largest score takes all: next to no two of a row's are within 32 bits of one another."""
+    for lens, had, prefix in SHAPES:
+        a = attention_inputs(lens, had, 4, 2, 64, BF, dev, prefix=prefix)
+        check_attention(ops.cached_attention, {**a, "cos": None, "sin": None, "sm_scale": scale}, HALF)
