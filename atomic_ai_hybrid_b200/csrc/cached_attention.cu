@@ -862,8 +862,9 @@ int64_t ahb_cached_attention_bytes(const Args& args) {
 int ahb_cached_attention(const Args& args, void* work, cudaStream_t st) {
   Args a = args;
   a.negate = a.scale2 < 0.f;  // the queries take the scale's sign: the largest product is then the largest score
-  // a masked score is -inf before it is scaled, and -inf times 0 is none: the least normal number gives the same weights
+  // A masked score is -inf before it is scaled, and -inf times 0 is none: the least normal number gives the same weights
   a.scale2 = fmaxf(a.scale2 < 0.f ? -a.scale2 : a.scale2, FLT_MIN);
+  a.rounded = a.scale2 * a.D * CLIP * CLIP > 268435456.f;  // queries and keys are clipped to CLIP
   lay_out(a, (char*)work);
   const bool vec = (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.cos | (uintptr_t)a.sin) & 15) == 0 && ((a.qs | a.ks | a.vs) & 7) == 0;
   const int per = 1 + (a.T - 1) / (8 * sm_count()), blocks = 1 + (a.T + per - 1) / per;  // eight blocks an SM at most

@@ -39,6 +39,10 @@ struct Args {
   int* held;
   float scale2;                  // sm_scale log2(e), without its sign
   bool negate;                   // the sign: the rotated queries are negated
+  // Exponents are s scale2 - m, in the tile kernel by one fused operation: the product is exact there and rounded in
+  // m, so that all of a row's weights and their sum carry one factor, up to 2^(half a step of m), and a quotient none.  Where scores can
+  // pass 2^28 that factor could leave 32 bits: there the product is rounded before too.
+  bool rounded;
   bf16* o;                       // (T, H, D)
   // workspace
   bf16* qw;                      // (T, H, 2, D) rotated queries rounded to bf16, and what the rounding left of them

@@ -212,7 +212,8 @@ struct RowsOut {
 // named barriers of the softmax warps: 1 both sides
 AHB_DEVICE void sides_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-template <int D>
+// ROUNDED: see Args::rounded
+template <int D, bool ROUNDED>
 __global__ void __launch_bounds__(NTHR, 1)
     ca_tiles(const Args a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
              const __grid_constant__ CUtensorMap mq) {
@@ -398,6 +399,7 @@ __global__ void __launch_bounds__(NTHR, 1)
     auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
       return (bool)__all_sync(0xffffffffu, mbar_wait(bar, phase & 1, abort_flag, a.err, code));
     };
+    const float2 scale = both(a.scale2);
     while (at.u < at.u_end) {
       const Item it = next_item(a, at);
       if (it.ke <= it.ks) break;
@@ -417,7 +419,6 @@ __global__ void __launch_bounds__(NTHR, 1)
 #pragma unroll 1
       for (int j = 0; j < cnt && ok; ++j, ++ns) {
         const int k0 = it.block(w, j) * TK;
-        float2 scale = both(a.scale2);
         ok = wait(s_full + w, ns, 66);
         if (!ok) break;
         tc_fence_after();
@@ -460,18 +461,14 @@ __global__ void __launch_bounds__(NTHR, 1)
           }
         }
         const float2 neg = both(m == -INFINITY ? 0.f : -m);
-        // The product s c is exact in the sum and rounded in m: a weight is off by what that rounding took, the same factor in all of a
-        // row's and in their sum.  From |m| = 2^24 on it would be more than 2^1, and soon past 32 bits: there it is rounded before too.
-        if (__any_sync(0xffffffffu, mine && fabsf(neg.x) > 16777216.f)) {
-#pragma unroll
-          for (int c = 0; c < TK; ++c) s[c] = __fmul_rn(s[c], a.scale2);
-          scale = both(1.f);
-        }
         float2 sum[2] = {both(0.f), both(0.f)};
         uint32_t p[TK / 2];
 #pragma unroll
         for (int e = 0; e < TK / 2; ++e) {
-          const float2 x = fma2(make_float2(s[2 * e], s[2 * e + 1]), scale, neg);
+          const float2 z = make_float2(s[2 * e], s[2 * e + 1]);
+          // (packed products and sums came out as one fused operation again)
+          const float2 x = ROUNDED ? make_float2(__fadd_rn(__fmul_rn(z.x, scale.x), neg.x), __fadd_rn(__fmul_rn(z.y, scale.y), neg.y))
+                                   : fma2(z, scale, neg);
           const float2 y = make_float2(ex2(x.x), ex2(x.y));
           sum[e & 1] = add2(sum[e & 1], y);
           p[e] = umma::pack_bf2(y.x, y.y);
@@ -618,8 +615,9 @@ int map_queries(CUtensorMap* m, const Args& a) {
 
 template <int D>
 int launch_dim(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, cudaStream_t st) {
-  if (cudaFuncSetAttribute(ca_tiles<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES) != cudaSuccess) return -3;
-  return launch_after(ca_tiles<D>, a.blocks, NTHR, (int)SMEM_BYTES, st, a, mk, mv, mq) == cudaSuccess ? 0 : -4;
+  auto kernel = a.rounded ? ca_tiles<D, true> : ca_tiles<D, false>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES) != cudaSuccess) return -3;
+  return launch_after(kernel, a.blocks, NTHR, (int)SMEM_BYTES, st, a, mk, mv, mq) == cudaSuccess ? 0 : -4;
 }
 
 }  // namespace
