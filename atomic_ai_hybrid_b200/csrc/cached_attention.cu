@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(RW * 32, RB) ca_rows(const Args a) {
       if (!final)
         *reinterpret_cast<float2*>((full ? full + out * (D + 4) : part + g * (D + 4)) + D) = make_float2(m, l);
       else if (a.lse)
-        a.lse[out] = m + log2f(l);
+        a.lse[out] = make_float2(m, inv);
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {  // rows 2 t4 and 2 t4 + 1
@@ -543,7 +543,7 @@ struct Joined {
     for (int c = 0; c < PL; ++c)
       if (64 * c + 2 * lane < D)
         *reinterpret_cast<uint32_t*>(a.o + out * D + 64 * c + 2 * lane) = pack2(o[c].x * inv, o[c].y * inv);
-    if (a.lse && lane == 0) a.lse[out] = m + log2f(l);
+    if (a.lse && lane == 0) a.lse[out] = make_float2(m, inv);
   }
 };
 
@@ -689,7 +689,8 @@ __global__ void __launch_bounds__(JW * 32) ca_join_tiles(const Args a) {
 // Bound by latency and the scores' bytes: 48 tokens of 32 heads over 200 to 4000 rows, 14 us beside the row kernel's 73.
 // Of the row kernel's groups, from the scores that it has kept (32 bytes a cache row, of its 4 D; made again from the
 // keys they took as long as the row kernel itself).  A warp goes through its share of the units; lane 4 r + k has query row r
-// and cache rows 4 k .. + 4.
+// and cache rows 4 k .. + 4.  A weight is 2^(s - m) / l, the softmax's own: with m + log2 l in one number large scores would round log2 l
+// away (at scores of 1e5 a token's weights came to 1.003 or 0.997).
 constexpr int MB = 12;  // blocks of ca_mass_rows on an SM
 __global__ void __launch_bounds__(RW * 32, MB) ca_mass_rows(const Args a, int warps) {
   next_may_start();
@@ -705,14 +706,14 @@ __global__ void __launch_bounds__(RW * 32, MB) ca_mass_rows(const Args a, int wa
     const int per_head = row_units(gr), h = (int)div64(u - units[i], per_head), c0 = (int)(u - units[i] - (int64_t)h * per_head);
     const int n = (int)min((int64_t)(per_head - c0), u_end - u);
     const bool in = r < gr.tokens * G;
-    const float lse = in ? a.lse[(int64_t)(gr.row0 + tt) * a.H + h * G + r - tt * G] : 0.f;
+    const float2 ml = in ? a.lse[(int64_t)(gr.row0 + tt) * a.H + h * G + r - tt * G] : make_float2(0.f, 0.f);
     float* m = a.mass + ((int64_t)gr.slot * a.Hk + h) * a.M;
 #pragma unroll 4
     for (int c = 0; c < n; ++c) {
       float4 p = make_float4(0.f, 0.f, 0.f, 0.f);
       if (in) {
         const float4 s = *reinterpret_cast<const float4*>(a.scores + (u + c) * RT * KU + lane * 4);
-        p = make_float4(ex2(s.x - lse), ex2(s.y - lse), ex2(s.z - lse), ex2(s.w - lse));
+        p = make_float4(ex2(s.x - ml.x) * ml.y, ex2(s.y - ml.x) * ml.y, ex2(s.z - ml.x) * ml.y, ex2(s.w - ml.x) * ml.y);
       }
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) {
@@ -730,10 +731,11 @@ __global__ void __launch_bounds__(RW * 32, MB) ca_mass_rows(const Args a, int wa
 }
 
 // Of the tile kernel's: a warp holds 64 cache rows and goes over the query rows that see them, eight at a time:
-// sum_t 2^(s_tj - lse_t).  Bound by the products, each query tile with its rounding remainders: a tracked prompt of 4000 tokens
+// sum_t 2^(s_tj - m_t) / l_t.  The scores are summed in another order than the tile kernel's, which moves a weight by some 2^-22 of its
+// row's largest score: next to nothing at scores of tens, 2 % at 1e5; more than the query rows that see a cache row it never gathers.  Bound by the products, each query tile with its rounding remainders: a tracked prompt of 4000 tokens
 // takes 673 us in all, under 200 untracked (16 cache rows a warp: 1017).
 constexpr int KM = 4;  // units of 16 cache rows that a warp holds
-template <int D>
+template <int D, bool ROUNDED>
 __global__ void __launch_bounds__(RW * 32, 2) ca_mass(const Args a) {
   next_may_start();
   after_previous();
@@ -755,7 +757,7 @@ __global__ void __launch_bounds__(RW * 32, 2) ca_mass(const Args a) {
     for (int r0 = max(0, j0 - gr.before) * G / RT * RT; r0 < rows; r0 += RT) {
       const int r = r0 + g, tt = per_group(r, G);
       const int64_t out = (int64_t)(gr.row0 + tt) * a.H + h * G + (r - tt * G);
-      const float lse = r < rows ? a.lse[out] : 0.f;
+      const float2 ml = r < rows ? a.lse[out] : make_float2(0.f, 0.f);
       const int last = r < rows ? gr.before + tt : -1;
       uint32_t qa[D / 16][4];
       load_q<D>(qa, r < rows ? a.qw + out * 2 * D : nullptr, t4);
@@ -767,7 +769,7 @@ __global__ void __launch_bounds__(RW * 32, 2) ca_mass(const Args a) {
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (j0 + y * KU + 8 * x + 2 * t4 + e <= last) sum[y][x][e] += ex2(s[x][e] * a.scale2 - lse);
+            if (j0 + y * KU + 8 * x + 2 * t4 + e <= last) sum[y][x][e] += ex2(ROUNDED ? __fadd_rn(__fmul_rn(s[x][e], a.scale2), -ml.x) : __fmaf_rn(s[x][e], a.scale2, -ml.x)) * ml.y;
       }
     }
 #pragma unroll
@@ -780,7 +782,7 @@ __global__ void __launch_bounds__(RW * 32, 2) ca_mass(const Args a) {
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
           const int j = j0 + y * KU + 8 * x + 2 * t4 + e;
-          if (g == 0 && j < gr.keys) a.mass[((int64_t)gr.slot * a.Hk + h) * a.M + j] += v;
+          if (g == 0 && j < gr.keys) a.mass[((int64_t)gr.slot * a.Hk + h) * a.M + j] += fminf(v, (float)rows);
         }
   }
 }
@@ -815,7 +817,7 @@ int64_t lay_out(Args& a, char* base) {
   a.run_end = (int*)place((int64_t)a.B * 4);
   for (int k = 0; k < (a.mass ? KINDS : 2); ++k) a.sums[k] = (int64_t*)place((int64_t)2 * (a.B + 1) * 8);
   a.scores = a.mass ? (float*)place((int64_t)a.B * a.Hk * ((a.M + KU - 1) / KU) * RT * KU * 4) : nullptr;
-  a.lse = a.mass ? (float*)place(rows * 4) : nullptr;
+  a.lse = a.mass ? (float2*)place(rows * 8) : nullptr;
   a.part = (float*)place((int64_t)2 * a.warps * RT * (a.D + 4) * 4);
   a.tile_part = (float*)place((int64_t)2 * a.blocks * 2 * TQ * (a.D + 4) * 4);
   a.shares = (int64_t*)place(2 * 8);
@@ -846,7 +848,7 @@ int launch(const Args& a, cudaStream_t st) {
   else then(launch_after(ca_join<D>, (unsigned)(blocks < 16 * sms ? blocks : 16 * sms), JW * 32, 0, st, a, heads));
   if (a.mass) {
     then(launch_after(ca_mass_rows, sms * MB, RW * 32, 0, st, a, sms * MB * RW));
-    if (a.blocks) then(launch_after(ca_mass<D>, sms * 2, RW * 32, 0, st, a));
+    if (a.blocks) then(launch_after(a.rounded ? ca_mass<D, true> : ca_mass<D, false>, sms * 2, RW * 32, 0, st, a));
   }
   if (e != cudaSuccess) return -4;
   return 0;

@@ -31,7 +31,6 @@ constexpr int TK = 64;    // tile kernel: cache rows of a block
 constexpr int TQ = 128;   // ... rows of a tensor-core tile, a.tile_rows of them used; an item has one or two tiles
 constexpr float CLIP = 1e3f;
 constexpr float SLACK = 8.f;  // the running maximum moves when a score passes it by more than 2^8: p <= 256, and no sum nears overflow
-
 AHB_DEVICE int ceil_div(int a, int b) { return (a + b - 1) / b; }
 // a / b of non-negative numbers that are seldom past 32 bits
 AHB_DEVICE int64_t div64(int64_t a, int64_t b) {

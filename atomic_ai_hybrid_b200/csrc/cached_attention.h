@@ -39,7 +39,7 @@ struct Args {
   int* held;
   float scale2;                  // sm_scale log2(e), without its sign
   bool negate;                   // the sign: the rotated queries are negated
-  // Exponents are s scale2 - m, in the tile kernel by one fused operation: the product is exact there and rounded in
+  // Exponents are s scale2 - m, in the tile kernel and for its masses by one fused operation: the product is exact there and rounded in
   // m, so that all of a row's weights and their sum carry one factor, up to 2^(half a step of m), and a quotient none.  Where scores can
   // pass 2^28 that factor could leave 32 bits: there the product is rounded before too.
   bool rounded;
@@ -51,7 +51,7 @@ struct Args {
   int *run_start, *run_end;      // a sequence's run: its first sequence (-1: no prefix), and that one's last
   int64_t* sums[KINDS];          // (2 B + 1) each
   float* scores;                 // the row kernel's, unit by unit (8 query rows of 16 cache rows), for mass
-  float* lse;                    // (T, H) log2 of the softmax's denominators, for mass
+  float2* lse;                   // (T, H) the softmax's maximum, as an exponent of 2, and one over its denominator, for mass
   float* part;                   // partial results of items that several warps share, two a warp
   float* tile_part;              // ... of items that several blocks share, two a block
   SharedItem* shared_items;      // (blocks)

@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(NTHR, 1)
             }
             rows.write(st, v, reinterpret_cast<unsigned char*>(a.o + 32 * c), D * 2);
           }
-          if (mine && a.lse) a.lse[out] = m + log2f(l);
+          if (mine && a.lse) a.lse[out] = make_float2(m, inv);
         } else {
           // among whole results, or among this block's partial ones
           float* y = it.whole ? a.full + (int64_t)(it.pre ? a.T : 0) * a.H * (D + 4)
