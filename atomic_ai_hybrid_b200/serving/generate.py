@@ -138,9 +138,10 @@ class Generator:
                 buf["tokens"].copy_(t.clamp(min=0))
                 return t, lp
 
-            # warm up and capture on a copy of what the step changes
+            # Warm up and capture on a copy of what the step changes.  Both runs count as a conversation's first token on the host, so that
+            # neither asks for room or cuts anything back; where the device's own counts leave no room, the warm-up's tokens are padding.
             st = self.state
-            st.cut_back(st.check_room(slots, [1] * B))  # outside the graph: the step itself then finds room
+            st.check_room(slots, [1] * B)
             changed = [c[n] for c in st.layers.values() for n in ("conv", "state", "mass", "held") if n in c]
             changed += [st.rows_dev, st.seen_dev] if st.has_mla else []
             kept = [t.clone() for t in changed]
@@ -149,9 +150,11 @@ class Generator:
             side.wait_stream(torch.cuda.current_stream(dev))
             graph = torch.cuda.CUDAGraph()
             try:
+                st.lengths, st.rows = [0] * st.slots, [0] * st.slots
                 with torch.cuda.stream(side):
                     run()
                 torch.cuda.current_stream(dev).wait_stream(side)
+                st.lengths, st.rows = [0] * st.slots, [0] * st.slots
                 with torch.cuda.graph(graph, pool=self._pool, stream=side):
                     buf["out"] = run()
             finally:
