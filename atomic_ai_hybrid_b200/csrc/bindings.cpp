@@ -475,25 +475,51 @@ int num_sms() {
   return n;
 }
 
+// Where a wait that runs out in a kernel leaves its code: one word a device, made at the first call there.
+struct ErrWords {
+  std::mutex m;
+  std::map<int, torch::Tensor> of;
+};
+ErrWords& err_words() {
+  static ErrWords* w = new ErrWords;  // never freed: kernels may outlive the process's other statics
+  return *w;
+}
+
+// The word of the current device.  Memory of its own, made beside a capture that may be running: a captured zero would clear it at every
+// replay, and the graph's memory goes with the graph.
 torch::Tensor& err_word() {
-  static torch::Tensor e;
-  if (!e.defined()) e = torch::zeros({1}, torch::dtype(torch::kInt32).device(torch::kCUDA));
+  int dev = 0;
+  C10_CUDA_CHECK(cudaGetDevice(&dev));
+  ErrWords& words = err_words();
+  std::lock_guard<std::mutex> lock(words.m);
+  torch::Tensor& e = words.of[dev];
+  if (!e.defined()) {
+    c10::cuda::CUDAStreamCaptureModeGuard beside(cudaStreamCaptureModeRelaxed);
+    void* p = nullptr;
+    cudaStream_t st = nullptr;
+    C10_CUDA_CHECK(cudaMalloc(&p, sizeof(int)));
+    C10_CUDA_CHECK(cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking));
+    C10_CUDA_CHECK(cudaMemsetAsync(p, 0, sizeof(int), st));
+    C10_CUDA_CHECK(cudaStreamSynchronize(st));
+    C10_CUDA_CHECK(cudaStreamDestroy(st));
+    e = torch::from_blob(p, {1}, torch::dtype(torch::kInt32).device(torch::kCUDA, dev));
+  }
   return e;
 }
 
-// the error word of kernels that run on any device: err_word() on its own one
-torch::Tensor& err_word_on(const torch::Device& device) {
-  static std::mutex m;
-  static std::map<int, torch::Tensor> words;
-  std::lock_guard<std::mutex> lock(m);
-  torch::Tensor& e = words[device.index()];
-  if (!e.defined())
-    e = err_word().device() == device ? err_word() : torch::zeros({1}, torch::dtype(torch::kInt32).device(device));
-  return e;
+// the first code that a device's word holds, of all devices
+int64_t gemm_error() {
+  ErrWords& words = err_words();
+  std::lock_guard<std::mutex> lock(words.m);
+  for (auto& w : words.of)
+    if (const int code = w.second.item<int>()) return code;
+  return 0;
 }
-
-int64_t gemm_error() { return err_word().item<int>(); }
-void gemm_error_reset() { err_word().zero_(); }
+void gemm_error_reset() {
+  ErrWords& words = err_words();
+  std::lock_guard<std::mutex> lock(words.m);
+  for (auto& w : words.of) w.second.zero_();
+}
 
 void gemm_check(int rc, const char* what) { TORCH_CHECK(rc == 0, "moe_gemm (", what, ") setup failed: code ", rc); }
 
@@ -1924,7 +1950,7 @@ torch::Tensor cached_attention(const torch::Tensor& q, const torch::Tensor& k, c
   a.D = (int)D;
   a.scale2 = (float)(scale * 1.4426950408889634);
   a.o = (ahb::cattn::bf16*)o.data_ptr();
-  a.err = err_word_on(q.device()).data_ptr<int>();
+  a.err = err_word().data_ptr<int>();
   auto work = new_output({ahb_cached_attention_bytes(a)}, at::kByte, q);
   const int rc = ahb_cached_attention(a, work.data_ptr(), cur_stream());
   TORCH_CHECK(rc == 0, op, ": failed with code ", rc, " for head dim ", D);

@@ -846,8 +846,17 @@ def moe_forward(flat, top_idx, gate, w1, w2, w3, shared, act):
 
 
 def gemm_error() -> int:
-    """Error word of the tcgen05 kernels (0 = no timed-out wait since the last reset)."""
+    """Error word of the kernels that wait (0: no wait ran out since the last reset), of every device that they ran on.  It is
+    read behind the current stream's work: wait for other streams first."""
     return int(ext().gemm_error())
+
+
+def check_waits() -> None:
+    """Raises where a kernel gave up waiting since the last check: what it was to write is not there."""
+    code = gemm_error()
+    if code:
+        ext().gemm_error_reset()
+        raise RuntimeError(f"a kernel gave up a wait (code {code}): results since the last check are not valid, nor the conversations behind them")
 
 
 def newton_schulz3(g, steps: int = 3, eps: float = 1e-4):

@@ -167,6 +167,12 @@ class Generator:
         self._graphs[key] = graph, buf
         return graph, buf
 
+    def _check_waits(self) -> None:
+        """Where the host has waited for the device anyway: no answers from kernels that gave up (``prefill`` and ``step`` do not wait)."""
+        if self.device.type == "cuda" and ops.get_impl() == "cuda":
+            from ..ops import kernels as K
+            K.check_waits()
+
     # ------------------------------------------------------------ scores
     def _check_prompts(self, prompts, prefix) -> None:
         room = self.state.slots - (prefix is not None)
@@ -210,6 +216,7 @@ class Generator:
         for a in range(0, max(1, len(rows)), step):
             logits = self._logits(h[rows[a:a + step]])
             parts.append([t.tolist() for t in ops.token_logprobs(logits, tokens[a:a + step], top=top, temperature=temperature)])
+        self._check_waits()
         names = ("logprobs", "entropy", "top_tokens", "top_logprobs")[:len(parts[0])]
         flat = [sum(p, []) for p in zip(*parts)]
         return {name: [v[a:e] for a, e in zip([0] + counts[:-1], counts)] for name, v in zip(names, flat)}
@@ -263,6 +270,7 @@ class Generator:
             done = done | (t < 0) | (t == stop_token) if stop_token is not None else done | (t < 0)
         tokens = torch.stack([s[0] for s in steps], 1).tolist()
         logprobs = torch.stack([s[1] for s in steps], 1).tolist()
+        self._check_waits()
         for ts, ls in zip(tokens, logprobs):
             end = next((i + (x >= 0) for i, x in enumerate(ts) if x < 0 or x == stop_token), len(ts))
             del ts[end:], ls[end:]
