@@ -60,22 +60,61 @@ def compute_loss(model, batch: Dict[str, torch.Tensor], deterministic: bool = Fa
     return total, info
 
 
-def token_scores(model, batch: Dict[str, torch.Tensor], temperature: float = 1.0, chunk: int = 2048):
-    """``(logprobs, entropy)``, fp32 and shaped like ``batch["labels"]``: the log-probability of every label under the model and the entropy of
-    the distribution that it is drawn from, with gradients (``ops.token_logprobs``), for objectives on the answers themselves
-    (preference pairs, policy gradients).  Labels of -100 have log-probability 0 and no gradient.  As in ``compute_loss`` the logits are made
-    ``chunk`` tokens at a time and again in the backward; they are rounded to the hidden states' type."""
-    import torch.utils.checkpoint as ckpt
+class _HeadScores(torch.autograd.Function):
+    """``ops.token_logprobs`` of ``h @ weight^T``, whose logits exist for ``chunk`` rows at a time, in the backward again.  The
+    weight's gradient is summed over all rows in fp32, in the parameter's accumulator where it has one, and else rounded once."""
 
+    @staticmethod
+    def forward(ctx, h, labels, weight, temperature, chunk):
+        ctx.save_for_backward(h, labels)
+        ctx.weight, ctx.temperature, ctx.chunk = weight, temperature, chunk
+        w = weight.to(h.dtype)
+        parts = [ops.token_logprobs(h[s:s + chunk] @ w.t(), labels[s:s + chunk], temperature=temperature)
+                 for s in range(0, max(1, h.shape[0]), chunk)]
+        return tuple(torch.cat(t) for t in zip(*parts))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, ge):
+        h, labels = ctx.saved_tensors
+        weight, chunk = ctx.weight, ctx.chunk
+        w = weight.detach().to(h.dtype)
+        dh = torch.empty_like(h) if ctx.needs_input_grad[0] else None
+        direct = sums = None
+        if ctx.needs_input_grad[2]:
+            direct = getattr(weight, "_ahb_grad_acc", None)
+            own = direct is None or direct.dtype != torch.float32
+            sums = torch.zeros(weight.shape, dtype=torch.promote_types(h.dtype, torch.float32), device=h.device) if own else direct.view(weight.shape)
+        for s in range(0, h.shape[0], chunk):
+            hc = h[s:s + chunk]
+            with torch.enable_grad():
+                logits = (hc @ w.t()).detach().requires_grad_()
+                out = ops.token_logprobs(logits, labels[s:s + chunk], temperature=ctx.temperature)
+            d, = torch.autograd.grad(out, [logits], [g[s:s + chunk], ge[s:s + chunk]])
+            if dh is not None:
+                torch.mm(d, w, out=dh[s:s + chunk])
+            if sums is None:
+                continue
+            if ops.use_cuda(h) and h.dtype == torch.bfloat16 and sums.dtype == torch.float32:
+                from ..ops import kernels as K
+                K._wgrad_acc(sums, d, hc)
+            else:
+                sums.addmm_(d.t().to(sums.dtype), hc.to(sums.dtype))
+        dw = None
+        if sums is not None and direct is None:
+            dw = sums.to(weight.dtype)
+        elif sums is not None and direct.dtype != torch.float32:
+            direct.view(weight.shape).add_(sums)
+        return dh, None, dw, None, None
+
+
+def token_scores(model, batch: Dict[str, torch.Tensor], temperature: float = 1.0, chunk: int = 2048):
+    """``(logprobs, entropy)``, fp32 and shaped like ``batch["labels"]`` (under tensor or context parallelism like the rank's shard of them):
+    the log-probability of every label under the model and the entropy of the distribution that it is drawn from, with
+    gradients (``ops.token_logprobs``), for objectives on the answers themselves (preference pairs, policy gradients).  Labels of -100
+    have log-probability 0 and no gradient.  As in ``compute_loss`` the logits are made ``chunk`` tokens at a time and again in
+    the backward, and the head's gradient is summed in fp32; logits are rounded to the hidden states' type, and so are their gradients."""
     hidden, _ = model(batch["input_ids"], return_hidden=True)
     labels = model.token_shard(batch["labels"]) if hasattr(model, "token_shard") else batch["labels"]
-    w = model.lm_weight()
-
-    def piece(h, y, w):
-        return ops.token_logprobs(h @ w.to(h.dtype).t(), y, temperature=temperature)
-
-    h, y = hidden.reshape(-1, hidden.shape[-1]), labels.reshape(-1)
-    parts = [ckpt.checkpoint(piece, h[s:s + chunk], y[s:s + chunk], w, use_reentrant=False) if torch.is_grad_enabled() else
-             piece(h[s:s + chunk], y[s:s + chunk], w) for s in range(0, max(1, h.shape[0]), chunk)]
-    lp, entropy = (torch.cat(t).view(labels.shape) for t in zip(*parts))
-    return lp, entropy
+    lp, entropy = _HeadScores.apply(hidden.reshape(-1, hidden.shape[-1]), labels.reshape(-1), model.lm_weight(), temperature, chunk)
+    return lp.view(labels.shape), entropy.view(labels.shape)
