@@ -482,10 +482,10 @@ def cache_evict(k_cache, v_cache, mass, held, lengths, seen, keep, recent=0, slo
         n = rows[slot]
         gathered = mass[slot, :, :n]
         low = torch.isnan(gathered) | (gathered == -math.inf)
-        rank = torch.where(held[slot, :, :n].long() >= at[slot] - recent, math.inf,
-                           torch.where(low, -math.inf, gathered.clamp(max=torch.finfo(gathered.dtype).max)))
-        order = torch.sort(rank, dim=-1, descending=True, stable=True).indices
-        kept = torch.zeros(rank.shape, dtype=torch.bool, device=rank.device).scatter_(-1, order[:, :keep], True)
+        newest = held[slot, :, :n].long() >= at[slot] - recent
+        order = torch.sort(torch.where(newest | low, -math.inf, gathered), dim=-1, descending=True, stable=True).indices
+        order = order.gather(1, torch.sort(newest.gather(1, order).int(), dim=-1, descending=True, stable=True).indices)
+        kept = torch.zeros_like(newest).scatter_(-1, order[:, :keep], True)
         h, hole = torch.nonzero(~kept[:, :keep], as_tuple=True)
         row = torch.nonzero(kept[:, keep:], as_tuple=True)[1] + keep
         for t in (k_cache, v_cache, mass, held):
