@@ -88,14 +88,17 @@ class Generator:
     def _read(self, prompts: Sequence[Sequence[int]], slots: List[int], fresh: bool):
         """The hidden rows of ``prompts``, packed, and where each one's last row is."""
         lens = [len(p) for p in prompts]
-        ids = torch.cat([torch.as_tensor(p, dtype=torch.long) for p in prompts])
-        if ids.numel() and not 0 <= int(ids.min()) <= int(ids.max()) < self.model.cfg.vocab_size:
-            raise ValueError(f"prompts need token ids of the vocabulary, [0, {self.model.cfg.vocab_size})")
-        ids = ids.to(self.device)
+        ids = self._ids(prompts).to(self.device)
         with serving(self.state, slots, lens, fresh=fresh) as call:
             h, _ = self.model(ids[None])
             last = call.cu[1:].long() - 1
         return h[0], last
+
+    def _ids(self, prompts: Sequence[Sequence[int]]) -> torch.Tensor:
+        ids = torch.cat([torch.as_tensor(p, dtype=torch.long) for p in prompts])
+        if ids.numel() and not 0 <= int(ids.min()) <= int(ids.max()) < self.model.cfg.vocab_size:
+            raise ValueError(f"prompts need token ids of the vocabulary, [0, {self.model.cfg.vocab_size})")
+        return ids
 
     def fork(self, source: int, slots: List[int]) -> None:
         """Makes the conversations in ``slots`` new ones that go on from the one in ``source`` (``DecodeState.fork``)."""
@@ -181,6 +184,14 @@ class Generator:
         if any(len(p) == 0 for p in prompts) or prefix is not None and len(prefix) == 0:
             raise ValueError("a prompt needs at least one token")
 
+    def _check_new(self, prompts, prefix) -> None:
+        """What reading ``prompts`` and ``prefix`` would be refused for, before any conversation is changed."""
+        before = 0 if prefix is None else len(prefix)
+        self._ids(prompts if prefix is None else [prefix, *prompts])
+        if before:
+            self.state.check_room([len(prompts)], [before], fresh=True)
+        self.state.check_room(list(range(len(prompts))), [len(p) for p in prompts], fresh=True, before=before)
+
     def _read_prefix(self, prefix: Sequence[int], B: int) -> torch.Tensor:
         """Reads ``prefix`` into slot ``B`` and forks slots 0 to ``B - 1`` from it; returns its last hidden row."""
         self.state.reset(list(range(B + 1)))
@@ -197,6 +208,9 @@ class Generator:
         drawn from, and with ``top`` the likeliest ``top_tokens`` and their ``top_logprobs`` (``ops.token_logprobs``).  Slots 0
         to ``len(sequences) - 1`` (the next one too with ``prefix``) hold new conversations afterwards."""
         self._check_prompts(sequences, prefix)
+        self._check_new(sequences, prefix)
+        V = self.model.cfg.vocab_size  # scores of no rows: what the settings are refused for
+        ops.token_logprobs(torch.empty(0, V), torch.empty(0, dtype=torch.long), top=top, temperature=temperature)
         B, slots, first = len(sequences), list(range(len(sequences))), None
         if prefix is not None:
             first = self._read_prefix(prefix, B)
@@ -212,7 +226,7 @@ class Generator:
         rows, tokens = torch.tensor(rows, dtype=torch.long).to(self.device), torch.tensor(tokens, dtype=torch.long).to(self.device)
         if first is not None:
             h = torch.cat([h, first])  # row -1
-        step, parts = max(1, SCORE_LOGITS // self.model.cfg.vocab_size), []
+        step, parts = max(1, SCORE_LOGITS // V), []
         for a in range(0, max(1, len(rows)), step):
             logits = self._logits(h[rows[a:a + step]])
             parts.append([t.tolist() for t in ops.token_logprobs(logits, tokens[a:a + step], top=top, temperature=temperature)])
@@ -238,11 +252,12 @@ class Generator:
         if max_new_tokens < 1:
             return [[] for _ in prompts], [[] for _ in prompts]
         slots = list(range(B))
-        if prefix is not None:
-            self._read_prefix(prefix, B)
         V, dev = self.model.cfg.vocab_size, self.device
         row = lambda v, dt: torch.as_tensor(v, dtype=dt).expand(B).contiguous().to(dev)  # noqa: E731
         rules = (row(temperature, torch.float32), row(top_k, torch.int32), row(top_p, torch.float32), row(min_p, torch.float32))
+        self._check_new(prompts, prefix)
+        if prefix is not None:
+            self._read_prefix(prefix, B)
         noise = lambda out: out.exponential_(generator=generator)  # noqa: E731
         t, lp = ops.sample(self.prefill(prompts, slots, fresh=prefix is None), noise(torch.empty(B, V, device=dev)), *rules)
         steps = [(t, lp)]

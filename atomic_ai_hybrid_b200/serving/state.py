@@ -151,15 +151,16 @@ class DecodeState:
             self.prefix[s] = source if self.has_mla else -1
         self._rows_to_device(slots)
 
-    def check_room(self, slots: List[int], lens: List[int], fresh: bool = False) -> List[int]:
-        """Raises where MLA layers cannot hold ``lens`` more tokens; returns the slots that are to be cut back for them."""
+    def check_room(self, slots: List[int], lens: List[int], fresh: bool = False, before: int = 0) -> List[int]:
+        """Raises where MLA layers cannot hold ``lens`` more tokens (``fresh``: of new conversations, behind ``before`` shared ones);
+        returns the slots that are to be cut back for them."""
         if not self.has_mla:
             return []
         if not fresh:
             self._check_unshared(slots)
         cut = []
         for s, n in zip(slots, lens):
-            if (0 if fresh else self.lengths[s]) + n > self.max_positions:
+            if (before if fresh else self.lengths[s]) + n > self.max_positions:
                 raise ValueError(f"a conversation would grow past max_positions={self.max_positions}")
             if (0 if fresh else self.rows[s]) + n > self.max_len:
                 if not self.budget or fresh or min(self.rows[s], self.budget) + n > self.max_len:
