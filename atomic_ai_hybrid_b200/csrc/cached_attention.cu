@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(AT) ca_append(const Args a, int per) {
   }
   __shared__ Seq s_sh;
   __shared__ int i_sh, end_sh;
-  const int t_end = min(a.T, (int)blockIdx.x * per), half = a.D >> 1, pc = half >> 3, heads = a.H + 2 * a.Hk, G = a.H / a.Hk;
+  const int t_end = min(a.T, (int)blockIdx.x * per), half = a.D >> 1, pc = half >> 3, heads = a.H + 2 * a.Hk;
   for (int t = (blockIdx.x - 1) * per; t < t_end;) {
     __syncthreads();
     if (threadIdx.x == 0) {  // the rows from t on that are of one sequence, or of none
@@ -601,7 +601,7 @@ AHB_DEVICE void join_row(const Args& a, int t, int h0, int h1) {
     // the head's results one after another: of own rows, of the prefix's, each whole or from one worker after another
     const float* from[2] = {nullptr, nullptr};
     int64_t w0[2] = {0, 0}, slot[2] = {0, 0};
-    int count[2] = {0, 0}, late[2] = {0, 0};
+    int count[2] = {0, 0};
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       if (x >= n) break;
@@ -610,7 +610,6 @@ AHB_DEVICE void join_row(const Args& a, int t, int h0, int h1) {
       w0[x] = div64(first, s.share);
       const int64_t rest = first + s.units - 1 - w0[x] * s.share;  // mostly one or two workers
       count[x] = rest < s.share ? 1 : rest < 2 * s.share ? 2 : 1 + (int)div64(rest, s.share);
-      late[x] = first >= w0[x] * s.share;  // the first one's second result; the others began before their worker's units
       slot[x] = (int64_t)s.rows * (D + 4);
       from[x] = count[x] > 1 ? (s.tiles ? a.tile_part : a.part) + (int64_t)(s.row + hq - h * G) * (D + 4)
                              : a.full + ((int64_t)x * a.T * a.H + out) * (D + 4);
@@ -619,7 +618,7 @@ AHB_DEVICE void join_row(const Args& a, int t, int h0, int h1) {
     auto place = [&](int k) {
       const bool x = k >= count[0];
       const int j = x ? k - count[0] : k;
-      const int64_t at = 2 * ((x ? w0[1] : w0[0]) + j) + (j > 0 ? 0 : x ? late[1] : late[0]);
+      const int64_t at = 2 * ((x ? w0[1] : w0[0]) + j) + (j > 0 ? 0 : 1);  // the first one's second result, the others' first ones
       return (x ? from[1] : from[0]) + ((x ? count[1] : count[0]) > 1 ? at * (x ? slot[1] : slot[0]) : 0);
     };
     const int all = count[0] + count[1], each = WIDE ? (all + JW - 1) / JW : all, k0 = WIDE ? warp * each : 0;

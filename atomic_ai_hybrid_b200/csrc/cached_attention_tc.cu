@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(NTHR, 1)
   if (warp == 3) sm100::tmem_dealloc(tmem, 512);
 }
 
-// bf16 caches (S Hk, M, D): boxes of 64 channels and 128 rows of one slot's head, rows past M as zeros
+// bf16 caches (S Hk, M, D): boxes of 64 channels and TK rows of one slot's head, rows past M as zeros
 int map_cache(CUtensorMap* m, const void* p, const Args& a) {
   TmapEncodeFn fn = tmap_encode_fn();
   if (!fn) return -1;
