@@ -95,3 +95,12 @@ def test_masses_add_up(lens, had, offset):
     want = 2.0 * torch.tensor(lens, dtype=torch.float64, device=dev)[:, None]
     # sums of thousands of weights in 32 bits, and the denominators' reciprocal and the hardware's exp2 (2^-22 each)
     assert ((total / want - 1).abs() <= 1e-5).all(), float((total / want - 1).abs().max())
+
+
+@pytest.mark.parametrize("D,H,Hk", [(96, 6, 2), (128, 3, 3), (128, 8, 1)])
+@pytest.mark.parametrize("scale", [2.0, 30.0, 1e9])
+def test_large_scales_of_other_heads(D, H, Hk, scale):
+    """Scales on both sides of the one from which products are rounded first, with the other head dims and groups."""
+    for lens, had, prefix in SHAPES:
+        a = attention_inputs(lens, had, H, Hk, D, BF, dev, prefix=prefix)
+        check_attention(ops.cached_attention, {**a, "cos": None, "sin": None, "sm_scale": scale}, HALF)
