@@ -732,7 +732,7 @@ __global__ void __launch_bounds__(RW * 32, MB) ca_mass_rows(const Args a, int wa
 // Of the tile kernel's: a warp holds 64 cache rows and goes over the query rows that see them, eight at a time:
 // sum_t 2^(s_tj - m_t) / l_t.  The scores are summed in another order than the tile kernel's, which moves a weight by some 2^-22 of its
 // row's largest score: next to nothing at scores of tens, 2 % at 1e5; more than the query rows that see a cache row it never gathers.  Bound by the products, each query tile with its rounding remainders: a tracked prompt of 4000 tokens
-// takes 673 us in all, under 200 untracked (16 cache rows a warp: 1017).
+// takes 694 us in all, 172 untracked (16 cache rows a warp: 1017).
 constexpr int KM = 4;  // units of 16 cache rows that a warp holds
 template <int D, bool ROUNDED>
 __global__ void __launch_bounds__(RW * 32, 2) ca_mass(const Args a) {

@@ -41,7 +41,8 @@ struct Args {
   bool negate;                   // the sign: the rotated queries are negated
   // Exponents are s scale2 - m, in the tile kernel and for its masses by one fused operation: the product is exact there and rounded in
   // m, so that all of a row's weights and their sum carry one factor, up to 2^(half a step of m), and a quotient none.  Where scores can
-  // pass 2^28 that factor could leave 32 bits: there the product is rounded before too.
+  // pass 2^28 that factor could leave 32 bits: there the product is rounded before too, with a product and a sum for each exponent (2407
+  // tokens on 4100 shared rows at the scales 1.4 and 1.5, fused and rounded: 278 and 290 us, a prompt of 8192 613 and 610).
   bool rounded;
   bf16* o;                       // (T, H, D)
   // workspace

@@ -4,7 +4,8 @@
 //   dx_v = (g ([v = y] - p_v) - gH p_v (log p_v + H)) / T
 //
 // Sums run over differences from the running maximum, in which nothing is lost to the size of the logits.  Two values
-// at a time where the GPU has instructions for it: a bf16 logit costs five, where the copy's rate leaves time for ten.
+// at a time where the GPU has instructions for it: a bf16 logit costs eleven all told (2048 x 128256: 93.1 M issued by warps), as many
+// as the SMs issue while the copy would bring it.
 //
 // Forward: one pass over a row, by one block or, where rows are few, by a cluster of up to eight.  A warp's sums refer
 // to its own running maximum, which moves a handful of times (with one for each thread some lane of a warp had a new one at

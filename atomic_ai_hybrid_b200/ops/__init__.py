@@ -231,15 +231,16 @@ def cached_attention(q, k, v, k_cache, v_cache, lengths, cos=None, sin=None, cu_
         q, k, v clipped to 1e3;  row lengths[s] + t of the cache <- k_t, v_t, rounded to its type
         o_t = sum_j p_tj v_j,  p_t = softmax_j(sm_scale q_t k_j)  over the prefix's rows and own rows j <= lengths[s] + t
 
-    Without tables nothing is rotated; ``sm_scale`` is ``1 / sqrt(D)`` by default.  ``prefix`` (int32, one a sequence): the
+    Without tables nothing is rotated; ``sm_scale``, at most 1e28 either way, is ``1 / sqrt(D)`` by default.  ``prefix`` (int32, one a sequence): the
     slot whose rows the sequence sees before its own, any value outside ``[0, S)`` for none; neighbours in the batch
     with the same one read its rows once for all.  ``seen`` (int32, one a slot) is the position of a slot's next token,
     by default its rows and its prefix's.  ``mass`` (fp32) and ``held`` (int32), both ``(S, Hk, M)`` or neither: new
     rows start with mass 0 and hold their position, then every own row's mass grows by the ``p_tj`` that it got from the call's
-    tokens and query heads (a prefix's rows gather none).
+    tokens and query heads (a prefix's rows gather none).  Scores have 32 bits: a mass is off by some 2^-22 of the size of its tokens' largest
+    scores, next to nothing where these are tens or hundreds.
 
     ``lengths`` and ``seen`` stay as they are, for the next layer's call: the caller moves them past the tokens.  The
-    cache is read below ``lengths`` only: what lies behind may be anything.  A
+    cache is read below ``lengths`` only, rows that earlier calls wrote, or others within the same clip: what lies behind may be anything.  A
     sequence whose slot is outside ``[0, S)``, whose rows would not fit into ``M`` or whose positions have no table row is
     padding: zeros come out and nothing is written.  Returns ``o`` shaped like ``q``."""
     if q.is_cuda and _IMPL == "cuda":
